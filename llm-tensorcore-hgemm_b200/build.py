@@ -7,8 +7,10 @@ Produces, next to the Python sources in ``llm_hgemm/``:
   static CUDA runtime, no torch);
 * ``libhgemm_sm100_debug.so`` - the same with ``-DHGEMM_DEBUG`` (device-side
   bounds checks that record a failure instead of trapping), for tests;
+* ``libhgemm_train_sm100.so`` - the training operators' kernels and the C ABI
+  of ``include/hgemm_sm100_train.h``, built the same way;
 * ``_C<EXT_SUFFIX>`` - the pybind11/torch host module (contract checks, name
-  dispatch, current-stream launch) linked against ``libhgemm_sm100.so``;
+  dispatch, autograd, current-stream launch) linked against both libraries;
 * ``_comparators<EXT_SUFFIX>`` - benchmark-only cuBLASLt comparator (never in
   the ``hgemm`` dispatch path).
 
@@ -48,9 +50,13 @@ DEBUG_LIB = OUT_DIR / "libhgemm_sm100_debug.so"
 KERNEL_SOURCES = [CSRC / "hgemm_sm100.cu"]
 KERNEL_DEPS = KERNEL_SOURCES + [CSRC / "hgemm_kernels.cuh", CSRC / "sm100_ptx.cuh", CSRC / "debug_checks.cuh",
                                 INCLUDE / "hgemm_sm100.h"]
+TRAIN_LIB = OUT_DIR / "libhgemm_train_sm100.so"
+TRAIN_SOURCES = [CSRC / "train_sm100.cu"]
+TRAIN_DEPS = TRAIN_SOURCES + [CSRC / "train_kernels.cuh", INCLUDE / "hgemm_sm100_train.h"] + KERNEL_DEPS[1:]
 HOST_SOURCES = [CSRC / "host" / "bindings.cpp", CSRC / "host" / "contract.cpp",
-                CSRC / "host" / "dispatch.cpp"]
-HOST_DEPS = HOST_SOURCES + [CSRC / "host" / "hgemm.h", INCLUDE / "hgemm_sm100.h"]
+                CSRC / "host" / "dispatch.cpp", CSRC / "host" / "training.cpp"]
+HOST_DEPS = HOST_SOURCES + [CSRC / "host" / "hgemm.h", CSRC / "host" / "training.h",
+                            INCLUDE / "hgemm_sm100.h", INCLUDE / "hgemm_sm100_train.h"]
 COMPARATOR_SOURCES = [CSRC / "comparators" / "cublaslt_comparator.cpp"]
 
 
@@ -94,6 +100,15 @@ def build_kernel_lib(force: bool = False, debug: bool = False) -> Path:
     return target
 
 
+def build_train_lib(force: bool = False) -> Path:
+    if not force and not _stale(TRAIN_LIB, TRAIN_DEPS):
+        return TRAIN_LIB
+    _run([NVCC, *ARCH_FLAGS, "-O3", "-std=c++17", "-lineinfo", "-Xptxas", "-v",
+          "-Xcompiler", "-fPIC", "-shared", "-cudart", "static",
+          f"-I{INCLUDE}", f"-I{CSRC}", *map(str, TRAIN_SOURCES), "-o", str(TRAIN_LIB)])
+    return TRAIN_LIB
+
+
 def _torch_flags() -> tuple[list[str], list[str]]:
     import torch
     from torch.utils import cpp_extension
@@ -121,12 +136,12 @@ def _compile_objects(sources: list[Path], cflags: list[str], tag: str) -> list[P
 
 def build_host_module(force: bool = False) -> Path:
     target = host_module()
-    if not force and not _stale(target, HOST_DEPS + [KERNEL_LIB]):
+    if not force and not _stale(target, HOST_DEPS + [KERNEL_LIB, TRAIN_LIB]):
         return target
     cflags, ldflags = _torch_flags()
     objs = _compile_objects(HOST_SOURCES, cflags + [f"-I{CSRC / 'host'}"], "host")
     _run(["g++", "-shared", *map(str, objs), "-o", str(target), f"-L{OUT_DIR}", "-lhgemm_sm100",
-          "-Wl,-rpath,$ORIGIN", *ldflags])
+          "-lhgemm_train_sm100", "-Wl,-rpath,$ORIGIN", *ldflags])
     return target
 
 
@@ -148,8 +163,8 @@ def build_comparator_module(force: bool = False) -> Path | None:
 def build(force: bool = False, debug: bool = True) -> None:
     if shutil.which(NVCC) is None and not Path(NVCC).exists():
         raise RuntimeError(f"nvcc not found at {NVCC}")
-    with ThreadPoolExecutor(max_workers=2) as pool:
-        jobs = [pool.submit(build_kernel_lib, force)]
+    with ThreadPoolExecutor(max_workers=3) as pool:
+        jobs = [pool.submit(build_kernel_lib, force), pool.submit(build_train_lib, force)]
         if debug:
             jobs.append(pool.submit(build_kernel_lib, force, True))
         for j in jobs:
@@ -164,7 +179,7 @@ def main() -> None:
     parser.add_argument("--no-debug", action="store_true", help="skip the -DHGEMM_DEBUG kernel library")
     args = parser.parse_args()
     build(args.force, debug=not args.no_debug)
-    print(f"built {KERNEL_LIB.name}, {'' if args.no_debug else DEBUG_LIB.name + ', '}{host_module().name}")
+    print(f"built {KERNEL_LIB.name}, {TRAIN_LIB.name}, {'' if args.no_debug else DEBUG_LIB.name + ', '}{host_module().name}")
 
 
 if __name__ == "__main__":

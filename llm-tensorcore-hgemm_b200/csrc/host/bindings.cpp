@@ -1,10 +1,12 @@
 // pybind11 module llm_hgemm._C: the four functions of the reference module
 // (reference csrc/bindings.cpp:6-14, same defaults) plus introspection and
-// the FP32-output entry used by the tensor-parallel MLP.
+// the FP32-output entry used by the tensor-parallel MLP, and the training
+// operators.
 #include <pybind11/stl.h>
 #include <torch/extension.h>
 
 #include "hgemm.h"
+#include "training.h"
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "B200 (sm_100a) tcgen05 HGEMM backends";
@@ -20,4 +22,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("implementation") = "auto");
     m.def("implementations", &implementations);
     m.def("resolve", &resolve, py::arg("a"), py::arg("b"), py::arg("implementation") = "auto");
+    m.def("gated_ffn", &gated_ffn, py::arg("x"), py::arg("gate"), py::arg("up"), py::arg("down"));
+    m.def("linear_cross_entropy", &linear_cross_entropy, py::arg("x"), py::arg("weight"), py::arg("target"),
+          py::arg("reduction") = "mean", py::arg("ignore_index") = -100);
+    m.def("orthogonalize", &orthogonalize, py::arg("g"), py::arg("steps"), py::arg("a"), py::arg("b"), py::arg("c"),
+          py::arg("eps"));
 }

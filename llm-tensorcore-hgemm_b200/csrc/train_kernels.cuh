@@ -1,0 +1,806 @@
+// sm_100a kernels of the training operators (gated feed-forward block and its
+// gradient, cross entropy from hidden states and its gradient, orthogonalised
+// updates). All of their matrix products run on one tcgen05 kernel template,
+//
+//   train_gemm_kernel<kPair, kEpi>:  acc[m, n] = sum_k A(m, k) B(k, n)
+//
+// for FP16 or BF16 operands and FP32 accumulators in TMEM. It differs from the
+// inference kernels of hgemm_kernels.cuh in what a training step needs:
+//
+//  * either operand lies either way in memory (rows along K, "K-major", or
+//    rows along M / N, "MN-major"), chosen per problem at run time: only the
+//    TMA boxes and the matrix descriptors differ, so x W^T, dy W and dy^T x
+//    all read the tensors where they are, without a transposed copy;
+//  * the sum over K may run over two operand pairs (dx = dg Wg + du Wu), and
+//    the columns of B may come from two tensors (gate and up), so no weight is
+//    packed: a training step changes the weights every time;
+//  * one launch takes up to four problems and walks their tiles as one list
+//    (dx, dWgate, dWup and dWdown fill the last wave together);
+//  * the epilogue finishes the operator (SwiGLU, its gradient, softmax
+//    statistics, the logits' gradient, a x X + acc) on the FP32 accumulators.
+//
+// kPair: tiles of 256 x tile_n per CTA pair (cta_group::2); otherwise 128 x
+// tile_n per CTA. tile_n is a run-time multiple of 32 (pairs: 64) up to 256,
+// so the host cuts the columns into a whole number of waves.
+// Roles per CTA: warps 0-3 epilogue (one TMEM lane = one output row per
+// thread), warp 4 TMA producer, warp 5 MMA issuer; two accumulators, so a
+// tile's epilogue runs under the next tile's MMAs. Every wait is bounded as
+// in the inference kernels (status word, drained copies, freed TMEM).
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "hgemm_kernels.cuh"
+
+namespace hgemm {
+
+constexpr int kTrainMaxProblems = 4;
+constexpr uint32_t kTrainRingBytes = 196608;               // stages of both operands
+constexpr uint32_t kTrainBoxBytes = 2048;                  // 32 rows x 32 16-bit columns
+constexpr uint32_t kTrainEpiBytes = 4u * 4u * kTrainBoxBytes;  // 4 warps x 4 boxes
+constexpr int kTrainMaxStages = 12;
+constexpr uint32_t kTrainDataBytes = kTrainRingBytes + kTrainEpiBytes;
+constexpr uint32_t kTrainSmemBytes = kTrainDataBytes + 256 + 1024;
+constexpr uint32_t kTrainAccCols = 256;                    // TMEM columns per accumulator
+static_assert(2 * kTrainMaxStages + 5 <= 30, "barrier area");
+static_assert(kTrainSmemBytes <= 232448, "shared memory");
+
+enum : int {
+    kTrainStore = 0,      // out = alpha acc + beta C (16 bits), or FP32 acc stored / added
+    kTrainGate = 1,       // acc = (gate | up): out = silu(gate) up, gate and up kept
+    kTrainGateGrad = 2,   // acc = dh: out = dh up silu'(gate), out2 = dh silu(gate)
+    kTrainLse = 3,        // per row: max and sum of exp over the tile's columns
+    kTrainLogitGrad = 4,  // out = (exp(acc - lse) - [column == target]) row factor
+};
+// How kTrainStore writes: 16-bit boxes, FP32 boxes, FP32 boxes added to memory.
+enum : int { kTrainOut16 = 0, kTrainOutF32 = 1, kTrainOutF32Add = 2 };
+
+struct alignas(64) TrainProblem {
+    CUtensorMap a[2];      // A of the first and second K segment
+    CUtensorMap b[2];      // B of the two segments, or (dual) the two column halves
+    CUtensorMap out[3];
+    int m, n;              // output rows and columns (dual: columns of one half)
+    int tile_n;            // accumulator columns of a tile (dual: both halves)
+    int nkb0, nkb;         // K blocks of the first segment, of both
+    int a_mn, b_mn, dual;
+    int tiles_m, tiles_n, group_m;
+    int out_kind;
+    float alpha, beta;
+    const float* alpha_ptr;    // multiplies alpha (device memory; may be null)
+    const void* c;             // 16-bit [m x ldc] for beta != 0
+    long long ldc;
+};
+
+struct alignas(64) TrainParams {
+    TrainProblem prob[kTrainMaxProblems];
+    int num_problems;
+    int heavy_tiles, light_tiles;  // tiles of problem 0 / of the others
+    int light_skip;                // waves the units with one heavy tile more sit out
+    int stages;
+    uint32_t stage_bytes;
+    int in_bf16, out_bf16;
+    int* status;
+    unsigned long long timeout_ns;
+    int inject;                    // test only: arm the first stage with 16 bytes more
+    // kTrainGateGrad: the saved pre-activations, 16-bit [m x ld_saved].
+    const void* gate;
+    const void* up;
+    long long ld_saved;
+    int keep;                      // kTrainGate: store gate and up too (out[1], out[2])
+    // kTrainLse / kTrainLogitGrad, per row.
+    const long long* target;
+    long long col_base;            // vocabulary index of column 0
+    float2* partial;               // kTrainLse: [tiles_n][m] (max, sum of exp(x - max))
+    float* target_logit;           // kTrainLse: written by the tile holding the target
+    const float* lse;
+    const float* row_scale;
+};
+
+// ------------------------------------------------------------- small parts ---
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, int bf16) {
+    if (bf16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, int bf16) {
+    if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ float to_f32(const void* base, long long i, int bf16) {
+    return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(base)[i])
+                : __half2float(static_cast<const __half*>(base)[i]);
+}
+
+// 2^x (about 2 ulp; -inf -> 0, NaN -> NaN).
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
+// sigmoid(x); x -> -inf gives 0 (1 / (1 + inf)).
+__device__ __forceinline__ float sigmoid_f(float x) { return __frcp_rn(1.f + exp2_fast(-x * kLog2e)); }
+
+// 32 16-bit values src[0 .. 31] of one row as floats; elements from `avail`
+// on are zero. src 16-byte aligned; whole 8-element vectors are read only
+// where avail > 0 (rows are padded to a multiple of 8 elements).
+__device__ __forceinline__ void load_row32(const void* base, long long off, int avail, int bf16, float (&v)[32]) {
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + off);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (8 * q < avail) w = __ldg(src + q);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack2(u[j], bf16);
+            v[8 * q + 2 * j] = f.x;
+            v[8 * q + 2 * j + 1] = f.y;
+        }
+    }
+}
+
+// Adds a 2-D box in shared memory to FP32 global memory (elements outside the
+// map are not written).
+__device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap* map, const void* src, int32_t x, int32_t y) {
+    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(src)), "r"(x), "r"(y)
+                 : "memory");
+}
+
+// One epilogue warp's output boxes: 32 rows (lane = row) x 32 columns through
+// shared memory to a TMA store, 16-bit boxes in a ring of four 2 KB buffers
+// (64-byte swizzle), FP32 boxes in a ring of two 4 KB buffers (128-byte
+// swizzle). Before a buffer is rewritten, the store that used it last must
+// have read it. Every value is rounded here, once.
+struct BoxWriter {
+    uint8_t* bufs;
+    uint32_t next;
+    uint32_t lane;
+
+    __device__ void put16(const CUtensorMap* map, const float (&v)[32], int bf16, int col, int row) {
+        if (lane == 0) bulk_wait_group_read<3>();
+        __syncwarp();
+        uint8_t* box = bufs + (next & 3u) * kTrainBoxBytes;
+        ++next;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            uint4 q;
+            q.x = pack2(v[8 * j + 0], v[8 * j + 1], bf16);
+            q.y = pack2(v[8 * j + 2], v[8 * j + 3], bf16);
+            q.z = pack2(v[8 * j + 4], v[8 * j + 5], bf16);
+            q.w = pack2(v[8 * j + 6], v[8 * j + 7], bf16);
+            *reinterpret_cast<uint4*>(box + lane * 64u + ((j ^ ((lane >> 1) & 3u)) << 4)) = q;
+        }
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+            tma_store_2d(map, box, col, row);
+            bulk_commit_group();
+        }
+    }
+
+    __device__ void put32(const CUtensorMap* map, const float (&v)[32], bool add, int col, int row) {
+        if (lane == 0) bulk_wait_group_read<1>();
+        __syncwarp();
+        uint8_t* box = bufs + (next & 1u) * (2u * kTrainBoxBytes);
+        ++next;
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j)
+            *reinterpret_cast<float4*>(box + lane * 128u + ((j ^ (lane & 7u)) << 4)) =
+                make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+            if (add)
+                tma_reduce_add_2d(map, box, col, row);
+            else
+                tma_store_2d(map, box, col, row);
+            bulk_commit_group();
+        }
+    }
+};
+
+__device__ __forceinline__ void tmem_ld32(uint32_t t, float (&v)[32]) {
+    uint32_t r[32];
+    tmem_ld_32x32b_x32(t, r);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// The tiles of one unit (CTA or pair) in order; every role iterates alike.
+// Problem 0's tiles ("heavy": the longest K) go round robin; where they do
+// not divide evenly the units that took one more sit out the first
+// `light_skip` waves of the other problems' tiles, which are shorter.
+struct TileIter {
+    int unit, units, next_heavy, wave;
+    __device__ TileIter(int u, int n) : unit(u), units(n), next_heavy(u), wave(0) {}
+    __device__ bool next(const TrainParams& p, int& prob, int& tm, int& tn, int& nth) {
+        int t;
+        if (next_heavy < p.heavy_tiles) {
+            prob = 0;
+            t = next_heavy;
+            nth = next_heavy / units;
+            next_heavy += units;
+        } else {
+            const int rest = p.heavy_tiles % units;
+            if (wave < p.light_skip && unit < rest) wave = p.light_skip;
+            t = wave < p.light_skip ? wave * (units - rest) + unit - rest
+                                    : p.light_skip * (units - rest) + (wave - p.light_skip) * units + unit;
+            nth = wave;
+            ++wave;
+            if (t >= p.light_tiles) return false;
+            prob = 1;
+            while (true) {
+                const int tiles = p.prob[prob].tiles_m * p.prob[prob].tiles_n;
+                if (t < tiles) break;
+                t -= tiles;
+                ++prob;
+            }
+        }
+        const TrainProblem& q = p.prob[prob];
+        tile_coords(t, q.tiles_m, q.tiles_n, q.group_m, tm, tn);
+        return true;
+    }
+};
+
+// ---------------------------------------------------------------- epilogues ---
+
+// One 32-row x tile_n accumulator slice at TMEM address `t`: rows row0 + lane,
+// columns of tile column tn. Called by the whole warp.
+template <int kEpi>
+__device__ __forceinline__ void train_epilogue(const TrainParams& p, const TrainProblem& q, BoxWriter& box,
+                                               uint32_t t, int row0, int tn) {
+    if (row0 >= q.m) return;
+    const int row = row0 + static_cast<int>(box.lane);
+    const bool in_rows = row < q.m;
+    if constexpr (kEpi == kTrainStore) {
+        const float alpha = q.alpha_ptr != nullptr ? q.alpha * __ldg(q.alpha_ptr) : q.alpha;
+#pragma unroll 1
+        for (int c = 0; c < q.tile_n; c += 32) {
+            const int col = tn * q.tile_n + c;
+            if (col >= q.n) break;
+            float v[32];
+            tmem_ld32(t + c, v);
+            if (q.out_kind != kTrainOut16) {
+                box.put32(&q.out[0], v, q.out_kind == kTrainOutF32Add, col, row0);
+                continue;
+            }
+            if (q.beta != 0.f) {
+                float w[32];
+                load_row32(q.c, row * q.ldc + col, in_rows ? q.n - col : 0, p.in_bf16, w);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = fmaf(alpha, v[i], q.beta * w[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] *= alpha;
+            }
+            box.put16(&q.out[0], v, p.out_bf16, col, row0);
+        }
+    } else if constexpr (kEpi == kTrainGate) {
+        const int half = q.tile_n / 2;
+#pragma unroll 1
+        for (int c = 0; c < half; c += 32) {
+            const int col = tn * half + c;
+            if (col >= q.n) break;
+            float g[32], u[32];
+            tmem_ld32(t + c, g);
+            tmem_ld32(t + half + c, u);
+            if (p.keep) {
+                box.put16(&q.out[1], g, p.out_bf16, col, row0);
+                box.put16(&q.out[2], u, p.out_bf16, col, row0);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) u[i] *= g[i] * sigmoid_f(g[i]);
+            box.put16(&q.out[0], u, p.out_bf16, col, row0);
+        }
+    } else if constexpr (kEpi == kTrainGateGrad) {
+#pragma unroll 1
+        for (int c = 0; c < q.tile_n; c += 32) {
+            const int col = tn * q.tile_n + c;
+            if (col >= q.n) break;
+            float g[32], u[32], v[32];
+            const int avail = in_rows ? q.n - col : 0;
+            load_row32(p.gate, row * p.ld_saved + col, avail, p.in_bf16, g);
+            load_row32(p.up, row * p.ld_saved + col, avail, p.in_bf16, u);
+            tmem_ld32(t + c, v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const float s = sigmoid_f(g[i]);
+                const float silu = g[i] * s;
+                // silu' = s (1 + g (1 - s)) = s + silu (1 - s)
+                g[i] = v[i] * u[i] * fmaf(silu, 1.f - s, s);
+                u[i] = v[i] * silu;
+            }
+            box.put16(&q.out[0], g, p.out_bf16, col, row0);
+            box.put16(&q.out[1], u, p.out_bf16, col, row0);
+        }
+    } else if constexpr (kEpi == kTrainLse) {
+        // Running maximum and sum over the tile's columns of this thread's row.
+        const long long want = in_rows ? p.target[row] - p.col_base : -1;
+        float top = __int_as_float(0xff800000), sum = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < q.tile_n; c += 32) {
+            const int col = tn * q.tile_n + c;
+            if (col >= q.n) break;
+            float v[32];
+            tmem_ld32(t + c, v);
+            if (want >= col && want < col + 32) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (col + i == want && want < q.n) p.target_logit[row] = v[i];
+            }
+            if (col + 32 > q.n) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (col + i >= q.n) v[i] = __int_as_float(0xff800000);
+            }
+            float best = v[0];
+#pragma unroll
+            for (int i = 1; i < 32; ++i) best = fmaxf(best, v[i]);
+            best = fmaxf(best, top);
+            // No column above -inf yet: subtract 0, so that exp gives 0, not NaN.
+            const float ref = best == __int_as_float(0xff800000) ? 0.f : best;
+            float part = 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) part += exp2_fast((v[i] - ref) * kLog2e);
+            sum = fmaf(sum, exp2_fast((top - ref) * kLog2e), part);
+            top = best;
+        }
+        if (in_rows) p.partial[static_cast<long long>(tn) * q.m + row] = make_float2(top, sum);
+    } else {
+        const long long want = in_rows ? p.target[row] - p.col_base : -1;
+        const float scale = in_rows ? p.row_scale[row] : 0.f;
+        const float lse = in_rows ? p.lse[row] : 0.f;
+#pragma unroll 1
+        for (int c = 0; c < q.tile_n; c += 32) {
+            const int col = tn * q.tile_n + c;
+            if (col >= q.n) break;
+            float v[32];
+            tmem_ld32(t + c, v);
+            // A row without a target has factor 0 and gradient 0, whatever its logits.
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = scale == 0.f ? 0.f : exp2_fast((v[i] - lse) * kLog2e) * scale;
+            if (want >= col && want < col + 32) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (col + i == want) v[i] -= scale;
+            }
+            box.put16(&q.out[0], v, p.out_bf16, col, row0);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ the GEMM ---
+
+template <bool kPair, int kEpi>
+__global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_constant__ TrainParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = align_1024(smem_raw);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kTrainDataBytes);   // pair: the even CTA's
+    uint64_t* empty = full + kTrainMaxStages;
+    uint64_t* tfull = empty + kTrainMaxStages;   // [2]
+    uint64_t* tempty = tfull + 2;                // [2], pair: the even CTA's
+    uint64_t* drain = tempty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    constexpr int kTileM = kPair ? 256 : 128;
+    constexpr uint32_t kABytes = 128u * 128u;    // 128 rows x 64 halves, either way round
+    const uint32_t warp = warp_index();
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint32_t rank = kPair ? cluster_ctarank() : 0u;
+    const bool leader = rank == 0;
+
+    if (warp == 4 && lane == 0) {
+        for (int s = 0; s < p.stages; ++s) {
+            mbar_init(&full[s], 1u);
+            mbar_init(&empty[s], 1u);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&tfull[i], 1u);
+            mbar_init(&tempty[i], kPair ? 8u : 4u);   // one lane of each epilogue warp
+        }
+        mbar_init(drain, 1u);
+        *abort_flag = 0;
+        mbar_init_fence();
+    }
+    if (warp == 5) {
+        if constexpr (kPair) {
+            tmem_alloc_pair(tmem_slot, 2 * kTrainAccCols);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(tmem_slot, 2 * kTrainAccCols);
+            tmem_relinquish();
+        }
+    }
+    tc_fence_before_sync();
+    if constexpr (kPair) cluster_sync();         // both CTAs' barriers exist before any remote op
+    else __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+    grid_dependents_launch();
+    grid_dependency_wait();                      // global memory only after the previous kernel
+    const WaitCtl wc{abort_flag, p.status, p.timeout_ns};
+    const int unit = kPair ? blockIdx.x >> 1 : blockIdx.x;
+    const int units = kPair ? gridDim.x >> 1 : gridDim.x;
+    TileIter it(unit, units);
+    int prob, tm, tn, nth;
+
+    if (warp == 4) {
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0, issued = 0;
+            bool ok = true;
+            while (ok && it.next(p, prob, tm, tn, nth)) {
+                const TrainProblem& q = p.prob[prob];
+                const int row0 = tm * kTileM + static_cast<int>(rank) * 128;
+                // Columns of B that this CTA loads: all, or its half of the pair's.
+                const int cols = kPair ? q.tile_n / 2 : q.tile_n;
+                const int col0 = q.dual ? tn * (q.tile_n / 2) : tn * q.tile_n + static_cast<int>(rank) * cols;
+                const uint32_t bytes = kABytes + (q.b_mn ? ((cols + 63) / 64) * kChunkBytes : cols * 128u);
+                // Odd waves walk K backwards: they start on the panels that the
+                // wave before read last, while those are in L2.
+                const bool back = (nth & 1) != 0;
+                for (int kq = 0; kq < q.nkb; ++kq) {
+                    const int kb = back ? q.nkb - 1 - kq : kq;
+                    if (!(kPair ? mbar_wait_cluster(&empty[stage], phase ^ 1u, wc)
+                                : mbar_wait(&empty[stage], phase ^ 1u, wc))) { ok = false; break; }
+                    uint8_t* s_a = smem + stage * p.stage_bytes;
+                    uint8_t* s_b = s_a + kABytes;
+                    if (leader) {
+                        const uint32_t extra = (p.inject && issued == 0) ? 16u : 0u;
+                        mbar_arrive_expect_tx(&full[stage], (kPair ? 2u : 1u) * bytes + extra);
+                    }
+                    const uint32_t bar = kPair ? map_to_rank(smem_addr(&full[stage]), 0) : 0u;
+                    auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y) {
+                        if constexpr (kPair) tma_load_2d_pair(dst, map, bar, x, y);
+                        else tma_load_2d(dst, map, &full[stage], x, y);
+                    };
+                    const int seg = kb >= q.nkb0 ? 1 : 0;
+                    const int k0 = (seg ? kb - q.nkb0 : kb) * kBlockK;
+                    if (q.a_mn) {
+                        load(s_a, &q.a[seg], row0, k0);
+                        load(s_a + kChunkBytes, &q.a[seg], row0 + 64, k0);
+                    } else {
+                        load(s_a, &q.a[seg], k0, row0);
+                    }
+                    if (q.dual) {
+                        if constexpr (kPair) {
+                            load(s_b, &q.b[rank], k0, col0);
+                        } else {
+                            load(s_b, &q.b[0], k0, col0);
+                            load(s_b + (cols / 2) * 128, &q.b[1], k0, col0);
+                        }
+                    } else if (q.b_mn) {
+                        for (int j = 0; j < cols; j += 64) load(s_b + j * 128, &q.b[seg], col0 + j, k0);
+                    } else {
+                        load(s_b, &q.b[seg], k0, col0);
+                    }
+                    ++issued;
+                    if (++stage == static_cast<uint32_t>(p.stages)) { stage = 0; phase ^= 1u; }
+                }
+            }
+            if (leader && (!ok || *abort_flag)) {
+                // In-flight copies land before the CTA (or its pair) leaves.
+                const uint32_t n = static_cast<uint32_t>(p.stages);
+                for (uint32_t s = 0; s < (issued < n ? issued : n); ++s) {
+                    const uint32_t arms = issued / n + (s < issued % n ? 1u : 0u);
+                    mbar_wait_drain(&full[s], (arms - 1u) & 1u, kDrainLimitNs);
+                }
+            }
+        }
+    } else if (warp == 5) {
+        if (lane == 0 && leader) {
+            uint32_t stage = 0, phase = 0, iter = 0;
+            bool ok = true;
+            const uint32_t format = p.in_bf16 ? (1u << 7) | (1u << 10) : 0u;
+            while (ok && it.next(p, prob, tm, tn, nth)) {
+                const TrainProblem& q = p.prob[prob];
+                const uint32_t idesc = make_idesc_f16(kTileM, 0, q.a_mn, q.b_mn) | format |
+                                       (static_cast<uint32_t>(q.tile_n >> 3) << 17);
+                // 16 of K further: 32 bytes along a K-major row, 16 rows of 128 bytes MN-major.
+                const uint64_t step_a = q.a_mn ? 2048u >> 4 : 32u >> 4;
+                const uint64_t step_b = q.b_mn ? 2048u >> 4 : 32u >> 4;
+                const uint32_t lbo_a = q.a_mn ? kChunkBytes : 16u, lbo_b = q.b_mn ? kChunkBytes : 16u;
+                const uint32_t acc = iter & 1u, acc_phase = (iter >> 1) & 1u;
+                ++iter;
+                if (!(kPair ? mbar_wait_cluster(&tempty[acc], acc_phase ^ 1u, wc)
+                            : mbar_wait(&tempty[acc], acc_phase ^ 1u, wc))) { ok = false; break; }
+                tc_fence_after_sync();
+                const uint32_t d = tmem_base + acc * kTrainAccCols;
+                for (int kb = 0; kb < q.nkb; ++kb) {
+                    if (!mbar_wait(&full[stage], phase, wc)) { ok = false; break; }
+                    tc_fence_after_sync();
+                    const uint32_t s_a = smem_addr(smem + stage * p.stage_bytes);
+                    const uint64_t da = make_smem_desc(s_a, lbo_a, 1024u);
+                    const uint64_t db = make_smem_desc(s_a + kABytes, lbo_b, 1024u);
+#pragma unroll
+                    for (int kk = 0; kk < kBlockK / 16; ++kk) {
+                        const uint32_t add = (kb > 0 || kk > 0) ? 1u : 0u;
+                        if constexpr (kPair) tc_mma_f16_pair(d, da + kk * step_a, db + kk * step_b, idesc, add);
+                        else tc_mma_f16(d, da + kk * step_a, db + kk * step_b, idesc, add);
+                    }
+                    if constexpr (kPair) tc_commit_pair_both(smem_addr(&empty[stage]));
+                    else tc_commit(&empty[stage]);
+                    if (++stage == static_cast<uint32_t>(p.stages)) { stage = 0; phase ^= 1u; }
+                }
+                if (ok) {
+                    if constexpr (kPair) tc_commit_pair_both(smem_addr(&tfull[acc]));
+                    else tc_commit(&tfull[acc]);
+                }
+            }
+            if (!ok) {
+                if constexpr (kPair) tc_commit_pair(smem_addr(drain));
+                else tc_commit(drain);
+                mbar_wait_drain(drain, 0, kDrainLimitNs);
+            }
+        }
+    } else {
+        const uint32_t tempty0 = kPair ? map_to_rank(smem_addr(&tempty[0]), 0) : 0u;
+        const uint32_t tempty1 = kPair ? map_to_rank(smem_addr(&tempty[1]), 0) : 0u;
+        BoxWriter box{smem + kTrainRingBytes + warp * 4u * kTrainBoxBytes, 0u, lane};
+        uint32_t iter = 0;
+        while (it.next(p, prob, tm, tn, nth)) {
+            const TrainProblem& q = p.prob[prob];
+            const uint32_t acc = iter & 1u, acc_phase = (iter >> 1) & 1u;
+            ++iter;
+            const bool got = kPair ? mbar_wait_cluster(&tfull[acc], acc_phase, wc) : mbar_wait(&tfull[acc], acc_phase, wc);
+            if (!__all_sync(0xffffffffu, got)) break;
+            tc_fence_after_sync();
+            const int row0 = tm * kTileM + static_cast<int>(rank) * 128 + static_cast<int>(warp) * 32;
+            train_epilogue<kEpi>(p, q, box, tmem_base + ((warp * 32u) << 16) + acc * kTrainAccCols, row0, tn);
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (kPair) mbar_arrive_cluster(acc ? tempty1 : tempty0);
+                else mbar_arrive(&tempty[acc]);
+            }
+        }
+        if (lane == 0) bulk_wait_group_all();
+    }
+
+    __syncwarp();
+    if (kPair && *abort_flag) settle_ns(2000000ull);   // the peer's copies towards this CTA land
+    tc_fence_before_sync();
+    if constexpr (kPair) cluster_sync();               // no CTA leaves while its pair may still touch it
+    else __syncthreads();
+    if (warp == 5) {
+        tc_fence_after_sync();
+        if constexpr (kPair) tmem_dealloc_pair(tmem_base, 2 * kTrainAccCols);
+        else tmem_dealloc(tmem_base, 2 * kTrainAccCols);
+    }
+}
+
+// -------------------------------------------------- cross entropy, row parts ---
+
+// Factor on the stored logit gradients, so that a probability of 1 / vocabulary
+// stays a normal FP16 number; the products' epilogues take it out again.
+constexpr float kLogitGradScale = 16384.f;
+
+// Joins a row's per-tile (max, sum) pairs: lse = max + log(sum), and its loss
+// lse - logit[target], formed as (max - logit) + log(sum). A row whose target
+// is `ignore` has loss 0; one outside the vocabulary gets NaN.
+// Block (32 rows, 32 slices of the tile list), joined in shared memory.
+__global__ void __launch_bounds__(1024) lse_join_kernel(const float2* __restrict__ partial, int tiles, int m,
+                                                        const float* __restrict__ target_logit,
+                                                        const long long* __restrict__ target, long long vocab,
+                                                        long long ignore, float* __restrict__ lse,
+                                                        float* __restrict__ loss) {
+    __shared__ float2 part[32][33];
+    grid_dependents_launch();
+    grid_dependency_wait();
+    const int row = blockIdx.x * 32 + threadIdx.x;
+    const float kNone = __int_as_float(0xff800000);
+    float top = kNone, sum = 0.f;   // a NaN sum stays NaN through every join
+    if (row < m) {
+        for (int t = threadIdx.y; t < tiles; t += 32) {
+            const float2 v = partial[static_cast<long long>(t) * m + row];
+            const float best = fmaxf(top, v.x);
+            const float ref = best == kNone ? 0.f : best;
+            sum = sum * exp2_fast((top - ref) * kLog2e) + v.y * exp2_fast((v.x - ref) * kLog2e);
+            top = best;
+        }
+    }
+    part[threadIdx.y][threadIdx.x] = make_float2(top, sum);
+    __syncthreads();
+    if (threadIdx.y != 0 || row >= m) return;
+    for (int t = 1; t < 32; ++t) {
+        const float2 v = part[t][threadIdx.x];
+        const float best = fmaxf(top, v.x);
+        const float ref = best == kNone ? 0.f : best;
+        sum = sum * exp2_fast((top - ref) * kLog2e) + v.y * exp2_fast((v.x - ref) * kLog2e);
+        top = best;
+    }
+    const float ls = logf(sum);
+    lse[row] = top + ls;
+    const long long want = target[row];
+    if (want == ignore) loss[row] = 0.f;
+    else loss[row] = (want >= 0 && want < vocab) ? (top - target_logit[row]) + ls : __int_as_float(0x7fffffff);
+}
+
+// Sum of the rows' losses (and their count for the mean), one block, in a
+// fixed order and 64 bits.
+__global__ void __launch_bounds__(1024) loss_reduce_kernel(const float* __restrict__ loss,
+                                                           const long long* __restrict__ target, int m,
+                                                           long long ignore, int mean, float* __restrict__ out) {
+    __shared__ double sums[32];
+    __shared__ int counts[32];
+    grid_dependents_launch();
+    grid_dependency_wait();
+    double s = 0.;
+    int c = 0;
+    for (int i = threadIdx.x; i < m; i += 1024) {
+        s += static_cast<double>(loss[i]);
+        c += target[i] != ignore;
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        c += __shfl_xor_sync(0xffffffffu, c, o);
+    }
+    if ((threadIdx.x & 31) == 0) {
+        sums[threadIdx.x >> 5] = s;
+        counts[threadIdx.x >> 5] = c;
+    }
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int i = 1; i < 32; ++i) {
+        s += sums[i];
+        c += counts[i];
+    }
+    *out = static_cast<float>(mean ? s / c : s);   // no target at all: 0 / 0 = NaN for the mean
+}
+
+// Row factors of the logits' gradient and the scalar that the products take:
+// dz[row] = row_scale[row] (p - onehot), gradient = alpha dz^T x and so on.
+// One loss per row: row_scale = dloss[row] / max |dloss|, so that any range of
+// incoming gradients fits 16 bits. One block.
+__global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* __restrict__ dloss, int per_row, int mean,
+                                                                const long long* __restrict__ target, int m,
+                                                                long long vocab, long long ignore,
+                                                                float* __restrict__ row_scale,
+                                                                float* __restrict__ alpha) {
+    __shared__ float tops[32];
+    __shared__ int counts[32];
+    grid_dependents_launch();
+    grid_dependency_wait();
+    float top = 0.f;
+    int c = 0;
+    bool odd = false;
+    for (int i = threadIdx.x; i < m; i += 1024) {
+        if (target[i] == ignore) continue;
+        ++c;
+        if (per_row) {
+            const float a = fabsf(dloss[i]);
+            odd |= !(a <= 3.4028235e38f);
+            top = fmaxf(top, a);
+        }
+    }
+    if (odd) top = __int_as_float(0x7f800000);
+    for (int o = 16; o > 0; o >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        c += __shfl_xor_sync(0xffffffffu, c, o);
+    }
+    if ((threadIdx.x & 31) == 0) {
+        tops[threadIdx.x >> 5] = top;
+        counts[threadIdx.x >> 5] = c;
+    }
+    __syncthreads();
+    top = 0.f;
+    c = 0;
+    for (int i = 0; i < 32; ++i) {
+        top = fmaxf(top, tops[i]);
+        c += counts[i];
+    }
+    const float nan = __int_as_float(0x7fffffff);
+    for (int i = threadIdx.x; i < m; i += 1024) {
+        const long long want = target[i];
+        float r = 0.f;
+        if (want != ignore) {
+            r = (want >= 0 && want < vocab) ? kLogitGradScale : nan;
+            if (per_row) r *= top > 0.f ? dloss[i] / top : 0.f;   // inf / inf: NaN, as it should be
+        }
+        row_scale[i] = r;
+    }
+    if (threadIdx.x == 0) {
+        float a = per_row ? top : dloss[0];
+        if (mean) a = c > 0 ? a / static_cast<float>(c) : 0.f;
+        *alpha = a / kLogitGradScale;
+    }
+}
+
+// out = alpha src, rounded once (8 elements per thread).
+__global__ void __launch_bounds__(256) scale_round_kernel(const float4* __restrict__ src, uint4* __restrict__ out,
+                                                          long long vecs, const float* __restrict__ alpha, int bf16) {
+    grid_dependents_launch();
+    grid_dependency_wait();
+    const float a = *alpha;
+    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < vecs;
+         i += static_cast<long long>(gridDim.x) * 256) {
+        const float4 x = src[2 * i], y = src[2 * i + 1];
+        uint4 q;
+        q.x = pack2(a * x.x, a * x.y, bf16);
+        q.y = pack2(a * x.z, a * x.w, bf16);
+        q.z = pack2(a * y.x, a * y.y, bf16);
+        q.w = pack2(a * y.z, a * y.w, bf16);
+        out[i] = q;
+    }
+}
+
+// ------------------------------------------------------ orthogonalised update ---
+
+// X is kept as FP16 times this power of two: a matrix of Frobenius norm 1 has
+// elements near (rows cols)^-1/2, close to FP16's subnormals for large
+// matrices; its largest element is at most 1 (and 1.3 after a step), so 256
+// leaves room on both sides.
+constexpr float kOrthScale = 256.f;
+
+// Sums of squares of matrix blockIdx.y, in 64 bits: sums[matrix][block].
+__global__ void __launch_bounds__(256) orth_square_kernel(const void* __restrict__ g, long long batch_stride, int rows,
+                                                          int cols, long long ld, int bf16,
+                                                          double* __restrict__ sums) {
+    __shared__ double part[8];
+    grid_dependents_launch();
+    grid_dependency_wait();
+    const long long base = blockIdx.y * batch_stride;
+    double s = 0.;
+    for (int r = blockIdx.x; r < rows; r += gridDim.x)
+        for (int c = threadIdx.x; c < cols; c += 256) {
+            const double v = static_cast<double>(to_f32(g, base + r * ld + c, bf16));
+            s += v * v;
+        }
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 8; ++i) s += part[i];
+        sums[static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x] = s;
+    }
+}
+
+// x = FP16(g kOrthScale / (norm + eps)), rows padded to ld_x columns.
+__global__ void __launch_bounds__(256) orth_scale_kernel(const void* __restrict__ g, long long batch_stride, int rows,
+                                                         int cols, long long ld, int bf16,
+                                                         const double* __restrict__ sums, int num_sums, double eps,
+                                                         __half* __restrict__ x, long long ld_x, long long x_stride) {
+    __shared__ float factor;
+    grid_dependents_launch();
+    grid_dependency_wait();
+    if (threadIdx.x < 32) {
+        double s = 0.;
+        for (int i = threadIdx.x; i < num_sums; i += 32) s += sums[static_cast<long long>(blockIdx.y) * num_sums + i];
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (threadIdx.x == 0) factor = static_cast<float>(static_cast<double>(kOrthScale) / (sqrt(s) + eps));
+    }
+    __syncthreads();
+    const float f = factor;
+    const long long base = blockIdx.y * batch_stride;
+    __half* dst = x + blockIdx.y * x_stride;
+    for (int r = blockIdx.x; r < rows; r += gridDim.x)
+        for (int c = threadIdx.x; c < cols; c += 256)
+            dst[r * ld_x + c] = __float2half_rn(to_f32(g, base + r * ld + c, bf16) * f);
+}
+
+// out[r, c] = scale src[r, c], for outputs whose rows TMA cannot store to (scale
+// 1, src in the output's type) and for no step at all (X itself).
+__global__ void __launch_bounds__(256) orth_copy_kernel(const void* __restrict__ src, long long ld_src,
+                                                        long long src_stride, int src_bf16, float scale,
+                                                        void* __restrict__ out, int rows, int cols, int out_bf16) {
+    grid_dependents_launch();
+    grid_dependency_wait();
+    const long long from = blockIdx.y * src_stride, to = static_cast<long long>(blockIdx.y) * rows * cols;
+    for (int r = blockIdx.x; r < rows; r += gridDim.x)
+        for (int c = threadIdx.x; c < cols; c += 256) {
+            const float v = scale * to_f32(src, from + r * ld_src + c, src_bf16);
+            const long long i = to + static_cast<long long>(r) * cols + c;
+            if (out_bf16) static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
+            else static_cast<__half*>(out)[i] = __float2half_rn(v);
+        }
+}
+
+}  // namespace hgemm

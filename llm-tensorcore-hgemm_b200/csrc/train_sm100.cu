@@ -1,0 +1,828 @@
+// C-ABI implementation of the training operators (include/hgemm_sm100_train.h):
+// argument checks, tile choice, TMA descriptors and launches on the caller's
+// stream. Descriptors are encoded per call and travel as kernel parameters.
+#include "hgemm_sm100_train.h"
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstring>
+#include <mutex>
+
+#include "train_kernels.cuh"
+
+namespace {
+
+using namespace hgemm;
+
+__device__ int g_train_status_word;  // status word used when the caller passes none
+
+constexpr int kMaxDevices = 64;
+constexpr uint64_t kDefaultTimeoutNs = 2000ull * 1000ull * 1000ull;
+constexpr int64_t kMaxSize = (int64_t{1} << 31) - 1024;
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t round_up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
+
+struct DeviceInfo {
+    int sms = 0;
+    int* status_word = nullptr;
+    int error = HGEMM_SM100_ERR_CUDA;
+    std::once_flag once;
+};
+DeviceInfo g_devices[kMaxDevices];
+
+int device_info(const DeviceInfo** out, int* id) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return HGEMM_SM100_ERR_CUDA;
+    // Binds the device's context to this thread: a thread that has made no CUDA
+    // call yet (autograd's) has none, and descriptor encoding needs it.
+    if (cudaSetDevice(dev) != cudaSuccess) return HGEMM_SM100_ERR_CUDA;
+    DeviceInfo& d = g_devices[dev];
+    std::call_once(d.once, [&d, dev] {
+        int major = 0, minor = 0;
+        if (cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+            cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
+            cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev) != cudaSuccess)
+            return;
+        if (major != 10 || minor != 0) {
+            d.error = HGEMM_SM100_ERR_UNSUPPORTED_DEVICE;
+            return;
+        }
+        if (cudaGetSymbolAddress(reinterpret_cast<void**>(&d.status_word), g_train_status_word) != cudaSuccess) return;
+        d.error = HGEMM_SM100_OK;
+    });
+    *out = &d;
+    *id = dev;
+    return d.error;
+}
+
+// ------------------------------------------------------------ tensor maps --
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+    static EncodeTiledFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            return static_cast<EncodeTiledFn>(nullptr);
+        return reinterpret_cast<EncodeTiledFn>(p);
+    }();
+    return fn;
+}
+
+// Row-major matrix [rows x cols], pitch ld elements, in boxes of box_rows x
+// box_cols; elements outside it read as zero and are not written.
+int tensor_map(CUtensorMap* out, const void* base, int64_t cols, int64_t rows, int64_t ld, uint32_t box_cols,
+               uint32_t box_rows, CUtensorMapDataType type, CUtensorMapSwizzle swizzle) {
+    EncodeTiledFn fn = encode_fn();
+    if (fn == nullptr) return HGEMM_SM100_ERR_TENSOR_MAP;
+    const cuuint64_t esize = type == CU_TENSOR_MAP_DATA_TYPE_FLOAT32 ? 4 : 2;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * esize};
+    const cuuint32_t box[2] = {box_cols, box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(out, type, 2, const_cast<void*>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? HGEMM_SM100_OK : HGEMM_SM100_ERR_TENSOR_MAP;
+}
+
+CUtensorMapDataType type16(int bf16) {
+    return bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
+// ---------------------------------------------------------------- kernels --
+
+using KernelFn = void (*)(TrainParams);
+struct KernelEntry {
+    KernelFn fn;
+    std::atomic<uint64_t> ready{0};   // bit d: attributes set on device d
+};
+#define HG_TRAIN(PAIR, EPI) KernelEntry { &train_gemm_kernel<PAIR, EPI> }
+KernelEntry g_kernels[2][5] = {
+    {HG_TRAIN(false, kTrainStore), HG_TRAIN(false, kTrainGate), HG_TRAIN(false, kTrainGateGrad),
+     HG_TRAIN(false, kTrainLse), HG_TRAIN(false, kTrainLogitGrad)},
+    {HG_TRAIN(true, kTrainStore), HG_TRAIN(true, kTrainGate), HG_TRAIN(true, kTrainGateGrad),
+     HG_TRAIN(true, kTrainLse), HG_TRAIN(true, kTrainLogitGrad)},
+};
+
+// Launch with programmatic stream serialisation (the kernels wait for the
+// previous kernel before they touch global memory).
+template <typename... P, typename... A>
+int launch(void (*fn)(P...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t stream, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    unsigned n = 0;
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = static_cast<unsigned>(cluster);
+        attr[n].val.clusterDim.y = 1;
+        attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    return cudaLaunchKernelEx(&cfg, fn, static_cast<P>(args)...) == cudaSuccess ? HGEMM_SM100_OK
+                                                                                 : HGEMM_SM100_ERR_LAUNCH;
+}
+
+// ---------------------------------------------------------- one GEMM launch --
+
+// An operand as it lies in memory. K-major: rows along M (or N), columns along
+// K; MN-major: rows along K.
+struct Operand {
+    const void* ptr = nullptr;
+    int64_t ld = 0;
+    bool mn = false;
+};
+
+struct Tile {
+    bool pair = false;
+    int n = 0;
+};
+
+// One product as the host describes it. Two segments where k1 > 0; with `dual`
+// b0 and b1 are the two column halves instead (n counts one half's columns).
+struct Product {
+    int64_t m = 0, n = 0, k0 = 0, k1 = 0;
+    Operand a0, b0, a1, b1;
+    bool dual = false;
+    void* out = nullptr;       // 16-bit (or FP32, see out_kind) [m x ld_out]
+    int64_t ld_out = 0;
+    void* out1 = nullptr;      // further 16-bit outputs of the same shape
+    void* out2 = nullptr;
+    int out_kind = kTrainOut16;
+    float alpha = 1.f, beta = 0.f;
+    const float* alpha_ptr = nullptr;
+    const void* c = nullptr;
+    int64_t ldc = 0;
+    int64_t kblocks() const { return cdiv(k0, kBlockK) + cdiv(k1, kBlockK); }
+};
+
+// Time of a problem's tiles in clock cycles, for comparing tiles of one
+// problem. A K block of 64 costs an SM 4 MMAs of max(46, tile_n / 2) cycles
+// and a hand-off that narrow tiles do not hide, and at least what its TMA
+// loads take; a tile adds its epilogue's last columns, a launch its fill.
+double tile_cost(const Product& p, bool pair, int tile_n, int sms) {
+    const int64_t cols = p.dual ? tile_n / 2 : tile_n;
+    const int64_t tiles = cdiv(p.m, pair ? 256 : 128) * cdiv(p.n, cols);
+    const int64_t units = pair ? sms / 2 : sms;
+    const double block = std::max(4.0 * std::max(46.0, tile_n / 2.0) + (pair ? 40.0 : 90.0), pair ? 400.0 : 420.0);
+    const double waves = static_cast<double>(cdiv(tiles, units));
+    return waves * (p.kblocks() * block + 300.0) + 3000.0 + 12.0 * tile_n;
+}
+
+Tile choose_tile(const Product& p, int sms, int32_t forced, int only_pair = -1) {
+    if (forced != 0) return {(forced & HGEMM_SM100_TRAIN_TILE_PAIR) != 0, forced & 0xfff};
+    Tile best;
+    double cost = 0;
+    for (int pair = 1; pair >= 0; --pair) {
+        if (only_pair >= 0 && pair != only_pair) continue;
+        for (int n = 256; n >= 64; n -= 64) {
+            const double c = tile_cost(p, pair != 0, n, sms);
+            if (best.n == 0 || c < cost) {
+                best = {pair != 0, n};
+                cost = c;
+            }
+        }
+    }
+    return best;
+}
+
+// Raster group height: the tallest of 8, 16, 32 tile rows whose one-wave
+// footprint of A and B panels stays within 48 MB (the pair kernels' rule).
+int group_height(int64_t m, int64_t k, bool pair, int units) {
+    const int rows = pair ? 256 : 128;
+    const double panel = 2.0 * rows * static_cast<double>(k);
+    int g = 8;
+    for (int h : {16, 32})
+        if (h <= cdiv(m, rows) && (h + static_cast<double>(units) / h) * panel <= 48e6) g = h;
+    return g;
+}
+
+int make_operand(CUtensorMap* map, const Operand& o, int64_t rows, int64_t k, uint32_t box_rows, int bf16) {
+    return o.mn ? tensor_map(map, o.ptr, rows, k, o.ld, 64, 64, type16(bf16), CU_TENSOR_MAP_SWIZZLE_128B)
+                : tensor_map(map, o.ptr, k, rows, o.ld, 64, box_rows, type16(bf16), CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+struct Context {
+    const DeviceInfo* dev = nullptr;
+    int id = 0;
+    cudaStream_t stream = nullptr;
+    HgemmSm100TrainCommon common{};
+};
+
+int begin(Context* c, const HgemmSm100TrainCommon& common, void* stream) {
+    if (common.dtype != HGEMM_SM100_TRAIN_F16 && common.dtype != HGEMM_SM100_TRAIN_BF16)
+        return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    if (common.flags & ~HGEMM_SM100_FLAG_TEST_INJECT_TX) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    if (common.tile != 0) {
+        const int n = common.tile & 0xfff;
+        if ((common.tile & ~(0xfff | HGEMM_SM100_TRAIN_TILE_PAIR)) || n < 64 || n > 256 || n % 64)
+            return HGEMM_SM100_ERR_UNKNOWN_CONFIG;
+    }
+    c->stream = static_cast<cudaStream_t>(stream);
+    c->common = common;
+    return device_info(&c->dev, &c->id);
+}
+
+// Common fields of a launch.
+void init_params(TrainParams& p, const Context& c) {
+    std::memset(static_cast<void*>(&p), 0, sizeof(p));
+    p.in_bf16 = p.out_bf16 = c.common.dtype == HGEMM_SM100_TRAIN_BF16;
+    p.status = c.common.status != nullptr ? c.common.status : c.dev->status_word;
+    p.timeout_ns = c.common.timeout_ns != 0 ? c.common.timeout_ns : kDefaultTimeoutNs;
+    p.inject = (c.common.flags & HGEMM_SM100_FLAG_TEST_INJECT_TX) ? 1 : 0;
+}
+
+// Fills the problems of `p` from `count` products (the first one with the most
+// K blocks) and launches them as one grid.
+int run_products(TrainParams& p, int epi, const Product* products, const Tile* tiles, int count, const Context& c) {
+    const bool pair = tiles[0].pair;
+    const int units = pair ? c.dev->sms / 2 : c.dev->sms;
+    uint32_t stage_bytes = 0;
+    int64_t total = 0, light = 0;
+    for (int i = 0; i < count; ++i) {
+        const Product& s = products[i];
+        TrainProblem& q = p.prob[i];
+        const int tile_n = tiles[i].n;
+        const int cols = s.dual ? tile_n / 2 : tile_n;          // output columns of a tile
+        const uint32_t b_box = static_cast<uint32_t>(s.dual || pair ? tile_n / 2 : tile_n);
+        const int bf16 = p.in_bf16;
+        q.m = static_cast<int>(s.m);
+        q.n = static_cast<int>(s.n);
+        q.tile_n = tile_n;
+        q.nkb0 = static_cast<int>(cdiv(s.k0, kBlockK));
+        q.nkb = static_cast<int>(s.kblocks());
+        q.a_mn = s.a0.mn;
+        q.b_mn = s.b0.mn;
+        q.dual = s.dual;
+        q.tiles_m = static_cast<int>(cdiv(s.m, pair ? 256 : 128));
+        q.tiles_n = static_cast<int>(cdiv(s.n, cols));
+        q.group_m = group_height(s.m, s.k0 + s.k1, pair, units);
+        q.out_kind = s.out_kind;
+        q.alpha = s.alpha;
+        q.beta = s.beta;
+        q.alpha_ptr = s.alpha_ptr;
+        q.c = s.c;
+        q.ldc = s.ldc;
+        int rc = make_operand(&q.a[0], s.a0, s.m, s.k0, 128, bf16);
+        if (rc == HGEMM_SM100_OK) rc = make_operand(&q.b[0], s.b0, s.n, s.k0, b_box, bf16);
+        if (rc == HGEMM_SM100_OK && s.dual) rc = make_operand(&q.b[1], s.b1, s.n, s.k0, b_box, bf16);
+        if (rc == HGEMM_SM100_OK && s.k1 > 0) {
+            rc = make_operand(&q.a[1], s.a1, s.m, s.k1, 128, bf16);
+            if (rc == HGEMM_SM100_OK) rc = make_operand(&q.b[1], s.b1, s.n, s.k1, b_box, bf16);
+        }
+        void* const outs[3] = {s.out, s.out1, s.out2};
+        for (int j = 0; j < 3 && rc == HGEMM_SM100_OK; ++j) {
+            if (outs[j] == nullptr) continue;
+            rc = s.out_kind == kTrainOut16
+                     ? tensor_map(&q.out[j], outs[j], s.n, s.m, s.ld_out, 32, 32, type16(p.out_bf16),
+                                  CU_TENSOR_MAP_SWIZZLE_64B)
+                     : tensor_map(&q.out[j], outs[j], s.n, s.m, s.ld_out, 32, 32, CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                                  CU_TENSOR_MAP_SWIZZLE_128B);
+        }
+        if (rc != HGEMM_SM100_OK) return rc;
+        const int64_t b_cols = pair ? tile_n / 2 : tile_n;
+        stage_bytes = std::max(stage_bytes, static_cast<uint32_t>(16384 + round_up(b_cols, 64) * 128));
+        const int64_t n = static_cast<int64_t>(q.tiles_m) * q.tiles_n;
+        total += n;
+        if (i > 0) light += n;
+    }
+    if (total >= (int64_t{1} << 31)) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    p.num_problems = count;
+    p.heavy_tiles = static_cast<int>(total - light);
+    p.light_tiles = static_cast<int>(light);
+    const int grid_units = static_cast<int>(std::min<int64_t>(total, units));
+    if (light > 0 && p.heavy_tiles % grid_units != 0) {
+        const double ratio = static_cast<double>(p.prob[0].nkb) * p.prob[0].tile_n /
+                             (static_cast<double>(p.prob[1].nkb) * p.prob[1].tile_n);
+        p.light_skip = static_cast<int>(ratio + 0.5);
+    }
+    p.stage_bytes = stage_bytes;
+    p.stages = static_cast<int>(std::min<uint32_t>(kTrainRingBytes / stage_bytes, kTrainMaxStages));
+
+    KernelEntry& k = g_kernels[pair ? 1 : 0][epi];
+    const uint64_t bit = 1ull << c.id;
+    if (!(k.ready.load(std::memory_order_acquire) & bit)) {
+        if (cudaFuncSetAttribute(reinterpret_cast<const void*>(k.fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(kTrainSmemBytes)) != cudaSuccess)
+            return HGEMM_SM100_ERR_LAUNCH;
+        k.ready.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    return launch(k.fn, dim3(static_cast<unsigned>(grid_units * (pair ? 2 : 1))), dim3(kThreads), kTrainSmemBytes,
+                  pair ? 2 : 1, c.stream, p);
+}
+
+int run_product(TrainParams& p, int epi, const Product& s, const Context& c) {
+    const Tile t = choose_tile(s, c.dev->sms, c.common.tile);
+    return run_products(p, epi, &s, &t, 1, c);
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool size_ok(int64_t v) { return v > 0 && v <= kMaxSize; }
+bool size8_ok(int64_t v) { return size_ok(v) && v % 8 == 0; }
+// A matrix operand: present, aligned, its pitch a multiple of 8 and at least `cols`.
+bool matrix_ok(const void* p, int64_t ld, int64_t cols) {
+    return p != nullptr && aligned16(p) && ld >= cols && ld % 8 == 0;
+}
+
+}  // namespace
+
+// ------------------------------------------------------------ feed-forward --
+
+extern "C" int hgemm_sm100_ffn_forward(const HgemmSm100FfnForward* a, void* stream) {
+    if (a == nullptr || !size_ok(a->tokens) || !size8_ok(a->hidden) || !size8_ok(a->inter) || !size8_ok(a->out))
+        return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    if (!matrix_ok(a->x, a->ldx, a->hidden) || !matrix_ok(a->gate, 8, 8) || !matrix_ok(a->up, 8, 8) ||
+        !matrix_ok(a->down, 8, 8) || !matrix_ok(a->y, 8, 8) || !matrix_ok(a->h, 8, 8))
+        return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    if ((a->gate_pre == nullptr) != (a->up_pre == nullptr) || !aligned16(a->gate_pre) || !aligned16(a->up_pre))
+        return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    Context c;
+    int rc = begin(&c, a->common, stream);
+    if (rc != HGEMM_SM100_OK) return rc;
+    TrainParams p;
+
+    Product g;
+    g.m = a->tokens;
+    g.n = a->inter;
+    g.k0 = a->hidden;
+    g.a0 = {a->x, a->ldx, false};
+    g.b0 = {a->gate, a->hidden, false};
+    g.b1 = {a->up, a->hidden, false};
+    g.dual = true;
+    g.out = a->h;
+    g.out1 = a->gate_pre;
+    g.out2 = a->up_pre;
+    g.ld_out = a->inter;
+    init_params(p, c);
+    p.keep = a->gate_pre != nullptr;
+    if ((rc = run_product(p, kTrainGate, g, c)) != HGEMM_SM100_OK) return rc;
+
+    Product d;
+    d.m = a->tokens;
+    d.n = a->out;
+    d.k0 = a->inter;
+    d.a0 = {a->h, a->inter, false};
+    d.b0 = {a->down, a->inter, false};
+    d.out = a->y;
+    d.ld_out = a->out;
+    init_params(p, c);
+    return run_product(p, kTrainStore, d, c);
+}
+
+extern "C" int hgemm_sm100_ffn_backward(const HgemmSm100FfnBackward* a, void* stream) {
+    if (a == nullptr || !size_ok(a->tokens) || !size8_ok(a->hidden) || !size8_ok(a->inter) || !size8_ok(a->out))
+        return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    if (!matrix_ok(a->dy, a->lddy, a->out) || !matrix_ok(a->x, a->ldx, a->hidden) || !matrix_ok(a->gate, 8, 8) ||
+        !matrix_ok(a->up, 8, 8) || !matrix_ok(a->down, 8, 8) || !matrix_ok(a->gate_pre, 8, 8) ||
+        !matrix_ok(a->up_pre, 8, 8) || !matrix_ok(a->h, 8, 8) || !matrix_ok(a->dgate_pre, 8, 8) ||
+        !matrix_ok(a->dup_pre, 8, 8) || !aligned16(a->dx) || !aligned16(a->dgate) || !aligned16(a->dup) ||
+        !aligned16(a->ddown))
+        return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    Context c;
+    int rc = begin(&c, a->common, stream);
+    if (rc != HGEMM_SM100_OK) return rc;
+    TrainParams p;
+
+    // dh = dy Wd; its epilogue turns it into dg and du.
+    if (a->dx != nullptr || a->dgate != nullptr || a->dup != nullptr) {
+        Product h;
+        h.m = a->tokens;
+        h.n = a->inter;
+        h.k0 = a->out;
+        h.a0 = {a->dy, a->lddy, false};
+        h.b0 = {a->down, a->inter, true};
+        h.out = a->dgate_pre;
+        h.out1 = a->dup_pre;
+        h.ld_out = a->inter;
+        init_params(p, c);
+        p.gate = a->gate_pre;
+        p.up = a->up_pre;
+        p.ld_saved = a->inter;
+        if ((rc = run_product(p, kTrainGateGrad, h, c)) != HGEMM_SM100_OK) return rc;
+    }
+
+    Product s[4];
+    int n = 0;
+    if (a->dx != nullptr) {
+        Product& q = s[n++];
+        q.m = a->tokens;
+        q.n = a->hidden;
+        q.k0 = q.k1 = a->inter;
+        q.a0 = {a->dgate_pre, a->inter, false};
+        q.b0 = {a->gate, a->hidden, true};
+        q.a1 = {a->dup_pre, a->inter, false};
+        q.b1 = {a->up, a->hidden, true};
+        q.out = a->dx;
+        q.ld_out = a->hidden;
+    }
+    auto weight = [&](void* out, const void* left, int64_t ld_left, int64_t rows, const void* right, int64_t ld_right,
+                      int64_t cols) {
+        if (out == nullptr) return;
+        Product& q = s[n++];
+        q.m = rows;
+        q.n = cols;
+        q.k0 = a->tokens;
+        q.a0 = {left, ld_left, true};
+        q.b0 = {right, ld_right, true};
+        q.out = out;
+        q.ld_out = cols;
+    };
+    weight(a->dgate, a->dgate_pre, a->inter, a->inter, a->x, a->ldx, a->hidden);
+    weight(a->dup, a->dup_pre, a->inter, a->inter, a->x, a->ldx, a->hidden);
+    weight(a->ddown, a->dy, a->lddy, a->out, a->h, a->inter, a->inter);
+    if (n == 0) return HGEMM_SM100_OK;
+    // The problem with the most K blocks goes first.
+    std::stable_sort(s, s + n, [](const Product& x, const Product& y) { return x.kblocks() > y.kblocks(); });
+    Tile t[4];
+    t[0] = choose_tile(s[0], c.dev->sms, c.common.tile);
+    // All of a launch's tiles are pairs or none: what the costlier set of products takes.
+    double cost[2] = {0, 0};
+    Tile by[2][4];
+    for (int pair = 0; pair < 2; ++pair)
+        for (int i = 0; i < n; ++i) {
+            by[pair][i] = choose_tile(s[i], c.dev->sms, c.common.tile, pair);
+            cost[pair] += tile_cost(s[i], pair != 0, by[pair][i].n, c.dev->sms);
+        }
+    const int pair = c.common.tile != 0 ? (t[0].pair ? 1 : 0) : (cost[1] <= cost[0] ? 1 : 0);
+    for (int i = 0; i < n; ++i) t[i] = by[pair][i];
+    init_params(p, c);
+    return run_products(p, kTrainStore, s, t, n, c);
+}
+
+// ------------------------------------------------------------ cross entropy --
+
+namespace {
+
+struct LossForwardPlan {
+    Product z;
+    Tile tile;
+    int64_t tiles_n = 0;
+    size_t partial_bytes = 0, row_bytes = 0;
+    size_t bytes() const { return partial_bytes + 2 * row_bytes; }
+};
+
+LossForwardPlan plan_loss_forward(const HgemmSm100LossForward& a, int sms) {
+    LossForwardPlan q;
+    q.z.m = a.tokens;
+    q.z.n = a.vocab;
+    q.z.k0 = a.hidden;
+    q.z.a0 = {a.x, a.ldx, false};
+    q.z.b0 = {a.weight, a.hidden, false};
+    q.tile = choose_tile(q.z, sms, a.common.tile);
+    q.tiles_n = cdiv(a.vocab, q.tile.n);
+    q.partial_bytes = static_cast<size_t>(round_up(q.tiles_n * a.tokens * 8, 256));
+    q.row_bytes = static_cast<size_t>(round_up(a.tokens * 4, 256));
+    return q;
+}
+
+// Vocabulary entries of a piece: as many as keep its dz (tokens x piece, 16
+// bits) within 96 MB, so that it stays in L2 between the product that writes
+// it and the two that read it, in whole 256-column tiles, at least 2048.
+int64_t loss_piece(const HgemmSm100LossBackward& a) {
+    if (a.piece > 0) return std::min<int64_t>(round_up(a.piece, 8), round_up(a.vocab, 8));
+    int64_t n = (int64_t{96} << 20) / (2 * a.tokens) / 256 * 256;
+    n = std::max<int64_t>(n, 2048);
+    if (n >= a.vocab) return round_up(a.vocab, 8);
+    return round_up(cdiv(a.vocab, cdiv(a.vocab, n)), 256);   // equal pieces
+}
+
+struct LossBackwardPlan {
+    int64_t piece = 0, pieces = 0;
+    size_t dz_bytes = 0, sum_bytes = 0, row_bytes = 0;
+    size_t bytes() const { return dz_bytes + sum_bytes + row_bytes + 256; }
+};
+
+LossBackwardPlan plan_loss_backward(const HgemmSm100LossBackward& a) {
+    LossBackwardPlan q;
+    q.piece = loss_piece(a);
+    q.pieces = cdiv(a.vocab, q.piece);
+    q.dz_bytes = static_cast<size_t>(round_up(a.tokens * q.piece * 2, 256));
+    q.sum_bytes = a.dx != nullptr && q.pieces > 1 ? static_cast<size_t>(round_up(a.tokens * a.hidden * 4, 256)) : 0;
+    q.row_bytes = static_cast<size_t>(round_up(a.tokens * 4, 256));
+    return q;
+}
+
+template <typename Args>
+bool loss_args_ok(const Args& a) {
+    return size_ok(a.tokens) && size8_ok(a.hidden) && size_ok(a.vocab) && matrix_ok(a.x, a.ldx, a.hidden) &&
+           matrix_ok(a.weight, 8, 8) && a.target != nullptr && a.lse != nullptr &&
+           a.reduction >= HGEMM_SM100_LOSS_NONE && a.reduction <= HGEMM_SM100_LOSS_SUM;
+}
+
+}  // namespace
+
+extern "C" size_t hgemm_sm100_loss_forward_workspace(const HgemmSm100LossForward* a) {
+    Context c;
+    if (a == nullptr || !size_ok(a->tokens) || !size_ok(a->vocab) || !size8_ok(a->hidden)) return 0;
+    if (begin(&c, a->common, nullptr) != HGEMM_SM100_OK) return 0;
+    return plan_loss_forward(*a, c.dev->sms).bytes();
+}
+
+extern "C" int hgemm_sm100_loss_forward(const HgemmSm100LossForward* a, void* stream) {
+    if (a == nullptr || !loss_args_ok(*a) || a->loss == nullptr || a->workspace == nullptr || !aligned16(a->workspace))
+        return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    Context c;
+    int rc = begin(&c, a->common, stream);
+    if (rc != HGEMM_SM100_OK) return rc;
+    const LossForwardPlan q = plan_loss_forward(*a, c.dev->sms);
+    if (a->workspace_bytes < q.bytes()) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+    float2* partial = reinterpret_cast<float2*>(ws);
+    float* target_logit = reinterpret_cast<float*>(ws + q.partial_bytes);
+    float* rows = reinterpret_cast<float*>(ws + q.partial_bytes + q.row_bytes);
+    float* loss = a->reduction == HGEMM_SM100_LOSS_NONE ? a->loss : rows;
+    const int m = static_cast<int>(a->tokens);
+    const long long* target = reinterpret_cast<const long long*>(a->target);
+
+    TrainParams p;
+    init_params(p, c);
+    p.target = target;
+    p.partial = partial;
+    p.target_logit = target_logit;
+    if ((rc = run_products(p, kTrainLse, &q.z, &q.tile, 1, c)) != HGEMM_SM100_OK) return rc;
+    rc = launch(&lse_join_kernel, dim3(static_cast<unsigned>(cdiv(m, 32))), dim3(32, 32), 0, 1, c.stream, partial,
+                static_cast<int>(q.tiles_n), m, target_logit, target, static_cast<long long>(a->vocab),
+                static_cast<long long>(a->ignore_index), a->lse, loss);
+    if (rc != HGEMM_SM100_OK || a->reduction == HGEMM_SM100_LOSS_NONE) return rc;
+    return launch(&loss_reduce_kernel, dim3(1), dim3(1024), 0, 1, c.stream, rows, target, m,
+                  static_cast<long long>(a->ignore_index), a->reduction == HGEMM_SM100_LOSS_MEAN ? 1 : 0, a->loss);
+}
+
+extern "C" size_t hgemm_sm100_loss_backward_workspace(const HgemmSm100LossBackward* a) {
+    if (a == nullptr || !size_ok(a->tokens) || !size_ok(a->vocab) || !size8_ok(a->hidden)) return 0;
+    return plan_loss_backward(*a).bytes();
+}
+
+extern "C" int hgemm_sm100_loss_backward(const HgemmSm100LossBackward* a, void* stream) {
+    if (a == nullptr || !loss_args_ok(*a) || a->dloss == nullptr || a->workspace == nullptr ||
+        !aligned16(a->workspace) || !aligned16(a->dx) || !aligned16(a->dweight) || a->piece < 0)
+        return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    Context c;
+    int rc = begin(&c, a->common, stream);
+    if (rc != HGEMM_SM100_OK) return rc;
+    const LossBackwardPlan q = plan_loss_backward(*a);
+    if (a->workspace_bytes < q.bytes()) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    if (a->dx == nullptr && a->dweight == nullptr) return HGEMM_SM100_OK;
+    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+    void* dz = ws;
+    float* sums = reinterpret_cast<float*>(ws + q.dz_bytes);
+    float* row_scale = reinterpret_cast<float*>(ws + q.dz_bytes + q.sum_bytes);
+    float* alpha = reinterpret_cast<float*>(ws + q.dz_bytes + q.sum_bytes + q.row_bytes);
+    const long long* target = reinterpret_cast<const long long*>(a->target);
+
+    rc = launch(&logit_grad_setup_kernel, dim3(1), dim3(1024), 0, 1, c.stream, a->dloss,
+                a->reduction == HGEMM_SM100_LOSS_NONE ? 1 : 0, a->reduction == HGEMM_SM100_LOSS_MEAN ? 1 : 0, target,
+                static_cast<int>(a->tokens), static_cast<long long>(a->vocab),
+                static_cast<long long>(a->ignore_index), row_scale, alpha);
+    if (rc != HGEMM_SM100_OK) return rc;
+
+    TrainParams p;
+    for (int64_t i = 0; i < q.pieces; ++i) {
+        const int64_t v0 = i * q.piece, nv = std::min(q.piece, a->vocab - v0);
+        const uint8_t* w = static_cast<const uint8_t*>(a->weight) + v0 * a->hidden * 2;
+        Product z;
+        z.m = a->tokens;
+        z.n = nv;
+        z.k0 = a->hidden;
+        z.a0 = {a->x, a->ldx, false};
+        z.b0 = {w, a->hidden, false};
+        z.out = dz;
+        z.ld_out = q.piece;
+        init_params(p, c);
+        p.target = target;
+        p.col_base = v0;
+        p.lse = a->lse;
+        p.row_scale = row_scale;
+        if ((rc = run_product(p, kTrainLogitGrad, z, c)) != HGEMM_SM100_OK) return rc;
+
+        Product s[2];
+        int n = 0;
+        if (a->dx != nullptr) {
+            Product& d = s[n++];
+            d.m = a->tokens;
+            d.n = a->hidden;
+            d.k0 = nv;
+            d.a0 = {dz, q.piece, false};
+            d.b0 = {w, a->hidden, true};
+            d.ld_out = a->hidden;
+            if (q.pieces == 1) {
+                d.out = a->dx;
+                d.alpha_ptr = alpha;
+            } else {
+                d.out = sums;
+                d.out_kind = i == 0 ? kTrainOutF32 : kTrainOutF32Add;
+            }
+        }
+        if (a->dweight != nullptr) {
+            Product& d = s[n++];
+            d.m = nv;
+            d.n = a->hidden;
+            d.k0 = a->tokens;
+            d.a0 = {dz, q.piece, true};
+            d.b0 = {a->x, a->ldx, true};
+            d.out = static_cast<uint8_t*>(a->dweight) + v0 * a->hidden * 2;
+            d.ld_out = a->hidden;
+            d.alpha_ptr = alpha;
+        }
+        if (n == 2 && s[1].kblocks() > s[0].kblocks()) std::swap(s[0], s[1]);
+        Tile by[2][2];
+        double cost[2] = {0, 0};
+        for (int pair = 0; pair < 2; ++pair)
+            for (int j = 0; j < n; ++j) {
+                by[pair][j] = choose_tile(s[j], c.dev->sms, c.common.tile, pair);
+                cost[pair] += tile_cost(s[j], pair != 0, by[pair][j].n, c.dev->sms);
+            }
+        const int pair = c.common.tile != 0 ? ((c.common.tile & HGEMM_SM100_TRAIN_TILE_PAIR) ? 1 : 0)
+                                            : (cost[1] <= cost[0] ? 1 : 0);
+        init_params(p, c);
+        if ((rc = run_products(p, kTrainStore, s, by[pair], n, c)) != HGEMM_SM100_OK) return rc;
+    }
+    if (a->dx != nullptr && q.pieces > 1) {
+        const int64_t vecs = a->tokens * a->hidden / 8;
+        const int64_t blocks = std::min<int64_t>(cdiv(vecs, 256), c.dev->sms * 8);
+        rc = launch(&scale_round_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, 1, c.stream,
+                    reinterpret_cast<const float4*>(sums), static_cast<uint4*>(a->dx), static_cast<long long>(vecs),
+                    alpha, a->common.dtype == HGEMM_SM100_TRAIN_BF16 ? 1 : 0);
+    }
+    return rc;
+}
+
+// ------------------------------------------------------ orthogonalised update --
+
+namespace {
+
+constexpr int kOrthSums = 148;   // partial sums of squares per matrix
+
+struct OrthPlan {
+    bool tall = false;
+    int64_t side = 0, ld = 0, ld_side = 0, x_stride = 0, side_stride = 0;
+    size_t sum_bytes = 0, x_bytes = 0, side_bytes = 0;
+    size_t bytes() const { return sum_bytes + 2 * x_bytes + 2 * side_bytes; }
+};
+
+OrthPlan plan_orth(const HgemmSm100Orthogonalize& a) {
+    OrthPlan q;
+    q.tall = a.rows > a.cols;
+    q.side = std::min(a.rows, a.cols);
+    q.ld = round_up(a.cols, 64);
+    q.ld_side = round_up(q.side, 64);
+    q.x_stride = a.rows * q.ld;
+    q.side_stride = q.side * q.ld_side;
+    q.sum_bytes = static_cast<size_t>(round_up(a.batch * kOrthSums * 8, 256));
+    q.x_bytes = static_cast<size_t>(round_up(a.batch * q.x_stride * 2, 256));
+    q.side_bytes = static_cast<size_t>(round_up(a.batch * q.side_stride * 2, 256));
+    return q;
+}
+
+bool orth_sizes_ok(const HgemmSm100Orthogonalize& a) {
+    return a.batch > 0 && a.batch <= 65535 && size_ok(a.rows) && size_ok(a.cols) && a.steps >= 0;
+}
+
+}  // namespace
+
+extern "C" size_t hgemm_sm100_orthogonalize_workspace(const HgemmSm100Orthogonalize* a) {
+    return a != nullptr && orth_sizes_ok(*a) ? plan_orth(*a).bytes() : 0;
+}
+
+extern "C" int hgemm_sm100_orthogonalize(const HgemmSm100Orthogonalize* a, void* stream) {
+    if (a == nullptr || !orth_sizes_ok(*a) || a->g == nullptr || a->out == nullptr || a->ldg < a->cols ||
+        a->batch_stride < 0 || a->workspace == nullptr || reinterpret_cast<uintptr_t>(a->workspace) % 256 != 0 ||
+        !(a->eps >= 0))
+        return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    Context c;
+    int rc = begin(&c, a->common, stream);
+    if (rc != HGEMM_SM100_OK) return rc;
+    const OrthPlan q = plan_orth(*a);
+    if (a->workspace_bytes < q.bytes()) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+    double* sums = reinterpret_cast<double*>(ws);
+    uint16_t* x = reinterpret_cast<uint16_t*>(ws + q.sum_bytes);
+    uint16_t* y = reinterpret_cast<uint16_t*>(ws + q.sum_bytes + q.x_bytes);
+    uint16_t* gram = reinterpret_cast<uint16_t*>(ws + q.sum_bytes + 2 * q.x_bytes);
+    uint16_t* poly = reinterpret_cast<uint16_t*>(ws + q.sum_bytes + 2 * q.x_bytes + q.side_bytes);
+    const int bf16 = a->common.dtype == HGEMM_SM100_TRAIN_BF16 ? 1 : 0;
+    const int rows = static_cast<int>(a->rows), cols = static_cast<int>(a->cols);
+    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(a->rows, kOrthSums));
+    const unsigned batch = static_cast<unsigned>(a->batch);
+
+    rc = launch(&orth_square_kernel, dim3(blocks, batch), dim3(256), 0, 1, c.stream, a->g,
+                static_cast<long long>(a->batch_stride), rows, cols, static_cast<long long>(a->ldg), bf16, sums);
+    if (rc != HGEMM_SM100_OK) return rc;
+    rc = launch(&orth_scale_kernel, dim3(static_cast<unsigned>(std::min<int64_t>(a->rows, 65535)), batch), dim3(256), 0,
+                1, c.stream, a->g, static_cast<long long>(a->batch_stride), rows, cols,
+                static_cast<long long>(a->ldg), bf16, sums, static_cast<int>(blocks), a->eps,
+                reinterpret_cast<__half*>(x), static_cast<long long>(q.ld), static_cast<long long>(q.x_stride));
+    if (rc != HGEMM_SM100_OK) return rc;
+
+    // The last step writes the result itself where TMA can store it.
+    const bool direct = aligned16(a->out) && a->cols % 8 == 0;
+    const float inv = 1.f / kOrthScale;
+    TrainParams p;
+    auto each = [&](auto&& make, int out_bf16) -> int {
+        for (int64_t first = 0; first < a->batch; first += kTrainMaxProblems) {
+            Product s[kTrainMaxProblems];
+            Tile t[kTrainMaxProblems];
+            const int n = static_cast<int>(std::min<int64_t>(kTrainMaxProblems, a->batch - first));
+            for (int i = 0; i < n; ++i) make(s[i], first + i);
+            Product all = s[0];
+            all.m = round_up(all.m, 256) * n;   // the launch's tiles, for the choice of the tile
+            for (int i = 0; i < n; ++i) t[i] = choose_tile(n > 1 ? all : s[0], c.dev->sms, c.common.tile);
+            init_params(p, c);
+            p.in_bf16 = 0;
+            p.out_bf16 = out_bf16;
+            const int r = run_products(p, kTrainStore, s, t, n, c);
+            if (r != HGEMM_SM100_OK) return r;
+        }
+        return HGEMM_SM100_OK;
+    };
+    for (int step = 0; step < a->steps; ++step) {
+        const bool last = step + 1 == a->steps;
+        // gram = X X^T or X^T X
+        rc = each([&](Product& s, int64_t i) {
+            const uint16_t* xi = x + i * q.x_stride;
+            s.m = s.n = q.side;
+            s.k0 = q.tall ? a->rows : a->cols;
+            s.a0 = {xi, q.ld, q.tall};
+            s.b0 = {xi, q.ld, q.tall};
+            s.out = gram + i * q.side_stride;
+            s.ld_out = q.ld_side;
+            s.alpha = inv * inv;
+        }, 0);
+        if (rc != HGEMM_SM100_OK) return rc;
+        // poly = b gram + c gram gram (symmetric)
+        rc = each([&](Product& s, int64_t i) {
+            const uint16_t* gi = gram + i * q.side_stride;
+            s.m = s.n = s.k0 = q.side;
+            s.a0 = {gi, q.ld_side, false};
+            s.b0 = {gi, q.ld_side, false};
+            s.out = poly + i * q.side_stride;
+            s.ld_out = q.ld_side;
+            s.alpha = a->c;
+            s.beta = a->b;
+            s.c = gi;
+            s.ldc = q.ld_side;
+        }, 0);
+        if (rc != HGEMM_SM100_OK) return rc;
+        // X <- a X + poly X, or a X + X poly
+        rc = each([&](Product& s, int64_t i) {
+            const uint16_t* xi = x + i * q.x_stride;
+            const uint16_t* pi = poly + i * q.side_stride;
+            s.m = a->rows;
+            s.n = a->cols;
+            s.k0 = q.side;
+            if (q.tall) {
+                s.a0 = {xi, q.ld, false};
+                s.b0 = {pi, q.ld_side, false};
+            } else {
+                s.a0 = {pi, q.ld_side, false};
+                s.b0 = {xi, q.ld, true};
+            }
+            s.c = xi;
+            s.ldc = q.ld;
+            s.alpha = last ? inv : 1.f;
+            s.beta = last ? a->a * inv : a->a;
+            if (last && direct) {
+                s.out = static_cast<uint16_t*>(a->out) + i * a->rows * a->cols;
+                s.ld_out = a->cols;
+            } else {
+                s.out = y + i * q.x_stride;
+                s.ld_out = q.ld;
+            }
+        }, last ? bf16 : 0);
+        if (rc != HGEMM_SM100_OK) return rc;
+        std::swap(x, y);
+    }
+    if (direct && a->steps > 0) return HGEMM_SM100_OK;
+    const bool none = a->steps == 0;
+    return launch(&orth_copy_kernel, dim3(static_cast<unsigned>(std::min<int64_t>(a->rows, 65535)), batch), dim3(256),
+                  0, 1, c.stream, x, static_cast<long long>(q.ld), static_cast<long long>(q.x_stride),
+                  none ? 0 : bf16, none ? inv : 1.f, a->out, rows, cols, bf16);
+}
+
+extern "C" int hgemm_sm100_train_read_status(int32_t* value, int clear) {
+    const DeviceInfo* dev = nullptr;
+    int id = 0;
+    const int rc = device_info(&dev, &id);
+    if (rc != HGEMM_SM100_OK) return rc;
+    if (value != nullptr && cudaMemcpy(value, dev->status_word, sizeof(int32_t), cudaMemcpyDeviceToHost) != cudaSuccess)
+        return HGEMM_SM100_ERR_CUDA;
+    if (clear && cudaMemset(dev->status_word, 0, sizeof(int32_t)) != cudaSuccess) return HGEMM_SM100_ERR_CUDA;
+    return HGEMM_SM100_OK;
+}

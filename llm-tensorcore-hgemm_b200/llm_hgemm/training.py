@@ -1,0 +1,91 @@
+"""Training operators on the library's tensor-core core: the gated feed-forward
+block, the loss of a language-model head and the orthogonalised update of a
+weight, each with hand-written sm_100a kernels (no reference counterpart: the
+reference, llm_hgemm/integration.py:8-46, is inference-only).
+
+They take FP16 or BF16 CUDA tensors and weights in ``nn.Linear``'s layout
+(``[out_features, in_features]``), which are read where they are: nothing is
+packed, so an optimizer may change them between calls. Sums are FP32. Launches
+go to the current stream of the tensors' device; scratch comes from torch's
+caching allocator, so calls on different streams and captured graphs do not
+share any. Like the rest of the package there is no CPU or library fallback.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch import nn
+
+from . import _C
+
+#: Coefficients of the quintic Newton-Schulz step of the Muon optimizer.
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+
+
+def gated_ffn(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor) -> torch.Tensor:
+    """SwiGLU block ``(silu(x @ gate.T) * (x @ up.T)) @ down.T``, differentiable in
+    all four tensors.
+
+    ``x`` is ``[..., H]`` (any strides), ``gate`` and ``up`` ``[I, H]``, ``down``
+    ``[O, I]``; the result is ``[..., O]``. Two launches: gate and up are one
+    product whose epilogue writes the gated activation, then the down
+    projection. Where a gradient is wanted the pre-activations and the gated
+    activation are kept (``3 * tokens * I`` elements); the backward pass is two
+    launches more, one whose epilogue turns the activation's gradient into
+    those of the pre-activations, and one for all wanted gradients together.
+    H, I and O that are no multiples of 8 work through padded copies.
+    Gradients of gradients are refused.
+    """
+    return _C.gated_ffn(x, gate, up, down)
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *,
+                         reduction: str = "mean", ignore_index: int = -100) -> torch.Tensor:
+    """``cross_entropy(x @ weight.T, target)`` without the logits, in FP32,
+    differentiable in ``x`` and ``weight``.
+
+    ``x`` is ``[..., H]``, ``weight`` ``[V, H]``, ``target`` ``[...]`` (int64 or
+    int32). ``reduction``: ``"none"`` (shape of ``target``), ``"mean"`` over the
+    targets that are not ``ignore_index`` (NaN when there is none) or
+    ``"sum"``. Ignored targets have loss 0 and gradient 0. A target outside
+    ``[0, V)`` that is not ``ignore_index`` gives that token a NaN loss (and NaN
+    gradients) instead of a device assertion. The forward pass keeps one number
+    per token; the backward pass forms the logits again, a piece of the
+    vocabulary at a time. Gradients of gradients are refused.
+    """
+    return _C.linear_cross_entropy(x, weight, target, reduction, ignore_index)
+
+
+def orthogonalize(g: torch.Tensor, *, steps: int = 5,
+                  coefficients: tuple[float, float, float] = NEWTON_SCHULZ,
+                  eps: float = 1e-7) -> torch.Tensor:
+    """The last two dimensions of ``g`` with all singular values moved towards 1
+    (the update direction of the Muon optimizer): ``X = g / (norm(g) + eps)``,
+    then ``steps`` times ``X = a X + (b A + c A A) X`` with ``A = X X^T`` (of the
+    shorter side).
+
+    Leading dimensions are a batch of matrices, each normalised by itself. A
+    zero matrix gives zeros. The steps run on FP16 elements (scaled by a power
+    of two) whatever the dtype of ``g``. No gradient is recorded.
+    """
+    a, b, c = coefficients
+    return _C.orthogonalize(g, steps, a, b, c, eps)
+
+
+class TrainableSwiGLU(nn.Module):
+    """SwiGLU MLP that trains through :func:`gated_ffn`; the counterpart of the
+    inference-only ``HgemmSwiGLU``. It holds the projections it is built from
+    as ``gate_proj``, ``up_proj`` and ``down_proj``, so parameters, state dict
+    and optimizers stay as they are."""
+
+    def __init__(self, gate: nn.Linear, up: nn.Linear, down: nn.Linear):
+        super().__init__()
+        for lin in (gate, up, down):
+            if not isinstance(lin, nn.Linear) or lin.bias is not None:
+                raise ValueError("requires bias-free nn.Linear projections")
+        if gate.weight.shape != up.weight.shape or down.in_features != gate.out_features:
+            raise ValueError("gate/up/down shapes do not form an MLP")
+        self.gate_proj, self.up_proj, self.down_proj = gate, up, down
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return gated_ffn(x, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight)

@@ -1,0 +1,568 @@
+"""Training operators against their formulas in 64 bits (GPU), with the error
+bounds of tests/training_reference.py: tile shapes, types, odd and ragged sizes,
+ignored and invalid targets, strides, streams, captured graphs, differences."""
+
+import pytest
+import torch
+from torch import nn
+
+import llm_hgemm
+from llm_hgemm import capi, train_capi
+from llm_hgemm.training import NEWTON_SCHULZ, TrainableSwiGLU
+from tests import training_reference as ref
+from tests.gpu_helpers import require_cuda
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float16, torch.bfloat16]
+IDS = ["fp16", "bf16"]
+
+
+@pytest.fixture(autouse=True, scope="module")
+def _cuda():
+    require_cuda()
+
+
+def normal(seed, *shape, dtype=torch.float16, scale=1.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=gen, device="cuda") * scale).to(dtype)
+
+
+def ffn_inputs(tokens, hidden, inter, out, dtype, seed=1):
+    return (normal(seed, tokens, hidden, dtype=dtype), normal(seed + 1, inter, hidden, dtype=dtype, scale=hidden ** -0.5),
+            normal(seed + 2, inter, hidden, dtype=dtype, scale=hidden ** -0.5),
+            normal(seed + 3, out, inter, dtype=dtype, scale=inter ** -0.5), normal(seed + 4, tokens, out, dtype=dtype))
+
+
+def loss_inputs(tokens, hidden, vocab, dtype, ignore=-100, seed=1):
+    w = normal(seed, vocab, hidden, dtype=dtype, scale=2 * hidden ** -0.5)
+    gen = torch.Generator(device="cuda").manual_seed(seed + 7)
+    t = torch.randint(0, vocab, (tokens,), generator=gen, device="cuda")
+    x = (normal(seed + 1, tokens, hidden, dtype=dtype).float() + 2 * w[t].float()).to(dtype)
+    t = torch.where(torch.rand(tokens, generator=gen, device="cuda") < 0.2, torch.full_like(t, ignore), t)
+    return x, w, t
+
+
+def within(got, want):
+    value, err = want
+    assert got.shape == value.shape
+    off = (got.double() - value).abs()
+    assert bool((off <= err).all()), f"off by {float((off / err).max()):.3g} times the bound"
+
+
+def grads_of(y, leaves, dy):
+    return torch.autograd.grad(y, leaves, dy)
+
+
+# ------------------------------------------------------------ feed-forward ---
+
+FFN_SIZES = [   # tokens, hidden, inter, out
+    (1, 64, 128, 64),
+    (1, 2560, 1024, 2560),
+    (3, 8, 8, 8),
+    (7, 72, 40, 136),
+    (33, 264, 1000, 200),
+    (127, 256, 688, 256),
+    (129, 512, 320, 512),
+    (257, 648, 1032, 640),
+    (509, 1024, 2816, 1024),
+    (1025, 768, 2048, 768),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("size", FFN_SIZES, ids=str)
+def test_ffn(size, dtype):
+    *leaves, dy = ffn_inputs(*size, dtype)
+    want = ref.ffn(*leaves, dy)
+    with torch.no_grad():
+        within(llm_hgemm.gated_ffn(*leaves), want[0])
+    leaves = [t.requires_grad_() for t in leaves]
+    y = llm_hgemm.gated_ffn(*leaves)
+    for got, w in zip([y.detach(), *grads_of(y, leaves, dy)], want):
+        assert got.dtype == dtype
+        within(got, w)
+
+
+@pytest.mark.parametrize("size", [(5, 37, 53, 29), (130, 100, 300, 100)], ids=str)
+def test_ffn_sizes_of_any_remainder(size):
+    *leaves, dy = ffn_inputs(*size, torch.float16)
+    leaves = [t.requires_grad_() for t in leaves]
+    y = llm_hgemm.gated_ffn(*leaves)
+    for got, w in zip([y.detach(), *grads_of(y, leaves, dy)], ref.ffn(*leaves, dy)):
+        within(got, w)
+
+
+TILES = [64, 128, 192, 256]
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def ffn_through_c(x, gate, up, down, dy, tile, flags=0, status=None, timeout_ns=0):
+    """Both calls of the C ABI with a forced tile; outputs pre-filled with NaN."""
+    (t, h), (i, _), o = x.shape, gate.shape, down.shape[0]
+    like = lambda *s: torch.full(s, float("nan"), dtype=x.dtype, device="cuda")   # noqa: E731
+    common = train_capi.Common(train_capi.BF16 if x.dtype == torch.bfloat16 else train_capi.F16, tile, flags, 0,
+                               None if status is None else status.data_ptr(), timeout_ns)
+    y, act, g, u, dg, du = like(t, o), like(t, i), like(t, i), like(t, i), like(t, i), like(t, i)
+    dx, dgate, dup, ddown = like(t, h), like(i, h), like(i, h), like(o, i)
+    p = lambda *ts: [a.data_ptr() for a in ts]   # noqa: E731
+    f = train_capi.FfnForward(common, *p(x, gate, up, down, y, act, g, u), t, h, i, o, h)
+    assert train_capi.run("ffn_forward", f, stream()) == capi.OK
+    b = train_capi.FfnBackward(common, *p(dy, x, gate, up, down, g, u, act, dg, du, dx, dgate, dup, ddown), t, h, i, o, h, o)
+    assert train_capi.run("ffn_backward", b, stream()) == capi.OK
+    return y, dx, dgate, dup, ddown
+
+
+@pytest.mark.parametrize("pair", [0, train_capi.TILE_PAIR], ids=["single", "pair"])
+@pytest.mark.parametrize("width", TILES)
+def test_ffn_every_tile(width, pair):
+    """Each tile shape of the GEMM, on sizes whose edges fall inside tiles and
+    with more tiles than one wave for the narrow ones."""
+    inputs = ffn_inputs(390, 1352, 1992, 1096, torch.bfloat16)
+    for got, w in zip(ffn_through_c(*inputs, width | pair), ref.ffn(*inputs)):
+        within(got, w)
+
+
+def test_ffn_only_the_wanted_gradients():
+    x, gate, up, down, dy = ffn_inputs(70, 128, 256, 128, torch.bfloat16)
+    want = ref.ffn(x, gate, up, down, dy)
+    for wanted in ([0], [1], [3], [0, 2], [1, 2, 3]):
+        tensors = [t.detach().clone().requires_grad_(k in wanted) for k, t in enumerate((x, gate, up, down))]
+        y = llm_hgemm.gated_ffn(*tensors)
+        y.backward(dy)
+        for k, t in enumerate(tensors):
+            if k in wanted:
+                within(t.grad, want[1 + k])
+            else:
+                assert t.grad is None
+
+
+def test_ffn_strides_and_leading_dimensions():
+    x, gate, up, down, dy = ffn_inputs(60, 128, 256, 64, torch.float16)
+    want = ref.ffn(x, gate, up, down, dy)
+    wide = normal(9, 60, 300)
+    wide[:, 40:168] = x                       # rows 300 apart, 16-byte aligned
+    odd = normal(9, 60, 301)
+    odd[:, 41:169] = x                        # rows 301 apart, at an odd offset
+    turned = x.t().contiguous().t()           # columns unit apart in the other dimension
+    gate_turned = gate.t().contiguous().t()
+    for v in (wide[:, 40:168], odd[:, 41:169], turned):
+        within(llm_hgemm.gated_ffn(v, gate_turned, up, down), want[0])
+    cube = x.view(3, 4, 5, 128).requires_grad_()
+    y = llm_hgemm.gated_ffn(cube, gate, up, down)
+    assert y.shape == (3, 4, 5, 64)
+    (dx,) = torch.autograd.grad(y, cube, dy.view(3, 4, 5, 64))
+    within(dx.view(60, 128), want[1])
+    # A broadcast incoming gradient (stride 0).
+    (dx,) = torch.autograd.grad(llm_hgemm.gated_ffn(cube, gate, up, down).sum(), cube)
+    within(dx.view(60, 128), ref.ffn(x, gate, up, down, torch.ones_like(dy))[1])
+
+
+def test_ffn_no_tokens_and_shared_weights():
+    x, gate, _, down, dy = ffn_inputs(20, 64, 128, 64, torch.float16)
+    none = x[:0].clone().requires_grad_()
+    g = gate.clone().requires_grad_()
+    y = llm_hgemm.gated_ffn(none, g, g, down)
+    assert y.shape == (0, 64)
+    y.sum().backward()
+    assert none.grad.shape == (0, 64) and not g.grad.any()
+    # gate and up the same tensor: both gradients add up.
+    g = gate.clone().requires_grad_()
+    llm_hgemm.gated_ffn(x, g, g, down).backward(dy)
+    want = ref.ffn(x, gate, gate, down, dy)
+    (a, ea), (b, eb) = want[2], want[3]
+    within(g.grad, (a + b, ea + eb + ref.unit(torch.float16) * (a + b).abs()))
+
+
+def test_ffn_special_values_stay_in_their_rows():
+    x, gate, up, down, _ = ffn_inputs(130, 64, 128, 64, torch.float16)
+    clean = llm_hgemm.gated_ffn(x, gate, up, down)
+    x[5] = float("nan")
+    x[128, 3] = float("inf")
+    y = llm_hgemm.gated_ffn(x, gate, up, down)
+    assert y[5].isnan().all() and not y[128].isfinite().all()
+    rest = [r for r in range(130) if r not in (5, 128)]
+    assert torch.equal(y[rest], clean[rest])
+    # Large negative pre-activations: silu is 0, not NaN.
+    big = torch.full((4, 64), 100.0, dtype=torch.float16, device="cuda")
+    y = llm_hgemm.gated_ffn(big, -torch.ones_like(gate), torch.ones_like(up), down)
+    assert bool((y == 0).all())
+
+
+def test_ffn_against_differences():
+    """The directional derivative by central differences of the 64-bit formula
+    at the same points: the two agree to the bound and the difference's own error."""
+    x, gate, up, down, dy = ffn_inputs(9, 40, 48, 32, torch.float16)
+    leaves = [t.requires_grad_() for t in (x, gate, up, down)]
+    grads = grads_of(llm_hgemm.gated_ffn(*leaves), leaves, dy)
+    want = ref.ffn(*leaves, dy)
+    for k in range(4):
+        direction = normal(50 + k, *leaves[k].shape).double()
+        step = 1e-4
+
+        def f(sign):
+            moved = [t.detach().double() + (sign * step * direction if j == k else 0) for j, t in enumerate(leaves)]
+            pre = moved[0] @ moved[1].T
+            return ((torch.nn.functional.silu(pre) * (moved[0] @ moved[2].T)) @ moved[3].T * dy.double()).sum()
+
+        diff = (f(1) - f(-1)) / (2 * step)
+        # Third derivatives are of order one here: the difference is off by about step^2 |d|^3.
+        slack = (want[1 + k][1] * direction.abs()).sum() + 1e-3 * (1 + diff.abs())
+        assert abs((grads[k].double() * direction).sum() - diff) <= slack
+
+
+# ------------------------------------------------------------ cross entropy ---
+
+LOSS_SIZES = [   # tokens, hidden, vocab
+    (1, 8, 2),
+    (1, 64, 1),
+    (2, 72, 31),
+    (17, 136, 257),
+    (24, 256, 4001),
+    (129, 64, 1000),
+    (300, 264, 513),
+    (1, 2560, 12345),
+    (257, 520, 10007),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+@pytest.mark.parametrize("size", LOSS_SIZES, ids=str)
+def test_loss(size, reduction, dtype):
+    x, w, t = loss_inputs(*size, dtype)
+    t[0] = size[2] - 1          # one target at least, in the last column
+    dl = (torch.rand(size[0], device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) * 100
+          if reduction == "none" else torch.tensor(64.0, device="cuda"))
+    want = ref.loss(x, w, t, reduction, -100, dl)
+    within(llm_hgemm.linear_cross_entropy(x, w, t, reduction=reduction), want[0])
+    x.requires_grad_(), w.requires_grad_()
+    value = llm_hgemm.linear_cross_entropy(x, w, t, reduction=reduction)
+    assert value.dtype == torch.float32
+    for got, v in zip([value.detach(), *grads_of(value, [x, w], dl)], want):
+        within(got, v)
+
+
+def loss_through_c(x, w, t, dl, tile=0, piece=0, reduction=train_capi.LOSS_MEAN):
+    """Forward and backward through the C ABI, workspaces pre-filled with NaN."""
+    n, h = x.shape
+    v = w.shape[0]
+    common = train_capi.Common(train_capi.BF16 if x.dtype == torch.bfloat16 else train_capi.F16, tile)
+    loss = torch.full((n if reduction == train_capi.LOSS_NONE else 1,), float("nan"), device="cuda")
+    lse = torch.full((n,), float("nan"), device="cuda")
+    f = train_capi.LossForward(common, x.data_ptr(), w.data_ptr(), t.data_ptr(), loss.data_ptr(), lse.data_ptr(), None, 0,
+                               n, h, v, h, -100, reduction, 0)
+    f.workspace_bytes = train_capi.workspace("loss_forward", f)
+    ws = torch.full((f.workspace_bytes // 4,), float("nan"), device="cuda")
+    f.workspace = ws.data_ptr()
+    assert train_capi.run("loss_forward", f, stream()) == capi.OK
+    dx, dw = torch.full_like(x, float("nan")), torch.full_like(w, float("nan"))
+    b = train_capi.LossBackward(common, x.data_ptr(), w.data_ptr(), t.data_ptr(), lse.data_ptr(), dl.data_ptr(),
+                                dx.data_ptr(), dw.data_ptr(), None, 0, n, h, v, h, -100, piece, reduction, 0)
+    b.workspace_bytes = train_capi.workspace("loss_backward", b)
+    ws2 = torch.full((b.workspace_bytes // 4,), float("nan"), device="cuda")
+    b.workspace = ws2.data_ptr()
+    assert train_capi.run("loss_backward", b, stream()) == capi.OK
+    torch.cuda.synchronize()
+    return loss, dx, dw
+
+
+@pytest.mark.parametrize("pair", [0, train_capi.TILE_PAIR], ids=["single", "pair"])
+@pytest.mark.parametrize("width", TILES)
+def test_loss_every_tile(width, pair):
+    x, w, t = loss_inputs(390, 328, 20011, torch.float16)
+    dl = torch.tensor([32.0], device="cuda")
+    want = ref.loss(x, w, t, "mean", -100, dl)
+    got = loss_through_c(x, w, t, dl, width | pair)
+    for g, v in zip((got[0][0], got[1], got[2]), want):
+        within(g, v)
+
+
+@pytest.mark.parametrize("piece", [8, 264, 1000, 2049, 5000, 100000])
+def test_loss_pieces_of_the_vocabulary(piece):
+    x, w, t = loss_inputs(200, 136, 4999, torch.bfloat16)
+    dl = torch.tensor([1.0], device="cuda")
+    want = ref.loss(x, w, t, "sum", -100, dl)
+    got = loss_through_c(x, w, t, dl, piece=piece, reduction=train_capi.LOSS_SUM)
+    for g, v in zip((got[0][0], got[1], got[2]), want):
+        within(g, v)
+
+
+def test_loss_odd_hidden_size_strides_and_int32_targets():
+    x, w, t = loss_inputs(45, 37, 300, torch.float16)
+    dl = torch.tensor(8.0, device="cuda")
+    want = ref.loss(x, w, t, "sum", -100, dl)
+    wide = normal(3, 45, 99)
+    wide[:, 11:48] = x
+    a, b = wide[:, 11:48].detach().view(3, 15, 37).requires_grad_(), w.requires_grad_()
+    value = llm_hgemm.linear_cross_entropy(a, b, t.int().view(3, 15), reduction="sum")
+    dx, dw = grads_of(value, [a, b], dl)
+    assert dx.shape == (3, 15, 37)
+    for got, v in zip((value.detach(), dx.reshape(45, 37), dw), want):
+        within(got, v)
+    each = llm_hgemm.linear_cross_entropy(a.detach(), b.detach(), t.view(3, 15), reduction="none")
+    assert each.shape == (3, 15)
+
+
+def test_loss_ignored_and_invalid_targets():
+    x, w, t = loss_inputs(40, 64, 500, torch.float16)
+    x.requires_grad_(), w.requires_grad_()
+    nothing = torch.full_like(t, -100)
+    for reduction, want in (("mean", float("nan")), ("sum", 0.0)):
+        value = llm_hgemm.linear_cross_entropy(x, w, nothing, reduction=reduction)
+        assert torch.equal(value, torch.tensor(want, device="cuda")) or value.isnan() and want != want
+        dx, dw = grads_of(value, [x, w], torch.ones((), device="cuda"))
+        assert not dx.any() and not dw.any()
+    # An ignored row may hold anything.
+    poisoned = x.detach().clone()
+    poisoned[3] = float("nan")
+    t[3] = -100
+    keep = torch.arange(40, device="cuda") != 3
+    p = poisoned.requires_grad_()
+    value = llm_hgemm.linear_cross_entropy(p, w, t, reduction="sum")
+    want = ref.loss(x.detach()[keep], w, t[keep], "sum", -100, torch.ones((), device="cuda"))
+    within(value.detach(), want[0])
+    (dx,) = torch.autograd.grad(value, p)
+    assert not dx[3].any()
+    within(dx[keep], want[1])
+    # Another ignore_index, among the valid classes.
+    got = llm_hgemm.linear_cross_entropy(x.detach(), w.detach(), t.clamp(min=0), reduction="none", ignore_index=0)
+    assert bool((got[t.clamp(min=0) == 0] == 0).all())
+    # Outside the vocabulary: NaN for that token, the others as they were.
+    for bad in (500, -1, 2 ** 40):
+        t2 = t.clone()
+        t2[7] = bad
+        each = llm_hgemm.linear_cross_entropy(x.detach(), w.detach(), t2, reduction="none")
+        assert each[7].isnan() and int(each.isnan().sum()) == 1
+        dx, = torch.autograd.grad(llm_hgemm.linear_cross_entropy(x, w.detach(), t2, reduction="sum"), x)
+        assert dx[7].isnan().all() and int(dx.isnan().any(dim=1).sum()) == 1
+
+
+def test_loss_extreme_logits_and_gradients():
+    """Logits of +-3000, rows with one certain class, and incoming gradients over
+    16 orders of magnitude or zero."""
+    w = torch.zeros(300, 64, dtype=torch.float16, device="cuda")
+    w[:, 0] = torch.linspace(-50, 50, 300, device="cuda").half()
+    x = torch.zeros(6, 64, dtype=torch.float16, device="cuda")
+    x[:, 0] = torch.tensor([60.0, -60.0, 0.0, 1e-3, 20.0, -1.0], device="cuda").half()
+    t = torch.tensor([299, 0, 5, 7, 299, 1], device="cuda")
+    x.requires_grad_(), w.requires_grad_()
+    for dl in (torch.tensor([1e4, 1e-12, 1.0, 3.0, 1e-3, 0.5], device="cuda"), torch.zeros(6, device="cuda")):
+        value = llm_hgemm.linear_cross_entropy(x, w, t, reduction="none")
+        want = ref.loss(x, w, t, "none", -100, dl)
+        for got, v in zip([value.detach(), *grads_of(value, [x, w], dl)], want):
+            within(got, v)
+
+
+def test_loss_no_tokens():
+    w = normal(1, 50, 64).requires_grad_()
+    x = normal(2, 0, 64).requires_grad_()
+    t = torch.zeros(0, dtype=torch.int64, device="cuda")
+    assert llm_hgemm.linear_cross_entropy(x, w, t).isnan()
+    value = llm_hgemm.linear_cross_entropy(x, w, t, reduction="sum")
+    value.backward()
+    assert value == 0 and not w.grad.any() and x.grad.shape == (0, 64)
+    assert llm_hgemm.linear_cross_entropy(x, w, t, reduction="none").shape == (0,)
+
+
+def test_loss_against_differences():
+    x, w, t = loss_inputs(11, 40, 77, torch.float16)
+    x.requires_grad_(), w.requires_grad_()
+    dl = torch.ones((), device="cuda")
+    grads = grads_of(llm_hgemm.linear_cross_entropy(x, w, t), [x, w], dl)
+    want = ref.loss(x, w, t, "mean", -100, dl)
+    for k in range(2):
+        d = normal(60 + k, *(x, w)[k].shape).double()
+
+        def f(sign):
+            a, b = (v.detach().double() + (sign * 1e-4 * d if j == k else 0) for j, v in enumerate((x, w)))
+            return torch.nn.functional.cross_entropy(a @ b.T, t)
+
+        diff = (f(1) - f(-1)) / 2e-4
+        slack = (want[1 + k][1] * d.abs()).sum() + 1e-3 * (1 + diff.abs())
+        assert abs((grads[k].double() * d).sum() - diff) <= slack
+
+
+# ------------------------------------------------------ orthogonalised update ---
+
+ORTH_SIZES = [(1, 1), (1, 9), (9, 1), (8, 8), (16, 40), (96, 256), (256, 96), (129, 131), (333, 1001), (513, 64),
+              (1000, 250), (512, 512)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("size", ORTH_SIZES, ids=str)
+def test_orthogonalize(size, dtype):
+    g = normal(5, *size, dtype=dtype, scale=1e-3)
+    value, err = ref.orthogonalize(g, 5, NEWTON_SCHULZ, 1e-7)
+    got = llm_hgemm.orthogonalize(g)
+    assert got.shape == g.shape and got.dtype == dtype and got.is_contiguous()
+    assert float(torch.linalg.vector_norm(got.double() - value)) <= err
+
+
+@pytest.mark.parametrize("batch", [(1,), (3,), (4,), (5,), (2, 3)], ids=str)
+def test_orthogonalize_batches_and_strides(batch):
+    g = normal(6, *batch, 40, 77, scale=0.1)
+    got = llm_hgemm.orthogonalize(g)
+    for k, m in enumerate(g.view(-1, 40, 77)):
+        assert torch.equal(got.view(-1, 40, 77)[k], llm_hgemm.orthogonalize(m))
+    wide = normal(7, *batch, 50, 200, scale=0.1)
+    assert torch.equal(llm_hgemm.orthogonalize(wide[..., 3:43, 5:82]), llm_hgemm.orthogonalize(wide[..., 3:43, 5:82].contiguous()))
+    assert torch.equal(llm_hgemm.orthogonalize(g.mT), llm_hgemm.orthogonalize(g.mT.contiguous()))
+
+
+def test_orthogonalize_steps_coefficients_and_zeros():
+    g = normal(8, 60, 90, dtype=torch.bfloat16)
+    for steps, co in ((0, NEWTON_SCHULZ), (1, NEWTON_SCHULZ), (10, (1.5, -0.5, 0.0))):
+        value, err = ref.orthogonalize(g, steps, co, 1e-7)
+        got = llm_hgemm.orthogonalize(g, steps=steps, coefficients=co)
+        assert float(torch.linalg.vector_norm(got.double() - value)) <= err
+    zero = torch.zeros(30, 50, dtype=torch.float16, device="cuda")
+    assert not llm_hgemm.orthogonalize(zero).any()
+    # Far outside FP32's squares, and with eps as the whole norm.
+    for scale in (1e30, 1e-30):
+        h = (normal(9, 24, 32, dtype=torch.bfloat16).float() * scale).bfloat16()
+        value, err = ref.orthogonalize(h, 5, NEWTON_SCHULZ, 0.0)
+        assert float(torch.linalg.vector_norm(llm_hgemm.orthogonalize(h, eps=0.0).double() - value)) <= err
+    assert llm_hgemm.orthogonalize(g.requires_grad_()).requires_grad is False
+    assert llm_hgemm.orthogonalize(zero[:0]).shape == (0, 50)
+
+
+@pytest.mark.parametrize("pair", [0, train_capi.TILE_PAIR], ids=["single", "pair"])
+@pytest.mark.parametrize("width", TILES)
+@pytest.mark.parametrize("size", [(300, 700), (700, 300)], ids=str)
+def test_orthogonalize_every_tile(size, width, pair):
+    g = normal(10, *size)
+    value, err = ref.orthogonalize(g, 5, NEWTON_SCHULZ, 1e-7)
+    out = torch.full_like(g, float("nan"))
+    a = train_capi.Orthogonalize(train_capi.Common(train_capi.F16, width | pair), g.data_ptr(), out.data_ptr(), None, 0,
+                                 1, *size, size[1], 0, 5, 0, *NEWTON_SCHULZ, 0.0, 1e-7)
+    a.workspace_bytes = train_capi.workspace("orthogonalize", a)
+    ws = torch.full((a.workspace_bytes // 2,), float("nan"), dtype=torch.float16, device="cuda")
+    a.workspace = ws.data_ptr()
+    assert train_capi.run("orthogonalize", a, stream()) == capi.OK
+    assert float(torch.linalg.vector_norm(out.double() - value)) <= err
+
+
+# -------------------------------------------------------- how they are called ---
+
+def run_all(x, gate, up, down, w, t, dy):
+    y = llm_hgemm.gated_ffn(x, gate, up, down)
+    value = llm_hgemm.linear_cross_entropy(y, w, t)
+    grads = torch.autograd.grad(value, [x, gate, up, down, w])
+    return [y.detach(), value.detach(), *grads, llm_hgemm.orthogonalize(grads[1])]
+
+
+def all_inputs(tokens=90, seed=1):
+    x, gate, up, down, dy = ffn_inputs(tokens, 128, 320, 128, torch.bfloat16, seed)
+    _, w, t = loss_inputs(tokens, 128, 3001, torch.bfloat16, seed=seed + 20)
+    return [v.requires_grad_() for v in (x, gate, up, down, w)][:4] + [w, t, dy]
+
+
+def test_same_result_every_time_and_on_another_stream():
+    inputs = all_inputs()
+    first = run_all(*inputs)
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    with torch.cuda.stream(other):
+        again = run_all(*inputs)
+    other.synchronize()
+    for a, b in zip(first, again):
+        assert torch.equal(a, b)
+
+
+def test_two_streams_at_once():
+    sets = [all_inputs(seed=s) for s in (1, 100)]
+    want = [run_all(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [None, None]
+    for _ in range(3):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k] = run_all(*sets[k])
+    torch.cuda.synchronize()
+    for k in range(2):
+        for a, b in zip(want[k], got[k]):
+            assert torch.equal(a, b)
+
+
+def test_captured_and_replayed():
+    """A whole step in a CUDA graph, replayed on new inputs in place, twice."""
+    inputs = all_inputs()
+    fresh = [all_inputs(seed=s) for s in (40, 80)]
+    want = [run_all(*f) for f in fresh]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run_all(*inputs)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run_all(*inputs)
+    for f, w in zip(fresh, want):
+        with torch.no_grad():
+            for dst, src in zip(inputs, f):
+                dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, w):
+            assert torch.equal(a, b)
+
+
+def test_injected_stall_times_out_and_context_survives():
+    inputs = ffn_inputs(390, 520, 712, 520, torch.bfloat16)
+    for tile in (128, 128 | train_capi.TILE_PAIR):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        ffn_through_c(*inputs, tile, flags=capi.FLAG_TEST_INJECT_TX, status=status, timeout_ns=50_000_000)
+        torch.cuda.synchronize()
+        assert int(status) == capi.ERR_PIPELINE_TIMEOUT
+        for got, w in zip(ffn_through_c(*inputs, tile), ref.ffn(*inputs)):
+            within(got, w)
+    assert train_capi.read_status() == (capi.OK, 0)
+
+
+def test_second_derivatives_and_changed_weights_are_refused():
+    x, gate, up, down, w, t, dy = all_inputs()
+    y = llm_hgemm.gated_ffn(x, gate, up, down)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(y, x, dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(llm_hgemm.linear_cross_entropy(x, w, t), x, create_graph=True)
+    y = llm_hgemm.gated_ffn(x, gate, up, down)
+    with torch.no_grad():
+        gate.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, x, dy)
+
+
+def test_a_training_step_of_a_small_model():
+    """Module, head loss and orthogonalised update together, against the same
+    step on the stock modules: the gradients to the formula's bounds."""
+    torch.manual_seed(0)
+    parts = [nn.Linear(128, 320, bias=False), nn.Linear(128, 320, bias=False), nn.Linear(320, 128, bias=False)]
+    block = TrainableSwiGLU(*parts).to("cuda", torch.bfloat16)
+    assert sorted(block.state_dict()) == ["down_proj.weight", "gate_proj.weight", "up_proj.weight"]
+    head = normal(3, 1001, 128, dtype=torch.bfloat16, scale=0.1).requires_grad_()
+    x = normal(4, 2, 35, 128, dtype=torch.bfloat16)
+    t = torch.randint(0, 1001, (2, 35), device="cuda")
+    for _ in range(2):
+        y = block(x)
+        y.retain_grad()
+        value = llm_hgemm.linear_cross_entropy(y, head, t)
+        value.backward()
+        weights = [block.gate_proj.weight, block.up_proj.weight, block.down_proj.weight]
+        want = ref.loss(y.detach().view(70, 128), head, t.view(70), "mean", -100, torch.ones((), device="cuda"))
+        for got, v in zip((value.detach(), y.grad.view(70, 128), head.grad), want):
+            within(got, v)
+        for p, v in zip(weights, ref.ffn(x.view(70, 128), *weights, y.grad.view(70, 128))[2:]):
+            within(p.grad, v)
+        with torch.no_grad():
+            for p in weights + [head]:
+                update = llm_hgemm.orthogonalize(p.grad)
+                value_, err = ref.orthogonalize(p.grad, 5, NEWTON_SCHULZ, 1e-7)
+                assert float(torch.linalg.vector_norm(update.double() - value_)) <= err
+                p -= 0.02 * update
+                p.grad = None
