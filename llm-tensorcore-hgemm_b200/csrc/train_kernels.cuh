@@ -379,6 +379,13 @@ __device__ __forceinline__ void train_epilogue(const TrainParams& p, const Train
 
 // ------------------------------------------------------------------ the GEMM ---
 
+// A compile-time argument of the producer's inner loop, and the ways B comes.
+template <int kValue>
+struct Is {
+    static constexpr int value = kValue;
+};
+enum : int { kBKMajor = 0, kBMnMajor = 1, kBTwoHalves = 2 };
+
 template <bool kPair, int kEpi>
 __global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_constant__ TrainParams p) {
     extern __shared__ uint8_t smem_raw[];
@@ -433,64 +440,97 @@ __global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_co
     TileIter it(unit, units);
     int prob, tm, tn, nth;
 
+    const uint32_t num_stages = static_cast<uint32_t>(p.stages), stage_bytes = p.stage_bytes;
+    const uint32_t ring = smem_addr(smem);
+
     if (warp == 4) {
         if (lane == 0) {
             uint32_t stage = 0, phase = 0, issued = 0;
             bool ok = true;
+            // Everything the inner loop needs is in registers: parameter loads
+            // between the copies cost 15-30 % of a 256 x 256 tile's K block.
+            const uint32_t full0 = kPair ? map_to_rank(smem_addr(full), 0) : smem_addr(full);
+            auto load = [](uint32_t dst, uint64_t map, uint32_t bar, int x, int y) {
+                if constexpr (kPair)
+                    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global"
+                                 ".mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+                else
+                    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+                                 " [%0], [%1, {%3, %4}], [%2];"
+                                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+            };
+            auto map_of = [](const CUtensorMap& m) { return reinterpret_cast<uint64_t>(&m); };
+            uint32_t extra = p.inject ? 16u : 0u;
+            // The K blocks [kb0, kb1) of one segment, forwards or backwards.
+            auto segment = [&](uint64_t ma, uint64_t mb, uint64_t mb2, auto a_mn_c, auto b_kind_c, int row0, int col0,
+                               int chunks, uint32_t half_bytes, uint32_t tx, int blocks, bool back) {
+                constexpr bool a_mn = decltype(a_mn_c)::value;
+                constexpr int b_kind = decltype(b_kind_c)::value;
+                int k = back ? (blocks - 1) * kBlockK : 0;
+                const int step = back ? -kBlockK : kBlockK;
+                for (int i = 0; i < blocks; ++i, k += step) {
+                    if (!(kPair ? mbar_wait_cluster(&empty[stage], phase ^ 1u, wc)
+                                : mbar_wait(&empty[stage], phase ^ 1u, wc))) return false;
+                    if (leader) mbar_arrive_expect_tx(&full[stage], tx + extra);
+                    extra = 0;
+                    const uint32_t bar = full0 + stage * 8u, s_a = ring + stage * stage_bytes, s_b = s_a + kABytes;
+                    if constexpr (a_mn) {
+                        load(s_a, ma, bar, row0, k);
+                        load(s_a + kChunkBytes, ma, bar, row0 + 64, k);
+                    } else {
+                        load(s_a, ma, bar, k, row0);
+                    }
+                    if constexpr (b_kind == kBMnMajor) {
+                        load(s_b, mb, bar, col0, k);
+                        if (chunks > 1) load(s_b + kChunkBytes, mb, bar, col0 + 64, k);
+                        if (!kPair && chunks > 2) load(s_b + 2 * kChunkBytes, mb, bar, col0 + 128, k);
+                        if (!kPair && chunks > 3) load(s_b + 3 * kChunkBytes, mb, bar, col0 + 192, k);
+                    } else {
+                        load(s_b, mb, bar, k, col0);
+                        if constexpr (b_kind == kBTwoHalves) load(s_b + half_bytes, mb2, bar, k, col0);
+                    }
+                    ++issued;
+                    if (++stage == num_stages) { stage = 0; phase ^= 1u; }
+                }
+                return true;
+            };
             while (ok && it.next(p, prob, tm, tn, nth)) {
                 const TrainProblem& q = p.prob[prob];
                 const int row0 = tm * kTileM + static_cast<int>(rank) * 128;
                 // Columns of B that this CTA loads: all, or its half of the pair's.
                 const int cols = kPair ? q.tile_n / 2 : q.tile_n;
-                const int col0 = q.dual ? tn * (q.tile_n / 2) : tn * q.tile_n + static_cast<int>(rank) * cols;
-                const uint32_t bytes = kABytes + (q.b_mn ? ((cols + 63) / 64) * kChunkBytes : cols * 128u);
+                const bool dual = kEpi == kTrainGate;
+                const int col0 = dual ? tn * (q.tile_n / 2) : tn * q.tile_n + static_cast<int>(rank) * cols;
+                const int chunks = (cols + 63) / 64;
+                const uint32_t bytes = kABytes + (q.b_mn ? chunks * kChunkBytes : cols * 128u);
+                const uint32_t tx = (kPair ? 2u : 1u) * bytes;
                 // Odd waves walk K backwards: they start on the panels that the
                 // wave before read last, while those are in L2.
                 const bool back = (nth & 1) != 0;
-                for (int kq = 0; kq < q.nkb; ++kq) {
-                    const int kb = back ? q.nkb - 1 - kq : kq;
-                    if (!(kPair ? mbar_wait_cluster(&empty[stage], phase ^ 1u, wc)
-                                : mbar_wait(&empty[stage], phase ^ 1u, wc))) { ok = false; break; }
-                    uint8_t* s_a = smem + stage * p.stage_bytes;
-                    uint8_t* s_b = s_a + kABytes;
-                    if (leader) {
-                        const uint32_t extra = (p.inject && issued == 0) ? 16u : 0u;
-                        mbar_arrive_expect_tx(&full[stage], (kPair ? 2u : 1u) * bytes + extra);
-                    }
-                    const uint32_t bar = kPair ? map_to_rank(smem_addr(&full[stage]), 0) : 0u;
-                    auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y) {
-                        if constexpr (kPair) tma_load_2d_pair(dst, map, bar, x, y);
-                        else tma_load_2d(dst, map, &full[stage], x, y);
-                    };
-                    const int seg = kb >= q.nkb0 ? 1 : 0;
-                    const int k0 = (seg ? kb - q.nkb0 : kb) * kBlockK;
-                    if (q.a_mn) {
-                        load(s_a, &q.a[seg], row0, k0);
-                        load(s_a + kChunkBytes, &q.a[seg], row0 + 64, k0);
+                for (int i = 0; i < 2 && ok; ++i) {
+                    const int seg = back ? 1 - i : i;
+                    const int blocks = seg ? q.nkb - q.nkb0 : q.nkb0;
+                    if (blocks == 0) continue;
+                    const uint64_t ma = map_of(q.a[seg]), mb = map_of(q.b[seg]);
+                    if constexpr (dual) {
+                        if constexpr (kPair)
+                            ok = segment(ma, map_of(q.b[rank]), 0ull, Is<0>{}, Is<kBKMajor>{}, row0, col0, chunks, 0u, tx, blocks, back);
+                        else
+                            ok = segment(ma, mb, map_of(q.b[1]), Is<0>{}, Is<kBTwoHalves>{}, row0, col0, chunks, cols * 64u, tx, blocks, back);
+                    } else if (q.a_mn) {
+                        ok = q.b_mn ? segment(ma, mb, 0ull, Is<1>{}, Is<kBMnMajor>{}, row0, col0, chunks, 0u, tx, blocks, back)
+                                    : segment(ma, mb, 0ull, Is<1>{}, Is<kBKMajor>{}, row0, col0, chunks, 0u, tx, blocks, back);
                     } else {
-                        load(s_a, &q.a[seg], k0, row0);
+                        ok = q.b_mn ? segment(ma, mb, 0ull, Is<0>{}, Is<kBMnMajor>{}, row0, col0, chunks, 0u, tx, blocks, back)
+                                    : segment(ma, mb, 0ull, Is<0>{}, Is<kBKMajor>{}, row0, col0, chunks, 0u, tx, blocks, back);
                     }
-                    if (q.dual) {
-                        if constexpr (kPair) {
-                            load(s_b, &q.b[rank], k0, col0);
-                        } else {
-                            load(s_b, &q.b[0], k0, col0);
-                            load(s_b + (cols / 2) * 128, &q.b[1], k0, col0);
-                        }
-                    } else if (q.b_mn) {
-                        for (int j = 0; j < cols; j += 64) load(s_b + j * 128, &q.b[seg], col0 + j, k0);
-                    } else {
-                        load(s_b, &q.b[seg], k0, col0);
-                    }
-                    ++issued;
-                    if (++stage == static_cast<uint32_t>(p.stages)) { stage = 0; phase ^= 1u; }
                 }
             }
             if (leader && (!ok || *abort_flag)) {
                 // In-flight copies land before the CTA (or its pair) leaves.
-                const uint32_t n = static_cast<uint32_t>(p.stages);
-                for (uint32_t s = 0; s < (issued < n ? issued : n); ++s) {
-                    const uint32_t arms = issued / n + (s < issued % n ? 1u : 0u);
+                for (uint32_t s = 0; s < (issued < num_stages ? issued : num_stages); ++s) {
+                    const uint32_t arms = issued / num_stages + (s < issued % num_stages ? 1u : 0u);
                     mbar_wait_drain(&full[s], (arms - 1u) & 1u, kDrainLimitNs);
                 }
             }
@@ -507,19 +547,20 @@ __global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_co
                 // 16 of K further: 32 bytes along a K-major row, 16 rows of 128 bytes MN-major.
                 const uint64_t step_a = q.a_mn ? 2048u >> 4 : 32u >> 4;
                 const uint64_t step_b = q.b_mn ? 2048u >> 4 : 32u >> 4;
-                const uint32_t lbo_a = q.a_mn ? kChunkBytes : 16u, lbo_b = q.b_mn ? kChunkBytes : 16u;
+                const uint64_t desc_a = make_smem_desc(ring, q.a_mn ? kChunkBytes : 16u, 1024u);
+                const uint64_t desc_b = make_smem_desc(ring + kABytes, q.b_mn ? kChunkBytes : 16u, 1024u);
+                const int nkb = q.nkb;
                 const uint32_t acc = iter & 1u, acc_phase = (iter >> 1) & 1u;
                 ++iter;
                 if (!(kPair ? mbar_wait_cluster(&tempty[acc], acc_phase ^ 1u, wc)
                             : mbar_wait(&tempty[acc], acc_phase ^ 1u, wc))) { ok = false; break; }
                 tc_fence_after_sync();
                 const uint32_t d = tmem_base + acc * kTrainAccCols;
-                for (int kb = 0; kb < q.nkb; ++kb) {
+                for (int kb = 0; kb < nkb; ++kb) {
                     if (!mbar_wait(&full[stage], phase, wc)) { ok = false; break; }
                     tc_fence_after_sync();
-                    const uint32_t s_a = smem_addr(smem + stage * p.stage_bytes);
-                    const uint64_t da = make_smem_desc(s_a, lbo_a, 1024u);
-                    const uint64_t db = make_smem_desc(s_a + kABytes, lbo_b, 1024u);
+                    const uint64_t off = (stage * stage_bytes) >> 4;
+                    const uint64_t da = desc_a + off, db = desc_b + off;
 #pragma unroll
                     for (int kk = 0; kk < kBlockK / 16; ++kk) {
                         const uint32_t add = (kb > 0 || kk > 0) ? 1u : 0u;
@@ -528,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_co
                     }
                     if constexpr (kPair) tc_commit_pair_both(smem_addr(&empty[stage]));
                     else tc_commit(&empty[stage]);
-                    if (++stage == static_cast<uint32_t>(p.stages)) { stage = 0; phase ^= 1u; }
+                    if (++stage == num_stages) { stage = 0; phase ^= 1u; }
                 }
                 if (ok) {
                     if constexpr (kPair) tc_commit_pair_both(smem_addr(&tfull[acc]));
