@@ -76,8 +76,8 @@ struct alignas(64) TrainParams {
     int num_problems;
     int heavy_tiles, light_tiles;  // tiles of problem 0 / of the others
     int light_skip;                // waves the units with one heavy tile more sit out
-    int stages;
-    uint32_t stage_bytes;
+    int stages, sub;               // ring stages, K blocks of 64 in each
+    uint32_t block_stride;         // bytes of one K block's tiles in a stage
     int in_bf16, out_bf16;
     int* status;
     unsigned long long timeout_ns;
@@ -379,6 +379,38 @@ __device__ __forceinline__ void train_epilogue(const TrainParams& p, const Train
 
 // ------------------------------------------------------------------ the GEMM ---
 
+// 1 in one lane of the (converged) warp, 0 in the others.
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
+}
+
+// tcgen05.mma and commit by the lane with `issuer` set; called by the whole warp.
+template <bool kPair>
+__device__ __forceinline__ void tc_mma_if(uint32_t issuer, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                          uint32_t idesc, uint32_t accumulate) {
+    if constexpr (kPair)
+        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                     "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(issuer) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                     "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(issuer) : "memory");
+}
+template <bool kPair>
+__device__ __forceinline__ void tc_commit_if(uint32_t issuer, uint32_t bar) {
+    if constexpr (kPair)   // the barrier at the same place in both CTAs
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+                     "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+                     " [%0], %1;\n\t}" ::"r"(bar), "h"(static_cast<uint16_t>(0x3)), "r"(issuer) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                     "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+                     ::"r"(bar), "r"(issuer) : "memory");
+}
+
 // A compile-time argument of the producer's inner loop, and the ways B comes.
 template <int kValue>
 struct Is {
@@ -417,6 +449,10 @@ __global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_co
         mbar_init(drain, 1u);
         *abort_flag = 0;
         mbar_init_fence();
+        tma_prefetch_map(&p.prob[0].a[0]);
+        tma_prefetch_map(&p.prob[0].b[0]);
+        if constexpr (kEpi == kTrainGate) tma_prefetch_map(&p.prob[0].b[1]);
+        if constexpr (kEpi != kTrainLse) tma_prefetch_map(&p.prob[0].out[0]);
     }
     if (warp == 5) {
         if constexpr (kPair) {
@@ -440,7 +476,9 @@ __global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_co
     TileIter it(unit, units);
     int prob, tm, tn, nth;
 
-    const uint32_t num_stages = static_cast<uint32_t>(p.stages), stage_bytes = p.stage_bytes;
+    const uint32_t num_stages = static_cast<uint32_t>(p.stages), block_stride = p.block_stride;
+    const int sub = p.sub;
+    const uint32_t stage_bytes = static_cast<uint32_t>(sub) * block_stride;
     const uint32_t ring = smem_addr(smem);
 
     if (warp == 4) {
@@ -462,33 +500,38 @@ __global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_co
             };
             auto map_of = [](const CUtensorMap& m) { return reinterpret_cast<uint64_t>(&m); };
             uint32_t extra = p.inject ? 16u : 0u;
-            // The K blocks [kb0, kb1) of one segment, forwards or backwards.
+            // The K blocks of one segment, forwards or backwards, two to a stage.
             auto segment = [&](uint64_t ma, uint64_t mb, uint64_t mb2, auto a_mn_c, auto b_kind_c, int row0, int col0,
-                               int chunks, uint32_t half_bytes, uint32_t tx, int blocks, bool back) {
+                               int chunks, uint32_t half_bytes, uint32_t block_bytes, int blocks, bool back) {
                 constexpr bool a_mn = decltype(a_mn_c)::value;
                 constexpr int b_kind = decltype(b_kind_c)::value;
                 int k = back ? (blocks - 1) * kBlockK : 0;
                 const int step = back ? -kBlockK : kBlockK;
-                for (int i = 0; i < blocks; ++i, k += step) {
+                for (int left = blocks; left > 0; left -= sub) {
                     if (!(kPair ? mbar_wait_cluster(&empty[stage], phase ^ 1u, wc)
                                 : mbar_wait(&empty[stage], phase ^ 1u, wc))) return false;
-                    if (leader) mbar_arrive_expect_tx(&full[stage], tx + extra);
+                    const int count = left < sub ? left : sub;
+                    if (leader) mbar_arrive_expect_tx(&full[stage], (kPair ? 2u : 1u) * count * block_bytes + extra);
                     extra = 0;
-                    const uint32_t bar = full0 + stage * 8u, s_a = ring + stage * stage_bytes, s_b = s_a + kABytes;
-                    if constexpr (a_mn) {
-                        load(s_a, ma, bar, row0, k);
-                        load(s_a + kChunkBytes, ma, bar, row0 + 64, k);
-                    } else {
-                        load(s_a, ma, bar, k, row0);
-                    }
-                    if constexpr (b_kind == kBMnMajor) {
-                        load(s_b, mb, bar, col0, k);
-                        if (chunks > 1) load(s_b + kChunkBytes, mb, bar, col0 + 64, k);
-                        if (!kPair && chunks > 2) load(s_b + 2 * kChunkBytes, mb, bar, col0 + 128, k);
-                        if (!kPair && chunks > 3) load(s_b + 3 * kChunkBytes, mb, bar, col0 + 192, k);
-                    } else {
-                        load(s_b, mb, bar, k, col0);
-                        if constexpr (b_kind == kBTwoHalves) load(s_b + half_bytes, mb2, bar, k, col0);
+                    const uint32_t bar = full0 + stage * 8u;
+                    uint32_t s_a = ring + stage * stage_bytes;
+                    for (int i = 0; i < count; ++i, s_a += block_stride, k += step) {
+                        const uint32_t s_b = s_a + kABytes;
+                        if constexpr (a_mn) {
+                            load(s_a, ma, bar, row0, k);
+                            load(s_a + kChunkBytes, ma, bar, row0 + 64, k);
+                        } else {
+                            load(s_a, ma, bar, k, row0);
+                        }
+                        if constexpr (b_kind == kBMnMajor) {
+                            load(s_b, mb, bar, col0, k);
+                            if (chunks > 1) load(s_b + kChunkBytes, mb, bar, col0 + 64, k);
+                            if (!kPair && chunks > 2) load(s_b + 2 * kChunkBytes, mb, bar, col0 + 128, k);
+                            if (!kPair && chunks > 3) load(s_b + 3 * kChunkBytes, mb, bar, col0 + 192, k);
+                        } else {
+                            load(s_b, mb, bar, k, col0);
+                            if constexpr (b_kind == kBTwoHalves) load(s_b + half_bytes, mb2, bar, k, col0);
+                        }
                     }
                     ++issued;
                     if (++stage == num_stages) { stage = 0; phase ^= 1u; }
@@ -504,7 +547,6 @@ __global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_co
                 const int col0 = dual ? tn * (q.tile_n / 2) : tn * q.tile_n + static_cast<int>(rank) * cols;
                 const int chunks = (cols + 63) / 64;
                 const uint32_t bytes = kABytes + (q.b_mn ? chunks * kChunkBytes : cols * 128u);
-                const uint32_t tx = (kPair ? 2u : 1u) * bytes;
                 // Odd waves walk K backwards: they start on the panels that the
                 // wave before read last, while those are in L2.
                 const bool back = (nth & 1) != 0;
@@ -515,15 +557,15 @@ __global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_co
                     const uint64_t ma = map_of(q.a[seg]), mb = map_of(q.b[seg]);
                     if constexpr (dual) {
                         if constexpr (kPair)
-                            ok = segment(ma, map_of(q.b[rank]), 0ull, Is<0>{}, Is<kBKMajor>{}, row0, col0, chunks, 0u, tx, blocks, back);
+                            ok = segment(ma, map_of(q.b[rank]), 0ull, Is<0>{}, Is<kBKMajor>{}, row0, col0, chunks, 0u, bytes, blocks, back);
                         else
-                            ok = segment(ma, mb, map_of(q.b[1]), Is<0>{}, Is<kBTwoHalves>{}, row0, col0, chunks, cols * 64u, tx, blocks, back);
+                            ok = segment(ma, mb, map_of(q.b[1]), Is<0>{}, Is<kBTwoHalves>{}, row0, col0, chunks, cols * 64u, bytes, blocks, back);
                     } else if (q.a_mn) {
-                        ok = q.b_mn ? segment(ma, mb, 0ull, Is<1>{}, Is<kBMnMajor>{}, row0, col0, chunks, 0u, tx, blocks, back)
-                                    : segment(ma, mb, 0ull, Is<1>{}, Is<kBKMajor>{}, row0, col0, chunks, 0u, tx, blocks, back);
+                        ok = q.b_mn ? segment(ma, mb, 0ull, Is<1>{}, Is<kBMnMajor>{}, row0, col0, chunks, 0u, bytes, blocks, back)
+                                    : segment(ma, mb, 0ull, Is<1>{}, Is<kBKMajor>{}, row0, col0, chunks, 0u, bytes, blocks, back);
                     } else {
-                        ok = q.b_mn ? segment(ma, mb, 0ull, Is<0>{}, Is<kBMnMajor>{}, row0, col0, chunks, 0u, tx, blocks, back)
-                                    : segment(ma, mb, 0ull, Is<0>{}, Is<kBKMajor>{}, row0, col0, chunks, 0u, tx, blocks, back);
+                        ok = q.b_mn ? segment(ma, mb, 0ull, Is<0>{}, Is<kBMnMajor>{}, row0, col0, chunks, 0u, bytes, blocks, back)
+                                    : segment(ma, mb, 0ull, Is<0>{}, Is<kBKMajor>{}, row0, col0, chunks, 0u, bytes, blocks, back);
                     }
                 }
             }
@@ -536,7 +578,11 @@ __global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_co
             }
         }
     } else if (warp == 5) {
-        if (lane == 0 && leader) {
+        if (leader) {
+            // The whole warp walks the loop and one elected lane issues: with
+            // warp-uniform control flow the descriptors stay in uniform
+            // registers, where one lane alone pays a move per operand and MMA.
+            const uint32_t issuer = elect_lane();
             uint32_t stage = 0, phase = 0, iter = 0;
             bool ok = true;
             const uint32_t format = p.in_bf16 ? (1u << 7) | (1u << 10) : 0u;
@@ -549,34 +595,36 @@ __global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_co
                 const uint64_t step_b = q.b_mn ? 2048u >> 4 : 32u >> 4;
                 const uint64_t desc_a = make_smem_desc(ring, q.a_mn ? kChunkBytes : 16u, 1024u);
                 const uint64_t desc_b = make_smem_desc(ring + kABytes, q.b_mn ? kChunkBytes : 16u, 1024u);
-                const int nkb = q.nkb;
                 const uint32_t acc = iter & 1u, acc_phase = (iter >> 1) & 1u;
                 ++iter;
-                if (!(kPair ? mbar_wait_cluster(&tempty[acc], acc_phase ^ 1u, wc)
-                            : mbar_wait(&tempty[acc], acc_phase ^ 1u, wc))) { ok = false; break; }
+                if (!__all_sync(0xffffffffu, kPair ? mbar_wait_cluster(&tempty[acc], acc_phase ^ 1u, wc)
+                                                   : mbar_wait(&tempty[acc], acc_phase ^ 1u, wc))) { ok = false; break; }
                 tc_fence_after_sync();
                 const uint32_t d = tmem_base + acc * kTrainAccCols;
-                for (int kb = 0; kb < nkb; ++kb) {
-                    if (!mbar_wait(&full[stage], phase, wc)) { ok = false; break; }
-                    tc_fence_after_sync();
-                    const uint64_t off = (stage * stage_bytes) >> 4;
+                uint32_t add = 0;
+                auto block = [&](uint64_t off) {
                     const uint64_t da = desc_a + off, db = desc_b + off;
 #pragma unroll
                     for (int kk = 0; kk < kBlockK / 16; ++kk) {
-                        const uint32_t add = (kb > 0 || kk > 0) ? 1u : 0u;
-                        if constexpr (kPair) tc_mma_f16_pair(d, da + kk * step_a, db + kk * step_b, idesc, add);
-                        else tc_mma_f16(d, da + kk * step_a, db + kk * step_b, idesc, add);
+                        tc_mma_if<kPair>(issuer, d, da + kk * step_a, db + kk * step_b, idesc, add);
+                        add = 1;
                     }
-                    if constexpr (kPair) tc_commit_pair_both(smem_addr(&empty[stage]));
-                    else tc_commit(&empty[stage]);
-                    if (++stage == num_stages) { stage = 0; phase ^= 1u; }
+                };
+                const bool back = (nth & 1) != 0;
+                for (int i = 0; i < 2 && ok; ++i) {
+                    const int seg = back ? 1 - i : i;
+                    for (int left = seg ? q.nkb - q.nkb0 : q.nkb0; left > 0; left -= sub) {
+                        if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, wc))) { ok = false; break; }
+                        const uint64_t off = (stage * stage_bytes) >> 4;
+                        block(off);
+                        if (sub > 1 && left > 1) block(off + (block_stride >> 4));
+                        tc_commit_if<kPair>(issuer, smem_addr(&empty[stage]));
+                        if (++stage == num_stages) { stage = 0; phase ^= 1u; }
+                    }
                 }
-                if (ok) {
-                    if constexpr (kPair) tc_commit_pair_both(smem_addr(&tfull[acc]));
-                    else tc_commit(&tfull[acc]);
-                }
+                if (ok) tc_commit_if<kPair>(issuer, smem_addr(&tfull[acc]));
             }
-            if (!ok) {
+            if (!ok && lane == 0) {
                 if constexpr (kPair) tc_commit_pair(smem_addr(drain));
                 else tc_commit(drain);
                 mbar_wait_drain(drain, 0, kDrainLimitNs);

@@ -251,10 +251,12 @@ void init_params(TrainParams& p, const Context& c) {
 
 // Fills the problems of `p` from `count` products (the first one with the most
 // K blocks) and launches them as one grid.
+int g_sub = getenv("TSUB") ? atoi(getenv("TSUB")) : 0;
+
 int run_products(TrainParams& p, int epi, const Product* products, const Tile* tiles, int count, const Context& c) {
     const bool pair = tiles[0].pair;
     const int units = pair ? c.dev->sms / 2 : c.dev->sms;
-    uint32_t stage_bytes = 0;
+    uint32_t block_stride = 0;
     int64_t total = 0, light = 0;
     for (int i = 0; i < count; ++i) {
         const Product& s = products[i];
@@ -298,7 +300,7 @@ int run_products(TrainParams& p, int epi, const Product* products, const Tile* t
         }
         if (rc != HGEMM_SM100_OK) return rc;
         const int64_t b_cols = pair ? tile_n / 2 : tile_n;
-        stage_bytes = std::max(stage_bytes, static_cast<uint32_t>(16384 + round_up(b_cols, 64) * 128));
+        block_stride = std::max(block_stride, static_cast<uint32_t>(16384 + round_up(b_cols, 64) * 128));
         const int64_t n = static_cast<int64_t>(q.tiles_m) * q.tiles_n;
         total += n;
         if (i > 0) light += n;
@@ -313,8 +315,9 @@ int run_products(TrainParams& p, int epi, const Product* products, const Tile* t
                              (static_cast<double>(p.prob[1].nkb) * p.prob[1].tile_n);
         p.light_skip = static_cast<int>(ratio + 0.5);
     }
-    p.stage_bytes = stage_bytes;
-    p.stages = static_cast<int>(std::min<uint32_t>(kTrainRingBytes / stage_bytes, kTrainMaxStages));
+    p.block_stride = block_stride;
+    p.sub = g_sub ? g_sub : (kTrainRingBytes / (2 * block_stride) >= 3 ? 2 : 1);
+    p.stages = static_cast<int>(std::min<uint32_t>(kTrainRingBytes / (p.sub * block_stride), kTrainMaxStages));
 
     KernelEntry& k = g_kernels[pair ? 1 : 0][epi];
     const uint64_t bit = 1ull << c.id;
