@@ -22,10 +22,13 @@
 // kPair: tiles of 256 x tile_n per CTA pair (cta_group::2); otherwise 128 x
 // tile_n per CTA. tile_n is a run-time multiple of 32 (pairs: 64) up to 256,
 // so the host cuts the columns into a whole number of waves.
-// Roles per CTA: warps 0-3 epilogue (one TMEM lane = one output row per
-// thread), warp 4 TMA producer, warp 5 MMA issuer; two accumulators, so a
-// tile's epilogue runs under the next tile's MMAs. Every wait is bounded as
-// in the inference kernels (status word, drained copies, freed TMEM).
+// Roles per CTA: warps 0-7 epilogue (one TMEM lane = one output row per
+// thread; warps w and w + 4 share a row quarter and take every second group of
+// 32 columns), warp 8 TMA producer, warp 9 MMA issuer; two accumulators, so a
+// tile's epilogue runs under the next tile's MMAs. The last tile's epilogue is
+// exposed, and it is what eight warps halve (6400 -> 3200 cycles of a 256-wide
+// tile). Every wait is bounded as in the inference kernels (status word,
+// drained copies, freed TMEM).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -37,7 +40,9 @@ namespace hgemm {
 constexpr int kTrainMaxProblems = 4;
 constexpr uint32_t kTrainRingBytes = 196608;               // stages of both operands
 constexpr uint32_t kTrainBoxBytes = 2048;                  // 32 rows x 32 16-bit columns
-constexpr uint32_t kTrainEpiBytes = 4u * 4u * kTrainBoxBytes;  // 4 warps x 4 boxes
+constexpr int kTrainEpiWarps = 8;
+constexpr int kTrainThreads = (kTrainEpiWarps + 2) * 32;
+constexpr uint32_t kTrainEpiBytes = kTrainEpiWarps * 2u * kTrainBoxBytes;  // 2 boxes a warp
 constexpr int kTrainMaxStages = 12;
 constexpr uint32_t kTrainDataBytes = kTrainRingBytes + kTrainEpiBytes;
 constexpr uint32_t kTrainSmemBytes = kTrainDataBytes + 256 + 1024;
@@ -90,7 +95,7 @@ struct alignas(64) TrainParams {
     // kTrainLse / kTrainLogitGrad, per row.
     const long long* target;
     long long col_base;            // vocabulary index of column 0
-    float2* partial;               // kTrainLse: [tiles_n][m] (max, sum of exp(x - max))
+    float2* partial;               // kTrainLse: [2 tiles_n][m] (max, sum of exp(x - max))
     float* target_logit;           // kTrainLse: written by the tile holding the target
     const float* lse;
     const float* row_scale;
@@ -123,27 +128,28 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 constexpr float kLog2e = 1.4426950408889634f;
 
-// sigmoid(x); x -> -inf gives 0 (1 / (1 + inf)).
-__device__ __forceinline__ float sigmoid_f(float x) { return __frcp_rn(1.f + exp2_fast(-x * kLog2e)); }
-
-// 32 16-bit values src[0 .. 31] of one row as floats; elements from `avail`
-// on are zero. src 16-byte aligned; whole 8-element vectors are read only
-// where avail > 0 (rows are padded to a multiple of 8 elements).
-__device__ __forceinline__ void load_row32(const void* base, long long off, int avail, int bf16, float (&v)[32]) {
-    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + off);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (8 * q < avail) w = __ldg(src + q);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 f = unpack2(u[j], bf16);
-            v[8 * q + 2 * j] = f.x;
-            v[8 * q + 2 * j + 1] = f.y;
-        }
-    }
+// sigmoid(x), both approximations good to 2^-22; x -> -inf gives 0 (1 / (1 + inf)).
+__device__ __forceinline__ float sigmoid_f(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.f + exp2_fast(-x * kLog2e)));
+    return y;
 }
+
+// 32 16-bit values of one row, loaded ahead of their use. 16-byte-aligned
+// vectors, read only where they hold elements of the row (rows are padded to a
+// multiple of 8 elements); the others are zero.
+struct Row32 {
+    uint4 w[4];
+    __device__ __forceinline__ void load(const void* base, long long off, int avail) {
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + off);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) w[q] = 8 * q < avail ? __ldg(src + q) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    __device__ __forceinline__ float2 pair(int i, int bf16) const {   // elements 2i, 2i + 1
+        const uint4& v = w[i >> 2];
+        return unpack2((i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w, bf16);
+    }
+};
 
 // Adds a 2-D box in shared memory to FP32 global memory (elements outside the
 // map are not written).
@@ -154,19 +160,19 @@ __device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap* map, const 
 }
 
 // One epilogue warp's output boxes: 32 rows (lane = row) x 32 columns through
-// shared memory to a TMA store, 16-bit boxes in a ring of four 2 KB buffers
-// (64-byte swizzle), FP32 boxes in a ring of two 4 KB buffers (128-byte
-// swizzle). Before a buffer is rewritten, the store that used it last must
-// have read it. Every value is rounded here, once.
+// shared memory to a TMA store, 16-bit boxes in two 2 KB buffers in turn
+// (64-byte swizzle), FP32 boxes in one of 4 KB (128-byte swizzle). Before a
+// buffer is rewritten, the store that used it last must have read it. Every
+// value is rounded here, once.
 struct BoxWriter {
     uint8_t* bufs;
     uint32_t next;
     uint32_t lane;
 
     __device__ void put16(const CUtensorMap* map, const float (&v)[32], int bf16, int col, int row) {
-        if (lane == 0) bulk_wait_group_read<3>();
+        if (lane == 0) bulk_wait_group_read<1>();
         __syncwarp();
-        uint8_t* box = bufs + (next & 3u) * kTrainBoxBytes;
+        uint8_t* box = bufs + (next & 1u) * kTrainBoxBytes;
         ++next;
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
@@ -186,10 +192,9 @@ struct BoxWriter {
     }
 
     __device__ void put32(const CUtensorMap* map, const float (&v)[32], bool add, int col, int row) {
-        if (lane == 0) bulk_wait_group_read<1>();
+        if (lane == 0) bulk_wait_group_read<0>();
         __syncwarp();
-        uint8_t* box = bufs + (next & 1u) * (2u * kTrainBoxBytes);
-        ++next;
+        uint8_t* box = bufs;
 #pragma unroll
         for (uint32_t j = 0; j < 8; ++j)
             *reinterpret_cast<float4*>(box + lane * 128u + ((j ^ (lane & 7u)) << 4)) =
@@ -252,130 +257,150 @@ struct TileIter {
 
 // ---------------------------------------------------------------- epilogues ---
 
-// One 32-row x tile_n accumulator slice at TMEM address `t`: rows row0 + lane,
-// columns of tile column tn. Called by the whole warp.
+// One epilogue warp's part of a tile: rows row0 + lane, the groups of 32 columns
+// with index group, group + 2, ... of tile column tn. begin() starts the loads
+// of the first group (before the accumulator is ready); run() goes through the
+// groups with the next one's loads in flight. Called by the whole warp.
 template <int kEpi>
-__device__ __forceinline__ void train_epilogue(const TrainParams& p, const TrainProblem& q, BoxWriter& box,
-                                               uint32_t t, int row0, int tn) {
-    if (row0 >= q.m) return;
-    const int row = row0 + static_cast<int>(box.lane);
-    const bool in_rows = row < q.m;
-    if constexpr (kEpi == kTrainStore) {
-        const float alpha = q.alpha_ptr != nullptr ? q.alpha * __ldg(q.alpha_ptr) : q.alpha;
-#pragma unroll 1
-        for (int c = 0; c < q.tile_n; c += 32) {
-            const int col = tn * q.tile_n + c;
-            if (col >= q.n) break;
-            float v[32];
-            tmem_ld32(t + c, v);
-            if (q.out_kind != kTrainOut16) {
-                box.put32(&q.out[0], v, q.out_kind == kTrainOutF32Add, col, row0);
-                continue;
-            }
-            if (q.beta != 0.f) {
-                float w[32];
-                load_row32(q.c, row * q.ldc + col, in_rows ? q.n - col : 0, p.in_bf16, w);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = fmaf(alpha, v[i], q.beta * w[i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] *= alpha;
-            }
-            box.put16(&q.out[0], v, p.out_bf16, col, row0);
-        }
-    } else if constexpr (kEpi == kTrainGate) {
-        const int half = q.tile_n / 2;
-#pragma unroll 1
-        for (int c = 0; c < half; c += 32) {
-            const int col = tn * half + c;
-            if (col >= q.n) break;
-            float g[32], u[32];
-            tmem_ld32(t + c, g);
-            tmem_ld32(t + half + c, u);
-            if (p.keep) {
-                box.put16(&q.out[1], g, p.out_bf16, col, row0);
-                box.put16(&q.out[2], u, p.out_bf16, col, row0);
-            }
-#pragma unroll
-            for (int i = 0; i < 32; ++i) u[i] *= g[i] * sigmoid_f(g[i]);
-            box.put16(&q.out[0], u, p.out_bf16, col, row0);
-        }
-    } else if constexpr (kEpi == kTrainGateGrad) {
-#pragma unroll 1
-        for (int c = 0; c < q.tile_n; c += 32) {
-            const int col = tn * q.tile_n + c;
-            if (col >= q.n) break;
-            float g[32], u[32], v[32];
-            const int avail = in_rows ? q.n - col : 0;
-            load_row32(p.gate, row * p.ld_saved + col, avail, p.in_bf16, g);
-            load_row32(p.up, row * p.ld_saved + col, avail, p.in_bf16, u);
-            tmem_ld32(t + c, v);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const float s = sigmoid_f(g[i]);
-                const float silu = g[i] * s;
-                // silu' = s (1 + g (1 - s)) = s + silu (1 - s)
-                g[i] = v[i] * u[i] * fmaf(silu, 1.f - s, s);
-                u[i] = v[i] * silu;
-            }
-            box.put16(&q.out[0], g, p.out_bf16, col, row0);
-            box.put16(&q.out[1], u, p.out_bf16, col, row0);
-        }
-    } else if constexpr (kEpi == kTrainLse) {
-        // Running maximum and sum over the tile's columns of this thread's row.
-        const long long want = in_rows ? p.target[row] - p.col_base : -1;
-        float top = __int_as_float(0xff800000), sum = 0.f;
-#pragma unroll 1
-        for (int c = 0; c < q.tile_n; c += 32) {
-            const int col = tn * q.tile_n + c;
-            if (col >= q.n) break;
-            float v[32];
-            tmem_ld32(t + c, v);
-            if (want >= col && want < col + 32) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (col + i == want && want < q.n) p.target_logit[row] = v[i];
-            }
-            if (col + 32 > q.n) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (col + i >= q.n) v[i] = __int_as_float(0xff800000);
-            }
-            float best = v[0];
-#pragma unroll
-            for (int i = 1; i < 32; ++i) best = fmaxf(best, v[i]);
-            best = fmaxf(best, top);
-            // No column above -inf yet: subtract 0, so that exp gives 0, not NaN.
-            const float ref = best == __int_as_float(0xff800000) ? 0.f : best;
-            float part = 0.f;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) part += exp2_fast((v[i] - ref) * kLog2e);
-            sum = fmaf(sum, exp2_fast((top - ref) * kLog2e), part);
-            top = best;
-        }
-        if (in_rows) p.partial[static_cast<long long>(tn) * q.m + row] = make_float2(top, sum);
-    } else {
-        const long long want = in_rows ? p.target[row] - p.col_base : -1;
-        const float scale = in_rows ? p.row_scale[row] : 0.f;
-        const float lse = in_rows ? p.lse[row] : 0.f;
-#pragma unroll 1
-        for (int c = 0; c < q.tile_n; c += 32) {
-            const int col = tn * q.tile_n + c;
-            if (col >= q.n) break;
-            float v[32];
-            tmem_ld32(t + c, v);
-            // A row without a target has factor 0 and gradient 0, whatever its logits.
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = scale == 0.f ? 0.f : exp2_fast((v[i] - lse) * kLog2e) * scale;
-            if (want >= col && want < col + 32) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (col + i == want) v[i] -= scale;
-            }
-            box.put16(&q.out[0], v, p.out_bf16, col, row0);
+struct TrainEpilogue {
+    const TrainParams& p;
+    const TrainProblem& q;
+    int row0, row, tn, width, first;   // width: output columns of the tile
+    bool in_rows;
+    Row32 x, y;
+
+    __device__ TrainEpilogue(const TrainParams& p_, const TrainProblem& q_, int row0_, int lane, int tn_, int group)
+        : p(p_), q(q_), row0(row0_), row(row0_ + lane), tn(tn_),
+          width(kEpi == kTrainGate ? q_.tile_n / 2 : q_.tile_n), first(32 * group), in_rows(row0_ + lane < q_.m) {}
+
+    __device__ __forceinline__ void fetch(int c, Row32& a, Row32& b) const {
+        const int col = tn * width + c;
+        const int avail = in_rows && c < width ? q.n - col : 0;
+        if constexpr (kEpi == kTrainStore) {
+            if (q.beta != 0.f) a.load(q.c, row * q.ldc + col, avail);
+        } else if constexpr (kEpi == kTrainGateGrad) {
+            a.load(p.gate, row * p.ld_saved + col, avail);
+            b.load(p.up, row * p.ld_saved + col, avail);
         }
     }
-}
+    // The rows of the saved pre-activations come from DRAM: one 128-byte line
+    // per row and 64 columns into L2 while the tile is still multiplied, or each
+    // group's loads would wait for memory in turn.
+    __device__ void begin() {
+        if constexpr (kEpi == kTrainGateGrad) {
+            const void* src = first == 0 ? p.gate : p.up;
+            for (int c = 0; c < width && in_rows && tn * width + c < q.n; c += 64)
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint16_t*>(src) + row * p.ld_saved + tn * width + c));
+        }
+        fetch(first, x, y);
+    }
+
+    // t: TMEM address of the accumulator, this warp's lane quarter.
+    __device__ void run(BoxWriter& box, uint32_t t) {
+        if (row0 >= q.m) return;
+        const float kNone = __int_as_float(0xff800000);
+        float alpha = 0.f, top = kNone, sum = 0.f, scale = 0.f, lse = 0.f;
+        long long want = -1;
+        if constexpr (kEpi == kTrainStore) alpha = q.alpha_ptr != nullptr ? q.alpha * __ldg(q.alpha_ptr) : q.alpha;
+        if constexpr (kEpi == kTrainLse || kEpi == kTrainLogitGrad)
+            if (in_rows) want = p.target[row] - p.col_base;
+        if constexpr (kEpi == kTrainLogitGrad)
+            if (in_rows) {
+                scale = p.row_scale[row];
+                lse = p.lse[row];
+            }
+#pragma unroll 1
+        for (int c = first; c < width; c += 64) {
+            const int col = tn * width + c;
+            if (col >= q.n) break;
+            Row32 nx, ny;
+            fetch(c + 64, nx, ny);
+            float v[32];
+            tmem_ld32(t + c, v);
+            if constexpr (kEpi == kTrainStore) {
+                if (q.out_kind != kTrainOut16) {
+                    box.put32(&q.out[0], v, q.out_kind == kTrainOutF32Add, col, row0);
+                    continue;
+                }
+                if (q.beta != 0.f) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 w = x.pair(i, p.in_bf16);
+                        v[2 * i] = fmaf(alpha, v[2 * i], q.beta * w.x);
+                        v[2 * i + 1] = fmaf(alpha, v[2 * i + 1], q.beta * w.y);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] *= alpha;
+                }
+                box.put16(&q.out[0], v, p.out_bf16, col, row0);
+            } else if constexpr (kEpi == kTrainGate) {
+                float u[32];
+                tmem_ld32(t + width + c, u);
+                if (p.keep) {
+                    box.put16(&q.out[1], v, p.out_bf16, col, row0);
+                    box.put16(&q.out[2], u, p.out_bf16, col, row0);
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) u[i] *= v[i] * sigmoid_f(v[i]);
+                box.put16(&q.out[0], u, p.out_bf16, col, row0);
+            } else if constexpr (kEpi == kTrainGateGrad) {
+                float du[32];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float2 g = x.pair(i, p.in_bf16), u = y.pair(i, p.in_bf16);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float gj = j ? g.y : g.x, uj = j ? u.y : u.x, dh = v[2 * i + j];
+                        const float s = sigmoid_f(gj), silu = gj * s;
+                        // silu' = s (1 + g (1 - s)) = s + silu (1 - s)
+                        v[2 * i + j] = dh * uj * fmaf(silu, 1.f - s, s);
+                        du[2 * i + j] = dh * silu;
+                    }
+                }
+                box.put16(&q.out[0], v, p.out_bf16, col, row0);
+                box.put16(&q.out[1], du, p.out_bf16, col, row0);
+            } else if constexpr (kEpi == kTrainLse) {
+                // Running maximum and sum over this thread's columns of the tile.
+                if (want >= col && want < col + 32 && want < q.n) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (col + i == want) p.target_logit[row] = v[i];
+                }
+                if (col + 32 > q.n) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (col + i >= q.n) v[i] = kNone;
+                }
+                float best = v[0];
+#pragma unroll
+                for (int i = 1; i < 32; ++i) best = fmaxf(best, v[i]);
+                best = fmaxf(best, top);
+                // No column above -inf yet: subtract 0, so that exp gives 0, not NaN.
+                const float ref = best == kNone ? 0.f : best;
+                float part = 0.f;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) part += exp2_fast((v[i] - ref) * kLog2e);
+                sum = fmaf(sum, exp2_fast((top - ref) * kLog2e), part);
+                top = best;
+            } else {
+                // A row without a target has factor 0 and gradient 0, whatever its logits.
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = scale == 0.f ? 0.f : exp2_fast((v[i] - lse) * kLog2e) * scale;
+                if (want >= col && want < col + 32) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (col + i == want) v[i] -= scale;
+                }
+                box.put16(&q.out[0], v, p.out_bf16, col, row0);
+            }
+            x = nx;
+            y = ny;
+        }
+        if constexpr (kEpi == kTrainLse)
+            if (in_rows) p.partial[static_cast<long long>(2 * tn + first / 32) * q.m + row] = make_float2(top, sum);
+    }
+};
 
 // ------------------------------------------------------------------ the GEMM ---
 
@@ -419,7 +444,7 @@ struct Is {
 enum : int { kBKMajor = 0, kBMnMajor = 1, kBTwoHalves = 2 };
 
 template <bool kPair, int kEpi>
-__global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_constant__ TrainParams p) {
+__global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __grid_constant__ TrainParams p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align_1024(smem_raw);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + kTrainDataBytes);   // pair: the even CTA's
@@ -437,14 +462,14 @@ __global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_co
     const uint32_t rank = kPair ? cluster_ctarank() : 0u;
     const bool leader = rank == 0;
 
-    if (warp == 4 && lane == 0) {
+    if (warp == kTrainEpiWarps && lane == 0) {
         for (int s = 0; s < p.stages; ++s) {
             mbar_init(&full[s], 1u);
             mbar_init(&empty[s], 1u);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&tfull[i], 1u);
-            mbar_init(&tempty[i], kPair ? 8u : 4u);   // one lane of each epilogue warp
+            mbar_init(&tempty[i], (kPair ? 2u : 1u) * kTrainEpiWarps);   // one lane of each epilogue warp
         }
         mbar_init(drain, 1u);
         *abort_flag = 0;
@@ -454,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_co
         if constexpr (kEpi == kTrainGate) tma_prefetch_map(&p.prob[0].b[1]);
         if constexpr (kEpi != kTrainLse) tma_prefetch_map(&p.prob[0].out[0]);
     }
-    if (warp == 5) {
+    if (warp == kTrainEpiWarps + 1) {
         if constexpr (kPair) {
             tmem_alloc_pair(tmem_slot, 2 * kTrainAccCols);
             tmem_relinquish_pair();
@@ -481,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_co
     const uint32_t stage_bytes = static_cast<uint32_t>(sub) * block_stride;
     const uint32_t ring = smem_addr(smem);
 
-    if (warp == 4) {
+    if (warp == kTrainEpiWarps) {
         if (lane == 0) {
             uint32_t stage = 0, phase = 0, issued = 0;
             bool ok = true;
@@ -577,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_co
                 }
             }
         }
-    } else if (warp == 5) {
+    } else if (warp == kTrainEpiWarps + 1) {
         if (leader) {
             // The whole warp walks the loop and one elected lane issues: with
             // warp-uniform control flow the descriptors stay in uniform
@@ -633,17 +658,19 @@ __global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_co
     } else {
         const uint32_t tempty0 = kPair ? map_to_rank(smem_addr(&tempty[0]), 0) : 0u;
         const uint32_t tempty1 = kPair ? map_to_rank(smem_addr(&tempty[1]), 0) : 0u;
-        BoxWriter box{smem + kTrainRingBytes + warp * 4u * kTrainBoxBytes, 0u, lane};
+        BoxWriter box{smem + kTrainRingBytes + warp * 2u * kTrainBoxBytes, 0u, lane};
+        const int quarter = static_cast<int>(warp & 3u), group = static_cast<int>(warp >> 2);
         uint32_t iter = 0;
         while (it.next(p, prob, tm, tn, nth)) {
-            const TrainProblem& q = p.prob[prob];
             const uint32_t acc = iter & 1u, acc_phase = (iter >> 1) & 1u;
             ++iter;
+            const int row0 = tm * kTileM + static_cast<int>(rank) * 128 + quarter * 32;
+            TrainEpilogue<kEpi> epi(p, p.prob[prob], row0, static_cast<int>(lane), tn, group);
+            epi.begin();
             const bool got = kPair ? mbar_wait_cluster(&tfull[acc], acc_phase, wc) : mbar_wait(&tfull[acc], acc_phase, wc);
             if (!__all_sync(0xffffffffu, got)) break;
             tc_fence_after_sync();
-            const int row0 = tm * kTileM + static_cast<int>(rank) * 128 + static_cast<int>(warp) * 32;
-            train_epilogue<kEpi>(p, q, box, tmem_base + ((warp * 32u) << 16) + acc * kTrainAccCols, row0, tn);
+            epi.run(box, tmem_base + ((quarter * 32u) << 16) + acc * kTrainAccCols);
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) {
@@ -659,7 +686,7 @@ __global__ void __launch_bounds__(kThreads, 1) train_gemm_kernel(const __grid_co
     tc_fence_before_sync();
     if constexpr (kPair) cluster_sync();               // no CTA leaves while its pair may still touch it
     else __syncthreads();
-    if (warp == 5) {
+    if (warp == kTrainEpiWarps + 1) {
         tc_fence_after_sync();
         if constexpr (kPair) tmem_dealloc_pair(tmem_base, 2 * kTrainAccCols);
         else tmem_dealloc(tmem_base, 2 * kTrainAccCols);
@@ -829,7 +856,29 @@ __global__ void __launch_bounds__(256) scale_round_kernel(const float4* __restri
 // leaves room on both sides.
 constexpr float kOrthScale = 256.f;
 
-// Sums of squares of matrix blockIdx.y, in 64 bits: sums[matrix][block].
+// Eight elements of a row from column c on, zero from `cols` on. kVec: rows are
+// 16-byte aligned and whole vectors.
+template <bool kVec>
+__device__ __forceinline__ void orth_load8(const void* g, long long row, int c, int cols, int bf16, float (&v)[8]) {
+    if constexpr (kVec) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(g) + row + c));
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack2(u[j], bf16);
+            v[2 * j] = f.x;
+            v[2 * j + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? to_f32(g, row + c + j, bf16) : 0.f;
+    }
+}
+
+// Sums of squares of matrix blockIdx.y: sums[matrix][block]. Eight squares are
+// added in FP32 after dividing by their largest power of two, everything above
+// in 64 bits, so that no size of element overflows or is lost. One pass over g.
+template <bool kVec>
 __global__ void __launch_bounds__(256) orth_square_kernel(const void* __restrict__ g, long long batch_stride, int rows,
                                                           int cols, long long ld, int bf16,
                                                           double* __restrict__ sums) {
@@ -837,12 +886,26 @@ __global__ void __launch_bounds__(256) orth_square_kernel(const void* __restrict
     grid_dependents_launch();
     grid_dependency_wait();
     const long long base = blockIdx.y * batch_stride;
+    const int groups = (cols + 7) / 8;
+    const long long total = static_cast<long long>(rows) * groups, stride = static_cast<long long>(gridDim.x) * 256;
     double s = 0.;
-    for (int r = blockIdx.x; r < rows; r += gridDim.x)
-        for (int c = threadIdx.x; c < cols; c += 256) {
-            const double v = static_cast<double>(to_f32(g, base + r * ld + c, bf16));
-            s += v * v;
-        }
+#pragma unroll 4
+    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total; i += stride) {
+        const long long r = i / groups;
+        float v[8];
+        orth_load8<kVec>(g, base + r * ld, static_cast<int>(i - r * groups) * 8, cols, bf16, v);
+        float top = 0.f, sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
+        // 2^-e of the largest element (its mantissa cleared); 1 for zeros, infinities and NaN.
+        const uint32_t e = __float_as_uint(top) & 0x7f800000u;
+        const bool plain = e >= 0x01000000u && e < 0x7e800000u;
+        const float down = plain ? __uint_as_float(0x7f000000u - e) : 1.f;
+        const double up = plain ? static_cast<double>(__uint_as_float(e)) : 1.;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = fmaf(v[j] * down, v[j] * down, sum);
+        s += static_cast<double>(sum) * up * up;
+    }
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
     __syncthreads();
@@ -852,7 +915,8 @@ __global__ void __launch_bounds__(256) orth_square_kernel(const void* __restrict
     }
 }
 
-// x = FP16(g kOrthScale / (norm + eps)), rows padded to ld_x columns.
+// x = FP16(g kOrthScale / (norm + eps)), rows padded to ld_x (a multiple of 8) columns.
+template <bool kVec>
 __global__ void __launch_bounds__(256) orth_scale_kernel(const void* __restrict__ g, long long batch_stride, int rows,
                                                          int cols, long long ld, int bf16,
                                                          const double* __restrict__ sums, int num_sums, double eps,
@@ -870,9 +934,21 @@ __global__ void __launch_bounds__(256) orth_scale_kernel(const void* __restrict_
     const float f = factor;
     const long long base = blockIdx.y * batch_stride;
     __half* dst = x + blockIdx.y * x_stride;
-    for (int r = blockIdx.x; r < rows; r += gridDim.x)
-        for (int c = threadIdx.x; c < cols; c += 256)
-            dst[r * ld_x + c] = __float2half_rn(to_f32(g, base + r * ld + c, bf16) * f);
+    const int groups = (cols + 7) / 8;
+    const long long total = static_cast<long long>(rows) * groups, stride = static_cast<long long>(gridDim.x) * 256;
+#pragma unroll 2
+    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total; i += stride) {
+        const long long r = i / groups;
+        const int c = static_cast<int>(i - r * groups) * 8;
+        float v[8];
+        orth_load8<kVec>(g, base + r * ld, c, cols, bf16, v);
+        uint4 w;
+        w.x = pack2(v[0] * f, v[1] * f, 0);
+        w.y = pack2(v[2] * f, v[3] * f, 0);
+        w.z = pack2(v[4] * f, v[5] * f, 0);
+        w.w = pack2(v[6] * f, v[7] * f, 0);
+        *reinterpret_cast<uint4*>(dst + r * ld_x + c) = w;
+    }
 }
 
 // out[r, c] = scale src[r, c], for outputs whose rows TMA cannot store to (scale

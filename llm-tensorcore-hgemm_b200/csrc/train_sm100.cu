@@ -173,25 +173,30 @@ struct Product {
     int64_t kblocks() const { return cdiv(k0, kBlockK) + cdiv(k1, kBlockK); }
 };
 
-// Time of a problem's tiles in clock cycles, for comparing tiles of one
-// problem. A K block of 64 costs an SM 4 MMAs of max(46, tile_n / 2) cycles
-// and a hand-off that narrow tiles do not hide, and at least what its TMA
-// loads take; a tile adds its epilogue's last columns, a launch its fill.
+// Cycles of one K block of 64 by tile, measured with every SM at work
+// (2560 x 2560 x 9728 and 2560 x 9728 x 2560): a 256-wide pair tile comes near
+// its MMAs' 512, narrow tiles meet the hand-off of a stage.
+double block_cycles(bool pair, int tile_n) {
+    static const double kSingle[4] = {310, 440, 560, 650}, kPairs[4] = {305, 335, 470, 595};
+    return (pair ? kPairs : kSingle)[tile_n / 64 - 1];
+}
+
+// Time of a product's tiles in clock cycles, for comparing tiles of one
+// product: waves of main loops, a change of tile each, the launch and the last
+// tile's epilogue.
 double tile_cost(const Product& p, bool pair, int tile_n, int sms) {
     const int64_t cols = p.dual ? tile_n / 2 : tile_n;
     const int64_t tiles = cdiv(p.m, pair ? 256 : 128) * cdiv(p.n, cols);
     const int64_t units = pair ? sms / 2 : sms;
-    const double block = std::max(4.0 * std::max(46.0, tile_n / 2.0) + (pair ? 40.0 : 90.0), pair ? 400.0 : 420.0);
     const double waves = static_cast<double>(cdiv(tiles, units));
-    return waves * (p.kblocks() * block + 300.0) + 3000.0 + 12.0 * tile_n;
+    return waves * (p.kblocks() * block_cycles(pair, tile_n) + 600.0) + (pair ? 10000.0 : 8500.0) + 16.0 * tile_n;
 }
 
-Tile choose_tile(const Product& p, int sms, int32_t forced, int only_pair = -1) {
+Tile choose_tile(const Product& p, int sms, int32_t forced) {
     if (forced != 0) return {(forced & HGEMM_SM100_TRAIN_TILE_PAIR) != 0, forced & 0xfff};
     Tile best;
     double cost = 0;
     for (int pair = 1; pair >= 0; --pair) {
-        if (only_pair >= 0 && pair != only_pair) continue;
         for (int n = 256; n >= 64; n -= 64) {
             const double c = tile_cost(p, pair != 0, n, sms);
             if (best.n == 0 || c < cost) {
@@ -201,6 +206,32 @@ Tile choose_tile(const Product& p, int sms, int32_t forced, int only_pair = -1) 
         }
     }
     return best;
+}
+
+// One launch of several products: all tiles pairs or none. Its units take the
+// tiles one after the other, so what counts is the whole work over all units,
+// plus the part of a last tile that some wait for; and the longest tile.
+void choose_tiles(const Product* s, int count, Tile* out, int sms, int32_t forced) {
+    double best = -1;
+    for (int pair = 1; pair >= 0; --pair) {
+        for (int n = 256; n >= 64; n -= 64) {
+            const Tile t = forced != 0 ? choose_tile(s[0], sms, forced) : Tile{pair != 0, n};
+            double work = 0, longest = 0, last = 0;
+            for (int i = 0; i < count; ++i) {
+                const double one = s[i].kblocks() * block_cycles(t.pair, t.n) + 600.0 + 4.0 * t.n;
+                work += one * static_cast<double>(cdiv(s[i].m, t.pair ? 256 : 128) * cdiv(s[i].n, t.n));
+                longest = std::max(longest, one);
+                last = one;
+            }
+            const double cost = std::max(longest, work / (t.pair ? sms / 2 : sms) + 0.5 * last) +
+                                (t.pair ? 10000.0 : 8500.0) + 16.0 * t.n;
+            if (best < 0 || cost < best) {
+                best = cost;
+                for (int i = 0; i < count; ++i) out[i] = t;
+            }
+            if (forced != 0) return;
+        }
+    }
 }
 
 // Raster group height: the tallest of 8, 16, 32 tile rows whose one-wave
@@ -251,8 +282,6 @@ void init_params(TrainParams& p, const Context& c) {
 
 // Fills the problems of `p` from `count` products (the first one with the most
 // K blocks) and launches them as one grid.
-int g_sub = getenv("TSUB") ? atoi(getenv("TSUB")) : 0;
-
 int run_products(TrainParams& p, int epi, const Product* products, const Tile* tiles, int count, const Context& c) {
     const bool pair = tiles[0].pair;
     const int units = pair ? c.dev->sms / 2 : c.dev->sms;
@@ -316,7 +345,9 @@ int run_products(TrainParams& p, int epi, const Product* products, const Tile* t
         p.light_skip = static_cast<int>(ratio + 0.5);
     }
     p.block_stride = block_stride;
-    p.sub = g_sub ? g_sub : (kTrainRingBytes / (2 * block_stride) >= 3 ? 2 : 1);
+    // Two K blocks to a stage where three stages fit: the hand-off of a stage
+    // costs about 280 cycles whatever the tile's width.
+    p.sub = kTrainRingBytes / (2 * block_stride) >= 3 ? 2 : 1;
     p.stages = static_cast<int>(std::min<uint32_t>(kTrainRingBytes / (p.sub * block_stride), kTrainMaxStages));
 
     KernelEntry& k = g_kernels[pair ? 1 : 0][epi];
@@ -327,7 +358,7 @@ int run_products(TrainParams& p, int epi, const Product* products, const Tile* t
             return HGEMM_SM100_ERR_LAUNCH;
         k.ready.fetch_or(bit, std::memory_order_acq_rel);
     }
-    return launch(k.fn, dim3(static_cast<unsigned>(grid_units * (pair ? 2 : 1))), dim3(kThreads), kTrainSmemBytes,
+    return launch(k.fn, dim3(static_cast<unsigned>(grid_units * (pair ? 2 : 1))), dim3(kTrainThreads), kTrainSmemBytes,
                   pair ? 2 : 1, c.stream, p);
 }
 
@@ -454,17 +485,7 @@ extern "C" int hgemm_sm100_ffn_backward(const HgemmSm100FfnBackward* a, void* st
     // The problem with the most K blocks goes first.
     std::stable_sort(s, s + n, [](const Product& x, const Product& y) { return x.kblocks() > y.kblocks(); });
     Tile t[4];
-    t[0] = choose_tile(s[0], c.dev->sms, c.common.tile);
-    // All of a launch's tiles are pairs or none: what the costlier set of products takes.
-    double cost[2] = {0, 0};
-    Tile by[2][4];
-    for (int pair = 0; pair < 2; ++pair)
-        for (int i = 0; i < n; ++i) {
-            by[pair][i] = choose_tile(s[i], c.dev->sms, c.common.tile, pair);
-            cost[pair] += tile_cost(s[i], pair != 0, by[pair][i].n, c.dev->sms);
-        }
-    const int pair = c.common.tile != 0 ? (t[0].pair ? 1 : 0) : (cost[1] <= cost[0] ? 1 : 0);
-    for (int i = 0; i < n; ++i) t[i] = by[pair][i];
+    choose_tiles(s, n, t, c.dev->sms, c.common.tile);
     init_params(p, c);
     return run_products(p, kTrainStore, s, t, n, c);
 }
@@ -476,7 +497,7 @@ namespace {
 struct LossForwardPlan {
     Product z;
     Tile tile;
-    int64_t tiles_n = 0;
+    int64_t parts = 0;
     size_t partial_bytes = 0, row_bytes = 0;
     size_t bytes() const { return partial_bytes + 2 * row_bytes; }
 };
@@ -489,8 +510,8 @@ LossForwardPlan plan_loss_forward(const HgemmSm100LossForward& a, int sms) {
     q.z.a0 = {a.x, a.ldx, false};
     q.z.b0 = {a.weight, a.hidden, false};
     q.tile = choose_tile(q.z, sms, a.common.tile);
-    q.tiles_n = cdiv(a.vocab, q.tile.n);
-    q.partial_bytes = static_cast<size_t>(round_up(q.tiles_n * a.tokens * 8, 256));
+    q.parts = 2 * cdiv(a.vocab, q.tile.n);   // two column groups a tile
+    q.partial_bytes = static_cast<size_t>(round_up(q.parts * a.tokens * 8, 256));
     q.row_bytes = static_cast<size_t>(round_up(a.tokens * 4, 256));
     return q;
 }
@@ -561,7 +582,7 @@ extern "C" int hgemm_sm100_loss_forward(const HgemmSm100LossForward* a, void* st
     p.target_logit = target_logit;
     if ((rc = run_products(p, kTrainLse, &q.z, &q.tile, 1, c)) != HGEMM_SM100_OK) return rc;
     rc = launch(&lse_join_kernel, dim3(static_cast<unsigned>(cdiv(m, 32))), dim3(32, 32), 0, 1, c.stream, partial,
-                static_cast<int>(q.tiles_n), m, target_logit, target, static_cast<long long>(a->vocab),
+                static_cast<int>(q.parts), m, target_logit, target, static_cast<long long>(a->vocab),
                 static_cast<long long>(a->ignore_index), a->lse, loss);
     if (rc != HGEMM_SM100_OK || a->reduction == HGEMM_SM100_LOSS_NONE) return rc;
     return launch(&loss_reduce_kernel, dim3(1), dim3(1024), 0, 1, c.stream, rows, target, m,
@@ -645,17 +666,10 @@ extern "C" int hgemm_sm100_loss_backward(const HgemmSm100LossBackward* a, void* 
             d.alpha_ptr = alpha;
         }
         if (n == 2 && s[1].kblocks() > s[0].kblocks()) std::swap(s[0], s[1]);
-        Tile by[2][2];
-        double cost[2] = {0, 0};
-        for (int pair = 0; pair < 2; ++pair)
-            for (int j = 0; j < n; ++j) {
-                by[pair][j] = choose_tile(s[j], c.dev->sms, c.common.tile, pair);
-                cost[pair] += tile_cost(s[j], pair != 0, by[pair][j].n, c.dev->sms);
-            }
-        const int pair = c.common.tile != 0 ? ((c.common.tile & HGEMM_SM100_TRAIN_TILE_PAIR) ? 1 : 0)
-                                            : (cost[1] <= cost[0] ? 1 : 0);
+        Tile t[2];
+        choose_tiles(s, n, t, c.dev->sms, c.common.tile);
         init_params(p, c);
-        if ((rc = run_products(p, kTrainStore, s, by[pair], n, c)) != HGEMM_SM100_OK) return rc;
+        if ((rc = run_products(p, kTrainStore, s, t, n, c)) != HGEMM_SM100_OK) return rc;
     }
     if (a->dx != nullptr && q.pieces > 1) {
         const int64_t vecs = a->tokens * a->hidden / 8;
@@ -671,7 +685,7 @@ extern "C" int hgemm_sm100_loss_backward(const HgemmSm100LossBackward* a, void* 
 
 namespace {
 
-constexpr int kOrthSums = 148;   // partial sums of squares per matrix
+constexpr int kOrthSums = 592;   // partial sums of squares per matrix, at most
 
 struct OrthPlan {
     bool tall = false;
@@ -722,16 +736,20 @@ extern "C" int hgemm_sm100_orthogonalize(const HgemmSm100Orthogonalize* a, void*
     uint16_t* poly = reinterpret_cast<uint16_t*>(ws + q.sum_bytes + 2 * q.x_bytes + q.side_bytes);
     const int bf16 = a->common.dtype == HGEMM_SM100_TRAIN_BF16 ? 1 : 0;
     const int rows = static_cast<int>(a->rows), cols = static_cast<int>(a->cols);
-    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(a->rows, kOrthSums));
+    // A block per 2048 elements, several waves of blocks at most.
+    const unsigned blocks =
+        static_cast<unsigned>(std::min<int64_t>(cdiv(a->rows * cdiv(a->cols, 8), 256), kOrthSums));
     const unsigned batch = static_cast<unsigned>(a->batch);
 
-    rc = launch(&orth_square_kernel, dim3(blocks, batch), dim3(256), 0, 1, c.stream, a->g,
-                static_cast<long long>(a->batch_stride), rows, cols, static_cast<long long>(a->ldg), bf16, sums);
+    const bool vec = aligned16(a->g) && a->cols % 8 == 0 && a->ldg % 8 == 0 && a->batch_stride % 8 == 0;
+    rc = launch(vec ? &orth_square_kernel<true> : &orth_square_kernel<false>, dim3(blocks, batch), dim3(256), 0, 1,
+                c.stream, a->g, static_cast<long long>(a->batch_stride), rows, cols, static_cast<long long>(a->ldg),
+                bf16, sums);
     if (rc != HGEMM_SM100_OK) return rc;
-    rc = launch(&orth_scale_kernel, dim3(static_cast<unsigned>(std::min<int64_t>(a->rows, 65535)), batch), dim3(256), 0,
-                1, c.stream, a->g, static_cast<long long>(a->batch_stride), rows, cols,
-                static_cast<long long>(a->ldg), bf16, sums, static_cast<int>(blocks), a->eps,
-                reinterpret_cast<__half*>(x), static_cast<long long>(q.ld), static_cast<long long>(q.x_stride));
+    rc = launch(vec ? &orth_scale_kernel<true> : &orth_scale_kernel<false>, dim3(2 * blocks, batch), dim3(256), 0, 1,
+                c.stream, a->g, static_cast<long long>(a->batch_stride), rows, cols, static_cast<long long>(a->ldg),
+                bf16, sums, static_cast<int>(blocks), a->eps, reinterpret_cast<__half*>(x),
+                static_cast<long long>(q.ld), static_cast<long long>(q.x_stride));
     if (rc != HGEMM_SM100_OK) return rc;
 
     // The last step writes the result itself where TMA can store it.
@@ -744,9 +762,8 @@ extern "C" int hgemm_sm100_orthogonalize(const HgemmSm100Orthogonalize* a, void*
             Tile t[kTrainMaxProblems];
             const int n = static_cast<int>(std::min<int64_t>(kTrainMaxProblems, a->batch - first));
             for (int i = 0; i < n; ++i) make(s[i], first + i);
-            Product all = s[0];
-            all.m = round_up(all.m, 256) * n;   // the launch's tiles, for the choice of the tile
-            for (int i = 0; i < n; ++i) t[i] = choose_tile(n > 1 ? all : s[0], c.dev->sms, c.common.tile);
+            if (n > 1) choose_tiles(s, n, t, c.dev->sms, c.common.tile);
+            else t[0] = choose_tile(s[0], c.dev->sms, c.common.tile);
             init_params(p, c);
             p.in_bf16 = 0;
             p.out_bf16 = out_bf16;
