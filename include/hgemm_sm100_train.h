@@ -33,13 +33,15 @@ enum { HGEMM_SM100_TRAIN_F16 = 0, HGEMM_SM100_TRAIN_BF16 = 1 };
 
 /* Common part of every call. `tile` forces the tile of all products: 0 = the
  * library chooses; else columns (a multiple of 64 up to 256), plus
- * HGEMM_SM100_TRAIN_TILE_PAIR for CTA pairs (256 rows instead of 128). */
+ * HGEMM_SM100_TRAIN_TILE_PAIR for CTA pairs (256 rows instead of 128).
+ * `splits` forces into how many parts the long sums (y, dx) are cut: 0 = the
+ * library chooses, at most 16. Workspace queries take both into account. */
 #define HGEMM_SM100_TRAIN_TILE_PAIR 0x1000
 typedef struct HgemmSm100TrainCommon {
     int32_t dtype;        /* HGEMM_SM100_TRAIN_F16 / _BF16                     */
     int32_t tile;         /* 0 = choose                                       */
     int32_t flags;        /* 0, or HGEMM_SM100_FLAG_TEST_INJECT_TX (tests)    */
-    int32_t reserved;     /* 0                                                */
+    int32_t splits;       /* 0 = choose                                       */
     int32_t* status;      /* device int32 set when a kernel wait runs out; NULL
                              = the library's own word                         */
     uint64_t timeout_ns;  /* per-wait limit inside the kernels; 0 = 2 s       */
@@ -57,8 +59,11 @@ typedef struct HgemmSm100FfnForward {
     void* h;               /* [tokens x inter]                                */
     void* gate_pre;        /* [tokens x inter] or NULL                        */
     void* up_pre;          /* [tokens x inter] or NULL                        */
+    void* workspace;       /* hgemm_sm100_ffn_forward_workspace bytes (may be 0) */
+    uint64_t workspace_bytes;
     int64_t tokens, hidden, inter, out, ldx;
 } HgemmSm100FfnForward;
+size_t hgemm_sm100_ffn_forward_workspace(const HgemmSm100FfnForward* args);
 int hgemm_sm100_ffn_forward(const HgemmSm100FfnForward* args, void* stream);
 
 /* Its gradient. dh = dy Wd, du = dh silu(g), dg = dh u silu'(g) (rounded to the
@@ -80,8 +85,11 @@ typedef struct HgemmSm100FfnBackward {
     void* dgate;           /* [inter x hidden] or NULL                        */
     void* dup;             /* [inter x hidden] or NULL                        */
     void* ddown;           /* [out x inter] or NULL                           */
+    void* workspace;       /* hgemm_sm100_ffn_backward_workspace bytes (may be 0) */
+    uint64_t workspace_bytes;
     int64_t tokens, hidden, inter, out, ldx, lddy;
 } HgemmSm100FfnBackward;
+size_t hgemm_sm100_ffn_backward_workspace(const HgemmSm100FfnBackward* args);
 int hgemm_sm100_ffn_backward(const HgemmSm100FfnBackward* args, void* stream);
 
 /* Softmax cross entropy of logits z = x W^T that are never stored.

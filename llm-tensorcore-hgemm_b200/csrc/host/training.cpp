@@ -120,6 +120,11 @@ FfnForward ffn_forward(const Tensor& x, const Tensor& gate, const Tensor& up, co
     a.inter = s.inter8;
     a.out = s.out8;
     a.ldx = xp.stride(0);
+    Tensor ws;
+    if ((a.workspace_bytes = hgemm_sm100_ffn_forward_workspace(&a)) > 0) {
+        ws = bytes(a.workspace_bytes, x);
+        a.workspace = ws.data_ptr();
+    }
     check_status(hgemm_sm100_ffn_forward(&a, c10::cuda::getCurrentCUDAStream(x.get_device()).stream()), "gated_ffn");
     return r;
 }
@@ -181,6 +186,11 @@ class GatedFfn : public torch::autograd::Function<GatedFfn> {
         a.out = s.out8;
         a.ldx = xp.stride(0);
         a.lddy = dy.stride(0);
+        Tensor ws;
+        if ((a.workspace_bytes = hgemm_sm100_ffn_backward_workspace(&a)) > 0) {
+            ws = bytes(a.workspace_bytes, x);
+            a.workspace = ws.data_ptr();
+        }
         check_status(hgemm_sm100_ffn_backward(&a, c10::cuda::getCurrentCUDAStream(x.get_device()).stream()),
                      "gated_ffn backward");
         if (need_x) dx = cut(dx, s.tokens, s.hidden).view(x.sizes());

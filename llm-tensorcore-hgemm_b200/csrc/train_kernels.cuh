@@ -14,6 +14,8 @@
 //  * the sum over K may run over two operand pairs (dx = dg Wg + du Wu), and
 //    the columns of B may come from two tensors (gate and up), so no weight is
 //    packed: a training step changes the weights every time;
+//  * the sum over K may be split over several tiles whose FP32 partial sums
+//    sum_round_kernel adds in a fixed order (few rows, long sums);
 //  * one launch takes up to four problems and walks their tiles as one list
 //    (dx, dWgate, dWup and dWdown fill the last wave together);
 //  * the epilogue finishes the operator (SwiGLU, its gradient, softmax
@@ -69,6 +71,9 @@ struct alignas(64) TrainProblem {
     int nkb0, nkb;         // K blocks of the first segment, of both
     int a_mn, b_mn, dual;
     int tiles_m, tiles_n, group_m;
+    int splits, kb_split;  // parts of the sum over K, K blocks of each (the last: the rest)
+    int pad_rows;          // output rows from one part's sums to the next one's
+    uint32_t a_tile_bytes; // what the loads of A bring per K block
     int out_kind;
     float alpha, beta;
     const float* alpha_ptr;    // multiplies alpha (device memory; may be null)
@@ -83,6 +88,7 @@ struct alignas(64) TrainParams {
     int light_skip;                // waves the units with one heavy tile more sit out
     int stages, sub;               // ring stages, K blocks of 64 in each
     uint32_t block_stride;         // bytes of one K block's tiles in a stage
+    uint32_t b_offset;             // where B starts among them
     int in_bf16, out_bf16;
     int* status;
     unsigned long long timeout_ns;
@@ -220,14 +226,17 @@ __device__ __forceinline__ void tmem_ld32(uint32_t t, float (&v)[32]) {
 }
 
 // The tiles of one unit (CTA or pair) in order; every role iterates alike.
-// Problem 0's tiles ("heavy": the longest K) go round robin; where they do
+// Problem 0's tiles ("heavy": the longest sums) go round robin; where they do
 // not divide evenly the units that took one more sit out the first
 // `light_skip` waves of the other problems' tiles, which are shorter.
 struct TileIter {
     int unit, units, next_heavy, wave;
+    int prob, tm, tn;      // the current tile
+    int split, kb0, kb1;   // its part of the sum: K blocks [kb0, kb1)
+    bool back;             // walk K from the end
     __device__ TileIter(int u, int n) : unit(u), units(n), next_heavy(u), wave(0) {}
-    __device__ bool next(const TrainParams& p, int& prob, int& tm, int& tn, int& nth) {
-        int t;
+    __device__ bool next(const TrainParams& p) {
+        int t, nth;
         if (next_heavy < p.heavy_tiles) {
             prob = 0;
             t = next_heavy;
@@ -243,15 +252,27 @@ struct TileIter {
             if (t >= p.light_tiles) return false;
             prob = 1;
             while (true) {
-                const int tiles = p.prob[prob].tiles_m * p.prob[prob].tiles_n;
+                const int tiles = p.prob[prob].tiles_m * p.prob[prob].tiles_n * p.prob[prob].splits;
                 if (t < tiles) break;
                 t -= tiles;
                 ++prob;
             }
         }
         const TrainProblem& q = p.prob[prob];
-        tile_coords(t, q.tiles_m, q.tiles_n, q.group_m, tm, tn);
+        const int plane = q.tiles_m * q.tiles_n;
+        split = q.splits > 1 ? t / plane : 0;
+        tile_coords(t - split * plane, q.tiles_m, q.tiles_n, q.group_m, tm, tn);
+        kb0 = split * q.kb_split;
+        kb1 = min(q.nkb, kb0 + q.kb_split);
+        // Odd waves walk K backwards: they start on the panels that the wave
+        // before read last, while those are in L2.
+        back = (nth & 1) != 0;
         return true;
+    }
+    // K blocks [from, to) of segment 0 or 1 in this part.
+    __device__ void segment(const TrainProblem& q, int seg, int& from, int& to) const {
+        from = seg ? max(kb0 - q.nkb0, 0) : min(kb0, q.nkb0);
+        to = seg ? max(kb1 - q.nkb0, 0) : min(kb1, q.nkb0);
     }
 };
 
@@ -265,12 +286,13 @@ template <int kEpi>
 struct TrainEpilogue {
     const TrainParams& p;
     const TrainProblem& q;
-    int row0, row, tn, width, first;   // width: output columns of the tile
+    int row0, row, tn, out_row, width, first;   // out_row: row0 in the output; width: the tile's output columns
     bool in_rows;
     Row32 x, y;
 
-    __device__ TrainEpilogue(const TrainParams& p_, const TrainProblem& q_, int row0_, int lane, int tn_, int group)
-        : p(p_), q(q_), row0(row0_), row(row0_ + lane), tn(tn_),
+    __device__ TrainEpilogue(const TrainParams& p_, const TrainProblem& q_, int row0_, int lane, int tn_, int split,
+                             int group)
+        : p(p_), q(q_), row0(row0_), row(row0_ + lane), tn(tn_), out_row(row0_ + split * q_.pad_rows),
           width(kEpi == kTrainGate ? q_.tile_n / 2 : q_.tile_n), first(32 * group), in_rows(row0_ + lane < q_.m) {}
 
     __device__ __forceinline__ void fetch(int c, Row32& a, Row32& b) const {
@@ -319,7 +341,7 @@ struct TrainEpilogue {
             tmem_ld32(t + c, v);
             if constexpr (kEpi == kTrainStore) {
                 if (q.out_kind != kTrainOut16) {
-                    box.put32(&q.out[0], v, q.out_kind == kTrainOutF32Add, col, row0);
+                    box.put32(&q.out[0], v, q.out_kind == kTrainOutF32Add, col, out_row);
                     continue;
                 }
                 if (q.beta != 0.f) {
@@ -456,8 +478,7 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     constexpr int kTileM = kPair ? 256 : 128;
-    constexpr uint32_t kABytes = 128u * 128u;    // 128 rows x 64 halves, either way round
-    const uint32_t warp = warp_index();
+        const uint32_t warp = warp_index();
     const uint32_t lane = threadIdx.x & 31u;
     const uint32_t rank = kPair ? cluster_ctarank() : 0u;
     const bool leader = rank == 0;
@@ -499,11 +520,10 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
     const int unit = kPair ? blockIdx.x >> 1 : blockIdx.x;
     const int units = kPair ? gridDim.x >> 1 : gridDim.x;
     TileIter it(unit, units);
-    int prob, tm, tn, nth;
 
     const uint32_t num_stages = static_cast<uint32_t>(p.stages), block_stride = p.block_stride;
     const int sub = p.sub;
-    const uint32_t stage_bytes = static_cast<uint32_t>(sub) * block_stride;
+    const uint32_t stage_bytes = static_cast<uint32_t>(sub) * block_stride, b_offset = p.b_offset;
     const uint32_t ring = smem_addr(smem);
 
     if (warp == kTrainEpiWarps) {
@@ -527,12 +547,12 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
             uint32_t extra = p.inject ? 16u : 0u;
             // The K blocks of one segment, forwards or backwards, two to a stage.
             auto segment = [&](uint64_t ma, uint64_t mb, uint64_t mb2, auto a_mn_c, auto b_kind_c, int row0, int col0,
-                               int chunks, uint32_t half_bytes, uint32_t block_bytes, int blocks, bool back) {
+                               int chunks, uint32_t half_bytes, uint32_t block_bytes, int from, int to, bool back) {
                 constexpr bool a_mn = decltype(a_mn_c)::value;
                 constexpr int b_kind = decltype(b_kind_c)::value;
-                int k = back ? (blocks - 1) * kBlockK : 0;
+                int k = (back ? to - 1 : from) * kBlockK;
                 const int step = back ? -kBlockK : kBlockK;
-                for (int left = blocks; left > 0; left -= sub) {
+                for (int left = to - from; left > 0; left -= sub) {
                     if (!(kPair ? mbar_wait_cluster(&empty[stage], phase ^ 1u, wc)
                                 : mbar_wait(&empty[stage], phase ^ 1u, wc))) return false;
                     const int count = left < sub ? left : sub;
@@ -541,7 +561,7 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
                     const uint32_t bar = full0 + stage * 8u;
                     uint32_t s_a = ring + stage * stage_bytes;
                     for (int i = 0; i < count; ++i, s_a += block_stride, k += step) {
-                        const uint32_t s_b = s_a + kABytes;
+                        const uint32_t s_b = s_a + b_offset;
                         if constexpr (a_mn) {
                             load(s_a, ma, bar, row0, k);
                             load(s_a + kChunkBytes, ma, bar, row0 + 64, k);
@@ -563,34 +583,38 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
                 }
                 return true;
             };
-            while (ok && it.next(p, prob, tm, tn, nth)) {
-                const TrainProblem& q = p.prob[prob];
-                const int row0 = tm * kTileM + static_cast<int>(rank) * 128;
+            while (ok && it.next(p)) {
+                const TrainProblem& q = p.prob[it.prob];
+                const int row0 = it.tm * kTileM + static_cast<int>(rank) * 128;
                 // Columns of B that this CTA loads: all, or its half of the pair's.
                 const int cols = kPair ? q.tile_n / 2 : q.tile_n;
-                const bool dual = kEpi == kTrainGate;
-                const int col0 = dual ? tn * (q.tile_n / 2) : tn * q.tile_n + static_cast<int>(rank) * cols;
+                const bool dual = kEpi == kTrainGate, back = it.back;
+                const int col0 = dual ? it.tn * (q.tile_n / 2) : it.tn * q.tile_n + static_cast<int>(rank) * cols;
                 const int chunks = (cols + 63) / 64;
-                const uint32_t bytes = kABytes + (q.b_mn ? chunks * kChunkBytes : cols * 128u);
-                // Odd waves walk K backwards: they start on the panels that the
-                // wave before read last, while those are in L2.
-                const bool back = (nth & 1) != 0;
+                const uint32_t bytes = q.a_tile_bytes + (q.b_mn ? chunks * kChunkBytes : cols * 128u);
                 for (int i = 0; i < 2 && ok; ++i) {
                     const int seg = back ? 1 - i : i;
-                    const int blocks = seg ? q.nkb - q.nkb0 : q.nkb0;
-                    if (blocks == 0) continue;
+                    int from, to;
+                    it.segment(q, seg, from, to);
+                    if (from >= to) continue;
                     const uint64_t ma = map_of(q.a[seg]), mb = map_of(q.b[seg]);
                     if constexpr (dual) {
                         if constexpr (kPair)
-                            ok = segment(ma, map_of(q.b[rank]), 0ull, Is<0>{}, Is<kBKMajor>{}, row0, col0, chunks, 0u, bytes, blocks, back);
+                            ok = segment(ma, map_of(q.b[rank]), 0ull, Is<0>{}, Is<kBKMajor>{}, row0, col0, chunks, 0u,
+                                         bytes, from, to, back);
                         else
-                            ok = segment(ma, mb, map_of(q.b[1]), Is<0>{}, Is<kBTwoHalves>{}, row0, col0, chunks, cols * 64u, bytes, blocks, back);
+                            ok = segment(ma, mb, map_of(q.b[1]), Is<0>{}, Is<kBTwoHalves>{}, row0, col0, chunks,
+                                         cols * 64u, bytes, from, to, back);
                     } else if (q.a_mn) {
-                        ok = q.b_mn ? segment(ma, mb, 0ull, Is<1>{}, Is<kBMnMajor>{}, row0, col0, chunks, 0u, bytes, blocks, back)
-                                    : segment(ma, mb, 0ull, Is<1>{}, Is<kBKMajor>{}, row0, col0, chunks, 0u, bytes, blocks, back);
+                        ok = q.b_mn ? segment(ma, mb, 0ull, Is<1>{}, Is<kBMnMajor>{}, row0, col0, chunks, 0u, bytes,
+                                              from, to, back)
+                                    : segment(ma, mb, 0ull, Is<1>{}, Is<kBKMajor>{}, row0, col0, chunks, 0u, bytes,
+                                              from, to, back);
                     } else {
-                        ok = q.b_mn ? segment(ma, mb, 0ull, Is<0>{}, Is<kBMnMajor>{}, row0, col0, chunks, 0u, bytes, blocks, back)
-                                    : segment(ma, mb, 0ull, Is<0>{}, Is<kBKMajor>{}, row0, col0, chunks, 0u, bytes, blocks, back);
+                        ok = q.b_mn ? segment(ma, mb, 0ull, Is<0>{}, Is<kBMnMajor>{}, row0, col0, chunks, 0u, bytes,
+                                              from, to, back)
+                                    : segment(ma, mb, 0ull, Is<0>{}, Is<kBKMajor>{}, row0, col0, chunks, 0u, bytes,
+                                              from, to, back);
                     }
                 }
             }
@@ -611,15 +635,15 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
             uint32_t stage = 0, phase = 0, iter = 0;
             bool ok = true;
             const uint32_t format = p.in_bf16 ? (1u << 7) | (1u << 10) : 0u;
-            while (ok && it.next(p, prob, tm, tn, nth)) {
-                const TrainProblem& q = p.prob[prob];
+            while (ok && it.next(p)) {
+                const TrainProblem& q = p.prob[it.prob];
                 const uint32_t idesc = make_idesc_f16(kTileM, 0, q.a_mn, q.b_mn) | format |
                                        (static_cast<uint32_t>(q.tile_n >> 3) << 17);
                 // 16 of K further: 32 bytes along a K-major row, 16 rows of 128 bytes MN-major.
                 const uint64_t step_a = q.a_mn ? 2048u >> 4 : 32u >> 4;
                 const uint64_t step_b = q.b_mn ? 2048u >> 4 : 32u >> 4;
                 const uint64_t desc_a = make_smem_desc(ring, q.a_mn ? kChunkBytes : 16u, 1024u);
-                const uint64_t desc_b = make_smem_desc(ring + kABytes, q.b_mn ? kChunkBytes : 16u, 1024u);
+                const uint64_t desc_b = make_smem_desc(ring + b_offset, q.b_mn ? kChunkBytes : 16u, 1024u);
                 const uint32_t acc = iter & 1u, acc_phase = (iter >> 1) & 1u;
                 ++iter;
                 if (!__all_sync(0xffffffffu, kPair ? mbar_wait_cluster(&tempty[acc], acc_phase ^ 1u, wc)
@@ -635,10 +659,10 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
                         add = 1;
                     }
                 };
-                const bool back = (nth & 1) != 0;
                 for (int i = 0; i < 2 && ok; ++i) {
-                    const int seg = back ? 1 - i : i;
-                    for (int left = seg ? q.nkb - q.nkb0 : q.nkb0; left > 0; left -= sub) {
+                    int from, to;
+                    it.segment(q, it.back ? 1 - i : i, from, to);
+                    for (int left = to - from; left > 0; left -= sub) {
                         if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, wc))) { ok = false; break; }
                         const uint64_t off = (stage * stage_bytes) >> 4;
                         block(off);
@@ -661,11 +685,11 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
         BoxWriter box{smem + kTrainRingBytes + warp * 2u * kTrainBoxBytes, 0u, lane};
         const int quarter = static_cast<int>(warp & 3u), group = static_cast<int>(warp >> 2);
         uint32_t iter = 0;
-        while (it.next(p, prob, tm, tn, nth)) {
+        while (it.next(p)) {
             const uint32_t acc = iter & 1u, acc_phase = (iter >> 1) & 1u;
             ++iter;
-            const int row0 = tm * kTileM + static_cast<int>(rank) * 128 + quarter * 32;
-            TrainEpilogue<kEpi> epi(p, p.prob[prob], row0, static_cast<int>(lane), tn, group);
+            const int row0 = it.tm * kTileM + static_cast<int>(rank) * 128 + quarter * 32;
+            TrainEpilogue<kEpi> epi(p, p.prob[it.prob], row0, static_cast<int>(lane), it.tn, it.split, group);
             epi.begin();
             const bool got = kPair ? mbar_wait_cluster(&tfull[acc], acc_phase, wc) : mbar_wait(&tfull[acc], acc_phase, wc);
             if (!__all_sync(0xffffffffu, got)) break;
@@ -830,15 +854,25 @@ __global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* __r
     }
 }
 
-// out = alpha src, rounded once (8 elements per thread).
-__global__ void __launch_bounds__(256) scale_round_kernel(const float4* __restrict__ src, uint4* __restrict__ out,
-                                                          long long vecs, const float* __restrict__ alpha, int bf16) {
+// out = alpha (part 0 + part 1 + ...) of FP32 sums `stride` elements apart,
+// added in that order and rounded once (8 elements per thread). alpha: a device
+// number, or null for 1.
+__global__ void __launch_bounds__(256) sum_round_kernel(const float* __restrict__ src, int parts, long long stride,
+                                                        uint4* __restrict__ out, long long vecs,
+                                                        const float* __restrict__ alpha, int bf16) {
     grid_dependents_launch();
     grid_dependency_wait();
-    const float a = *alpha;
+    const float a = alpha != nullptr ? *alpha : 1.f;
     for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < vecs;
          i += static_cast<long long>(gridDim.x) * 256) {
-        const float4 x = src[2 * i], y = src[2 * i + 1];
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+        const float4* p = reinterpret_cast<const float4*>(src) + 2 * i;
+#pragma unroll 4
+        for (int k = 0; k < parts; ++k, p += stride / 4) {
+            const float4 u = p[0], v = p[1];
+            x.x += u.x; x.y += u.y; x.z += u.z; x.w += u.w;
+            y.x += v.x; y.y += v.y; y.z += v.z; y.w += v.w;
+        }
         uint4 q;
         q.x = pack2(a * x.x, a * x.y, bf16);
         q.y = pack2(a * x.z, a * x.w, bf16);

@@ -170,6 +170,8 @@ struct Product {
     const float* alpha_ptr = nullptr;
     const void* c = nullptr;
     int64_t ldc = 0;
+    int splits = 1;            // > 1: FP32 partial sums [splits][whole tiles of rows][ld_out]
+    bool splittable = false;
     int64_t kblocks() const { return cdiv(k0, kBlockK) + cdiv(k1, kBlockK); }
 };
 
@@ -181,57 +183,82 @@ double block_cycles(bool pair, int tile_n) {
     return (pair ? kPairs : kSingle)[tile_n / 64 - 1];
 }
 
-// Time of a product's tiles in clock cycles, for comparing tiles of one
-// product: waves of main loops, a change of tile each, the launch and the last
-// tile's epilogue.
-double tile_cost(const Product& p, bool pair, int tile_n, int sms) {
-    const int64_t cols = p.dual ? tile_n / 2 : tile_n;
-    const int64_t tiles = cdiv(p.m, pair ? 256 : 128) * cdiv(p.n, cols);
-    const int64_t units = pair ? sms / 2 : sms;
-    const double waves = static_cast<double>(cdiv(tiles, units));
-    return waves * (p.kblocks() * block_cycles(pair, tile_n) + 600.0) + (pair ? 10000.0 : 8500.0) + 16.0 * tile_n;
+int64_t tile_rows(bool pair) { return pair ? 256 : 128; }
+
+// What a launch of `count` products is estimated to take with tile t, in
+// cycles. One product: its waves. Several: units take the tiles one after the
+// other, so the whole work over all units, plus half a last tile that some wait
+// for. Never less than the longest tile, nor than the operands' way from memory
+// (3600 bytes a cycle). Partial sums are written, read and launched for.
+double launch_cost(const Product* s, int count, const Tile& t, int sms) {
+    const double units = t.pair ? sms / 2 : sms;
+    double work = 0, longest = 0, last = 0, bytes = 0, more = 0;
+    int64_t tiles = 0;
+    for (int i = 0; i < count; ++i) {
+        const Product& p = s[i];
+        const int64_t kb = cdiv(p.kblocks(), p.splits), cols = p.dual ? t.n / 2 : t.n;
+        const int64_t n = cdiv(p.m, tile_rows(t.pair)) * cdiv(p.n, cols) * p.splits;
+        const double one = static_cast<double>(kb) * block_cycles(t.pair, t.n) + 600.0;
+        work += one * static_cast<double>(n);
+        tiles += n;
+        longest = std::max(longest, one);
+        last = one;
+        bytes += 2.0 * static_cast<double>(p.k0 + p.k1) * static_cast<double>(p.m + (p.dual ? 2 : 1) * p.n);
+        if (p.splits > 1)
+            more += 6000.0 + 8.0 * p.splits * static_cast<double>(cdiv(p.m, tile_rows(t.pair)) * tile_rows(t.pair)) *
+                                 static_cast<double>(p.n) / 3600.0;
+    }
+    const double main = count == 1 ? longest * static_cast<double>(cdiv(tiles, static_cast<int64_t>(units)))
+                                   : std::max(longest, work / units + 0.5 * last);
+    return std::max(main, bytes / 3600.0) + more + (t.pair ? 10000.0 : 8500.0) + 16.0 * t.n;
 }
 
-Tile choose_tile(const Product& p, int sms, int32_t forced) {
-    if (forced != 0) return {(forced & HGEMM_SM100_TRAIN_TILE_PAIR) != 0, forced & 0xfff};
+// The tile of a launch (all its products alike), and the splits of the products
+// that may be split.
+Tile choose_tile(Product* s, int count, int sms, const HgemmSm100TrainCommon& forced) {
     Tile best;
-    double cost = 0;
+    int best_splits = 1;
+    double cost = -1;
     for (int pair = 1; pair >= 0; --pair) {
         for (int n = 256; n >= 64; n -= 64) {
-            const double c = tile_cost(p, pair != 0, n, sms);
-            if (best.n == 0 || c < cost) {
-                best = {pair != 0, n};
-                cost = c;
+            const Tile t{pair != 0, n};
+            if (forced.tile != 0 && forced.tile != (n | (pair ? HGEMM_SM100_TRAIN_TILE_PAIR : 0))) continue;
+            for (int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {
+                bool any = false;
+                for (int i = 0; i < count; ++i)
+                    if (s[i].splittable) {
+                        const int64_t want = forced.splits != 0 ? forced.splits : splits;
+                        // Whole parts of at least four K blocks (one where forced).
+                        const int64_t most = std::max<int64_t>(1, s[i].kblocks() / (forced.splits != 0 ? 1 : 4));
+                        s[i].splits = static_cast<int>(std::min(want, most));
+                        any = true;
+                    }
+                const double c = launch_cost(s, count, t, sms);
+                if (cost < 0 || c < cost) {
+                    best = t;
+                    best_splits = splits;
+                    cost = c;
+                }
+                if (!any || forced.splits != 0) break;
             }
         }
     }
+    for (int i = 0; i < count; ++i)
+        if (s[i].splittable) {
+            const int64_t want = forced.splits != 0 ? forced.splits : best_splits;
+            const int64_t most = std::max<int64_t>(1, s[i].kblocks() / (forced.splits != 0 ? 1 : 4));
+            const int64_t kb = cdiv(s[i].kblocks(), std::min(want, most));
+            s[i].splits = static_cast<int>(cdiv(s[i].kblocks(), kb));   // no part without K blocks
+        }
     return best;
 }
 
-// One launch of several products: all tiles pairs or none. Its units take the
-// tiles one after the other, so what counts is the whole work over all units,
-// plus the part of a last tile that some wait for; and the longest tile.
-void choose_tiles(const Product* s, int count, Tile* out, int sms, int32_t forced) {
-    double best = -1;
-    for (int pair = 1; pair >= 0; --pair) {
-        for (int n = 256; n >= 64; n -= 64) {
-            const Tile t = forced != 0 ? choose_tile(s[0], sms, forced) : Tile{pair != 0, n};
-            double work = 0, longest = 0, last = 0;
-            for (int i = 0; i < count; ++i) {
-                const double one = s[i].kblocks() * block_cycles(t.pair, t.n) + 600.0 + 4.0 * t.n;
-                work += one * static_cast<double>(cdiv(s[i].m, t.pair ? 256 : 128) * cdiv(s[i].n, t.n));
-                longest = std::max(longest, one);
-                last = one;
-            }
-            const double cost = std::max(longest, work / (t.pair ? sms / 2 : sms) + 0.5 * last) +
-                                (t.pair ? 10000.0 : 8500.0) + 16.0 * t.n;
-            if (best < 0 || cost < best) {
-                best = cost;
-                for (int i = 0; i < count; ++i) out[i] = t;
-            }
-            if (forced != 0) return;
-        }
-    }
+// FP32 elements of one part of a split product, and bytes of all parts.
+int64_t part_elements(const Product& p, const Tile& t) {
+    return cdiv(p.m, tile_rows(t.pair)) * tile_rows(t.pair) * p.ld_out;
+}
+size_t part_bytes(const Product& p, const Tile& t) {
+    return p.splits > 1 ? static_cast<size_t>(p.splits * part_elements(p, t)) * 4 : 0;
 }
 
 // Raster group height: the tallest of 8, 16, 32 tile rows whose one-wave
@@ -261,6 +288,7 @@ int begin(Context* c, const HgemmSm100TrainCommon& common, void* stream) {
     if (common.dtype != HGEMM_SM100_TRAIN_F16 && common.dtype != HGEMM_SM100_TRAIN_BF16)
         return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     if (common.flags & ~HGEMM_SM100_FLAG_TEST_INJECT_TX) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    if (common.splits < 0 || common.splits > 16) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     if (common.tile != 0) {
         const int n = common.tile & 0xfff;
         if ((common.tile & ~(0xfff | HGEMM_SM100_TRAIN_TILE_PAIR)) || n < 64 || n > 256 || n % 64)
@@ -282,15 +310,15 @@ void init_params(TrainParams& p, const Context& c) {
 
 // Fills the problems of `p` from `count` products (the first one with the most
 // K blocks) and launches them as one grid.
-int run_products(TrainParams& p, int epi, const Product* products, const Tile* tiles, int count, const Context& c) {
-    const bool pair = tiles[0].pair;
+int run_products(TrainParams& p, int epi, const Product* products, const Tile& tile, int count, const Context& c) {
+    const bool pair = tile.pair;
+    const int tile_n = tile.n;
     const int units = pair ? c.dev->sms / 2 : c.dev->sms;
-    uint32_t block_stride = 0;
+    uint32_t a_bytes = 0, b_bytes = 0;
     int64_t total = 0, light = 0;
     for (int i = 0; i < count; ++i) {
         const Product& s = products[i];
         TrainProblem& q = p.prob[i];
-        const int tile_n = tiles[i].n;
         const int cols = s.dual ? tile_n / 2 : tile_n;          // output columns of a tile
         const uint32_t b_box = static_cast<uint32_t>(s.dual || pair ? tile_n / 2 : tile_n);
         const int bf16 = p.in_bf16;
@@ -311,26 +339,36 @@ int run_products(TrainParams& p, int epi, const Product* products, const Tile* t
         q.alpha_ptr = s.alpha_ptr;
         q.c = s.c;
         q.ldc = s.ldc;
-        int rc = make_operand(&q.a[0], s.a0, s.m, s.k0, 128, bf16);
+        q.splits = s.splits;
+        q.kb_split = static_cast<int>(cdiv(s.kblocks(), s.splits));
+        q.pad_rows = static_cast<int>(q.tiles_m * tile_rows(pair));
+        // Few rows (K-major): only those are loaded. What the MMA reads in place
+        // of the others is some other part of the ring, and gives accumulator
+        // rows that nothing stores.
+        const uint32_t a_rows = s.a0.mn || pair ? 128u : static_cast<uint32_t>(std::min<int64_t>(128, round_up(s.m, 8)));
+        q.a_tile_bytes = a_rows * 128u;
+        int rc = make_operand(&q.a[0], s.a0, s.m, s.k0, a_rows, bf16);
         if (rc == HGEMM_SM100_OK) rc = make_operand(&q.b[0], s.b0, s.n, s.k0, b_box, bf16);
         if (rc == HGEMM_SM100_OK && s.dual) rc = make_operand(&q.b[1], s.b1, s.n, s.k0, b_box, bf16);
         if (rc == HGEMM_SM100_OK && s.k1 > 0) {
-            rc = make_operand(&q.a[1], s.a1, s.m, s.k1, 128, bf16);
+            rc = make_operand(&q.a[1], s.a1, s.m, s.k1, a_rows, bf16);
             if (rc == HGEMM_SM100_OK) rc = make_operand(&q.b[1], s.b1, s.n, s.k1, b_box, bf16);
         }
         void* const outs[3] = {s.out, s.out1, s.out2};
         for (int j = 0; j < 3 && rc == HGEMM_SM100_OK; ++j) {
             if (outs[j] == nullptr) continue;
+            const int64_t rows = s.splits > 1 ? static_cast<int64_t>(s.splits) * q.pad_rows : s.m;
             rc = s.out_kind == kTrainOut16
-                     ? tensor_map(&q.out[j], outs[j], s.n, s.m, s.ld_out, 32, 32, type16(p.out_bf16),
+                     ? tensor_map(&q.out[j], outs[j], s.n, rows, s.ld_out, 32, 32, type16(p.out_bf16),
                                   CU_TENSOR_MAP_SWIZZLE_64B)
-                     : tensor_map(&q.out[j], outs[j], s.n, s.m, s.ld_out, 32, 32, CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                     : tensor_map(&q.out[j], outs[j], s.n, rows, s.ld_out, 32, 32, CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
                                   CU_TENSOR_MAP_SWIZZLE_128B);
         }
         if (rc != HGEMM_SM100_OK) return rc;
         const int64_t b_cols = pair ? tile_n / 2 : tile_n;
-        block_stride = std::max(block_stride, static_cast<uint32_t>(16384 + round_up(b_cols, 64) * 128));
-        const int64_t n = static_cast<int64_t>(q.tiles_m) * q.tiles_n;
+        a_bytes = std::max(a_bytes, q.a_tile_bytes);
+        b_bytes = std::max(b_bytes, static_cast<uint32_t>(round_up(b_cols, 64) * 128));
+        const int64_t n = static_cast<int64_t>(q.tiles_m) * q.tiles_n * q.splits;
         total += n;
         if (i > 0) light += n;
     }
@@ -340,15 +378,14 @@ int run_products(TrainParams& p, int epi, const Product* products, const Tile* t
     p.light_tiles = static_cast<int>(light);
     const int grid_units = static_cast<int>(std::min<int64_t>(total, units));
     if (light > 0 && p.heavy_tiles % grid_units != 0) {
-        const double ratio = static_cast<double>(p.prob[0].nkb) * p.prob[0].tile_n /
-                             (static_cast<double>(p.prob[1].nkb) * p.prob[1].tile_n);
-        p.light_skip = static_cast<int>(ratio + 0.5);
+        p.light_skip = static_cast<int>(static_cast<double>(p.prob[0].kb_split) / p.prob[1].kb_split + 0.5);
     }
-    p.block_stride = block_stride;
+    p.b_offset = a_bytes;
+    p.block_stride = a_bytes + b_bytes;
     // Two K blocks to a stage where three stages fit: the hand-off of a stage
     // costs about 280 cycles whatever the tile's width.
-    p.sub = kTrainRingBytes / (2 * block_stride) >= 3 ? 2 : 1;
-    p.stages = static_cast<int>(std::min<uint32_t>(kTrainRingBytes / (p.sub * block_stride), kTrainMaxStages));
+    p.sub = kTrainRingBytes / (2 * p.block_stride) >= 3 ? 2 : 1;
+    p.stages = static_cast<int>(std::min<uint32_t>(kTrainRingBytes / (p.sub * p.block_stride), kTrainMaxStages));
 
     KernelEntry& k = g_kernels[pair ? 1 : 0][epi];
     const uint64_t bit = 1ull << c.id;
@@ -362,9 +399,17 @@ int run_products(TrainParams& p, int epi, const Product* products, const Tile* t
                   pair ? 2 : 1, c.stream, p);
 }
 
-int run_product(TrainParams& p, int epi, const Product& s, const Context& c) {
-    const Tile t = choose_tile(s, c.dev->sms, c.common.tile);
-    return run_products(p, epi, &s, &t, 1, c);
+int run_product(TrainParams& p, int epi, Product& s, const Context& c) {
+    return run_products(p, epi, &s, choose_tile(&s, 1, c.dev->sms, c.common), 1, c);
+}
+
+// The parts of a split product, joined and rounded into `out` [m x ld_out].
+int join_parts(const float* parts, const Product& s, const Tile& t, void* out, const float* alpha, const Context& c) {
+    const int64_t vecs = s.m * s.ld_out / 8;
+    const int64_t blocks = std::min<int64_t>(cdiv(vecs, 256), c.dev->sms * 8);
+    return launch(&sum_round_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, 1, c.stream, parts, s.splits,
+                  static_cast<long long>(part_elements(s, t)), static_cast<uint4*>(out), static_cast<long long>(vecs),
+                  alpha, c.common.dtype == HGEMM_SM100_TRAIN_BF16 ? 1 : 0);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -379,9 +424,87 @@ bool matrix_ok(const void* p, int64_t ld, int64_t cols) {
 
 // ------------------------------------------------------------ feed-forward --
 
+namespace {
+
+bool ffn_sizes_ok(int64_t tokens, int64_t hidden, int64_t inter, int64_t out) {
+    return size_ok(tokens) && size8_ok(hidden) && size8_ok(inter) && size8_ok(out);
+}
+
+// y = h Wd^T
+Product ffn_down(const HgemmSm100FfnForward& a) {
+    Product d;
+    d.m = a.tokens;
+    d.n = a.out;
+    d.k0 = a.inter;
+    d.a0 = {a.h, a.inter, false};
+    d.b0 = {a.down, a.inter, false};
+    d.out = a.y;
+    d.ld_out = a.out;
+    d.splittable = true;
+    return d;
+}
+
+// The gradients that are wanted, the one with the longest sums first.
+struct FfnGradPlan {
+    Product s[4];
+    int count = 0, dx = -1;
+    Tile tile;
+    size_t bytes() const { return dx >= 0 ? part_bytes(s[dx], tile) : 0; }
+};
+
+FfnGradPlan plan_ffn_backward(const HgemmSm100FfnBackward& a, int sms) {
+    FfnGradPlan g;
+    if (a.dx != nullptr) {
+        Product& q = g.s[g.count++];
+        q.m = a.tokens;
+        q.n = a.hidden;
+        q.k0 = q.k1 = a.inter;
+        q.a0 = {a.dgate_pre, a.inter, false};
+        q.b0 = {a.gate, a.hidden, true};
+        q.a1 = {a.dup_pre, a.inter, false};
+        q.b1 = {a.up, a.hidden, true};
+        q.out = a.dx;
+        q.ld_out = a.hidden;
+        q.splittable = true;
+    }
+    auto weight = [&](void* out, const void* left, int64_t ld_left, int64_t rows, const void* right, int64_t ld_right,
+                      int64_t cols) {
+        if (out == nullptr) return;
+        Product& q = g.s[g.count++];
+        q.m = rows;
+        q.n = cols;
+        q.k0 = a.tokens;
+        q.a0 = {left, ld_left, true};
+        q.b0 = {right, ld_right, true};
+        q.out = out;
+        q.ld_out = cols;
+    };
+    weight(a.dgate, a.dgate_pre, a.inter, a.inter, a.x, a.ldx, a.hidden);
+    weight(a.dup, a.dup_pre, a.inter, a.inter, a.x, a.ldx, a.hidden);
+    weight(a.ddown, a.dy, a.lddy, a.out, a.h, a.inter, a.inter);
+    if (g.count == 0) return g;
+    g.tile = choose_tile(g.s, g.count, sms, a.common);
+    std::stable_sort(g.s, g.s + g.count, [](const Product& x, const Product& y) {
+        return cdiv(x.kblocks(), x.splits) > cdiv(y.kblocks(), y.splits);
+    });
+    for (int i = 0; i < g.count; ++i)
+        if (g.s[i].splittable) g.dx = i;
+    return g;
+}
+
+}  // namespace
+
+extern "C" size_t hgemm_sm100_ffn_forward_workspace(const HgemmSm100FfnForward* a) {
+    Context c;
+    if (a == nullptr || !ffn_sizes_ok(a->tokens, a->hidden, a->inter, a->out)) return 0;
+    if (begin(&c, a->common, nullptr) != HGEMM_SM100_OK) return 0;
+    Product d = ffn_down(*a);
+    const Tile t = choose_tile(&d, 1, c.dev->sms, c.common);
+    return part_bytes(d, t);
+}
+
 extern "C" int hgemm_sm100_ffn_forward(const HgemmSm100FfnForward* a, void* stream) {
-    if (a == nullptr || !size_ok(a->tokens) || !size8_ok(a->hidden) || !size8_ok(a->inter) || !size8_ok(a->out))
-        return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    if (a == nullptr || !ffn_sizes_ok(a->tokens, a->hidden, a->inter, a->out)) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     if (!matrix_ok(a->x, a->ldx, a->hidden) || !matrix_ok(a->gate, 8, 8) || !matrix_ok(a->up, 8, 8) ||
         !matrix_ok(a->down, 8, 8) || !matrix_ok(a->y, 8, 8) || !matrix_ok(a->h, 8, 8))
         return HGEMM_SM100_ERR_INVALID_ARGUMENT;
@@ -390,6 +513,11 @@ extern "C" int hgemm_sm100_ffn_forward(const HgemmSm100FfnForward* a, void* stre
     Context c;
     int rc = begin(&c, a->common, stream);
     if (rc != HGEMM_SM100_OK) return rc;
+    Product d = ffn_down(*a);
+    const Tile down_tile = choose_tile(&d, 1, c.dev->sms, c.common);
+    const size_t need = part_bytes(d, down_tile);
+    if (need > 0 && (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < need))
+        return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     TrainParams p;
 
     Product g;
@@ -408,21 +536,24 @@ extern "C" int hgemm_sm100_ffn_forward(const HgemmSm100FfnForward* a, void* stre
     p.keep = a->gate_pre != nullptr;
     if ((rc = run_product(p, kTrainGate, g, c)) != HGEMM_SM100_OK) return rc;
 
-    Product d;
-    d.m = a->tokens;
-    d.n = a->out;
-    d.k0 = a->inter;
-    d.a0 = {a->h, a->inter, false};
-    d.b0 = {a->down, a->inter, false};
-    d.out = a->y;
-    d.ld_out = a->out;
+    if (need > 0) {
+        d.out = a->workspace;
+        d.out_kind = kTrainOutF32;
+    }
     init_params(p, c);
-    return run_product(p, kTrainStore, d, c);
+    if ((rc = run_products(p, kTrainStore, &d, down_tile, 1, c)) != HGEMM_SM100_OK || need == 0) return rc;
+    return join_parts(static_cast<const float*>(a->workspace), d, down_tile, a->y, nullptr, c);
+}
+
+extern "C" size_t hgemm_sm100_ffn_backward_workspace(const HgemmSm100FfnBackward* a) {
+    Context c;
+    if (a == nullptr || !ffn_sizes_ok(a->tokens, a->hidden, a->inter, a->out)) return 0;
+    if (begin(&c, a->common, nullptr) != HGEMM_SM100_OK) return 0;
+    return plan_ffn_backward(*a, c.dev->sms).bytes();
 }
 
 extern "C" int hgemm_sm100_ffn_backward(const HgemmSm100FfnBackward* a, void* stream) {
-    if (a == nullptr || !size_ok(a->tokens) || !size8_ok(a->hidden) || !size8_ok(a->inter) || !size8_ok(a->out))
-        return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    if (a == nullptr || !ffn_sizes_ok(a->tokens, a->hidden, a->inter, a->out)) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     if (!matrix_ok(a->dy, a->lddy, a->out) || !matrix_ok(a->x, a->ldx, a->hidden) || !matrix_ok(a->gate, 8, 8) ||
         !matrix_ok(a->up, 8, 8) || !matrix_ok(a->down, 8, 8) || !matrix_ok(a->gate_pre, 8, 8) ||
         !matrix_ok(a->up_pre, 8, 8) || !matrix_ok(a->h, 8, 8) || !matrix_ok(a->dgate_pre, 8, 8) ||
@@ -432,6 +563,11 @@ extern "C" int hgemm_sm100_ffn_backward(const HgemmSm100FfnBackward* a, void* st
     Context c;
     int rc = begin(&c, a->common, stream);
     if (rc != HGEMM_SM100_OK) return rc;
+    FfnGradPlan g = plan_ffn_backward(*a, c.dev->sms);
+    const size_t need = g.bytes();
+    if (need > 0 && (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < need))
+        return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    if (g.count == 0) return HGEMM_SM100_OK;
     TrainParams p;
 
     // dh = dy Wd; its epilogue turns it into dg and du.
@@ -451,43 +587,13 @@ extern "C" int hgemm_sm100_ffn_backward(const HgemmSm100FfnBackward* a, void* st
         p.ld_saved = a->inter;
         if ((rc = run_product(p, kTrainGateGrad, h, c)) != HGEMM_SM100_OK) return rc;
     }
-
-    Product s[4];
-    int n = 0;
-    if (a->dx != nullptr) {
-        Product& q = s[n++];
-        q.m = a->tokens;
-        q.n = a->hidden;
-        q.k0 = q.k1 = a->inter;
-        q.a0 = {a->dgate_pre, a->inter, false};
-        q.b0 = {a->gate, a->hidden, true};
-        q.a1 = {a->dup_pre, a->inter, false};
-        q.b1 = {a->up, a->hidden, true};
-        q.out = a->dx;
-        q.ld_out = a->hidden;
+    if (need > 0) {
+        g.s[g.dx].out = a->workspace;
+        g.s[g.dx].out_kind = kTrainOutF32;
     }
-    auto weight = [&](void* out, const void* left, int64_t ld_left, int64_t rows, const void* right, int64_t ld_right,
-                      int64_t cols) {
-        if (out == nullptr) return;
-        Product& q = s[n++];
-        q.m = rows;
-        q.n = cols;
-        q.k0 = a->tokens;
-        q.a0 = {left, ld_left, true};
-        q.b0 = {right, ld_right, true};
-        q.out = out;
-        q.ld_out = cols;
-    };
-    weight(a->dgate, a->dgate_pre, a->inter, a->inter, a->x, a->ldx, a->hidden);
-    weight(a->dup, a->dup_pre, a->inter, a->inter, a->x, a->ldx, a->hidden);
-    weight(a->ddown, a->dy, a->lddy, a->out, a->h, a->inter, a->inter);
-    if (n == 0) return HGEMM_SM100_OK;
-    // The problem with the most K blocks goes first.
-    std::stable_sort(s, s + n, [](const Product& x, const Product& y) { return x.kblocks() > y.kblocks(); });
-    Tile t[4];
-    choose_tiles(s, n, t, c.dev->sms, c.common.tile);
     init_params(p, c);
-    return run_products(p, kTrainStore, s, t, n, c);
+    if ((rc = run_products(p, kTrainStore, g.s, g.tile, g.count, c)) != HGEMM_SM100_OK || need == 0) return rc;
+    return join_parts(static_cast<const float*>(a->workspace), g.s[g.dx], g.tile, a->dx, nullptr, c);
 }
 
 // ------------------------------------------------------------ cross entropy --
@@ -509,7 +615,7 @@ LossForwardPlan plan_loss_forward(const HgemmSm100LossForward& a, int sms) {
     q.z.k0 = a.hidden;
     q.z.a0 = {a.x, a.ldx, false};
     q.z.b0 = {a.weight, a.hidden, false};
-    q.tile = choose_tile(q.z, sms, a.common.tile);
+    q.tile = choose_tile(&q.z, 1, sms, a.common);
     q.parts = 2 * cdiv(a.vocab, q.tile.n);   // two column groups a tile
     q.partial_bytes = static_cast<size_t>(round_up(q.parts * a.tokens * 8, 256));
     q.row_bytes = static_cast<size_t>(round_up(a.tokens * 4, 256));
@@ -527,19 +633,67 @@ int64_t loss_piece(const HgemmSm100LossBackward& a) {
     return round_up(cdiv(a.vocab, cdiv(a.vocab, n)), 256);   // equal pieces
 }
 
+// dx and dW of one piece (nv vocabulary entries), as long sums first.
+struct LossPiece {
+    Product s[2];
+    int count = 0, dx = -1;
+    Tile tile;
+};
+
+LossPiece plan_piece(const HgemmSm100LossBackward& a, int64_t nv, int64_t piece, int sms) {
+    LossPiece g;
+    if (a.dx != nullptr) {
+        Product& d = g.s[g.count++];
+        d.m = a.tokens;
+        d.n = d.ld_out = a.hidden;
+        d.k0 = nv;
+        d.a0 = {nullptr, piece, false};
+        d.b0 = {nullptr, a.hidden, true};
+        d.splittable = true;
+    }
+    if (a.dweight != nullptr) {
+        Product& d = g.s[g.count++];
+        d.m = nv;
+        d.n = d.ld_out = a.hidden;
+        d.k0 = a.tokens;
+        d.a0 = {nullptr, piece, true};
+        d.b0 = {a.x, a.ldx, true};
+    }
+    g.tile = choose_tile(g.s, g.count, sms, a.common);
+    return g;
+}
+
 struct LossBackwardPlan {
     int64_t piece = 0, pieces = 0;
+    bool sums = false;     // dx goes through FP32 sums: several pieces, or parts of one
+    int splits = 1;        // of dx, in every piece alike
+    Tile tile;
     size_t dz_bytes = 0, sum_bytes = 0, row_bytes = 0;
     size_t bytes() const { return dz_bytes + sum_bytes + row_bytes + 256; }
 };
 
-LossBackwardPlan plan_loss_backward(const HgemmSm100LossBackward& a) {
+LossBackwardPlan plan_loss_backward(const HgemmSm100LossBackward& a, int sms) {
     LossBackwardPlan q;
     q.piece = loss_piece(a);
     q.pieces = cdiv(a.vocab, q.piece);
     q.dz_bytes = static_cast<size_t>(round_up(a.tokens * q.piece * 2, 256));
-    q.sum_bytes = a.dx != nullptr && q.pieces > 1 ? static_cast<size_t>(round_up(a.tokens * a.hidden * 4, 256)) : 0;
     q.row_bytes = static_cast<size_t>(round_up(a.tokens * 4, 256));
+    if (a.dx == nullptr && a.dweight == nullptr) return q;
+    const int64_t last = a.vocab - (q.pieces - 1) * q.piece;
+    const LossPiece g = plan_piece(a, std::min(q.piece, a.vocab), q.piece, sms);
+    q.tile = g.tile;
+    if (a.dx != nullptr) {
+        // In whole pieces and the last one alike, each part has K blocks.
+        auto parts_ok = [](int64_t n, int64_t splits) {
+            const int64_t kb = cdiv(n, kBlockK);
+            return (splits - 1) * cdiv(kb, splits) < kb;
+        };
+        q.splits = g.s[0].splits;
+        while (!parts_ok(std::min(q.piece, a.vocab), q.splits) || !parts_ok(last, q.splits)) --q.splits;
+        q.sums = q.pieces > 1 || q.splits > 1;
+        if (q.sums)
+            q.sum_bytes = static_cast<size_t>(round_up(q.splits * part_elements(g.s[0], q.tile) * 4, 256));
+    }
     return q;
 }
 
@@ -580,7 +734,7 @@ extern "C" int hgemm_sm100_loss_forward(const HgemmSm100LossForward* a, void* st
     p.target = target;
     p.partial = partial;
     p.target_logit = target_logit;
-    if ((rc = run_products(p, kTrainLse, &q.z, &q.tile, 1, c)) != HGEMM_SM100_OK) return rc;
+    if ((rc = run_products(p, kTrainLse, &q.z, q.tile, 1, c)) != HGEMM_SM100_OK) return rc;
     rc = launch(&lse_join_kernel, dim3(static_cast<unsigned>(cdiv(m, 32))), dim3(32, 32), 0, 1, c.stream, partial,
                 static_cast<int>(q.parts), m, target_logit, target, static_cast<long long>(a->vocab),
                 static_cast<long long>(a->ignore_index), a->lse, loss);
@@ -590,8 +744,10 @@ extern "C" int hgemm_sm100_loss_forward(const HgemmSm100LossForward* a, void* st
 }
 
 extern "C" size_t hgemm_sm100_loss_backward_workspace(const HgemmSm100LossBackward* a) {
-    if (a == nullptr || !size_ok(a->tokens) || !size_ok(a->vocab) || !size8_ok(a->hidden)) return 0;
-    return plan_loss_backward(*a).bytes();
+    Context c;
+    if (a == nullptr || !size_ok(a->tokens) || !size_ok(a->vocab) || !size8_ok(a->hidden) || a->piece < 0) return 0;
+    if (begin(&c, a->common, nullptr) != HGEMM_SM100_OK) return 0;
+    return plan_loss_backward(*a, c.dev->sms).bytes();
 }
 
 extern "C" int hgemm_sm100_loss_backward(const HgemmSm100LossBackward* a, void* stream) {
@@ -601,7 +757,7 @@ extern "C" int hgemm_sm100_loss_backward(const HgemmSm100LossBackward* a, void* 
     Context c;
     int rc = begin(&c, a->common, stream);
     if (rc != HGEMM_SM100_OK) return rc;
-    const LossBackwardPlan q = plan_loss_backward(*a);
+    const LossBackwardPlan q = plan_loss_backward(*a, c.dev->sms);
     if (a->workspace_bytes < q.bytes()) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     if (a->dx == nullptr && a->dweight == nullptr) return HGEMM_SM100_OK;
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
@@ -636,49 +792,33 @@ extern "C" int hgemm_sm100_loss_backward(const HgemmSm100LossBackward* a, void* 
         p.row_scale = row_scale;
         if ((rc = run_product(p, kTrainLogitGrad, z, c)) != HGEMM_SM100_OK) return rc;
 
-        Product s[2];
+        LossPiece g = plan_piece(*a, nv, q.piece, c.dev->sms);
         int n = 0;
         if (a->dx != nullptr) {
-            Product& d = s[n++];
-            d.m = a->tokens;
-            d.n = a->hidden;
-            d.k0 = nv;
-            d.a0 = {dz, q.piece, false};
-            d.b0 = {w, a->hidden, true};
-            d.ld_out = a->hidden;
-            if (q.pieces == 1) {
-                d.out = a->dx;
-                d.alpha_ptr = alpha;
-            } else {
-                d.out = sums;
-                d.out_kind = i == 0 ? kTrainOutF32 : kTrainOutF32Add;
-            }
+            Product& d = g.s[n++];
+            d.a0.ptr = dz;
+            d.b0.ptr = w;
+            d.splits = q.splits;
+            d.out = q.sums ? static_cast<void*>(sums) : a->dx;
+            d.out_kind = !q.sums ? kTrainOut16 : i == 0 ? kTrainOutF32 : kTrainOutF32Add;
+            if (!q.sums) d.alpha_ptr = alpha;
         }
         if (a->dweight != nullptr) {
-            Product& d = s[n++];
-            d.m = nv;
-            d.n = a->hidden;
-            d.k0 = a->tokens;
-            d.a0 = {dz, q.piece, true};
-            d.b0 = {a->x, a->ldx, true};
+            Product& d = g.s[n++];
+            d.a0.ptr = dz;
             d.out = static_cast<uint8_t*>(a->dweight) + v0 * a->hidden * 2;
-            d.ld_out = a->hidden;
             d.alpha_ptr = alpha;
         }
-        if (n == 2 && s[1].kblocks() > s[0].kblocks()) std::swap(s[0], s[1]);
-        Tile t[2];
-        choose_tiles(s, n, t, c.dev->sms, c.common.tile);
+        if (n == 2 && g.s[1].kblocks() > cdiv(g.s[0].kblocks(), g.s[0].splits)) std::swap(g.s[0], g.s[1]);
         init_params(p, c);
-        if ((rc = run_products(p, kTrainStore, s, t, n, c)) != HGEMM_SM100_OK) return rc;
+        if ((rc = run_products(p, kTrainStore, g.s, q.tile, n, c)) != HGEMM_SM100_OK) return rc;
     }
-    if (a->dx != nullptr && q.pieces > 1) {
-        const int64_t vecs = a->tokens * a->hidden / 8;
-        const int64_t blocks = std::min<int64_t>(cdiv(vecs, 256), c.dev->sms * 8);
-        rc = launch(&scale_round_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, 1, c.stream,
-                    reinterpret_cast<const float4*>(sums), static_cast<uint4*>(a->dx), static_cast<long long>(vecs),
-                    alpha, a->common.dtype == HGEMM_SM100_TRAIN_BF16 ? 1 : 0);
-    }
-    return rc;
+    if (!q.sums) return HGEMM_SM100_OK;
+    Product d;
+    d.m = a->tokens;
+    d.n = d.ld_out = a->hidden;
+    d.splits = q.splits;
+    return join_parts(sums, d, q.tile, a->dx, alpha, c);
 }
 
 // ------------------------------------------------------ orthogonalised update --
@@ -759,11 +899,9 @@ extern "C" int hgemm_sm100_orthogonalize(const HgemmSm100Orthogonalize* a, void*
     auto each = [&](auto&& make, int out_bf16) -> int {
         for (int64_t first = 0; first < a->batch; first += kTrainMaxProblems) {
             Product s[kTrainMaxProblems];
-            Tile t[kTrainMaxProblems];
             const int n = static_cast<int>(std::min<int64_t>(kTrainMaxProblems, a->batch - first));
             for (int i = 0; i < n; ++i) make(s[i], first + i);
-            if (n > 1) choose_tiles(s, n, t, c.dev->sms, c.common.tile);
-            else t[0] = choose_tile(s[0], c.dev->sms, c.common.tile);
+            const Tile t = choose_tile(s, n, c.dev->sms, c.common);
             init_params(p, c);
             p.in_bf16 = 0;
             p.out_bf16 = out_bf16;

@@ -17,7 +17,7 @@ LOSS_NONE, LOSS_MEAN, LOSS_SUM = 0, 1, 2
 
 
 class Common(ctypes.Structure):
-    _fields_ = [("dtype", c_int32), ("tile", c_int32), ("flags", c_int32), ("reserved", c_int32),
+    _fields_ = [("dtype", c_int32), ("tile", c_int32), ("flags", c_int32), ("splits", c_int32),
                 ("status", c_void_p), ("timeout_ns", c_uint64)]
 
 
@@ -28,9 +28,10 @@ def _struct(name: str, pointers: str, sizes: str, rest=()):
     return type(name, (ctypes.Structure,), {"_fields_": fields + list(rest)})
 
 
-FfnForward = _struct("FfnForward", "x gate up down y h gate_pre up_pre", "tokens hidden inter out ldx")
-FfnBackward = _struct("FfnBackward", "dy x gate up down gate_pre up_pre h dgate_pre dup_pre dx dgate dup ddown",
-                      "tokens hidden inter out ldx lddy")
+FfnForward = _struct("FfnForward", "x gate up down y h gate_pre up_pre workspace",
+                     "workspace_bytes tokens hidden inter out ldx")
+FfnBackward = _struct("FfnBackward", "dy x gate up down gate_pre up_pre h dgate_pre dup_pre dx dgate dup ddown workspace",
+                      "workspace_bytes tokens hidden inter out ldx lddy")
 _REDUCTION = [("reduction", c_int32), ("reserved", c_int32)]
 LossForward = _struct("LossForward", "x weight target loss lse workspace",
                       "workspace_bytes tokens hidden vocab ldx ignore_index", _REDUCTION)
@@ -52,9 +53,8 @@ def load() -> ctypes.CDLL:
                              ("orthogonalize", Orthogonalize)):
             fn = getattr(lib, f"hgemm_sm100_{name}")
             fn.argtypes, fn.restype = [ctypes.POINTER(struct), c_void_p], ctypes.c_int
-            if not name.startswith("ffn"):
-                size = getattr(lib, f"hgemm_sm100_{name}_workspace")
-                size.argtypes, size.restype = [ctypes.POINTER(struct)], ctypes.c_size_t
+            size = getattr(lib, f"hgemm_sm100_{name}_workspace")
+            size.argtypes, size.restype = [ctypes.POINTER(struct)], ctypes.c_size_t
         lib.hgemm_sm100_train_read_status.argtypes = [ctypes.POINTER(c_int32), ctypes.c_int]
         lib.hgemm_sm100_train_read_status.restype = ctypes.c_int
         _lib = lib

@@ -100,20 +100,48 @@ def stream():
     return torch.cuda.current_stream().cuda_stream
 
 
-def ffn_through_c(x, gate, up, down, dy, tile, flags=0, status=None, timeout_ns=0):
+def with_workspace(name, args):
+    """The call's workspace, filled with NaN; returned so that it lives on."""
+    args.workspace_bytes = train_capi.workspace(name, args)
+    ws = torch.full((args.workspace_bytes // 4,), float("nan"), device="cuda")
+    args.workspace = ws.data_ptr() if args.workspace_bytes else None
+    return ws
+
+
+def ffn_through_c(x, gate, up, down, dy, tile, flags=0, splits=0, status=None, timeout_ns=0):
     """Both calls of the C ABI with a forced tile; outputs pre-filled with NaN."""
     (t, h), (i, _), o = x.shape, gate.shape, down.shape[0]
     like = lambda *s: torch.full(s, float("nan"), dtype=x.dtype, device="cuda")   # noqa: E731
-    common = train_capi.Common(train_capi.BF16 if x.dtype == torch.bfloat16 else train_capi.F16, tile, flags, 0,
+    common = train_capi.Common(train_capi.BF16 if x.dtype == torch.bfloat16 else train_capi.F16, tile, flags, splits,
                                None if status is None else status.data_ptr(), timeout_ns)
     y, act, g, u, dg, du = like(t, o), like(t, i), like(t, i), like(t, i), like(t, i), like(t, i)
     dx, dgate, dup, ddown = like(t, h), like(i, h), like(i, h), like(o, i)
     p = lambda *ts: [a.data_ptr() for a in ts]   # noqa: E731
-    f = train_capi.FfnForward(common, *p(x, gate, up, down, y, act, g, u), t, h, i, o, h)
+    f = train_capi.FfnForward(common, *p(x, gate, up, down, y, act, g, u), None, 0, t, h, i, o, h)
+    ws = with_workspace("ffn_forward", f)
     assert train_capi.run("ffn_forward", f, stream()) == capi.OK
-    b = train_capi.FfnBackward(common, *p(dy, x, gate, up, down, g, u, act, dg, du, dx, dgate, dup, ddown), t, h, i, o, h, o)
+    b = train_capi.FfnBackward(common, *p(dy, x, gate, up, down, g, u, act, dg, du, dx, dgate, dup, ddown), None, 0,
+                               t, h, i, o, h, o)
+    ws2 = with_workspace("ffn_backward", b)
     assert train_capi.run("ffn_backward", b, stream()) == capi.OK
+    if ws.numel() + ws2.numel():
+        torch.cuda.synchronize()
+        # Less than the call asks for is refused.
+        for name, args in (("ffn_forward", f), ("ffn_backward", b)):
+            if args.workspace_bytes:
+                args.workspace_bytes -= 1
+                assert train_capi.run(name, args, stream()) == capi.ERR_INVALID_ARGUMENT
     return y, dx, dgate, dup, ddown
+
+
+@pytest.mark.parametrize("splits", [1, 2, 3, 5, 16])
+@pytest.mark.parametrize("size", [(5, 72, 1000, 136), (130, 264, 584, 200), (300, 520, 1352, 640)], ids=str)
+def test_ffn_sums_in_parts(size, splits):
+    """y and dx as sums of parts, whose borders fall inside either segment of dx's sum."""
+    inputs = ffn_inputs(*size, torch.bfloat16)
+    for tile in (64, 192, 128 | train_capi.TILE_PAIR):
+        for got, w in zip(ffn_through_c(*inputs, tile, splits=splits), ref.ffn(*inputs)):
+            within(got, w)
 
 
 @pytest.mark.parametrize("pair", [0, train_capi.TILE_PAIR], ids=["single", "pair"])
@@ -246,28 +274,44 @@ def test_loss(size, reduction, dtype):
         within(got, v)
 
 
-def loss_through_c(x, w, t, dl, tile=0, piece=0, reduction=train_capi.LOSS_MEAN):
-    """Forward and backward through the C ABI, workspaces pre-filled with NaN."""
+def loss_through_c(x, w, t, dl, tile=0, piece=0, reduction=train_capi.LOSS_MEAN, splits=0):
+    """Forward and backward through the C ABI, outputs and workspaces pre-filled with NaN."""
     n, h = x.shape
     v = w.shape[0]
-    common = train_capi.Common(train_capi.BF16 if x.dtype == torch.bfloat16 else train_capi.F16, tile)
+    common = train_capi.Common(train_capi.BF16 if x.dtype == torch.bfloat16 else train_capi.F16, tile, 0, splits)
     loss = torch.full((n if reduction == train_capi.LOSS_NONE else 1,), float("nan"), device="cuda")
     lse = torch.full((n,), float("nan"), device="cuda")
     f = train_capi.LossForward(common, x.data_ptr(), w.data_ptr(), t.data_ptr(), loss.data_ptr(), lse.data_ptr(), None, 0,
                                n, h, v, h, -100, reduction, 0)
-    f.workspace_bytes = train_capi.workspace("loss_forward", f)
-    ws = torch.full((f.workspace_bytes // 4,), float("nan"), device="cuda")
-    f.workspace = ws.data_ptr()
+    keep = [with_workspace("loss_forward", f)]
     assert train_capi.run("loss_forward", f, stream()) == capi.OK
     dx, dw = torch.full_like(x, float("nan")), torch.full_like(w, float("nan"))
     b = train_capi.LossBackward(common, x.data_ptr(), w.data_ptr(), t.data_ptr(), lse.data_ptr(), dl.data_ptr(),
                                 dx.data_ptr(), dw.data_ptr(), None, 0, n, h, v, h, -100, piece, reduction, 0)
-    b.workspace_bytes = train_capi.workspace("loss_backward", b)
-    ws2 = torch.full((b.workspace_bytes // 4,), float("nan"), device="cuda")
-    b.workspace = ws2.data_ptr()
+    keep.append(with_workspace("loss_backward", b))
     assert train_capi.run("loss_backward", b, stream()) == capi.OK
     torch.cuda.synchronize()
     return loss, dx, dw
+
+
+@pytest.mark.parametrize("splits", [1, 2, 7, 16])
+@pytest.mark.parametrize("piece", [64, 320, 1000, 5000])
+def test_loss_sums_in_parts(piece, splits):
+    """dx in pieces of the vocabulary and parts of each, the last piece short."""
+    x, w, t = loss_inputs(70, 136, 2100, torch.bfloat16)
+    dl = torch.tensor([1.0], device="cuda")
+    want = ref.loss(x, w, t, "sum", -100, dl)
+    got = loss_through_c(x, w, t, dl, piece=piece, reduction=train_capi.LOSS_SUM, splits=splits)
+    for g, v in zip((got[0][0], got[1], got[2]), want):
+        within(g, v)
+
+
+def test_loss_workspace_holds_one_piece():
+    a = train_capi.LossBackward(tokens=1000, hidden=64, vocab=150000, dx=1 << 20)
+    # At most 96 MB of 16-bit logit gradients (and the sums of dx), not the 300 MB of all.
+    assert 0 < train_capi.workspace("loss_backward", a) < 140 << 20
+    a.tokens = 0
+    assert train_capi.workspace("loss_backward", a) == 0
 
 
 @pytest.mark.parametrize("pair", [0, train_capi.TILE_PAIR], ids=["single", "pair"])
