@@ -144,8 +144,8 @@ typedef struct HgemmSm100Orthogonalize {
     const void* g;         /* [batch][rows x ldg], batch_stride elements apart,
                               2-byte aligned, any ldg >= cols                 */
     void* out;             /* [batch][rows x cols], 2-byte aligned            */
-    void* workspace;       /* hgemm_sm100_orthogonalize_workspace bytes,
-                              256-byte aligned                                */
+    void* workspace;       /* hgemm_sm100_orthogonalize_workspace bytes (0 for
+                              small matrices), 256-byte aligned               */
     uint64_t workspace_bytes;
     int64_t batch, rows, cols, ldg, batch_stride;
     int32_t steps;         /* >= 0                                            */

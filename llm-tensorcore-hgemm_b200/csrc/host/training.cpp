@@ -377,9 +377,11 @@ Tensor orthogonalize(const Tensor& g, int64_t steps, double a, double b, double 
     args.b = static_cast<float>(b);
     args.c = static_cast<float>(c);
     args.eps = eps;
-    args.workspace_bytes = hgemm_sm100_orthogonalize_workspace(&args);
-    const Tensor ws = bytes(args.workspace_bytes, g);
-    args.workspace = ws.data_ptr();
+    Tensor ws;
+    if ((args.workspace_bytes = hgemm_sm100_orthogonalize_workspace(&args)) > 0) {
+        ws = bytes(args.workspace_bytes, g);
+        args.workspace = ws.data_ptr();
+    }
     check_status(hgemm_sm100_orthogonalize(&args, c10::cuda::getCurrentCUDAStream(g.get_device()).stream()),
                  "orthogonalize");
     return out;

@@ -1002,4 +1002,345 @@ __global__ void __launch_bounds__(256) orth_copy_kernel(const void* __restrict__
         }
 }
 
+// All steps of a matrix whose shorter side is at most 128, in one launch: as
+// separate launches a step is three kernels of about 4 us each, whose products
+// take a tenth of that. A cluster of 1 to 16 CTAs keeps X (shorter side = 128
+// rows, zeros below) in shared memory, each CTA `slice` columns of it, in the
+// 128-byte-swizzled blocks of 64 columns that serve tcgen05 both as K-major
+// operand of X X^T and as MN-major operand of poly X. Per step each CTA
+// multiplies its slice's part of X X^T; the parts meet in distributed shared
+// memory (CTA r sums rows [128 r / C, 128 (r + 1) / C) of all of them in the
+// order of the CTAs and hands the rounded rows to everyone); the polynomial is
+// computed by everyone; X is updated in place. Rounding as in the launches per
+// product: FP16 X, X X^T and polynomial, FP32 sums.
+// A wait that runs out is recorded and the rest runs on without waiting, since
+// all CTAs have to reach the same cluster barriers.
+constexpr int kOrthThreads = 256;
+constexpr int kOrthMaxSlice = 640;
+constexpr uint32_t kOrthBlockBytes = 128u * 128u;                 // 128 rows x 64 halves
+constexpr uint32_t kOrthSquareBytes = 2u * kOrthBlockBytes;       // 128 x 128 halves
+constexpr uint32_t kOrthMaxSmem = (kOrthMaxSlice / 64) * kOrthBlockBytes + 2 * kOrthSquareBytes + 1024 + 512;
+static_assert(kOrthMaxSmem <= 232448, "shared memory");
+
+struct OrthClusterParams {
+    const void* g;
+    void* out;
+    long long batch_stride, ld;
+    int side, length;      // shorter and longer side
+    int tall;              // the longer side is the rows of g
+    int slice;             // columns of X per CTA, a multiple of 64
+    int bf16, steps;
+    float a, b, c;
+    double eps;
+    int* status;
+    unsigned long long timeout_ns;
+};
+
+__device__ __forceinline__ void st_dsmem_b64(uint32_t addr, uint32_t lo, uint32_t hi) {
+    asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(lo), "r"(hi) : "memory");
+}
+__device__ __forceinline__ void st_dsmem_f64(uint32_t addr, double v) {
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
+}
+
+__global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const OrthClusterParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = align_1024(smem_raw);
+    const uint32_t blocks = static_cast<uint32_t>(p.slice) / 64u;
+    uint8_t* xs = smem;                                            // X
+    uint8_t* ps = smem + blocks * kOrthBlockBytes;                 // X X^T
+    uint8_t* qs = ps + kOrthSquareBytes;                           // polynomial
+    float* parts = reinterpret_cast<float*>(ps);                   // [C][128 / C][128] over both
+    uint64_t* bars = reinterpret_cast<uint64_t*>(qs + kOrthSquareBytes);   // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* factor = reinterpret_cast<float*>(tmem_slot + 2);
+    double* warp_sums = reinterpret_cast<double*>(bars + 4);       // [8]
+    double* cta_sums = warp_sums + 8;                              // [16]
+
+    const uint32_t warp = warp_index(), lane = threadIdx.x & 31u;
+    const uint32_t rank = cluster_ctarank();
+    uint32_t ctas;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+    auto join_cluster = [&]() {
+        __syncwarp();
+        cluster_sync();
+    };
+    const long long base = blockIdx.y * p.batch_stride;
+    const int side = p.side, n16 = (side + 15) / 16 * 16;
+    const int first = static_cast<int>(rank) * p.slice;
+    const int valid = max(0, min(p.slice, p.length - first));      // columns of this slice inside X
+
+    if (threadIdx.x == 0) {
+        mbar_init(&bars[0], 1u);
+        mbar_init(&bars[1], 1u);
+        *abort_flag = 0;
+        mbar_init_fence();
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    for (uint32_t i = threadIdx.x; i < blocks * (kOrthBlockBytes / 16u); i += kOrthThreads)
+        reinterpret_cast<uint4*>(xs)[i] = make_uint4(0u, 0u, 0u, 0u);
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    grid_dependents_launch();
+    grid_dependency_wait();
+    const WaitCtl wc{abort_flag, p.status, p.timeout_ns};
+
+    // Rows of the walk (of g: its contiguous dimension across lanes), eight
+    // elements of a row a lane and turn.
+    const int outer = p.tall ? valid : side, inner = p.tall ? side : valid;
+    auto address = [&](int o, int i) {
+        return base + (p.tall ? (static_cast<long long>(first) + o) * p.ld + i : o * p.ld + first + i);
+    };
+    double sum = 0.;
+    for (int o = static_cast<int>(warp); o < outer; o += kOrthThreads / 32)
+        for (int i0 = static_cast<int>(lane); i0 < inner; i0 += 256) {
+            float v[8], top = 0.f, s = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = i0 + 32 * j < inner ? to_f32(p.g, address(o, i0 + 32 * j), p.bf16) : 0.f;
+                top = fmaxf(top, fabsf(v[j]));
+            }
+            // As in orth_square_kernel: no size of element overflows or is lost.
+            const uint32_t e = __float_as_uint(top) & 0x7f800000u;
+            const bool plain = e >= 0x01000000u && e < 0x7e800000u;
+            const float down = plain ? __uint_as_float(0x7f000000u - e) : 1.f;
+            const double up = plain ? static_cast<double>(__uint_as_float(e)) : 1.;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s = fmaf(v[j] * down, v[j] * down, s);
+            sum += static_cast<double>(s) * up * up;
+        }
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) warp_sums[warp] = sum;
+    __syncthreads();
+    if (ctas > 1) join_cluster();   // every CTA of the cluster runs before it is written to
+    if (threadIdx.x < ctas) {
+        sum = 0.;
+        for (int i = 0; i < kOrthThreads / 32; ++i) sum += warp_sums[i];
+        st_dsmem_f64(map_to_rank(smem_addr(&cta_sums[rank]), threadIdx.x), sum);
+    }
+    if (ctas > 1) join_cluster();
+    else __syncthreads();
+    if (threadIdx.x == 0) {
+        sum = 0.;
+        for (uint32_t i = 0; i < ctas; ++i) sum += cta_sums[i];
+        *factor = static_cast<float>(static_cast<double>(kOrthScale) / (sqrt(sum) + p.eps));
+    }
+    __syncthreads();
+    const float f = *factor;
+    for (int o = static_cast<int>(warp); o < outer; o += kOrthThreads / 32)
+#pragma unroll 8
+        for (int i = static_cast<int>(lane); i < inner; i += 32) {
+            const uint32_t row = static_cast<uint32_t>(p.tall ? i : o), col = static_cast<uint32_t>(p.tall ? o : i);
+            *reinterpret_cast<__half*>(xs + (col >> 6) * kOrthBlockBytes + swz128(row, (col & 63u) * 2u)) =
+                __float2half_rn(to_f32(p.g, address(o, i), p.bf16) * f);
+        }
+
+    const uint32_t x_addr = smem_addr(xs), p_addr = smem_addr(ps), q_addr = smem_addr(qs);
+    const uint32_t quarter = warp & 3u, group = warp >> 2;
+    const uint32_t row = quarter * 32u + lane;                     // of an accumulator: this thread's
+    const bool rows_used = static_cast<int>(quarter * 32u) < side;
+    const uint32_t t_row = tmem + ((quarter * 32u) << 16);
+    uint32_t phase[2] = {0u, 0u};
+    auto wait = [&](int i) {
+        mbar_wait(&bars[i], phase[i], wc);
+        phase[i] ^= 1u;
+        tc_fence_after_sync();
+    };
+    // Shared-memory writes of all threads before, MMAs after.
+    auto hand_over = [&]() {
+        fence_async_shared();
+        tc_fence_before_sync();
+        __syncthreads();
+        tc_fence_after_sync();
+    };
+    // 32 columns from `col` of this thread's row in a square matrix, as FP16.
+    auto put_square = [&](uint8_t* dst, uint32_t col, const float (&v)[32]) {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            uint4 w;
+            w.x = pack2(v[8 * j], v[8 * j + 1], 0);
+            w.y = pack2(v[8 * j + 2], v[8 * j + 3], 0);
+            w.z = pack2(v[8 * j + 4], v[8 * j + 5], 0);
+            w.w = pack2(v[8 * j + 6], v[8 * j + 7], 0);
+            *reinterpret_cast<uint4*>(dst + (col >> 6) * kOrthBlockBytes + swz128(row, (col & 63u) * 2u + 16u * j)) = w;
+        }
+    };
+    auto get_row = [&](const uint8_t* src, uint32_t col, float (&v)[32]) {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            const uint4 w = *reinterpret_cast<const uint4*>(src + (col >> 6) * kOrthBlockBytes +
+                                                            swz128(row, (col & 63u) * 2u + 16u * j));
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 h = unpack2(u[i], 0);
+                v[8 * j + 2 * i] = h.x;
+                v[8 * j + 2 * i + 1] = h.y;
+            }
+        }
+    };
+    const uint32_t square_idesc = make_idesc_f16(128, 0, false, false) | (static_cast<uint32_t>(n16 >> 3) << 17);
+    const float inv = 1.f / kOrthScale;
+    const uint32_t own = 128u / ctas;                              // rows of X X^T that this CTA sums
+
+    for (int step = 0; step < p.steps; ++step) {
+        const bool last = step + 1 == p.steps;
+        // X X^T of this slice.
+        hand_over();
+        if (warp == 0) {
+            const uint32_t issuer = elect_lane();
+            uint32_t add = 0;
+            for (uint32_t j = 0; j < blocks; ++j) {
+                const uint64_t d = make_smem_desc(x_addr + j * kOrthBlockBytes, 16u, 1024u);
+#pragma unroll
+                for (uint32_t kk = 0; kk < 4; ++kk) {
+                    tc_mma_if<false>(issuer, tmem, d + kk * 2u, d + kk * 2u, square_idesc, add);
+                    add = 1;
+                }
+            }
+            tc_commit_if<false>(issuer, smem_addr(&bars[0]));
+        }
+        wait(0);
+        if (ctas == 1) {
+            for (uint32_t c = 32u * group; rows_used && static_cast<int>(c) < n16; c += 64u) {
+                float v[32];
+                tmem_ld32(t_row + c, v);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] *= inv * inv;
+                put_square(ps, c, v);
+            }
+        } else {
+            // The other CTAs' polynomial products are done (barrier of the last
+            // step's end), so their squares may be written over.
+            for (uint32_t c = 32u * group; rows_used && static_cast<int>(c) < n16; c += 64u) {
+                float v[32];
+                tmem_ld32(t_row + c, v);
+                const uint32_t dst = map_to_rank(smem_addr(parts + (rank * own + row % own) * 128u + c), row / own);
+#pragma unroll
+                for (uint32_t i = 0; i < 32; i += 4) st_dsmem_f4(dst + i * 4u, v[i], v[i + 1], v[i + 2], v[i + 3]);
+            }
+            tc_fence_before_sync();
+            join_cluster();
+            // Sums of this CTA's rows, four columns a thread and turn (at most 8).
+            float4 acc[8];
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) {
+                const uint32_t q = k * kOrthThreads + threadIdx.x;
+                acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (q >= own * 32u) break;
+                const float4* src = reinterpret_cast<const float4*>(parts) + q;
+                for (uint32_t r = 0; r < ctas; ++r) {
+                    const float4 w = src[r * own * 32u];
+                    acc[k].x += w.x; acc[k].y += w.y; acc[k].z += w.z; acc[k].w += w.w;
+                }
+            }
+            join_cluster();
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) {
+                const uint32_t q = k * kOrthThreads + threadIdx.x;
+                if (q >= own * 32u) break;
+                const uint32_t r = rank * own + q / 32u, col = (q & 31u) * 4u;
+                const bool wanted = static_cast<int>(r) < n16 && static_cast<int>(col) < n16;
+                const uint32_t lo = pack2(acc[k].x * inv * inv, acc[k].y * inv * inv, 0);
+                const uint32_t hi = pack2(acc[k].z * inv * inv, acc[k].w * inv * inv, 0);
+                const uint32_t at = p_addr + (col >> 6) * kOrthBlockBytes + swz128(r, (col & 63u) * 2u);
+                for (uint32_t to = 0; wanted && to < ctas; ++to) st_dsmem_b64(map_to_rank(at, to), lo, hi);
+            }
+            // The rows come from other CTAs: each side orders them towards the MMAs.
+            fence_async_shared();
+            join_cluster();
+        }
+        // b P + c P P
+        hand_over();
+        if (warp == 0) {
+            const uint32_t issuer = elect_lane();
+            for (int k = 0; k < n16; k += 16) {
+                const uint64_t d = make_smem_desc(p_addr + (k >> 6) * kOrthBlockBytes, 16u, 1024u) + ((k & 63) >> 3);
+                tc_mma_if<false>(issuer, tmem + 256u, d, d, square_idesc, k > 0 ? 1u : 0u);
+            }
+            tc_commit_if<false>(issuer, smem_addr(&bars[0]));
+        }
+        wait(0);
+        for (uint32_t c = 32u * group; rows_used && static_cast<int>(c) < n16; c += 64u) {
+            float v[32], w[32];
+            tmem_ld32(t_row + 256u + c, v);
+            get_row(ps, c, w);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = fmaf(p.c, v[i], p.b * w[i]);
+            put_square(qs, c, v);
+        }
+        // X <- a X + poly X, 256 columns at a time, two accumulators in turn.
+        hand_over();
+        const int turns = (p.slice + 255) / 256;
+        auto update = [&](int turn) {
+            if (warp != 0) return;
+            const uint32_t issuer = elect_lane();
+            const int width = min(256, p.slice - 256 * turn);
+            const uint32_t idesc = make_idesc_f16(128, 0, false, true) | (static_cast<uint32_t>(width >> 3) << 17);
+            const uint64_t db = make_smem_desc(x_addr + turn * 4 * kOrthBlockBytes, kOrthBlockBytes, 1024u);
+            for (int k = 0; k < n16; k += 16) {
+                const uint64_t da = make_smem_desc(q_addr + (k >> 6) * kOrthBlockBytes, 16u, 1024u) + ((k & 63) >> 3);
+                tc_mma_if<false>(issuer, tmem + (turn & 1) * 256u, da, db + static_cast<uint64_t>(k) * 8u, idesc,
+                                 k > 0 ? 1u : 0u);
+            }
+            tc_commit_if<false>(issuer, smem_addr(&bars[turn & 1]));
+        };
+        update(0);
+        if (turns > 1) update(1);
+        for (int turn = 0; turn < turns; ++turn) {
+            wait(turn & 1);
+            const uint32_t width = static_cast<uint32_t>(min(256, p.slice - 256 * turn));
+            for (uint32_t c = 32u * group; rows_used && c < width; c += 64u) {
+                const uint32_t col = 256u * turn + c;
+                if (static_cast<int>(col) >= valid) break;
+                float v[32], w[32];
+                tmem_ld32(t_row + (turn & 1) * 256u + c, v);
+                get_row(xs, col, w);
+                const float a = last ? p.a * inv : p.a, scale = last ? inv : 1.f;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = fmaf(scale, v[i], a * w[i]);
+                if (static_cast<int>(row) < side && !last) put_square(xs, col, v);
+                if (static_cast<int>(row) < side && last) {
+                    // Tall: lanes are neighbours in a row of the output; else a lane has 32 of them.
+                    const long long at = static_cast<long long>(blockIdx.y) * side * p.length;
+                    const int left = valid - static_cast<int>(col);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        if (i >= left) break;
+                        const long long l = first + static_cast<int>(col) + i;
+                        const long long k = at + (p.tall ? l * side + row : static_cast<long long>(row) * p.length + l);
+                        if (p.bf16) static_cast<__nv_bfloat16*>(p.out)[k] = __float2bfloat16_rn(v[i]);
+                        else static_cast<__half*>(p.out)[k] = __float2half_rn(v[i]);
+                    }
+                }
+                __syncwarp();
+            }
+            if (turn + 2 < turns) {
+                tc_fence_before_sync();
+                __syncthreads();
+                tc_fence_after_sync();
+                update(turn + 2);
+            }
+        }
+        // No CTA's squares are written over while it still multiplies with them.
+        if (ctas > 1) {
+            tc_fence_before_sync();
+            join_cluster();
+        }
+    }
+    tc_fence_before_sync();
+    if (ctas > 1) join_cluster();
+    else __syncthreads();
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
 }  // namespace hgemm

@@ -848,6 +848,50 @@ OrthPlan plan_orth(const HgemmSm100Orthogonalize& a) {
     return q;
 }
 
+// The one-launch form for a shorter side of at most 128 rows: CTAs of a cluster
+// (each 128 rows x `slice` columns), 0 where it does not fit.
+int orth_cluster_ctas(const HgemmSm100Orthogonalize& a) {
+    const int64_t side = std::min(a.rows, a.cols), length = std::max(a.rows, a.cols);
+    if (a.common.tile != 0 || a.steps < 1 || side > 128) return 0;
+    for (int n : {1, 2, 4, 8, 16})
+        if (round_up(cdiv(length, n), 64) <= kOrthMaxSlice) return n;
+    return 0;
+}
+
+std::atomic<uint64_t> g_orth_ready{0};
+
+int run_orth_cluster(const HgemmSm100Orthogonalize& a, int ctas, const Context& c) {
+    const uint64_t bit = 1ull << c.id;
+    if (!(g_orth_ready.load(std::memory_order_acquire) & bit)) {
+        const void* fn = reinterpret_cast<const void*>(&orth_cluster_kernel);
+        if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kOrthMaxSmem)) !=
+                cudaSuccess ||
+            cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+            return HGEMM_SM100_ERR_LAUNCH;
+        g_orth_ready.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    OrthClusterParams p{};
+    p.g = a.g;
+    p.out = a.out;
+    p.batch_stride = a.batch_stride;
+    p.ld = a.ldg;
+    p.side = static_cast<int>(std::min(a.rows, a.cols));
+    p.length = static_cast<int>(std::max(a.rows, a.cols));
+    p.tall = a.rows > a.cols;
+    p.slice = static_cast<int>(round_up(cdiv(p.length, ctas), 64));
+    p.bf16 = a.common.dtype == HGEMM_SM100_TRAIN_BF16;
+    p.steps = a.steps;
+    p.a = a.a;
+    p.b = a.b;
+    p.c = a.c;
+    p.eps = a.eps;
+    p.status = a.common.status != nullptr ? a.common.status : c.dev->status_word;
+    p.timeout_ns = a.common.timeout_ns != 0 ? a.common.timeout_ns : kDefaultTimeoutNs;
+    const size_t smem = static_cast<size_t>(p.slice / 64) * kOrthBlockBytes + 2 * kOrthSquareBytes + 1024 + 512;
+    return launch(&orth_cluster_kernel, dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(a.batch)),
+                  dim3(kOrthThreads), smem, ctas, c.stream, p);
+}
+
 bool orth_sizes_ok(const HgemmSm100Orthogonalize& a) {
     return a.batch > 0 && a.batch <= 65535 && size_ok(a.rows) && size_ok(a.cols) && a.steps >= 0;
 }
@@ -855,19 +899,23 @@ bool orth_sizes_ok(const HgemmSm100Orthogonalize& a) {
 }  // namespace
 
 extern "C" size_t hgemm_sm100_orthogonalize_workspace(const HgemmSm100Orthogonalize* a) {
-    return a != nullptr && orth_sizes_ok(*a) ? plan_orth(*a).bytes() : 0;
+    if (a == nullptr || !orth_sizes_ok(*a) || orth_cluster_ctas(*a) > 0) return 0;
+    return plan_orth(*a).bytes();
 }
 
 extern "C" int hgemm_sm100_orthogonalize(const HgemmSm100Orthogonalize* a, void* stream) {
     if (a == nullptr || !orth_sizes_ok(*a) || a->g == nullptr || a->out == nullptr || a->ldg < a->cols ||
-        a->batch_stride < 0 || a->workspace == nullptr || reinterpret_cast<uintptr_t>(a->workspace) % 256 != 0 ||
-        !(a->eps >= 0))
+        a->batch_stride < 0 || !(a->eps >= 0))
+        return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    const OrthPlan q = plan_orth(*a);
+    const int ctas = orth_cluster_ctas(*a);
+    if (ctas == 0 && (a->workspace == nullptr || reinterpret_cast<uintptr_t>(a->workspace) % 256 != 0 ||
+                      a->workspace_bytes < q.bytes()))
         return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     Context c;
     int rc = begin(&c, a->common, stream);
     if (rc != HGEMM_SM100_OK) return rc;
-    const OrthPlan q = plan_orth(*a);
-    if (a->workspace_bytes < q.bytes()) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+    if (ctas > 0) return run_orth_cluster(*a, ctas, c);
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     double* sums = reinterpret_cast<double*>(ws);
     uint16_t* x = reinterpret_cast<uint16_t*>(ws + q.sum_bytes);

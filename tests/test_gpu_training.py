@@ -446,12 +446,25 @@ def test_orthogonalize(size, dtype):
     assert float(torch.linalg.vector_norm(got.double() - value)) <= err
 
 
+@pytest.mark.parametrize("turn", [False, True], ids=["wide", "tall"])
+@pytest.mark.parametrize("size", [(1, 640), (2, 641), (17, 1280), (128, 1283), (31, 2560), (96, 2600), (65, 5119),
+                                  (128, 9728), (48, 10240), (33, 10241), (128, 64), (129, 300)], ids=str)
+def test_orthogonalize_one_launch_and_its_limits(size, turn):
+    """A shorter side of at most 128 is one launch of 1 to 16 CTAs a matrix; around its limits."""
+    g = normal(11, 3, *(size[::-1] if turn else size), dtype=torch.bfloat16)
+    out = llm_hgemm.orthogonalize(g)
+    for k in range(3):
+        value, err = ref.orthogonalize(g[k], 5, NEWTON_SCHULZ, 1e-7)
+        assert float(torch.linalg.vector_norm(out[k].double() - value)) <= err
+
+
 @pytest.mark.parametrize("batch", [(1,), (3,), (4,), (5,), (2, 3)], ids=str)
 def test_orthogonalize_batches_and_strides(batch):
-    g = normal(6, *batch, 40, 77, scale=0.1)
-    got = llm_hgemm.orthogonalize(g)
-    for k, m in enumerate(g.view(-1, 40, 77)):
-        assert torch.equal(got.view(-1, 40, 77)[k], llm_hgemm.orthogonalize(m))
+    for size in ((40, 77), (150, 177)):
+        g = normal(6, *batch, *size, scale=0.1)
+        got = llm_hgemm.orthogonalize(g)
+        for k, m in enumerate(g.view(-1, *size)):
+            assert torch.equal(got.view(-1, *size)[k], llm_hgemm.orthogonalize(m))
     wide = normal(7, *batch, 50, 200, scale=0.1)
     assert torch.equal(llm_hgemm.orthogonalize(wide[..., 3:43, 5:82]), llm_hgemm.orthogonalize(wide[..., 3:43, 5:82].contiguous()))
     assert torch.equal(llm_hgemm.orthogonalize(g.mT), llm_hgemm.orthogonalize(g.mT.contiguous()))

@@ -87,7 +87,7 @@ def test_c_abi_refuses_loss_gradient_arguments(change):
 ], ids=str)
 def test_c_abi_refuses_orthogonalize_arguments(change):
     p = 1 << 20
-    a = train_capi.Orthogonalize(train_capi.Common(), p, p, p, 1 << 30, 1, 8, 8, 8, 0, 5, 0, *NEWTON_SCHULZ, 0.0, 1e-7)
+    a = train_capi.Orthogonalize(train_capi.Common(), p, p, p, 1 << 30, 1, 200, 300, 300, 0, 5, 0, *NEWTON_SCHULZ, 0.0, 1e-7)
     for k, v in change.items():
         setattr(a, k, v)
     assert train_capi.run("orthogonalize", a) == capi.ERR_INVALID_ARGUMENT
@@ -98,9 +98,12 @@ def test_null_arguments_and_workspaces():
     for name in ("ffn_forward", "ffn_backward", "loss_forward", "loss_backward", "orthogonalize"):
         assert getattr(lib, f"hgemm_sm100_{name}")(None, None) == capi.ERR_INVALID_ARGUMENT
         assert getattr(lib, f"hgemm_sm100_{name}_workspace")(None) == 0
-    o = train_capi.Orthogonalize(batch=2, rows=100, cols=300)
+    o = train_capi.Orthogonalize(batch=2, rows=200, cols=300, steps=5)
     # X twice and two square matrices, rows padded to 64 elements.
-    assert train_capi.workspace("orthogonalize", o) >= 2 * 2 * (2 * 100 * 320 + 2 * 100 * 128)
+    assert train_capi.workspace("orthogonalize", o) >= 2 * 2 * (2 * 200 * 320 + 2 * 200 * 256)
+    # One launch that keeps everything on chip.
+    o.rows = 128
+    assert train_capi.workspace("orthogonalize", o) == 0
 
 
 def test_module_refuses_other_linears():
