@@ -35,7 +35,8 @@ enum { HGEMM_SM100_TRAIN_F16 = 0, HGEMM_SM100_TRAIN_BF16 = 1 };
  * library chooses; else columns (a multiple of 64 up to 256), plus
  * HGEMM_SM100_TRAIN_TILE_PAIR for CTA pairs (256 rows instead of 128).
  * `splits` forces into how many parts the long sums (y, dx) are cut: 0 = the
- * library chooses, at most 16. Workspace queries take both into account. */
+ * library chooses, at most 16; for a small orthogonalised matrix the CTAs of
+ * its cluster (1, 2, 4, 8 or 16). Workspace queries take both into account. */
 #define HGEMM_SM100_TRAIN_TILE_PAIR 0x1000
 typedef struct HgemmSm100TrainCommon {
     int32_t dtype;        /* HGEMM_SM100_TRAIN_F16 / _BF16                     */

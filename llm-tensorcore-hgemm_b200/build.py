@@ -121,7 +121,7 @@ def _torch_flags() -> tuple[list[str], list[str]]:
     cflags += [f"-I{p}" for p in cpp_extension.include_paths()]
     lib_dirs = cpp_extension.library_paths()
     ldflags = [f"-L{p}" for p in lib_dirs] + [f"-Wl,-rpath,{p}" for p in lib_dirs]
-    ldflags += ["-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10_cuda"]
+    ldflags += ["-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10_cuda"]
     return cflags, ldflags
 
 

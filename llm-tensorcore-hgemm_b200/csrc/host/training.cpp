@@ -1,6 +1,7 @@
 // Argument checks, autograd and launches of the training operators.
 #include "training.h"
 
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -65,9 +66,15 @@ void no_double_backward(const char* what) {
     TORCH_CHECK(!torch::GradMode::is_enabled(), what, " has no second derivative (create_graph=True)");
 }
 
-Tensor bytes(size_t n, const Tensor& like) {
-    return torch::empty({static_cast<int64_t>(n)}, like.options().dtype(torch::kUInt8));
+// An uninitialised tensor on the device of `like`, without the dispatcher's way.
+Tensor fresh(at::IntArrayRef shape, torch::ScalarType dtype, const Tensor& like) {
+    return at::detail::empty_cuda(shape, dtype, like.device(), std::nullopt);
 }
+
+Tensor bytes(size_t n, const Tensor& like) { return fresh({static_cast<int64_t>(n)}, torch::kUInt8, like); }
+
+// [tokens, n] view of an activation.
+Tensor rows_of(const Tensor& t, int64_t tokens, int64_t n) { return t.dim() == 2 ? t : t.reshape({tokens, n}); }
 
 // ------------------------------------------------------------ feed-forward --
 
@@ -89,22 +96,22 @@ FfnSizes ffn_sizes(const Tensor& x, const Tensor& gate, const Tensor& down) {
 }
 
 struct FfnForward {
-    Tensor y, h, gate_pre, up_pre;   // padded sizes
+    Tensor y;
+    Tensor kept;   // [tokens, inter] (h), or [3, tokens, inter]: h, gate and up pre-activations; padded sizes
 };
 
 FfnForward ffn_forward(const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, const FfnSizes& s,
                        bool keep) {
     const c10::cuda::CUDAGuard device_guard(x.device());
-    const Tensor xp = operand(x.reshape({s.tokens, s.hidden}), s.tokens, s.hidden8, false);
+    const Tensor xp = operand(rows_of(x, s.tokens, s.hidden), s.tokens, s.hidden8, false);
     const Tensor gp = operand(gate, s.inter8, s.hidden8, true), up_ = operand(up, s.inter8, s.hidden8, true);
     const Tensor dp = operand(down, s.out8, s.inter8, true);
     FfnForward r;
-    r.y = torch::empty({s.tokens, s.out8}, x.options());
-    r.h = torch::empty({s.tokens, s.inter8}, x.options());
-    if (keep) {
-        r.gate_pre = torch::empty_like(r.h);
-        r.up_pre = torch::empty_like(r.h);
-    }
+    const torch::ScalarType dtype = x.scalar_type();
+    const int64_t plane = s.tokens * s.inter8 * 2;   // a multiple of 16 bytes
+    r.y = fresh({s.tokens, s.out8}, dtype, x);
+    r.kept = keep ? fresh({3, s.tokens, s.inter8}, dtype, x) : fresh({s.tokens, s.inter8}, dtype, x);
+    uint8_t* kept = static_cast<uint8_t*>(r.kept.data_ptr());
     HgemmSm100FfnForward a{};
     a.common = common_of(x);
     a.x = xp.data_ptr();
@@ -112,9 +119,9 @@ FfnForward ffn_forward(const Tensor& x, const Tensor& gate, const Tensor& up, co
     a.up = up_.data_ptr();
     a.down = dp.data_ptr();
     a.y = r.y.data_ptr();
-    a.h = r.h.data_ptr();
-    a.gate_pre = keep ? r.gate_pre.data_ptr() : nullptr;
-    a.up_pre = keep ? r.up_pre.data_ptr() : nullptr;
+    a.h = kept;
+    a.gate_pre = keep ? kept + plane : nullptr;
+    a.up_pre = keep ? kept + 2 * plane : nullptr;
     a.tokens = s.tokens;
     a.hidden = s.hidden8;
     a.inter = s.inter8;
@@ -141,8 +148,9 @@ class GatedFfn : public torch::autograd::Function<GatedFfn> {
                           const Tensor& down) {
         const FfnSizes s = ffn_sizes(x, gate, down);
         FfnForward r = ffn_forward(x, gate, up, down, s, true);
-        ctx->save_for_backward({x, gate, up, down, r.gate_pre, r.up_pre, r.h});
-        return cut(r.y, s.tokens, s.out).view(with_last(x, s.out));
+        ctx->save_for_backward({x, gate, up, down, r.kept});
+        const Tensor y = cut(r.y, s.tokens, s.out);
+        return x.dim() == 2 ? y : y.view(with_last(x, s.out));
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -152,18 +160,21 @@ class GatedFfn : public torch::autograd::Function<GatedFfn> {
         const FfnSizes s = ffn_sizes(x, gate, down);
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
         const c10::cuda::CUDAGuard device_guard(x.device());
-        const Tensor dy = operand(grads[0].to(x.scalar_type()).reshape({s.tokens, s.out}), s.tokens, s.out8, false);
-        const Tensor xp = operand(x.reshape({s.tokens, s.hidden}), s.tokens, s.hidden8, false);
+        const Tensor dy = operand(rows_of(grads[0], s.tokens, s.out), s.tokens, s.out8, false);
+        const Tensor xp = operand(rows_of(x, s.tokens, s.hidden), s.tokens, s.hidden8, false);
         const Tensor gp = operand(gate, s.inter8, s.hidden8, true), up_ = operand(up, s.inter8, s.hidden8, true);
         const Tensor dp = operand(down, s.out8, s.inter8, true);
         const bool need_x = ctx->needs_input_grad(0), need_g = ctx->needs_input_grad(1);
         const bool need_u = ctx->needs_input_grad(2), need_d = ctx->needs_input_grad(3);
-        const Tensor dg = torch::empty_like(v[4]), du = torch::empty_like(v[4]);
+        const torch::ScalarType dtype = x.scalar_type();
+        const int64_t plane = s.tokens * s.inter8 * 2;
+        const uint8_t* kept = static_cast<const uint8_t*>(v[4].const_data_ptr());
+        const Tensor pre = fresh({2, s.tokens, s.inter8}, dtype, x);
         Tensor dx, dgate, dup, ddown;
-        if (need_x) dx = torch::empty({s.tokens, s.hidden8}, x.options());
-        if (need_g) dgate = torch::empty({s.inter8, s.hidden8}, x.options());
-        if (need_u) dup = torch::empty({s.inter8, s.hidden8}, x.options());
-        if (need_d) ddown = torch::empty({s.out8, s.inter8}, x.options());
+        if (need_x) dx = fresh({s.tokens, s.hidden8}, dtype, x);
+        if (need_g) dgate = fresh({s.inter8, s.hidden8}, dtype, x);
+        if (need_u) dup = fresh({s.inter8, s.hidden8}, dtype, x);
+        if (need_d) ddown = fresh({s.out8, s.inter8}, dtype, x);
         HgemmSm100FfnBackward a{};
         a.common = common_of(x);
         a.dy = dy.data_ptr();
@@ -171,11 +182,11 @@ class GatedFfn : public torch::autograd::Function<GatedFfn> {
         a.gate = gp.data_ptr();
         a.up = up_.data_ptr();
         a.down = dp.data_ptr();
-        a.gate_pre = v[4].data_ptr();
-        a.up_pre = v[5].data_ptr();
-        a.h = v[6].data_ptr();
-        a.dgate_pre = dg.data_ptr();
-        a.dup_pre = du.data_ptr();
+        a.h = kept;
+        a.gate_pre = kept + plane;
+        a.up_pre = kept + 2 * plane;
+        a.dgate_pre = pre.data_ptr();
+        a.dup_pre = static_cast<uint8_t*>(pre.data_ptr()) + plane;
         a.dx = need_x ? dx.data_ptr() : nullptr;
         a.dgate = need_g ? dgate.data_ptr() : nullptr;
         a.dup = need_u ? dup.data_ptr() : nullptr;
@@ -193,7 +204,8 @@ class GatedFfn : public torch::autograd::Function<GatedFfn> {
         }
         check_status(hgemm_sm100_ffn_backward(&a, c10::cuda::getCurrentCUDAStream(x.get_device()).stream()),
                      "gated_ffn backward");
-        if (need_x) dx = cut(dx, s.tokens, s.hidden).view(x.sizes());
+        if (need_x) dx = cut(dx, s.tokens, s.hidden);
+        if (need_x && x.dim() != 2) dx = dx.view(x.sizes());
         if (need_g) dgate = cut(dgate, s.inter, s.hidden);
         if (need_u) dup = cut(dup, s.inter, s.hidden);
         if (need_d) ddown = cut(ddown, s.out, s.inter);
@@ -211,12 +223,11 @@ LossForward loss_forward(const Tensor& x, const Tensor& weight, const Tensor& ta
                          int32_t reduction, int64_t ignore_index) {
     const c10::cuda::CUDAGuard device_guard(x.device());
     const int64_t hidden = weight.size(1), hidden8 = round8(hidden);
-    const Tensor xp = operand(x.reshape({tokens, hidden}), tokens, hidden8, false);
+    const Tensor xp = operand(rows_of(x, tokens, hidden), tokens, hidden8, false);
     const Tensor wp = operand(weight, weight.size(0), hidden8, true);
-    const auto f32 = x.options().dtype(torch::kFloat32);
     LossForward r;
-    r.lse = torch::empty({tokens}, f32);
-    r.loss = reduction == HGEMM_SM100_LOSS_NONE ? torch::empty({tokens}, f32) : torch::empty({}, f32);
+    r.lse = fresh({tokens}, torch::kFloat32, x);
+    r.loss = reduction == HGEMM_SM100_LOSS_NONE ? fresh({tokens}, torch::kFloat32, x) : fresh({}, torch::kFloat32, x);
     HgemmSm100LossForward a{};
     a.common = common_of(x);
     a.x = xp.data_ptr();
@@ -257,13 +268,13 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
         const Tensor &x = v[0], &weight = v[1], &target = v[2], &lse = v[3];
         const c10::cuda::CUDAGuard device_guard(x.device());
         const int64_t tokens = target.numel(), hidden = weight.size(1), hidden8 = round8(hidden);
-        const Tensor xp = operand(x.reshape({tokens, hidden}), tokens, hidden8, false);
+        const Tensor xp = operand(rows_of(x, tokens, hidden), tokens, hidden8, false);
         const Tensor wp = operand(weight, weight.size(0), hidden8, true);
-        const Tensor dloss = grads[0].to(torch::kFloat32).contiguous();
+        const Tensor dloss = grads[0].contiguous();
         const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
         Tensor dx, dw;
-        if (need_x) dx = torch::empty({tokens, hidden8}, x.options());
-        if (need_w) dw = torch::empty({weight.size(0), hidden8}, x.options());
+        if (need_x) dx = fresh({tokens, hidden8}, x.scalar_type(), x);
+        if (need_w) dw = fresh({weight.size(0), hidden8}, x.scalar_type(), x);
         HgemmSm100LossBackward a{};
         a.common = common_of(x);
         a.x = xp.data_ptr();
@@ -284,7 +295,8 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
         a.workspace = ws.data_ptr();
         check_status(hgemm_sm100_loss_backward(&a, c10::cuda::getCurrentCUDAStream(x.get_device()).stream()),
                      "linear_cross_entropy backward");
-        if (need_x) out[0] = cut(dx, tokens, hidden).view(x.sizes());
+        if (need_x) out[0] = cut(dx, tokens, hidden);
+        if (need_x && x.dim() != 2) out[0] = out[0].view(x.sizes());
         if (need_w) out[1] = cut(dw, weight.size(0), hidden);
         return out;
     }
@@ -339,12 +351,14 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
         return kind == HGEMM_SM100_LOSS_NONE ? each : kind == HGEMM_SM100_LOSS_MEAN ? each.mean() : each.sum();
     }
     const c10::cuda::CUDAGuard device_guard(x.device());
-    const Tensor flat = target.reshape({tokens}).to(torch::kInt64).contiguous();
+    Tensor flat = target.dim() == 1 ? target : target.reshape({tokens});
+    if (flat.scalar_type() != torch::kInt64) flat = flat.to(torch::kInt64);
+    flat = flat.contiguous();
     const bool keep = torch::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad());
     const Tensor loss = keep ? LinearCrossEntropy::apply(x, weight, flat, tokens, static_cast<int64_t>(kind),
                                                          ignore_index)
                              : loss_forward(x, weight, flat, tokens, kind, ignore_index).loss;
-    return kind == HGEMM_SM100_LOSS_NONE ? loss.view(target.sizes()) : loss;
+    return kind == HGEMM_SM100_LOSS_NONE && target.dim() != 1 ? loss.view(target.sizes()) : loss;
 }
 
 Tensor orthogonalize(const Tensor& g, int64_t steps, double a, double b, double c, double eps) {
@@ -357,7 +371,7 @@ Tensor orthogonalize(const Tensor& g, int64_t steps, double a, double b, double 
     TORCH_CHECK(eps >= 0 && std::isfinite(eps), "eps must be finite and not negative");
     const torch::NoGradGuard no_grad;
     const c10::cuda::CUDAGuard device_guard(g.device());
-    const Tensor out = torch::empty(g.sizes(), g.options());
+    const Tensor out = fresh(g.sizes(), g.scalar_type(), g);
     if (g.numel() == 0) return out;
     const int64_t rows = g.size(-2), cols = g.size(-1), batch = g.numel() / (rows * cols);
     TORCH_CHECK(batch <= 65535, "at most 65535 matrices in one call, got ", batch);

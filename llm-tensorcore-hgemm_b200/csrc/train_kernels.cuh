@@ -1008,10 +1008,10 @@ __global__ void __launch_bounds__(256) orth_copy_kernel(const void* __restrict__
 // rows, zeros below) in shared memory, each CTA `slice` columns of it, in the
 // 128-byte-swizzled blocks of 64 columns that serve tcgen05 both as K-major
 // operand of X X^T and as MN-major operand of poly X. Per step each CTA
-// multiplies its slice's part of X X^T; the parts meet in distributed shared
-// memory (CTA r sums rows [128 r / C, 128 (r + 1) / C) of all of them in the
-// order of the CTAs and hands the rounded rows to everyone); the polynomial is
-// computed by everyone; X is updated in place. Rounding as in the launches per
+// multiplies its slice's part of X X^T; the parts meet through distributed
+// shared memory (CTA r reads rows [128 r / C, 128 (r + 1) / C) of all of them,
+// adds them in the order of the CTAs and hands the rounded rows to everyone);
+// the polynomial is computed by everyone; X is updated in place. Rounding as in the launches per
 // product: FP16 X, X X^T and polynomial, FP32 sums.
 // A wait that runs out is recorded and the rest runs on without waiting, since
 // all CTAs have to reach the same cluster barriers.
@@ -1030,6 +1030,7 @@ struct OrthClusterParams {
     int tall;              // the longer side is the rows of g
     int slice;             // columns of X per CTA, a multiple of 64
     int bf16, steps;
+    int vec_in, vec_out;   // rows of g / out are 16-byte aligned whole vectors
     float a, b, c;
     double eps;
     int* status;
@@ -1039,10 +1040,17 @@ struct OrthClusterParams {
 __device__ __forceinline__ void st_dsmem_b64(uint32_t addr, uint32_t lo, uint32_t hi) {
     asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(lo), "r"(hi) : "memory");
 }
+__device__ __forceinline__ float4 ld_dsmem_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ void st_dsmem_f64(uint32_t addr, double v) {
     asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
 }
 
+template <uint32_t ctas>
 __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const OrthClusterParams p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align_1024(smem_raw);
@@ -1050,7 +1058,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const Ort
     uint8_t* xs = smem;                                            // X
     uint8_t* ps = smem + blocks * kOrthBlockBytes;                 // X X^T
     uint8_t* qs = ps + kOrthSquareBytes;                           // polynomial
-    float* parts = reinterpret_cast<float*>(ps);                   // [C][128 / C][128] over both
+    float* parts = reinterpret_cast<float*>(ps);                   // [128][128] over both
     uint64_t* bars = reinterpret_cast<uint64_t*>(qs + kOrthSquareBytes);   // [2]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -1060,8 +1068,6 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const Ort
 
     const uint32_t warp = warp_index(), lane = threadIdx.x & 31u;
     const uint32_t rank = cluster_ctarank();
-    uint32_t ctas;
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
     auto join_cluster = [&]() {
         __syncwarp();
         cluster_sync();
@@ -1091,30 +1097,71 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const Ort
     grid_dependency_wait();
     const WaitCtl wc{abort_flag, p.status, p.timeout_ns};
 
-    // Rows of the walk (of g: its contiguous dimension across lanes), eight
-    // elements of a row a lane and turn.
-    const int outer = p.tall ? valid : side, inner = p.tall ? side : valid;
-    auto address = [&](int o, int i) {
-        return base + (p.tall ? (static_cast<long long>(first) + o) * p.ld + i : o * p.ld + first + i);
+    // Where element (s, l) of X lies in shared memory; l counts from this slice.
+    auto x_at = [&](int s, int l) {
+        return xs + (l >> 6) * kOrthBlockBytes + swz128(static_cast<uint32_t>(s), (l & 63) * 2u);
     };
+    // and in g / out, rows `ld` elements apart.
+    auto far = [&](long long ld, int s, int l) {
+        return p.tall ? (static_cast<long long>(first) + l) * ld + s : s * ld + first + l;
+    };
+    // Every piece of eight neighbours of a row of g (vector form) or every
+    // element, spread over the threads: work(s, l, count). Wide: threads go
+    // along the rows. Tall: in the vector form lanes take 32 rows of g, so that
+    // their shared-memory accesses are neighbours; else lanes go along a row.
+    auto walk = [&](bool vec, auto&& work) {
+        if (vec && !p.tall) {
+            const int per = valid / 8, n = per * side;
+#pragma unroll 4
+            for (int q = static_cast<int>(threadIdx.x); q < n; q += kOrthThreads) work(q / per, q % per * 8);
+        } else if (vec) {
+            const int per = side / 8, n = per * ((valid + 31) / 32);
+#pragma unroll 4
+            for (int q = static_cast<int>(warp); q < n; q += kOrthThreads / 32) {
+                const int l = q / per * 32 + static_cast<int>(lane);
+                if (l < valid) work(q % per * 8, l);
+            }
+        } else {
+            const int per = p.tall ? side : valid, n = side * valid;
+#pragma unroll 8
+            for (int q = static_cast<int>(threadIdx.x); q < n; q += kOrthThreads) {
+                const int o = q / per, i = q - o * per;
+                work(p.tall ? i : o, p.tall ? o : i);
+            }
+        }
+    };
+    // Raw elements into place, and the sum of squares (in 64 bits by pieces, as
+    // in orth_square_kernel: no size of element overflows or is lost).
     double sum = 0.;
-    for (int o = static_cast<int>(warp); o < outer; o += kOrthThreads / 32)
-        for (int i0 = static_cast<int>(lane); i0 < inner; i0 += 256) {
-            float v[8], top = 0.f, s = 0.f;
+    if (p.vec_in) {
+        walk(true, [&](int s, int l) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.g) + base + far(p.ld, s, l)));
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+            float v[8], top = 0.f, part = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                v[j] = i0 + 32 * j < inner ? to_f32(p.g, address(o, i0 + 32 * j), p.bf16) : 0.f;
+                const float2 h = unpack2(u[j >> 1], p.bf16);
+                v[j] = (j & 1) ? h.y : h.x;
                 top = fmaxf(top, fabsf(v[j]));
+                if (p.tall) *reinterpret_cast<uint16_t*>(x_at(s + j, l)) = static_cast<uint16_t>(u[j >> 1] >> ((j & 1) * 16));
             }
-            // As in orth_square_kernel: no size of element overflows or is lost.
+            if (!p.tall) *reinterpret_cast<uint4*>(x_at(s, l)) = w;
             const uint32_t e = __float_as_uint(top) & 0x7f800000u;
             const bool plain = e >= 0x01000000u && e < 0x7e800000u;
             const float down = plain ? __uint_as_float(0x7f000000u - e) : 1.f;
             const double up = plain ? static_cast<double>(__uint_as_float(e)) : 1.;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s = fmaf(v[j] * down, v[j] * down, s);
-            sum += static_cast<double>(s) * up * up;
-        }
+            for (int j = 0; j < 8; ++j) part = fmaf(v[j] * down, v[j] * down, part);
+            sum += static_cast<double>(part) * up * up;
+        });
+    } else {
+        walk(false, [&](int s, int l) {
+            const uint16_t w = __ldg(static_cast<const uint16_t*>(p.g) + base + far(p.ld, s, l));
+            *reinterpret_cast<uint16_t*>(x_at(s, l)) = w;
+            const double v = static_cast<double>(to_f32(&w, 0, p.bf16));
+            sum += v * v;
+        });
+    }
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) warp_sums[warp] = sum;
     __syncthreads();
@@ -1133,13 +1180,17 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const Ort
     }
     __syncthreads();
     const float f = *factor;
-    for (int o = static_cast<int>(warp); o < outer; o += kOrthThreads / 32)
-#pragma unroll 8
-        for (int i = static_cast<int>(lane); i < inner; i += 32) {
-            const uint32_t row = static_cast<uint32_t>(p.tall ? i : o), col = static_cast<uint32_t>(p.tall ? o : i);
-            *reinterpret_cast<__half*>(xs + (col >> 6) * kOrthBlockBytes + swz128(row, (col & 63u) * 2u)) =
-                __float2half_rn(to_f32(p.g, address(o, i), p.bf16) * f);
+    // Scaled in place (columns outside X are zero).
+    for (uint32_t i = threadIdx.x; i < blocks * (kOrthBlockBytes / 16u); i += kOrthThreads) {
+        uint4 w = reinterpret_cast<uint4*>(xs)[i];
+        uint32_t* u = &w.x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 h = unpack2(u[j], p.bf16);
+            u[j] = pack2(h.x * f, h.y * f, 0);
         }
+        reinterpret_cast<uint4*>(xs)[i] = w;
+    }
 
     const uint32_t x_addr = smem_addr(xs), p_addr = smem_addr(ps), q_addr = smem_addr(qs);
     const uint32_t quarter = warp & 3u, group = warp >> 2;
@@ -1159,15 +1210,15 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const Ort
         __syncthreads();
         tc_fence_after_sync();
     };
-    // 32 columns from `col` of this thread's row in a square matrix, as FP16.
-    auto put_square = [&](uint8_t* dst, uint32_t col, const float (&v)[32]) {
+    // 32 columns from `col` of this thread's row in swizzled blocks, as FP16 (or BF16).
+    auto put_square = [&](uint8_t* dst, uint32_t col, const float (&v)[32], int bf16 = 0) {
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
             uint4 w;
-            w.x = pack2(v[8 * j], v[8 * j + 1], 0);
-            w.y = pack2(v[8 * j + 2], v[8 * j + 3], 0);
-            w.z = pack2(v[8 * j + 4], v[8 * j + 5], 0);
-            w.w = pack2(v[8 * j + 6], v[8 * j + 7], 0);
+            w.x = pack2(v[8 * j], v[8 * j + 1], bf16);
+            w.y = pack2(v[8 * j + 2], v[8 * j + 3], bf16);
+            w.z = pack2(v[8 * j + 4], v[8 * j + 5], bf16);
+            w.w = pack2(v[8 * j + 6], v[8 * j + 7], bf16);
             *reinterpret_cast<uint4*>(dst + (col >> 6) * kOrthBlockBytes + swz128(row, (col & 63u) * 2u + 16u * j)) = w;
         }
     };
@@ -1187,7 +1238,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const Ort
     };
     const uint32_t square_idesc = make_idesc_f16(128, 0, false, false) | (static_cast<uint32_t>(n16 >> 3) << 17);
     const float inv = 1.f / kOrthScale;
-    const uint32_t own = 128u / ctas;                              // rows of X X^T that this CTA sums
+    constexpr uint32_t own = 128u / ctas;                          // rows of X X^T that this CTA sums
 
     for (int step = 0; step < p.steps; ++step) {
         const bool last = step + 1 == p.steps;
@@ -1207,7 +1258,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const Ort
             tc_commit_if<false>(issuer, smem_addr(&bars[0]));
         }
         wait(0);
-        if (ctas == 1) {
+        if constexpr (ctas == 1) {
             for (uint32_t c = 32u * group; rows_used && static_cast<int>(c) < n16; c += 64u) {
                 float v[32];
                 tmem_ld32(t_row + c, v);
@@ -1216,41 +1267,54 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const Ort
                 put_square(ps, c, v);
             }
         } else {
-            // The other CTAs' polynomial products are done (barrier of the last
-            // step's end), so their squares may be written over.
+            // This slice's part over both squares, which no MMA reads now; a
+            // row's 16-byte pieces are permuted by its number, so that lanes
+            // (rows) write to different banks.
             for (uint32_t c = 32u * group; rows_used && static_cast<int>(c) < n16; c += 64u) {
                 float v[32];
                 tmem_ld32(t_row + c, v);
-                const uint32_t dst = map_to_rank(smem_addr(parts + (rank * own + row % own) * 128u + c), row / own);
 #pragma unroll
-                for (uint32_t i = 0; i < 32; i += 4) st_dsmem_f4(dst + i * 4u, v[i], v[i + 1], v[i + 2], v[i + 3]);
+                for (uint32_t i = 0; i < 8; ++i)
+                    reinterpret_cast<float4*>(parts)[row * 32u + ((c / 4u + i) ^ (row & 7u))] =
+                        make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
             }
             tc_fence_before_sync();
             join_cluster();
-            // Sums of this CTA's rows, four columns a thread and turn (at most 8).
-            float4 acc[8];
+            // This CTA's rows of all the parts: 16 pieces of four columns a thread
+            // whatever the cluster's size, all in flight, then added in order.
+            constexpr uint32_t kTurns = 16 / ctas;
+            float4 w[16];
 #pragma unroll
-            for (uint32_t k = 0; k < 8; ++k) {
-                const uint32_t q = k * kOrthThreads + threadIdx.x;
-                acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (q >= own * 32u) break;
-                const float4* src = reinterpret_cast<const float4*>(parts) + q;
-                for (uint32_t r = 0; r < ctas; ++r) {
-                    const float4 w = src[r * own * 32u];
-                    acc[k].x += w.x; acc[k].y += w.y; acc[k].z += w.z; acc[k].w += w.w;
+            for (uint32_t k = 0; k < kTurns; ++k) {
+                const uint32_t q = k * kOrthThreads + threadIdx.x, r = rank * own + q / 32u, piece = q & 31u;
+                const uint32_t at = smem_addr(parts) + (r * 32u + (piece ^ (r & 7u))) * 16u;
+                const bool wanted = static_cast<int>(r) < n16 && static_cast<int>(piece * 4u) < n16;
+#pragma unroll
+                for (uint32_t from = 0; from < ctas; ++from)
+                    w[k * ctas + from] = wanted ? ld_dsmem_f4(map_to_rank(at, from)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            uint32_t sums[kTurns][2];
+#pragma unroll
+            for (uint32_t k = 0; k < kTurns; ++k) {
+                float4 a = w[k * ctas];
+#pragma unroll
+                for (uint32_t from = 1; from < ctas; ++from) {
+                    const float4 u = w[k * ctas + from];
+                    a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
                 }
+                sums[k][0] = pack2(a.x * inv * inv, a.y * inv * inv, 0);
+                sums[k][1] = pack2(a.z * inv * inv, a.w * inv * inv, 0);
             }
             join_cluster();
 #pragma unroll
-            for (uint32_t k = 0; k < 8; ++k) {
+            for (uint32_t k = 0; k < kTurns; ++k) {
                 const uint32_t q = k * kOrthThreads + threadIdx.x;
-                if (q >= own * 32u) break;
                 const uint32_t r = rank * own + q / 32u, col = (q & 31u) * 4u;
-                const bool wanted = static_cast<int>(r) < n16 && static_cast<int>(col) < n16;
-                const uint32_t lo = pack2(acc[k].x * inv * inv, acc[k].y * inv * inv, 0);
-                const uint32_t hi = pack2(acc[k].z * inv * inv, acc[k].w * inv * inv, 0);
-                const uint32_t at = p_addr + (col >> 6) * kOrthBlockBytes + swz128(r, (col & 63u) * 2u);
-                for (uint32_t to = 0; wanted && to < ctas; ++to) st_dsmem_b64(map_to_rank(at, to), lo, hi);
+                if (static_cast<int>(r) < n16 && static_cast<int>(col) < n16) {
+                    const uint32_t at = p_addr + (col >> 6) * kOrthBlockBytes + swz128(r, (col & 63u) * 2u);
+#pragma unroll
+                    for (uint32_t to = 0; to < ctas; ++to) st_dsmem_b64(map_to_rank(at, to), sums[k][0], sums[k][1]);
+                }
             }
             // The rows come from other CTAs: each side orders them towards the MMAs.
             fence_async_shared();
@@ -1305,20 +1369,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const Ort
                 const float a = last ? p.a * inv : p.a, scale = last ? inv : 1.f;
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] = fmaf(scale, v[i], a * w[i]);
-                if (static_cast<int>(row) < side && !last) put_square(xs, col, v);
-                if (static_cast<int>(row) < side && last) {
-                    // Tall: lanes are neighbours in a row of the output; else a lane has 32 of them.
-                    const long long at = static_cast<long long>(blockIdx.y) * side * p.length;
-                    const int left = valid - static_cast<int>(col);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        if (i >= left) break;
-                        const long long l = first + static_cast<int>(col) + i;
-                        const long long k = at + (p.tall ? l * side + row : static_cast<long long>(row) * p.length + l);
-                        if (p.bf16) static_cast<__nv_bfloat16*>(p.out)[k] = __float2bfloat16_rn(v[i]);
-                        else static_cast<__half*>(p.out)[k] = __float2half_rn(v[i]);
-                    }
-                }
+                if (static_cast<int>(row) < side) put_square(xs, col, v, last ? p.bf16 : 0);
                 __syncwarp();
             }
             if (turn + 2 < turns) {
@@ -1328,19 +1379,35 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const Ort
                 update(turn + 2);
             }
         }
-        // No CTA's squares are written over while it still multiplies with them.
-        if (ctas > 1) {
-            tc_fence_before_sync();
-            join_cluster();
-        }
+        // A CTA's squares are next written by itself, and by others only once it
+        // has come to the next step's second barrier.
     }
     tc_fence_before_sync();
-    if (ctas > 1) join_cluster();
-    else __syncthreads();
+    __syncthreads();
+    // X, now in the type of the result, to memory.
+    uint16_t* out = static_cast<uint16_t*>(p.out) + static_cast<long long>(blockIdx.y) * side * p.length;
+    const long long ld_out = p.tall ? side : p.length;
+    if (p.vec_out) {
+        walk(true, [&](int s, int l) {
+            uint4 w;
+            if (!p.tall) {
+                w = *reinterpret_cast<const uint4*>(x_at(s, l));
+            } else {
+                uint32_t u[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) u[j] = *reinterpret_cast<const uint16_t*>(x_at(s + j, l));
+                w = make_uint4(u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16);
+            }
+            *reinterpret_cast<uint4*>(out + far(ld_out, s, l)) = w;
+        });
+    } else {
+        walk(false, [&](int s, int l) { out[far(ld_out, s, l)] = *reinterpret_cast<const uint16_t*>(x_at(s, l)); });
+    }
     if (warp == 1) {
         tc_fence_after_sync();
         tmem_dealloc(tmem, 512);
     }
+    if (ctas > 1) join_cluster();   // no CTA leaves while others may read its part
 }
 
 }  // namespace hgemm

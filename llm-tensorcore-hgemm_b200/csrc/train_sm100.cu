@@ -213,9 +213,19 @@ double launch_cost(const Product* s, int count, const Tile& t, int sms) {
     return std::max(main, bytes / 3600.0) + more + (t.pair ? 10000.0 : 8500.0) + 16.0 * t.n;
 }
 
-// The tile of a launch (all its products alike), and the splits of the products
-// that may be split.
+// Parts of a product's sum for `want` parts: whole numbers of K blocks, none
+// empty, at least `least` blocks in each.
+int whole_parts(const Product& p, int64_t want, int64_t least) {
+    const int64_t kb = p.kblocks(), most = std::max<int64_t>(1, kb / least);
+    return static_cast<int>(cdiv(kb, cdiv(kb, std::min(want, most))));
+}
+
+// The tile of a launch (all its products alike), and the splits of the product
+// that may be split (one at most).
 Tile choose_tile(Product* s, int count, int sms, const HgemmSm100TrainCommon& forced) {
+    Product* split = nullptr;
+    for (int i = 0; i < count; ++i)
+        if (s[i].splittable) split = &s[i];
     Tile best;
     int best_splits = 1;
     double cost = -1;
@@ -223,33 +233,24 @@ Tile choose_tile(Product* s, int count, int sms, const HgemmSm100TrainCommon& fo
         for (int n = 256; n >= 64; n -= 64) {
             const Tile t{pair != 0, n};
             if (forced.tile != 0 && forced.tile != (n | (pair ? HGEMM_SM100_TRAIN_TILE_PAIR : 0))) continue;
+            double before = -1;
             for (int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {
-                bool any = false;
-                for (int i = 0; i < count; ++i)
-                    if (s[i].splittable) {
-                        const int64_t want = forced.splits != 0 ? forced.splits : splits;
-                        // Whole parts of at least four K blocks (one where forced).
-                        const int64_t most = std::max<int64_t>(1, s[i].kblocks() / (forced.splits != 0 ? 1 : 4));
-                        s[i].splits = static_cast<int>(std::min(want, most));
-                        any = true;
-                    }
+                // Parts of four K blocks at least (of one where forced).
+                if (split != nullptr)
+                    split->splits = forced.splits != 0 ? whole_parts(*split, forced.splits, 1) : whole_parts(*split, splits, 4);
                 const double c = launch_cost(s, count, t, sms);
                 if (cost < 0 || c < cost) {
                     best = t;
-                    best_splits = splits;
+                    best_splits = split != nullptr ? split->splits : 1;
                     cost = c;
                 }
-                if (!any || forced.splits != 0) break;
+                // More parts only as long as they help.
+                if (split == nullptr || forced.splits != 0 || (before >= 0 && c >= before)) break;
+                before = c;
             }
         }
     }
-    for (int i = 0; i < count; ++i)
-        if (s[i].splittable) {
-            const int64_t want = forced.splits != 0 ? forced.splits : best_splits;
-            const int64_t most = std::max<int64_t>(1, s[i].kblocks() / (forced.splits != 0 ? 1 : 4));
-            const int64_t kb = cdiv(s[i].kblocks(), std::min(want, most));
-            s[i].splits = static_cast<int>(cdiv(s[i].kblocks(), kb));   // no part without K blocks
-        }
+    if (split != nullptr) split->splits = best_splits;
     return best;
 }
 
@@ -849,26 +850,43 @@ OrthPlan plan_orth(const HgemmSm100Orthogonalize& a) {
 }
 
 // The one-launch form for a shorter side of at most 128 rows: CTAs of a cluster
-// (each 128 rows x `slice` columns), 0 where it does not fit.
+// (each 128 rows x `slice` columns), 0 where it does not fit. The fewest with
+// slices of at most 256 columns: a step's exchange between CTAs costs about 3 us
+// and 256 columns of a step 3.8 (128 x 640: 50, 48, 43, 44 and 46 us with 1 to
+// 16 CTAs; 128 x 256: 27 and 35 with 1 and 2).
 int orth_cluster_ctas(const HgemmSm100Orthogonalize& a) {
     const int64_t side = std::min(a.rows, a.cols), length = std::max(a.rows, a.cols);
     if (a.common.tile != 0 || a.steps < 1 || side > 128) return 0;
-    for (int n : {1, 2, 4, 8, 16})
-        if (round_up(cdiv(length, n), 64) <= kOrthMaxSlice) return n;
+    for (int n : {1, 2, 4, 8, 16}) {
+        const int64_t slice = round_up(cdiv(length, n), 64);
+        if (a.common.splits != 0 ? a.common.splits == n && slice <= kOrthMaxSlice
+                                 : slice <= 256 || (n == 16 && slice <= kOrthMaxSlice))
+            return n;
+    }
     return 0;
 }
 
-std::atomic<uint64_t> g_orth_ready{0};
+using OrthFn = void (*)(OrthClusterParams);
+struct OrthEntry {
+    OrthFn fn;
+    std::atomic<uint64_t> ready{0};
+};
+OrthEntry g_orth[5] = {{&orth_cluster_kernel<1>},
+                       {&orth_cluster_kernel<2>},
+                       {&orth_cluster_kernel<4>},
+                       {&orth_cluster_kernel<8>},
+                       {&orth_cluster_kernel<16>}};
 
 int run_orth_cluster(const HgemmSm100Orthogonalize& a, int ctas, const Context& c) {
+    OrthEntry& k = g_orth[ctas == 1 ? 0 : ctas == 2 ? 1 : ctas == 4 ? 2 : ctas == 8 ? 3 : 4];
     const uint64_t bit = 1ull << c.id;
-    if (!(g_orth_ready.load(std::memory_order_acquire) & bit)) {
-        const void* fn = reinterpret_cast<const void*>(&orth_cluster_kernel);
+    if (!(k.ready.load(std::memory_order_acquire) & bit)) {
+        const void* fn = reinterpret_cast<const void*>(k.fn);
         if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kOrthMaxSmem)) !=
                 cudaSuccess ||
             cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
             return HGEMM_SM100_ERR_LAUNCH;
-        g_orth_ready.fetch_or(bit, std::memory_order_acq_rel);
+        k.ready.fetch_or(bit, std::memory_order_acq_rel);
     }
     OrthClusterParams p{};
     p.g = a.g;
@@ -880,6 +898,9 @@ int run_orth_cluster(const HgemmSm100Orthogonalize& a, int ctas, const Context& 
     p.tall = a.rows > a.cols;
     p.slice = static_cast<int>(round_up(cdiv(p.length, ctas), 64));
     p.bf16 = a.common.dtype == HGEMM_SM100_TRAIN_BF16;
+    // Rows of g and out in 16-byte pieces. A slice begins at a multiple of 64.
+    p.vec_in = aligned16(a.g) && a.cols % 8 == 0 && a.ldg % 8 == 0 && a.batch_stride % 8 == 0;
+    p.vec_out = aligned16(a.out) && a.cols % 8 == 0;
     p.steps = a.steps;
     p.a = a.a;
     p.b = a.b;
@@ -888,7 +909,7 @@ int run_orth_cluster(const HgemmSm100Orthogonalize& a, int ctas, const Context& 
     p.status = a.common.status != nullptr ? a.common.status : c.dev->status_word;
     p.timeout_ns = a.common.timeout_ns != 0 ? a.common.timeout_ns : kDefaultTimeoutNs;
     const size_t smem = static_cast<size_t>(p.slice / 64) * kOrthBlockBytes + 2 * kOrthSquareBytes + 1024 + 512;
-    return launch(&orth_cluster_kernel, dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(a.batch)),
+    return launch(k.fn, dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(a.batch)),
                   dim3(kOrthThreads), smem, ctas, c.stream, p);
 }
 

@@ -458,6 +458,20 @@ def test_orthogonalize_one_launch_and_its_limits(size, turn):
         assert float(torch.linalg.vector_norm(out[k].double() - value)) <= err
 
 
+@pytest.mark.parametrize("ctas", [1, 2, 4, 8, 16])
+@pytest.mark.parametrize("size", [(40, 300), (300, 40), (128, 1), (128, 600), (600, 128)], ids=str)
+def test_orthogonalize_every_cluster(size, ctas):
+    """Every size of cluster, also with CTAs that hold no column at all."""
+    g = normal(12, *size)
+    value, err = ref.orthogonalize(g, 5, NEWTON_SCHULZ, 1e-7)
+    out = torch.full_like(g, float("nan"))
+    a = train_capi.Orthogonalize(train_capi.Common(train_capi.F16, 0, 0, ctas), g.data_ptr(), out.data_ptr(), None, 0,
+                                 1, *size, size[1], 0, 5, 0, *NEWTON_SCHULZ, 0.0, 1e-7)
+    assert train_capi.workspace("orthogonalize", a) == 0
+    assert train_capi.run("orthogonalize", a, stream()) == capi.OK
+    assert float(torch.linalg.vector_norm(out.double() - value)) <= err
+
+
 @pytest.mark.parametrize("batch", [(1,), (3,), (4,), (5,), (2, 3)], ids=str)
 def test_orthogonalize_batches_and_strides(batch):
     for size in ((40, 77), (150, 177)):
