@@ -14,8 +14,11 @@
 //  * the sum over K may run over two operand pairs (dx = dg Wg + du Wu), and
 //    the columns of B may come from two tensors (gate and up), so no weight is
 //    packed: a training step changes the weights every time;
-//  * the sum over K may be split over several tiles whose FP32 partial sums
-//    sum_round_kernel adds in a fixed order (few rows, long sums);
+//  * the last tiles' sums over K may be cut into parts, whose FP32 sums
+//    join_parts_kernel adds in a fixed order: all tiles where there are fewer
+//    than SMs (few rows, long sums), else those of a nearly empty last wave;
+//  * of a symmetric product only the tiles on and above the diagonal are
+//    computed, and stored both ways;
 //  * one launch takes up to four problems and walks their tiles as one list
 //    (dx, dWgate, dWup and dWdown fill the last wave together);
 //  * the epilogue finishes the operator (SwiGLU, its gradient, softmax
@@ -39,7 +42,7 @@
 
 namespace hgemm {
 
-constexpr int kTrainMaxProblems = 4;
+constexpr int kTrainMaxProblems = 4;   // of one launch
 constexpr uint32_t kTrainRingBytes = 196608;               // stages of both operands
 constexpr uint32_t kTrainBoxBytes = 2048;                  // 32 rows x 32 16-bit columns
 constexpr int kTrainEpiWarps = 8;
@@ -71,8 +74,10 @@ struct alignas(64) TrainProblem {
     int nkb0, nkb;         // K blocks of the first segment, of both
     int a_mn, b_mn, dual;
     int tiles_m, tiles_n, group_m;
+    int symmetric;         // tiles are those of the upper triangle, row by row
+    int tile0, tiles;      // this problem's tiles of all: tile0 .. tile0 + tiles - 1
     int splits, kb_split;  // parts of the sum over K, K blocks of each (the last: the rest)
-    int pad_rows;          // output rows from one part's sums to the next one's
+    int parted;            // out[0] holds FP32 tiles, [part][tile][rows of a tile][tile_n]
     uint32_t a_tile_bytes; // what the loads of A bring per K block
     int out_kind;
     float alpha, beta;
@@ -197,6 +202,27 @@ struct BoxWriter {
         }
     }
 
+    // The transposed box: lane = column `col` + lane, v = rows row .. row + 31.
+    __device__ void put16_turned(const CUtensorMap* map, const float (&v)[32], int bf16, int col, int row) {
+        if (lane == 0) bulk_wait_group_read<1>();
+        __syncwarp();
+        uint8_t* box = bufs + (next & 1u) * kTrainBoxBytes;
+        ++next;
+#pragma unroll
+        for (uint32_t i = 0; i < 32; i += 2) {
+            const uint32_t w = pack2(v[i], v[i + 1], bf16);
+            const uint32_t at = (((lane >> 3) ^ ((i >> 1) & 3u)) << 4) + (lane & 7u) * 2u;   // alike for i and i + 1
+            *reinterpret_cast<uint16_t*>(box + i * 64u + at) = static_cast<uint16_t>(w);
+            *reinterpret_cast<uint16_t*>(box + i * 64u + 64u + at) = static_cast<uint16_t>(w >> 16);
+        }
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+            tma_store_2d(map, box, col, row);
+            bulk_commit_group();
+        }
+    }
+
     __device__ void put32(const CUtensorMap* map, const float (&v)[32], bool add, int col, int row) {
         if (lane == 0) bulk_wait_group_read<0>();
         __syncwarp();
@@ -225,6 +251,24 @@ __device__ __forceinline__ void tmem_ld32(uint32_t t, float (&v)[32]) {
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// Row and column of a problem's tile t: grouped raster order, or the upper
+// triangle row by row.
+__device__ __forceinline__ void tile_place(int t, int tiles_m, int tiles_n, int group_m, int symmetric, int& tm, int& tn) {
+    if (!symmetric) {
+        tile_coords(t, tiles_m, tiles_n, group_m, tm, tn);
+        return;
+    }
+    tm = 0;
+    for (int left = tiles_n; t >= left; --left) {
+        t -= left;
+        ++tm;
+    }
+    tn = tm + t;
+}
+__device__ __forceinline__ void tile_place(const TrainProblem& q, int t, int& tm, int& tn) {
+    tile_place(t, q.tiles_m, q.tiles_n, q.group_m, q.symmetric, tm, tn);
+}
+
 // The tiles of one unit (CTA or pair) in order; every role iterates alike.
 // Problem 0's tiles ("heavy": the longest sums) go round robin; where they do
 // not divide evenly the units that took one more sit out the first
@@ -232,6 +276,7 @@ __device__ __forceinline__ void tmem_ld32(uint32_t t, float (&v)[32]) {
 struct TileIter {
     int unit, units, next_heavy, wave;
     int prob, tm, tn;      // the current tile
+    int local;             // its number among the problem's
     int split, kb0, kb1;   // its part of the sum: K blocks [kb0, kb1)
     bool back;             // walk K from the end
     __device__ TileIter(int u, int n) : unit(u), units(n), next_heavy(u), wave(0) {}
@@ -251,17 +296,15 @@ struct TileIter {
             ++wave;
             if (t >= p.light_tiles) return false;
             prob = 1;
-            while (true) {
-                const int tiles = p.prob[prob].tiles_m * p.prob[prob].tiles_n * p.prob[prob].splits;
-                if (t < tiles) break;
-                t -= tiles;
+            while (t >= p.prob[prob].tiles * p.prob[prob].splits) {
+                t -= p.prob[prob].tiles * p.prob[prob].splits;
                 ++prob;
             }
         }
         const TrainProblem& q = p.prob[prob];
-        const int plane = q.tiles_m * q.tiles_n;
-        split = q.splits > 1 ? t / plane : 0;
-        tile_coords(t - split * plane, q.tiles_m, q.tiles_n, q.group_m, tm, tn);
+        split = q.splits > 1 ? t / q.tiles : 0;
+        local = t - split * q.tiles;
+        tile_place(q, q.tile0 + local, tm, tn);
         kb0 = split * q.kb_split;
         kb1 = min(q.nkb, kb0 + q.kb_split);
         // Odd waves walk K backwards: they start on the panels that the wave
@@ -286,14 +329,18 @@ template <int kEpi>
 struct TrainEpilogue {
     const TrainParams& p;
     const TrainProblem& q;
-    int row0, row, tn, out_row, width, first;   // out_row: row0 in the output; width: the tile's output columns
+    int row0, row, tn, width, first;   // width: the tile's output columns
+    int out_row, mirror;               // row0 in the output; the tile is stored transposed too
     bool in_rows;
     Row32 x, y;
 
-    __device__ TrainEpilogue(const TrainParams& p_, const TrainProblem& q_, int row0_, int lane, int tn_, int split,
-                             int group)
-        : p(p_), q(q_), row0(row0_), row(row0_ + lane), tn(tn_), out_row(row0_ + split * q_.pad_rows),
-          width(kEpi == kTrainGate ? q_.tile_n / 2 : q_.tile_n), first(32 * group), in_rows(row0_ + lane < q_.m) {}
+    // in_tile: this warp's first row in the tile.
+    __device__ TrainEpilogue(const TrainParams& p_, const TrainProblem& q_, const TileIter& it, int tile_m, int in_tile,
+                             int lane, int group)
+        : p(p_), q(q_), row0(it.tm * tile_m + in_tile), row(row0 + lane), tn(it.tn),
+          width(kEpi == kTrainGate ? q_.tile_n / 2 : q_.tile_n), first(32 * group),
+          out_row(q_.parted ? (it.split * q_.tiles + it.local) * tile_m + in_tile : row0),
+          mirror(q_.symmetric && it.tn > it.tm), in_rows(row < q_.m) {}
 
     __device__ __forceinline__ void fetch(int c, Row32& a, Row32& b) const {
         const int col = tn * width + c;
@@ -341,7 +388,7 @@ struct TrainEpilogue {
             tmem_ld32(t + c, v);
             if constexpr (kEpi == kTrainStore) {
                 if (q.out_kind != kTrainOut16) {
-                    box.put32(&q.out[0], v, q.out_kind == kTrainOutF32Add, col, out_row);
+                    box.put32(&q.out[0], v, q.out_kind == kTrainOutF32Add, c, out_row);
                     continue;
                 }
                 if (q.beta != 0.f) {
@@ -356,6 +403,7 @@ struct TrainEpilogue {
                     for (int i = 0; i < 32; ++i) v[i] *= alpha;
                 }
                 box.put16(&q.out[0], v, p.out_bf16, col, row0);
+                if (mirror) box.put16_turned(&q.out[0], v, p.out_bf16, row0, col);
             } else if constexpr (kEpi == kTrainGate) {
                 float u[32];
                 tmem_ld32(t + width + c, u);
@@ -688,8 +736,8 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
         while (it.next(p)) {
             const uint32_t acc = iter & 1u, acc_phase = (iter >> 1) & 1u;
             ++iter;
-            const int row0 = it.tm * kTileM + static_cast<int>(rank) * 128 + quarter * 32;
-            TrainEpilogue<kEpi> epi(p, p.prob[it.prob], row0, static_cast<int>(lane), it.tn, it.split, group);
+            TrainEpilogue<kEpi> epi(p, p.prob[it.prob], it, kTileM, static_cast<int>(rank) * 128 + quarter * 32,
+                                    static_cast<int>(lane), group);
             epi.begin();
             const bool got = kPair ? mbar_wait_cluster(&tfull[acc], acc_phase, wc) : mbar_wait(&tfull[acc], acc_phase, wc);
             if (!__all_sync(0xffffffffu, got)) break;
@@ -854,32 +902,59 @@ __global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* __r
     }
 }
 
-// out = alpha (part 0 + part 1 + ...) of FP32 sums `stride` elements apart,
-// added in that order and rounded once (8 elements per thread). alpha: a device
-// number, or null for 1.
-__global__ void __launch_bounds__(256) sum_round_kernel(const float* __restrict__ src, int parts, long long stride,
-                                                        uint4* __restrict__ out, long long vecs,
-                                                        const float* __restrict__ alpha, int bf16) {
+// The tiles of a product whose sums came in parts: out = alpha (part 0 + part 1
+// + ...) + beta C, added in that order and rounded once. Block (x, y): some rows
+// of tile tile0 + y; eight columns per thread.
+struct JoinParams {
+    const float* parts;
+    int splits, tiles, tile0, tiles_m, tiles_n, group_m, tile_m, tile_n, m, n;
+    float alpha, beta;
+    const float* alpha_ptr;    // multiplies alpha; may be null
+    const void* c;
+    long long ldc;
+    void* out;                 // 16-byte aligned rows
+    long long ld_out;
+    int in_bf16, out_bf16;
+};
+
+__global__ void __launch_bounds__(256) join_parts_kernel(const JoinParams p) {
     grid_dependents_launch();
     grid_dependency_wait();
-    const float a = alpha != nullptr ? *alpha : 1.f;
-    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < vecs;
-         i += static_cast<long long>(gridDim.x) * 256) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-        const float4* p = reinterpret_cast<const float4*>(src) + 2 * i;
+    int tm, tn;
+    tile_coords(p.tile0 + static_cast<int>(blockIdx.y), p.tiles_m, p.tiles_n, p.group_m, tm, tn);
+    const int per_row = p.tile_n / 8, in_row = static_cast<int>(threadIdx.x) / per_row;
+    const int rows = 256 / per_row;                  // of this block; threads beyond have none
+    const int r = static_cast<int>(blockIdx.x) * rows + in_row, c = (static_cast<int>(threadIdx.x) - in_row * per_row) * 8;
+    const int row = tm * p.tile_m + r, col = tn * p.tile_n + c;
+    if (in_row >= rows || r >= p.tile_m || row >= p.m || col >= p.n) return;
+    const long long stride = static_cast<long long>(p.tiles) * p.tile_m * p.tile_n;
+    const float* src = p.parts + (static_cast<long long>(blockIdx.y) * p.tile_m + r) * p.tile_n + c;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-        for (int k = 0; k < parts; ++k, p += stride / 4) {
-            const float4 u = p[0], v = p[1];
-            x.x += u.x; x.y += u.y; x.z += u.z; x.w += u.w;
-            y.x += v.x; y.y += v.y; y.z += v.z; y.w += v.w;
-        }
-        uint4 q;
-        q.x = pack2(a * x.x, a * x.y, bf16);
-        q.y = pack2(a * x.z, a * x.w, bf16);
-        q.z = pack2(a * y.x, a * y.y, bf16);
-        q.w = pack2(a * y.z, a * y.w, bf16);
-        out[i] = q;
+    for (int k = 0; k < p.splits; ++k, src += stride) {
+        const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+        v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
     }
+    const float alpha = p.alpha_ptr != nullptr ? p.alpha * *p.alpha_ptr : p.alpha;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= alpha;
+    if (p.beta != 0.f) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.c) + row * p.ldc + col));
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack2(u[i], p.in_bf16);
+            v[2 * i] = fmaf(p.beta, f.x, v[2 * i]);
+            v[2 * i + 1] = fmaf(p.beta, f.y, v[2 * i + 1]);
+        }
+    }
+    uint4 q;
+    q.x = pack2(v[0], v[1], p.out_bf16);
+    q.y = pack2(v[2], v[3], p.out_bf16);
+    q.z = pack2(v[4], v[5], p.out_bf16);
+    q.w = pack2(v[6], v[7], p.out_bf16);
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.ld_out + col) = q;
 }
 
 // ------------------------------------------------------ orthogonalised update ---

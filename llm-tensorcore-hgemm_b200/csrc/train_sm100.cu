@@ -161,17 +161,23 @@ struct Product {
     int64_t m = 0, n = 0, k0 = 0, k1 = 0;
     Operand a0, b0, a1, b1;
     bool dual = false;
-    void* out = nullptr;       // 16-bit (or FP32, see out_kind) [m x ld_out]
+    void* out = nullptr;       // 16-bit [m x ld_out]
     int64_t ld_out = 0;
     void* out1 = nullptr;      // further 16-bit outputs of the same shape
     void* out2 = nullptr;
-    int out_kind = kTrainOut16;
     float alpha = 1.f, beta = 0.f;
     const float* alpha_ptr = nullptr;
     const void* c = nullptr;
     int64_t ldc = 0;
-    int splits = 1;            // > 1: FP32 partial sums [splits][whole tiles of rows][ld_out]
-    bool splittable = false;
+    bool splittable = false;   // sums may be cut into parts
+    bool symmetric = false;    // the product is symmetric (m == n)
+    // Chosen with the tile: the last `parted` tiles in `splits` parts each, to
+    // `parts` (FP32; added to what is there with add_parts); upper triangle only.
+    int64_t parted = 0;
+    int splits = 1;
+    float* parts = nullptr;
+    bool add_parts = false;
+    bool triangle = false;
     int64_t kblocks() const { return cdiv(k0, kBlockK) + cdiv(k1, kBlockK); }
 };
 
@@ -185,32 +191,16 @@ double block_cycles(bool pair, int tile_n) {
 
 int64_t tile_rows(bool pair) { return pair ? 256 : 128; }
 
-// What a launch of `count` products is estimated to take with tile t, in
-// cycles. One product: its waves. Several: units take the tiles one after the
-// other, so the whole work over all units, plus half a last tile that some wait
-// for. Never less than the longest tile, nor than the operands' way from memory
-// (3600 bytes a cycle). Partial sums are written, read and launched for.
-double launch_cost(const Product* s, int count, const Tile& t, int sms) {
-    const double units = t.pair ? sms / 2 : sms;
-    double work = 0, longest = 0, last = 0, bytes = 0, more = 0;
-    int64_t tiles = 0;
-    for (int i = 0; i < count; ++i) {
-        const Product& p = s[i];
-        const int64_t kb = cdiv(p.kblocks(), p.splits), cols = p.dual ? t.n / 2 : t.n;
-        const int64_t n = cdiv(p.m, tile_rows(t.pair)) * cdiv(p.n, cols) * p.splits;
-        const double one = static_cast<double>(kb) * block_cycles(t.pair, t.n) + 600.0;
-        work += one * static_cast<double>(n);
-        tiles += n;
-        longest = std::max(longest, one);
-        last = one;
-        bytes += 2.0 * static_cast<double>(p.k0 + p.k1) * static_cast<double>(p.m + (p.dual ? 2 : 1) * p.n);
-        if (p.splits > 1)
-            more += 6000.0 + 8.0 * p.splits * static_cast<double>(cdiv(p.m, tile_rows(t.pair)) * tile_rows(t.pair)) *
-                                 static_cast<double>(p.n) / 3600.0;
-    }
-    const double main = count == 1 ? longest * static_cast<double>(cdiv(tiles, static_cast<int64_t>(units)))
-                                   : std::max(longest, work / units + 0.5 * last);
-    return std::max(main, bytes / 3600.0) + more + (t.pair ? 10000.0 : 8500.0) + 16.0 * t.n;
+int64_t tile_count(const Product& p, const Tile& t) {
+    const int64_t rows = cdiv(p.m, tile_rows(t.pair)), cols = cdiv(p.n, p.dual ? t.n / 2 : t.n);
+    return p.triangle ? rows * (rows + 1) / 2 : rows * cols;
+}
+
+double tile_time(int64_t kb, const Tile& t) { return static_cast<double>(kb) * block_cycles(t.pair, t.n) + 600.0; }
+
+// Writing the parts of a product's last tiles, reading them, and one launch more.
+double parts_time(const Product& p, const Tile& t) {
+    return 6000.0 + 8.0 * p.splits * static_cast<double>(p.parted * tile_rows(t.pair) * t.n) / 3600.0;
 }
 
 // Parts of a product's sum for `want` parts: whole numbers of K blocks, none
@@ -220,46 +210,108 @@ int whole_parts(const Product& p, int64_t want, int64_t least) {
     return static_cast<int>(cdiv(kb, cdiv(kb, std::min(want, most))));
 }
 
-// The tile of a launch (all its products alike), and the splits of the product
-// that may be split (one at most).
+// Operands' way from memory, 3600 bytes a cycle.
+double memory_time(const Product& p) {
+    return 2.0 * static_cast<double>(p.k0 + p.k1) * static_cast<double>(p.m + (p.dual ? 2 : 1) * p.n) / 3600.0;
+}
+
+double launch_time(const Tile& t) { return (t.pair ? 10000.0 : 8500.0) + 16.0 * t.n; }
+
+// Time of one product with tile t: its full waves, and the last one, whose
+// tiles may be cut into parts that fill it (or all tiles' parts, where there are
+// fewer tiles than units). Sets the product's choices.
+double plan_product(Product& p, const Tile& t, int sms, int forced_splits) {
+    p.parted = 0;
+    p.splits = 1;
+    p.triangle = p.symmetric && t.n == tile_rows(t.pair);
+    const int64_t units = t.pair ? sms / 2 : sms, tiles = tile_count(p, t), kb = p.kblocks();
+    const int64_t rest = tiles % units;
+    double best = static_cast<double>(cdiv(tiles, units)) * tile_time(kb, t);
+    if (p.splittable && !p.triangle && (forced_splits != 0 || (rest != 0 && rest <= units / 2))) {
+        Product q = p;
+        q.parted = forced_splits != 0 && rest == 0 ? tiles : rest;
+        for (int splits : {2, 3, 4, 5, 6, 8, 10, 12, 16}) {
+            if (forced_splits != 0) splits = forced_splits;
+            // Parts of four K blocks at least (of one where forced).
+            q.splits = whole_parts(p, splits, forced_splits != 0 ? 1 : 4);
+            if (q.splits < 2 && forced_splits == 0) break;
+            const double time = static_cast<double>((tiles - q.parted) / units) * tile_time(kb, t) +
+                                static_cast<double>(cdiv(q.parted * q.splits, units)) * tile_time(cdiv(kb, q.splits), t) +
+                                parts_time(q, t);
+            if (time < best || forced_splits != 0) {
+                best = time;
+                p.parted = q.parted;
+                p.splits = q.splits;
+            }
+            if (forced_splits != 0 || q.parted * splits >= 2 * units) break;
+        }
+    }
+    return std::max(best, memory_time(p)) + launch_time(t);
+}
+
+// Time of several products in one launch: units take the tiles one after the
+// other, so the whole work over all units plus half a last tile that some wait
+// for, and never less than the longest tile. A splittable product's tiles all
+// come in `splits` parts (or whole, for 1).
+double plan_group(Product* s, int count, const Tile& t, int sms, int splits) {
+    double work = 0, longest = 0, last = 0, more = 0, memory = 0;
+    for (int i = 0; i < count; ++i) {
+        Product& p = s[i];
+        p.triangle = p.symmetric && t.n == tile_rows(t.pair);
+        p.splits = p.splittable ? splits : 1;
+        p.parted = p.splits > 1 ? tile_count(p, t) : 0;
+        const double one = tile_time(cdiv(p.kblocks(), p.splits), t);
+        work += one * static_cast<double>(tile_count(p, t) * p.splits);
+        longest = std::max(longest, one);
+        last = one;
+        memory += memory_time(p);
+        if (p.splits > 1) more += parts_time(p, t);
+    }
+    return std::max({longest, work / (t.pair ? sms / 2 : sms) + 0.5 * last, memory}) + more + launch_time(t);
+}
+
+// The tile of a launch (all its products alike), and the products' parts.
 Tile choose_tile(Product* s, int count, int sms, const HgemmSm100TrainCommon& forced) {
-    Product* split = nullptr;
+    const Product* split = nullptr;
     for (int i = 0; i < count; ++i)
         if (s[i].splittable) split = &s[i];
     Tile best;
     int best_splits = 1;
     double cost = -1;
+    auto take = [&](const Tile& t, int splits, double c) {
+        if (cost >= 0 && c >= cost) return;
+        best = t;
+        best_splits = splits;
+        cost = c;
+    };
     for (int pair = 1; pair >= 0; --pair) {
         for (int n = 256; n >= 64; n -= 64) {
             const Tile t{pair != 0, n};
             if (forced.tile != 0 && forced.tile != (n | (pair ? HGEMM_SM100_TRAIN_TILE_PAIR : 0))) continue;
+            if (count == 1) {
+                take(t, 1, plan_product(s[0], t, sms, forced.splits));
+                continue;
+            }
             double before = -1;
-            for (int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {
-                // Parts of four K blocks at least (of one where forced).
-                if (split != nullptr)
-                    split->splits = forced.splits != 0 ? whole_parts(*split, forced.splits, 1) : whole_parts(*split, splits, 4);
-                const double c = launch_cost(s, count, t, sms);
-                if (cost < 0 || c < cost) {
-                    best = t;
-                    best_splits = split != nullptr ? split->splits : 1;
-                    cost = c;
-                }
+            for (int want : {1, 2, 3, 4, 6, 8, 12, 16}) {
+                const int splits = split == nullptr      ? 1
+                                   : forced.splits != 0 ? whole_parts(*split, forced.splits, 1)
+                                                        : whole_parts(*split, want, 4);
+                const double c = plan_group(s, count, t, sms, splits);
+                take(t, splits, c);
                 // More parts only as long as they help.
                 if (split == nullptr || forced.splits != 0 || (before >= 0 && c >= before)) break;
                 before = c;
             }
         }
     }
-    if (split != nullptr) split->splits = best_splits;
+    if (count == 1) plan_product(s[0], best, sms, forced.splits);
+    else plan_group(s, count, best, sms, best_splits);
     return best;
 }
 
-// FP32 elements of one part of a split product, and bytes of all parts.
-int64_t part_elements(const Product& p, const Tile& t) {
-    return cdiv(p.m, tile_rows(t.pair)) * tile_rows(t.pair) * p.ld_out;
-}
-size_t part_bytes(const Product& p, const Tile& t) {
-    return p.splits > 1 ? static_cast<size_t>(p.splits * part_elements(p, t)) * 4 : 0;
+size_t parts_bytes(const Product& p, const Tile& t) {
+    return static_cast<size_t>(p.parted) * p.splits * tile_rows(t.pair) * t.n * 4;
 }
 
 // Raster group height: the tallest of 8, 16, 32 tile rows whose one-wave
@@ -309,20 +361,26 @@ void init_params(TrainParams& p, const Context& c) {
     p.inject = (c.common.flags & HGEMM_SM100_FLAG_TEST_INJECT_TX) ? 1 : 0;
 }
 
-// Fills the problems of `p` from `count` products (the first one with the most
-// K blocks) and launches them as one grid.
+// Fills the problems of `p` from `count` products (the one with the longest
+// sums first; one whose last tiles are parted makes two problems) and launches
+// them as one grid.
 int run_products(TrainParams& p, int epi, const Product* products, const Tile& tile, int count, const Context& c) {
     const bool pair = tile.pair;
     const int tile_n = tile.n;
     const int units = pair ? c.dev->sms / 2 : c.dev->sms;
     uint32_t a_bytes = 0, b_bytes = 0;
     int64_t total = 0, light = 0;
-    for (int i = 0; i < count; ++i) {
-        const Product& s = products[i];
-        TrainProblem& q = p.prob[i];
+    int problems = 0;
+    const int bf16 = p.in_bf16;
+    for (int i = 0; i < 2 * count; ++i) {
+        const Product& s = products[i / 2];
+        const bool parted = i % 2 != 0;
+        const int64_t all = tile_count(s, tile), tiles = parted ? s.parted : all - s.parted;
+        if (tiles == 0) continue;
+        if (problems == kTrainMaxProblems || all >= (int64_t{1} << 30)) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
+        TrainProblem& q = p.prob[problems++];
         const int cols = s.dual ? tile_n / 2 : tile_n;          // output columns of a tile
         const uint32_t b_box = static_cast<uint32_t>(s.dual || pair ? tile_n / 2 : tile_n);
-        const int bf16 = p.in_bf16;
         q.m = static_cast<int>(s.m);
         q.n = static_cast<int>(s.n);
         q.tile_n = tile_n;
@@ -331,18 +389,21 @@ int run_products(TrainParams& p, int epi, const Product* products, const Tile& t
         q.a_mn = s.a0.mn;
         q.b_mn = s.b0.mn;
         q.dual = s.dual;
-        q.tiles_m = static_cast<int>(cdiv(s.m, pair ? 256 : 128));
+        q.tiles_m = static_cast<int>(cdiv(s.m, tile_rows(pair)));
         q.tiles_n = static_cast<int>(cdiv(s.n, cols));
         q.group_m = group_height(s.m, s.k0 + s.k1, pair, units);
-        q.out_kind = s.out_kind;
+        q.symmetric = s.triangle;
+        q.tile0 = static_cast<int>(parted ? all - s.parted : 0);
+        q.tiles = static_cast<int>(tiles);
+        q.splits = parted ? s.splits : 1;
+        q.kb_split = static_cast<int>(cdiv(s.kblocks(), q.splits));
+        q.parted = parted;
+        q.out_kind = !parted ? kTrainOut16 : s.add_parts ? kTrainOutF32Add : kTrainOutF32;
         q.alpha = s.alpha;
-        q.beta = s.beta;
+        q.beta = parted ? 0.f : s.beta;   // the join adds it
         q.alpha_ptr = s.alpha_ptr;
         q.c = s.c;
         q.ldc = s.ldc;
-        q.splits = s.splits;
-        q.kb_split = static_cast<int>(cdiv(s.kblocks(), s.splits));
-        q.pad_rows = static_cast<int>(q.tiles_m * tile_rows(pair));
         // Few rows (K-major): only those are loaded. What the MMA reads in place
         // of the others is some other part of the ring, and gives accumulator
         // rows that nothing stores.
@@ -355,26 +416,22 @@ int run_products(TrainParams& p, int epi, const Product* products, const Tile& t
             rc = make_operand(&q.a[1], s.a1, s.m, s.k1, a_rows, bf16);
             if (rc == HGEMM_SM100_OK) rc = make_operand(&q.b[1], s.b1, s.n, s.k1, b_box, bf16);
         }
+        if (rc == HGEMM_SM100_OK && parted)
+            rc = tensor_map(&q.out[0], s.parts, tile_n, q.splits * tiles * tile_rows(pair), tile_n, 32, 32,
+                            CU_TENSOR_MAP_DATA_TYPE_FLOAT32, CU_TENSOR_MAP_SWIZZLE_128B);
         void* const outs[3] = {s.out, s.out1, s.out2};
-        for (int j = 0; j < 3 && rc == HGEMM_SM100_OK; ++j) {
-            if (outs[j] == nullptr) continue;
-            const int64_t rows = s.splits > 1 ? static_cast<int64_t>(s.splits) * q.pad_rows : s.m;
-            rc = s.out_kind == kTrainOut16
-                     ? tensor_map(&q.out[j], outs[j], s.n, rows, s.ld_out, 32, 32, type16(p.out_bf16),
-                                  CU_TENSOR_MAP_SWIZZLE_64B)
-                     : tensor_map(&q.out[j], outs[j], s.n, rows, s.ld_out, 32, 32, CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
-                                  CU_TENSOR_MAP_SWIZZLE_128B);
-        }
+        for (int j = 0; j < 3 && rc == HGEMM_SM100_OK && !parted; ++j)
+            if (outs[j] != nullptr)
+                rc = tensor_map(&q.out[j], outs[j], s.n, s.m, s.ld_out, 32, 32, type16(p.out_bf16),
+                                CU_TENSOR_MAP_SWIZZLE_64B);
         if (rc != HGEMM_SM100_OK) return rc;
-        const int64_t b_cols = pair ? tile_n / 2 : tile_n;
         a_bytes = std::max(a_bytes, q.a_tile_bytes);
-        b_bytes = std::max(b_bytes, static_cast<uint32_t>(round_up(b_cols, 64) * 128));
-        const int64_t n = static_cast<int64_t>(q.tiles_m) * q.tiles_n * q.splits;
-        total += n;
-        if (i > 0) light += n;
+        b_bytes = std::max(b_bytes, static_cast<uint32_t>(round_up(pair ? tile_n / 2 : tile_n, 64) * 128));
+        total += tiles * q.splits;
+        if (problems > 1) light += tiles * q.splits;
     }
     if (total >= (int64_t{1} << 31)) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
-    p.num_problems = count;
+    p.num_problems = problems;
     p.heavy_tiles = static_cast<int>(total - light);
     p.light_tiles = static_cast<int>(light);
     const int grid_units = static_cast<int>(std::min<int64_t>(total, units));
@@ -404,13 +461,51 @@ int run_product(TrainParams& p, int epi, Product& s, const Context& c) {
     return run_products(p, epi, &s, choose_tile(&s, 1, c.dev->sms, c.common), 1, c);
 }
 
-// The parts of a split product, joined and rounded into `out` [m x ld_out].
-int join_parts(const float* parts, const Product& s, const Tile& t, void* out, const float* alpha, const Context& c) {
-    const int64_t vecs = s.m * s.ld_out / 8;
-    const int64_t blocks = std::min<int64_t>(cdiv(vecs, 256), c.dev->sms * 8);
-    return launch(&sum_round_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, 1, c.stream, parts, s.splits,
-                  static_cast<long long>(part_elements(s, t)), static_cast<uint4*>(out), static_cast<long long>(vecs),
-                  alpha, c.common.dtype == HGEMM_SM100_TRAIN_BF16 ? 1 : 0);
+// The parted tiles of a product (if any), joined into its output.
+int join_parts(const Product& s, const Tile& t, const Context& c, int in_bf16, int out_bf16) {
+    if (s.parted == 0) return HGEMM_SM100_OK;
+    JoinParams p{};
+    p.parts = s.parts;
+    p.splits = s.splits;
+    p.tiles = static_cast<int>(s.parted);
+    p.tile0 = static_cast<int>(tile_count(s, t) - s.parted);
+    p.tile_m = static_cast<int>(tile_rows(t.pair));
+    p.tile_n = t.n;
+    p.tiles_m = static_cast<int>(cdiv(s.m, p.tile_m));
+    p.tiles_n = static_cast<int>(cdiv(s.n, t.n));
+    p.group_m = group_height(s.m, s.k0 + s.k1, t.pair, t.pair ? c.dev->sms / 2 : c.dev->sms);
+    p.m = static_cast<int>(s.m);
+    p.n = static_cast<int>(s.n);
+    p.alpha = s.alpha;
+    p.beta = s.beta;
+    p.alpha_ptr = s.alpha_ptr;
+    p.c = s.c;
+    p.ldc = s.ldc;
+    p.out = s.out;
+    p.ld_out = s.ld_out;
+    p.in_bf16 = in_bf16;
+    p.out_bf16 = out_bf16;
+    const int64_t rows = std::min<int64_t>(p.tile_m, s.m), per_block = 256 / (t.n / 8);
+    // Grid rows are limited to 65535; more tiles are taken by further launches.
+    for (int first = 0; first < p.tiles; first += 65535) {
+        JoinParams q = p;
+        q.tile0 += first;
+        q.parts += static_cast<int64_t>(first) * p.tile_m * p.tile_n;
+        const int rc = launch(&join_parts_kernel, dim3(static_cast<unsigned>(cdiv(rows, per_block)),
+                                                       static_cast<unsigned>(std::min(p.tiles - first, 65535))),
+                              dim3(256), 0, 1, c.stream, q);
+        if (rc != HGEMM_SM100_OK) return rc;
+    }
+    return HGEMM_SM100_OK;
+}
+
+// A single product, with its parts at `parts` (of parts_bytes).
+int run_and_join(Product& s, const Tile& t, void* parts, const Context& c) {
+    TrainParams p;
+    init_params(p, c);
+    s.parts = static_cast<float*>(parts);
+    const int rc = run_products(p, kTrainStore, &s, t, 1, c);
+    return rc != HGEMM_SM100_OK ? rc : join_parts(s, t, c, p.in_bf16, p.out_bf16);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -450,7 +545,7 @@ struct FfnGradPlan {
     Product s[4];
     int count = 0, dx = -1;
     Tile tile;
-    size_t bytes() const { return dx >= 0 ? part_bytes(s[dx], tile) : 0; }
+    size_t bytes() const { return dx >= 0 ? parts_bytes(s[dx], tile) : 0; }
 };
 
 FfnGradPlan plan_ffn_backward(const HgemmSm100FfnBackward& a, int sms) {
@@ -501,7 +596,7 @@ extern "C" size_t hgemm_sm100_ffn_forward_workspace(const HgemmSm100FfnForward* 
     if (begin(&c, a->common, nullptr) != HGEMM_SM100_OK) return 0;
     Product d = ffn_down(*a);
     const Tile t = choose_tile(&d, 1, c.dev->sms, c.common);
-    return part_bytes(d, t);
+    return parts_bytes(d, t);
 }
 
 extern "C" int hgemm_sm100_ffn_forward(const HgemmSm100FfnForward* a, void* stream) {
@@ -516,7 +611,7 @@ extern "C" int hgemm_sm100_ffn_forward(const HgemmSm100FfnForward* a, void* stre
     if (rc != HGEMM_SM100_OK) return rc;
     Product d = ffn_down(*a);
     const Tile down_tile = choose_tile(&d, 1, c.dev->sms, c.common);
-    const size_t need = part_bytes(d, down_tile);
+    const size_t need = parts_bytes(d, down_tile);
     if (need > 0 && (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < need))
         return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     TrainParams p;
@@ -537,13 +632,7 @@ extern "C" int hgemm_sm100_ffn_forward(const HgemmSm100FfnForward* a, void* stre
     p.keep = a->gate_pre != nullptr;
     if ((rc = run_product(p, kTrainGate, g, c)) != HGEMM_SM100_OK) return rc;
 
-    if (need > 0) {
-        d.out = a->workspace;
-        d.out_kind = kTrainOutF32;
-    }
-    init_params(p, c);
-    if ((rc = run_products(p, kTrainStore, &d, down_tile, 1, c)) != HGEMM_SM100_OK || need == 0) return rc;
-    return join_parts(static_cast<const float*>(a->workspace), d, down_tile, a->y, nullptr, c);
+    return run_and_join(d, down_tile, a->workspace, c);
 }
 
 extern "C" size_t hgemm_sm100_ffn_backward_workspace(const HgemmSm100FfnBackward* a) {
@@ -588,13 +677,10 @@ extern "C" int hgemm_sm100_ffn_backward(const HgemmSm100FfnBackward* a, void* st
         p.ld_saved = a->inter;
         if ((rc = run_product(p, kTrainGateGrad, h, c)) != HGEMM_SM100_OK) return rc;
     }
-    if (need > 0) {
-        g.s[g.dx].out = a->workspace;
-        g.s[g.dx].out_kind = kTrainOutF32;
-    }
+    if (g.dx >= 0) g.s[g.dx].parts = static_cast<float*>(a->workspace);
     init_params(p, c);
-    if ((rc = run_products(p, kTrainStore, g.s, g.tile, g.count, c)) != HGEMM_SM100_OK || need == 0) return rc;
-    return join_parts(static_cast<const float*>(a->workspace), g.s[g.dx], g.tile, a->dx, nullptr, c);
+    if ((rc = run_products(p, kTrainStore, g.s, g.tile, g.count, c)) != HGEMM_SM100_OK || g.dx < 0) return rc;
+    return join_parts(g.s[g.dx], g.tile, c, p.in_bf16, p.out_bf16);
 }
 
 // ------------------------------------------------------------ cross entropy --
@@ -691,9 +777,13 @@ LossBackwardPlan plan_loss_backward(const HgemmSm100LossBackward& a, int sms) {
         };
         q.splits = g.s[0].splits;
         while (!parts_ok(std::min(q.piece, a.vocab), q.splits) || !parts_ok(last, q.splits)) --q.splits;
-        q.sums = q.pieces > 1 || q.splits > 1;
-        if (q.sums)
-            q.sum_bytes = static_cast<size_t>(round_up(q.splits * part_elements(g.s[0], q.tile) * 4, 256));
+        // Several pieces add up in FP32 tiles, in as many parts.
+        Product d = g.s[0];
+        d.splits = q.splits;
+        if (q.pieces > 1 || q.splits > 1) d.parted = tile_count(d, q.tile);
+        else d.parted = 0;
+        q.sums = d.parted > 0;
+        q.sum_bytes = static_cast<size_t>(round_up(static_cast<int64_t>(parts_bytes(d, q.tile)), 256));
     }
     return q;
 }
@@ -800,9 +890,11 @@ extern "C" int hgemm_sm100_loss_backward(const HgemmSm100LossBackward* a, void* 
             d.a0.ptr = dz;
             d.b0.ptr = w;
             d.splits = q.splits;
-            d.out = q.sums ? static_cast<void*>(sums) : a->dx;
-            d.out_kind = !q.sums ? kTrainOut16 : i == 0 ? kTrainOutF32 : kTrainOutF32Add;
-            if (!q.sums) d.alpha_ptr = alpha;
+            d.parted = q.sums ? tile_count(d, q.tile) : 0;
+            d.parts = sums;
+            d.add_parts = i > 0;
+            d.out = a->dx;
+            d.alpha_ptr = alpha;
         }
         if (a->dweight != nullptr) {
             Product& d = g.s[n++];
@@ -815,11 +907,13 @@ extern "C" int hgemm_sm100_loss_backward(const HgemmSm100LossBackward* a, void* 
         if ((rc = run_products(p, kTrainStore, g.s, q.tile, n, c)) != HGEMM_SM100_OK) return rc;
     }
     if (!q.sums) return HGEMM_SM100_OK;
-    Product d;
-    d.m = a->tokens;
-    d.n = d.ld_out = a->hidden;
+    Product d = plan_piece(*a, std::min(q.piece, a->vocab), q.piece, c.dev->sms).s[0];
     d.splits = q.splits;
-    return join_parts(sums, d, q.tile, a->dx, alpha, c);
+    d.parted = tile_count(d, q.tile);
+    d.parts = sums;
+    d.out = a->dx;
+    d.alpha_ptr = alpha;
+    return join_parts(d, q.tile, c, p.in_bf16, p.out_bf16);
 }
 
 // ------------------------------------------------------ orthogonalised update --
@@ -831,11 +925,23 @@ constexpr int kOrthSums = 592;   // partial sums of squares per matrix, at most
 struct OrthPlan {
     bool tall = false;
     int64_t side = 0, ld = 0, ld_side = 0, x_stride = 0, side_stride = 0;
-    size_t sum_bytes = 0, x_bytes = 0, side_bytes = 0;
-    size_t bytes() const { return sum_bytes + 2 * x_bytes + 2 * side_bytes; }
+    size_t sum_bytes = 0, x_bytes = 0, side_bytes = 0, parts_bytes = 0;
+    size_t bytes() const { return sum_bytes + 2 * x_bytes + 2 * side_bytes + parts_bytes; }
 };
 
-OrthPlan plan_orth(const HgemmSm100Orthogonalize& a) {
+// The three products of a step, with their sizes only.
+Product orth_product(const HgemmSm100Orthogonalize& a, int which) {
+    const int64_t side = std::min(a.rows, a.cols);
+    Product s;
+    s.m = which < 2 ? side : a.rows;
+    s.n = which < 2 ? side : a.cols;
+    s.k0 = which == 0 ? std::max(a.rows, a.cols) : side;
+    s.symmetric = which < 2;
+    s.splittable = which != 1 && a.batch == 1;
+    return s;
+}
+
+OrthPlan plan_orth(const HgemmSm100Orthogonalize& a, int sms) {
     OrthPlan q;
     q.tall = a.rows > a.cols;
     q.side = std::min(a.rows, a.cols);
@@ -846,6 +952,12 @@ OrthPlan plan_orth(const HgemmSm100Orthogonalize& a) {
     q.sum_bytes = static_cast<size_t>(round_up(a.batch * kOrthSums * 8, 256));
     q.x_bytes = static_cast<size_t>(round_up(a.batch * q.x_stride * 2, 256));
     q.side_bytes = static_cast<size_t>(round_up(a.batch * q.side_stride * 2, 256));
+    for (int which : {0, 2}) {
+        Product s = orth_product(a, which);
+        if (!s.splittable) continue;
+        const Tile t = choose_tile(&s, 1, sms, a.common);
+        q.parts_bytes = std::max(q.parts_bytes, static_cast<size_t>(round_up(static_cast<int64_t>(parts_bytes(s, t)), 256)));
+    }
     return q;
 }
 
@@ -920,29 +1032,32 @@ bool orth_sizes_ok(const HgemmSm100Orthogonalize& a) {
 }  // namespace
 
 extern "C" size_t hgemm_sm100_orthogonalize_workspace(const HgemmSm100Orthogonalize* a) {
+    Context c;
     if (a == nullptr || !orth_sizes_ok(*a) || orth_cluster_ctas(*a) > 0) return 0;
-    return plan_orth(*a).bytes();
+    if (begin(&c, a->common, nullptr) != HGEMM_SM100_OK) return 0;
+    return plan_orth(*a, c.dev->sms).bytes();
 }
 
 extern "C" int hgemm_sm100_orthogonalize(const HgemmSm100Orthogonalize* a, void* stream) {
     if (a == nullptr || !orth_sizes_ok(*a) || a->g == nullptr || a->out == nullptr || a->ldg < a->cols ||
         a->batch_stride < 0 || !(a->eps >= 0))
         return HGEMM_SM100_ERR_INVALID_ARGUMENT;
-    const OrthPlan q = plan_orth(*a);
     const int ctas = orth_cluster_ctas(*a);
-    if (ctas == 0 && (a->workspace == nullptr || reinterpret_cast<uintptr_t>(a->workspace) % 256 != 0 ||
-                      a->workspace_bytes < q.bytes()))
+    if (ctas == 0 && (a->workspace == nullptr || reinterpret_cast<uintptr_t>(a->workspace) % 256 != 0))
         return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     Context c;
     int rc = begin(&c, a->common, stream);
     if (rc != HGEMM_SM100_OK) return rc;
     if (ctas > 0) return run_orth_cluster(*a, ctas, c);
+    const OrthPlan q = plan_orth(*a, c.dev->sms);
+    if (a->workspace_bytes < q.bytes()) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     double* sums = reinterpret_cast<double*>(ws);
     uint16_t* x = reinterpret_cast<uint16_t*>(ws + q.sum_bytes);
     uint16_t* y = reinterpret_cast<uint16_t*>(ws + q.sum_bytes + q.x_bytes);
     uint16_t* gram = reinterpret_cast<uint16_t*>(ws + q.sum_bytes + 2 * q.x_bytes);
     uint16_t* poly = reinterpret_cast<uint16_t*>(ws + q.sum_bytes + 2 * q.x_bytes + q.side_bytes);
+    float* parts = reinterpret_cast<float*>(ws + q.sum_bytes + 2 * q.x_bytes + 2 * q.side_bytes);
     const int bf16 = a->common.dtype == HGEMM_SM100_TRAIN_BF16 ? 1 : 0;
     const int rows = static_cast<int>(a->rows), cols = static_cast<int>(a->cols);
     // A block per 2048 elements, several waves of blocks at most.
@@ -965,16 +1080,22 @@ extern "C" int hgemm_sm100_orthogonalize(const HgemmSm100Orthogonalize* a, void*
     const bool direct = aligned16(a->out) && a->cols % 8 == 0;
     const float inv = 1.f / kOrthScale;
     TrainParams p;
-    auto each = [&](auto&& make, int out_bf16) -> int {
+    // Product `which` of every matrix, up to four to a launch; make() adds the operands.
+    auto each = [&](int which, auto&& make, int out_bf16) -> int {
         for (int64_t first = 0; first < a->batch; first += kTrainMaxProblems) {
             Product s[kTrainMaxProblems];
             const int n = static_cast<int>(std::min<int64_t>(kTrainMaxProblems, a->batch - first));
-            for (int i = 0; i < n; ++i) make(s[i], first + i);
+            for (int i = 0; i < n; ++i) {
+                s[i] = orth_product(*a, which);
+                make(s[i], first + i);
+                s[i].parts = parts;
+            }
             const Tile t = choose_tile(s, n, c.dev->sms, c.common);
             init_params(p, c);
             p.in_bf16 = 0;
             p.out_bf16 = out_bf16;
-            const int r = run_products(p, kTrainStore, s, t, n, c);
+            int r = run_products(p, kTrainStore, s, t, n, c);
+            if (r == HGEMM_SM100_OK && n == 1) r = join_parts(s[0], t, c, 0, out_bf16);
             if (r != HGEMM_SM100_OK) return r;
         }
         return HGEMM_SM100_OK;
@@ -982,10 +1103,8 @@ extern "C" int hgemm_sm100_orthogonalize(const HgemmSm100Orthogonalize* a, void*
     for (int step = 0; step < a->steps; ++step) {
         const bool last = step + 1 == a->steps;
         // gram = X X^T or X^T X
-        rc = each([&](Product& s, int64_t i) {
+        rc = each(0, [&](Product& s, int64_t i) {
             const uint16_t* xi = x + i * q.x_stride;
-            s.m = s.n = q.side;
-            s.k0 = q.tall ? a->rows : a->cols;
             s.a0 = {xi, q.ld, q.tall};
             s.b0 = {xi, q.ld, q.tall};
             s.out = gram + i * q.side_stride;
@@ -994,9 +1113,8 @@ extern "C" int hgemm_sm100_orthogonalize(const HgemmSm100Orthogonalize* a, void*
         }, 0);
         if (rc != HGEMM_SM100_OK) return rc;
         // poly = b gram + c gram gram (symmetric)
-        rc = each([&](Product& s, int64_t i) {
+        rc = each(1, [&](Product& s, int64_t i) {
             const uint16_t* gi = gram + i * q.side_stride;
-            s.m = s.n = s.k0 = q.side;
             s.a0 = {gi, q.ld_side, false};
             s.b0 = {gi, q.ld_side, false};
             s.out = poly + i * q.side_stride;
@@ -1008,12 +1126,9 @@ extern "C" int hgemm_sm100_orthogonalize(const HgemmSm100Orthogonalize* a, void*
         }, 0);
         if (rc != HGEMM_SM100_OK) return rc;
         // X <- a X + poly X, or a X + X poly
-        rc = each([&](Product& s, int64_t i) {
+        rc = each(2, [&](Product& s, int64_t i) {
             const uint16_t* xi = x + i * q.x_stride;
             const uint16_t* pi = poly + i * q.side_stride;
-            s.m = a->rows;
-            s.n = a->cols;
-            s.k0 = q.side;
             if (q.tall) {
                 s.a0 = {xi, q.ld, false};
                 s.b0 = {pi, q.ld_side, false};

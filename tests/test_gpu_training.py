@@ -135,9 +135,11 @@ def ffn_through_c(x, gate, up, down, dy, tile, flags=0, splits=0, status=None, t
 
 
 @pytest.mark.parametrize("splits", [1, 2, 3, 5, 16])
-@pytest.mark.parametrize("size", [(5, 72, 1000, 136), (130, 264, 584, 200), (300, 520, 1352, 640)], ids=str)
+@pytest.mark.parametrize("size", [(5, 72, 1000, 136), (130, 264, 584, 200), (300, 520, 1352, 640), (1100, 136, 584, 1352)],
+                         ids=str)
 def test_ffn_sums_in_parts(size, splits):
-    """y and dx as sums of parts, whose borders fall inside either segment of dx's sum."""
+    """y and dx as sums of parts, whose borders fall inside either segment of dx's
+    sum; of all tiles, or of those after the last full wave."""
     inputs = ffn_inputs(*size, torch.bfloat16)
     for tile in (64, 192, 128 | train_capi.TILE_PAIR):
         for got, w in zip(ffn_through_c(*inputs, tile, splits=splits), ref.ffn(*inputs)):
@@ -458,6 +460,25 @@ def test_orthogonalize_one_launch_and_its_limits(size, turn):
         assert float(torch.linalg.vector_norm(out[k].double() - value)) <= err
 
 
+@pytest.mark.parametrize("splits", [0, 1, 2, 5])
+@pytest.mark.parametrize("tile", [0, 64, 128, 256 | train_capi.TILE_PAIR])
+@pytest.mark.parametrize("size", [(140, 1100), (1500, 1010), (1003, 2100)], ids=str)
+def test_orthogonalize_triangles_and_parts(size, tile, splits):
+    """Symmetric products by their upper triangle, the others' last wave in parts."""
+    g = normal(13, *size)
+    value, err = ref.orthogonalize(g, 5, NEWTON_SCHULZ, 1e-7)
+    out = torch.full_like(g, float("nan"))
+    a = train_capi.Orthogonalize(train_capi.Common(train_capi.F16, tile, 0, splits), g.data_ptr(), out.data_ptr(), None,
+                                 0, 1, *size, size[1], 0, 5, 0, *NEWTON_SCHULZ, 0.0, 1e-7)
+    ws = with_workspace("orthogonalize", a)
+    # X twice and two square matrices, rows padded to 64 elements.
+    assert ws.numel() * 2 >= 2 * size[0] * size[1] + 2 * min(size) ** 2
+    assert train_capi.run("orthogonalize", a, stream()) == capi.OK
+    assert float(torch.linalg.vector_norm(out.double() - value)) <= err
+    a.workspace_bytes -= 1
+    assert train_capi.run("orthogonalize", a, stream()) == capi.ERR_INVALID_ARGUMENT
+
+
 @pytest.mark.parametrize("ctas", [1, 2, 4, 8, 16])
 @pytest.mark.parametrize("size", [(40, 300), (300, 40), (128, 1), (128, 600), (600, 128)], ids=str)
 def test_orthogonalize_every_cluster(size, ctas):
@@ -510,9 +531,8 @@ def test_orthogonalize_every_tile(size, width, pair):
     out = torch.full_like(g, float("nan"))
     a = train_capi.Orthogonalize(train_capi.Common(train_capi.F16, width | pair), g.data_ptr(), out.data_ptr(), None, 0,
                                  1, *size, size[1], 0, 5, 0, *NEWTON_SCHULZ, 0.0, 1e-7)
-    a.workspace_bytes = train_capi.workspace("orthogonalize", a)
-    ws = torch.full((a.workspace_bytes // 2,), float("nan"), dtype=torch.float16, device="cuda")
-    a.workspace = ws.data_ptr()
+    ws = with_workspace("orthogonalize", a)
+    assert ws.numel() > 0
     assert train_capi.run("orthogonalize", a, stream()) == capi.OK
     assert float(torch.linalg.vector_norm(out.double() - value)) <= err
 
