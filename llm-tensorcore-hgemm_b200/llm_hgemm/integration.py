@@ -13,6 +13,10 @@ GEMM over the concatenated q|k|v weights (:class:`FusedQKV`) and each SwiGLU
 MLP one GEMM over interleaved gate/up weights whose ``silu_mul`` epilogue
 writes ``silu(gate) * up`` directly (:class:`HgemmSwiGLU`), followed by the
 down projection.
+
+Training (no reference counterpart): :func:`trainable_mlps` gives each SwiGLU
+MLP the differentiable block of :mod:`llm_hgemm.training`, on the same
+parameters.
 """
 
 import torch
@@ -21,6 +25,7 @@ from torch import nn
 
 from .dispatch import last_selected
 from .ops import hgemm, interleave_gate_up
+from .training import TrainableSwiGLU
 
 
 class FrozenHgemmLinear(nn.Module):
@@ -241,3 +246,22 @@ def fuse_projections(module: nn.Module, implementation: str = "shape_auto") -> d
         counts["qkv"] += sub["qkv"]
         counts["mlp"] += sub["mlp"]
     return counts
+
+
+def trainable_mlps(module: nn.Module) -> int:
+    """Replaces every SwiGLU MLP below ``module`` (children ``gate_proj``,
+    ``up_proj``, ``down_proj``, bias-free FP16 or BF16, with a SiLU ``act_fn``)
+    by a ``TrainableSwiGLU`` holding the same linears: forward and backward run
+    on this library's kernels, parameters and their names stay. Returns how
+    many were replaced."""
+    count = 0
+    for name, child in list(module.named_children()):
+        mlp = [getattr(child, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
+        if (all(isinstance(lin, nn.Linear) and lin.bias is None
+                and lin.weight.dtype in (torch.float16, torch.bfloat16) for lin in mlp)
+                and _is_silu(getattr(child, "act_fn", None))):
+            setattr(module, name, TrainableSwiGLU(*mlp))
+            count += 1
+        else:
+            count += trainable_mlps(child)
+    return count

@@ -9,6 +9,7 @@ available here, so the weights are the architecture's own random init
 
     python llm-tensorcore-hgemm_b200/model_check.py            # Qwen3-4B sizes
     python llm-tensorcore-hgemm_b200/model_check.py --layers 2 --hidden 256 ...
+    python llm-tensorcore-hgemm_b200/model_check.py --train    # a training step instead
 
 Prints one JSON line: for prefill (batch 1 x 2048 tokens, last-token logits)
 and cached decode (batch 16, one token at context 2048), the logits gate of
@@ -24,6 +25,12 @@ models' errors against it are reported beside it. Two FP16 models whose GEMMs
 round differently drift apart through 36 layers even when each GEMM is within
 its own tolerance; the floor shows how far the stock FP16 model itself sits
 from the FP32 result.
+
+``--train`` checks a training step instead: the loss and every parameter's
+gradient of the stock model (``F.cross_entropy`` on its logits) and of the
+model with ``trainable_mlps`` and ``linear_cross_entropy``, both against the
+same seeded weights in FP32, the times of forward and backward, and of the
+orthogonalised updates of the MLP weights.
 """
 
 from __future__ import annotations
@@ -206,6 +213,65 @@ def check(args) -> dict:
     }
 
 
+LOSS_SCALE = 1024.0     # of the FP16 training step (gradients of FP16 weights are FP16)
+
+
+def training_step(model, prompt, loss_of):
+    """Loss of the prompt's next tokens, every parameter's gradient (unscaled,
+    FP32) and the step's device time; ``loss_of(hidden, head_weight, labels)``."""
+    model.zero_grad(set_to_none=True)
+    labels = prompt[:, 1:]
+
+    def step():
+        hidden = model.model(prompt).last_hidden_state[:, :-1]
+        loss = loss_of(hidden, model.lm_head.weight, labels)
+        (loss * LOSS_SCALE).backward()
+        return loss.detach()
+
+    step()                       # warm-up at full size
+    model.zero_grad(set_to_none=True)
+    loss, ms = timed(step)
+    grads = {n: p.grad.float() / LOSS_SCALE for n, p in model.named_parameters()}
+    return float(loss), grads, ms
+
+
+def stock_loss(hidden, weight, labels):
+    logits = torch.nn.functional.linear(hidden, weight)
+    return torch.nn.functional.cross_entropy(logits.float().flatten(0, 1), labels.flatten())
+
+
+def train_check(args) -> dict:
+    """The training-step check described in the module docstring."""
+    from llm_hgemm import linear_cross_entropy, orthogonalize
+    from llm_hgemm.integration import trainable_mlps
+
+    g = torch.Generator(device="cuda").manual_seed(args.seed + 1)
+    prompt = torch.randint(0, args.vocab, (1, args.prefill_tokens), device="cuda", generator=g)
+
+    model = build_model(args).float()
+    exact_loss, exact, _ = training_step(model, prompt, stock_loss)
+    del model
+    torch.cuda.empty_cache()
+
+    model = build_model(args)
+    result = {"fp32_loss": exact_loss}
+    for name in ("stock", "hgemm"):
+        if name == "hgemm":
+            result["mlps"] = trainable_mlps(model)
+        loss, grads, ms = training_step(model, prompt, stock_loss if name == "stock" else linear_cross_entropy)
+        errors = {n: float(torch.linalg.vector_norm(v - exact[n]) / torch.linalg.vector_norm(exact[n]).clamp_min(1e-12))
+                  for n, v in grads.items()}
+        worst = max(errors, key=errors.get)
+        result[name] = {"loss": loss, "step_ms": round(ms, 3), "worst_gradient": worst,
+                        "worst_gradient_relative_l2": errors[worst],
+                        "mean_gradient_relative_l2": sum(errors.values()) / len(errors)}
+        del grads
+    updates = [p.grad for n, p in model.named_parameters() if ".mlp." in n]
+    _, ms = timed(lambda: [orthogonalize(u) for u in updates])
+    result["updates"] = {"matrices": len(updates), "ms": round(ms, 3)}
+    return result
+
+
 def parser() -> argparse.ArgumentParser:
     p = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     p.add_argument("--layers", type=int, default=36)
@@ -224,11 +290,13 @@ def parser() -> argparse.ArgumentParser:
                    help="skip the fused-projection variant (second model copy)")
     p.add_argument("--no-fp32", action="store_true",
                    help="skip the FP32 model (the FP16-propagation floor)")
+    p.add_argument("--train", action="store_true", help="check a training step instead of the rollout")
     return p
 
 
 def main() -> None:
-    print(json.dumps(check(parser().parse_args())), flush=True)
+    args = parser().parse_args()
+    print(json.dumps(train_check(args) if args.train else check(args)), flush=True)
 
 
 if __name__ == "__main__":

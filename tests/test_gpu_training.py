@@ -657,3 +657,26 @@ def test_a_training_step_of_a_small_model():
                 assert float(torch.linalg.vector_norm(update.double() - value_)) <= err
                 p -= 0.02 * update
                 p.grad = None
+
+
+def test_model_training_step():
+    """A small decoder with ``trainable_mlps`` and ``linear_cross_entropy``: each
+    FP16 model's gradients against the FP32 model's. Ours round the MLP three
+    times (gate and up pre-activations, product) where the stock model rounds
+    four times, and the logits never: no parameter may be further off than 1.5
+    times the stock model's worst."""
+    import importlib.util
+
+    from tests.conftest import PKG
+
+    spec = importlib.util.spec_from_file_location("model_check", PKG / "model_check.py")
+    mc = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mc)
+    args = mc.parser().parse_args(["--train", "--layers", "2", "--hidden", "256", "--intermediate", "704", "--heads", "4",
+                                   "--kv-heads", "2", "--head-dim", "64", "--vocab", "1000", "--prefill-tokens", "96",
+                                   "--context", "64"])
+    res = mc.train_check(args)
+    assert res["mlps"] == 2 and res["updates"]["matrices"] == 6
+    assert res["hgemm"]["worst_gradient_relative_l2"] <= 1.5 * res["stock"]["worst_gradient_relative_l2"], res
+    # Losses of about 7, each in FP32 from FP16 activations: 2^-11 relative is a wide margin.
+    assert abs(res["hgemm"]["loss"] - res["fp32_loss"]) <= 2 ** -11 * res["fp32_loss"], res

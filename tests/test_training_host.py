@@ -140,3 +140,33 @@ def test_reference_orthogonalize_matches_the_steps():
         x = a * x + (b * p + c * (p @ p)) @ x
     value, err = ref.orthogonalize(g, 5, NEWTON_SCHULZ, 1e-7)
     assert torch.allclose(value, x, atol=1e-9) and 0 < err < 1
+
+
+def test_fingerprint_leaves_the_training_operators_out(tmp_path, monkeypatch):
+    """A dispatch table stays valid when only the training operators change."""
+    from llm_hgemm import provenance
+
+    names = {rel for rel, _ in provenance._sources()}
+    assert not names & provenance._APART
+    assert all((provenance.REPO_ROOT / rel).is_file() for rel in provenance._APART)
+    assert {"include/hgemm_sm100.h", "llm-tensorcore-hgemm_b200/csrc/hgemm_kernels.cuh",
+            "llm-tensorcore-hgemm_b200/csrc/host/bindings.cpp"} <= names
+
+
+def test_trainable_mlps_keeps_the_parameters():
+    from llm_hgemm.integration import trainable_mlps
+
+    class Mlp(nn.Module):
+        def __init__(self, act, dtype=torch.float16):
+            super().__init__()
+            self.gate_proj, self.up_proj = (nn.Linear(8, 16, bias=False, dtype=dtype) for _ in range(2))
+            self.down_proj = nn.Linear(16, 8, bias=False, dtype=dtype)
+            self.act_fn = act
+
+    model = nn.ModuleDict({"a": Mlp(nn.SiLU()), "b": nn.ModuleList([Mlp(nn.SiLU()), Mlp(nn.GELU())]),
+                           "c": Mlp(nn.SiLU(), torch.float32)})
+    before = {n: id(p) for n, p in model.named_parameters()}
+    assert trainable_mlps(model) == 2
+    assert isinstance(model["a"], TrainableSwiGLU) and isinstance(model["b"][0], TrainableSwiGLU)
+    assert not isinstance(model["b"][1], TrainableSwiGLU) and not isinstance(model["c"], TrainableSwiGLU)
+    assert {n: id(p) for n, p in model.named_parameters()} == before
