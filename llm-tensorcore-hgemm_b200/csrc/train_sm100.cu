@@ -580,9 +580,9 @@ FfnGradPlan plan_ffn_backward(const HgemmSm100FfnBackward& a, int sms) {
     weight(a.ddown, a.dy, a.lddy, a.out, a.h, a.inter, a.inter);
     if (g.count == 0) return g;
     g.tile = choose_tile(g.s, g.count, sms, a.common);
-    std::stable_sort(g.s, g.s + g.count, [](const Product& x, const Product& y) {
-        return cdiv(x.kblocks(), x.splits) > cdiv(y.kblocks(), y.splits);
-    });
+    auto length = [](const Product& p) { return cdiv(p.kblocks(), p.splits); };
+    for (int i = 1; i < g.count; ++i)
+        for (int j = i; j > 0 && length(g.s[j]) > length(g.s[j - 1]); --j) std::swap(g.s[j], g.s[j - 1]);
     for (int i = 0; i < g.count; ++i)
         if (g.s[i].splittable) g.dx = i;
     return g;
@@ -1020,7 +1020,10 @@ int run_orth_cluster(const HgemmSm100Orthogonalize& a, int ctas, const Context& 
     p.eps = a.eps;
     p.status = a.common.status != nullptr ? a.common.status : c.dev->status_word;
     p.timeout_ns = a.common.timeout_ns != 0 ? a.common.timeout_ns : kDefaultTimeoutNs;
-    const size_t smem = static_cast<size_t>(p.slice / 64) * kOrthBlockBytes + 2 * kOrthSquareBytes + 1024 + 512;
+    // One CTA to an SM: two of different clusters would wait for the one's TMEM
+    // while their clusters wait for them.
+    const size_t smem = std::max<size_t>(
+        static_cast<size_t>(p.slice / 64) * kOrthBlockBytes + 2 * kOrthSquareBytes + 1024 + 512, 120 * 1024);
     return launch(k.fn, dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(a.batch)),
                   dim3(kOrthThreads), smem, ctas, c.stream, p);
 }

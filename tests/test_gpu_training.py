@@ -403,6 +403,25 @@ def test_loss_extreme_logits_and_gradients():
             within(got, v)
 
 
+def test_one_token_without_a_token_dimension():
+    x, gate, up, down, dy = ffn_inputs(1, 64, 128, 72, torch.float16)
+    v = x[0].clone().requires_grad_()
+    y = llm_hgemm.gated_ffn(v, gate, up, down)
+    want = ref.ffn(x, gate, up, down, dy)
+    assert y.shape == (72,)
+    (dx,) = torch.autograd.grad(y, v, dy[0])
+    within(y.detach()[None], want[0])
+    within(dx[None], want[1])
+    w = normal(3, 90, 64)
+    t = torch.tensor(5, device="cuda")
+    each = llm_hgemm.linear_cross_entropy(v, w, t, reduction="none")
+    assert each.shape == ()
+    (dx,) = torch.autograd.grad(each, v, torch.tensor(2.0, device="cuda"))
+    want = ref.loss(x, w, t[None], "none", -100, torch.tensor([2.0], device="cuda"))
+    within(each.detach()[None], want[0])
+    within(dx[None], want[1])
+
+
 def test_loss_no_tokens():
     w = normal(1, 50, 64).requires_grad_()
     x = normal(2, 0, 64).requires_grad_()
@@ -535,6 +554,24 @@ def test_orthogonalize_every_tile(size, width, pair):
     assert ws.numel() > 0
     assert train_capi.run("orthogonalize", a, stream()) == capi.OK
     assert float(torch.linalg.vector_norm(out.double() - value)) <= err
+
+
+def test_orthogonalize_many_clusters_on_two_streams():
+    """More clusters than fit the GPU at once, of two calls at the same time."""
+    g = [normal(14 + k, 40, *size) for k, size in enumerate(((16, 2100), (100, 700)))]
+    want = [llm_hgemm.orthogonalize(t) for t in g]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in g]
+    got = [[], []]
+    for _ in range(5):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(llm_hgemm.orthogonalize(g[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert torch.equal(want[k][7], llm_hgemm.orthogonalize(g[k][7]))
+        for t in got[k]:
+            assert torch.equal(t, want[k])
 
 
 # -------------------------------------------------------- how they are called ---
