@@ -30,10 +30,19 @@
 // Roles per CTA: warps 0-7 epilogue (one TMEM lane = one output row per
 // thread; warps w and w + 4 share a row quarter and take every second group of
 // 32 columns), warp 8 TMA producer, warp 9 MMA issuer; two accumulators, so a
-// tile's epilogue runs under the next tile's MMAs. The last tile's epilogue is
-// exposed, and it is what eight warps halve (6400 -> 3200 cycles of a 256-wide
-// tile). Every wait is bounded as in the inference kernels (status word,
-// drained copies, freed TMEM).
+// tile's epilogue runs under the next tile's MMAs; eight warps, because the last
+// tile's epilogue is exposed and the gradient of the gate is a long one (dh at
+// 4096 x 9728 x 2560: 278 us with four, 192 with eight). Every wait is bounded
+// as in the inference kernels (status word, drained copies, freed TMEM).
+//
+// What bounds it (2048 tokens, hidden 2560, under ncu): the tensor pipe where
+// the epilogue stores nothing (softmax statistics: 91 % active, 1.7 PFLOP/s in
+// a burst); 80-85 % where it stores 16 bits (logit gradients, the weights'
+// gradients); 73 % with three outputs (gate, kept pre-activations); 46 % where
+// it reads two matrices and writes two (gradient of the gate), DRAM at 24 % and
+// L2 at 50 % throughout. Long back-to-back runs are held by the power limit
+// instead (1.2-1.35 PFLOP/s). A K block of a 256 x 256 pair tile takes about
+// 590 cycles of which the MMAs are 512.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -82,7 +91,7 @@ struct alignas(64) TrainProblem {
     int out_kind;
     float alpha, beta;
     const float* alpha_ptr;    // multiplies alpha (device memory; may be null)
-    const void* c;             // 16-bit [m x ldc] for beta != 0
+    const void* c;             // FP16 [m x ldc] for beta != 0
     long long ldc;
 };
 
@@ -114,13 +123,17 @@ struct alignas(64) TrainParams {
 
 // ------------------------------------------------------------- small parts ---
 
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, int bf16) {
-    if (bf16) {
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (kBf16) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
         return *reinterpret_cast<const uint32_t*>(&h);
     }
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, int bf16) {
+    return bf16 ? pack2<true>(lo, hi) : pack2<false>(lo, hi);
 }
 __device__ __forceinline__ float2 unpack2(uint32_t w, int bf16) {
     if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
@@ -156,9 +169,10 @@ struct Row32 {
 #pragma unroll
         for (int q = 0; q < 4; ++q) w[q] = 8 * q < avail ? __ldg(src + q) : make_uint4(0u, 0u, 0u, 0u);
     }
-    __device__ __forceinline__ float2 pair(int i, int bf16) const {   // elements 2i, 2i + 1
+    template <bool kBf16>
+    __device__ __forceinline__ float2 pair(int i) const {   // elements 2i, 2i + 1
         const uint4& v = w[i >> 2];
-        return unpack2((i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w, bf16);
+        return unpack2((i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w, kBf16);
     }
 };
 
@@ -180,20 +194,25 @@ struct BoxWriter {
     uint32_t next;
     uint32_t lane;
 
-    __device__ void put16(const CUtensorMap* map, const float (&v)[32], int bf16, int col, int row) {
+    // The next buffer, once the store that used it last has read it.
+    __device__ __forceinline__ uint8_t* take() {
         if (lane == 0) bulk_wait_group_read<1>();
         __syncwarp();
-        uint8_t* box = bufs + (next & 1u) * kTrainBoxBytes;
-        ++next;
+        return bufs + (next++ & 1u) * kTrainBoxBytes;
+    }
+    template <bool kBf16>
+    __device__ __forceinline__ void fill(uint8_t* box, const float (&v)[32]) const {
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
             uint4 q;
-            q.x = pack2(v[8 * j + 0], v[8 * j + 1], bf16);
-            q.y = pack2(v[8 * j + 2], v[8 * j + 3], bf16);
-            q.z = pack2(v[8 * j + 4], v[8 * j + 5], bf16);
-            q.w = pack2(v[8 * j + 6], v[8 * j + 7], bf16);
+            q.x = pack2<kBf16>(v[8 * j + 0], v[8 * j + 1]);
+            q.y = pack2<kBf16>(v[8 * j + 2], v[8 * j + 3]);
+            q.z = pack2<kBf16>(v[8 * j + 4], v[8 * j + 5]);
+            q.w = pack2<kBf16>(v[8 * j + 6], v[8 * j + 7]);
             *reinterpret_cast<uint4*>(box + lane * 64u + ((j ^ ((lane >> 1) & 3u)) << 4)) = q;
         }
+    }
+    __device__ __forceinline__ void send(const CUtensorMap* map, const uint8_t* box, int col, int row) const {
         fence_async_shared();
         __syncwarp();
         if (lane == 0) {
@@ -202,25 +221,42 @@ struct BoxWriter {
         }
     }
 
-    // The transposed box: lane = column `col` + lane, v = rows row .. row + 31.
-    __device__ void put16_turned(const CUtensorMap* map, const float (&v)[32], int bf16, int col, int row) {
-        if (lane == 0) bulk_wait_group_read<1>();
+    template <bool kBf16>
+    __device__ __forceinline__ void put16(const CUtensorMap* map, const float (&v)[32], int col, int row) {
+        uint8_t* box = take();
+        fill<kBf16>(box, v);
+        send(map, box, col, row);
+    }
+
+    // Two boxes (the second one with `two`) with one hand-over to the stores.
+    template <bool kBf16>
+    __device__ __forceinline__ void put16_two(const CUtensorMap* map, const float (&v)[32], const float (&w)[32],
+                                              bool two, int col, int col_two, int row) {
+        if (lane == 0) bulk_wait_group_read<0>();
         __syncwarp();
-        uint8_t* box = bufs + (next & 1u) * kTrainBoxBytes;
-        ++next;
+        fill<kBf16>(bufs, v);
+        if (two) fill<kBf16>(bufs + kTrainBoxBytes, w);
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+            tma_store_2d(map, bufs, col, row);
+            if (two) tma_store_2d(map, bufs + kTrainBoxBytes, col_two, row);
+            bulk_commit_group();
+        }
+    }
+
+    // The transposed box: lane = column `col` + lane, v = rows row .. row + 31.
+    template <bool kBf16>
+    __device__ __forceinline__ void put16_turned(const CUtensorMap* map, const float (&v)[32], int col, int row) {
+        uint8_t* box = take();
 #pragma unroll
         for (uint32_t i = 0; i < 32; i += 2) {
-            const uint32_t w = pack2(v[i], v[i + 1], bf16);
+            const uint32_t w = pack2<kBf16>(v[i], v[i + 1]);
             const uint32_t at = (((lane >> 3) ^ ((i >> 1) & 3u)) << 4) + (lane & 7u) * 2u;   // alike for i and i + 1
             *reinterpret_cast<uint16_t*>(box + i * 64u + at) = static_cast<uint16_t>(w);
             *reinterpret_cast<uint16_t*>(box + i * 64u + 64u + at) = static_cast<uint16_t>(w >> 16);
         }
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) {
-            tma_store_2d(map, box, col, row);
-            bulk_commit_group();
-        }
+        send(map, box, col, row);
     }
 
     __device__ void put32(const CUtensorMap* map, const float (&v)[32], bool add, int col, int row) {
@@ -242,6 +278,19 @@ struct BoxWriter {
         }
     }
 };
+
+// Two accumulator groups (the second one with `two`), loaded together.
+__device__ __forceinline__ void tmem_ld32_two(uint32_t t, uint32_t t_two, bool two, float (&v)[32], float (&w)[32]) {
+    uint32_t a[32], b[32];
+    tmem_ld_32x32b_x32(t, a);
+    if (two) tmem_ld_32x32b_x32(t_two, b);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        v[i] = __uint_as_float(a[i]);
+        w[i] = __uint_as_float(b[i]);
+    }
+}
 
 __device__ __forceinline__ void tmem_ld32(uint32_t t, float (&v)[32]) {
     uint32_t r[32];
@@ -346,7 +395,7 @@ struct TrainEpilogue {
         const int col = tn * width + c;
         const int avail = in_rows && c < width ? q.n - col : 0;
         if constexpr (kEpi == kTrainStore) {
-            if (q.beta != 0.f) a.load(q.c, row * q.ldc + col, avail);
+            a.load(q.c, row * q.ldc + col, q.beta != 0.f ? avail : 0);
         } else if constexpr (kEpi == kTrainGateGrad) {
             a.load(p.gate, row * p.ld_saved + col, avail);
             b.load(p.up, row * p.ld_saved + col, avail);
@@ -354,7 +403,10 @@ struct TrainEpilogue {
     }
     // The rows of the saved pre-activations come from DRAM: one 128-byte line
     // per row and 64 columns into L2 while the tile is still multiplied, or each
-    // group's loads would wait for memory in turn.
+    // group's loads would wait for memory in turn (192 -> 175 us for dh at
+    // 4096 x 9728 x 2560, with the approximate reciprocal). Boxes through TMA
+    // instead took a stage from the ring and gained 2 % there, and lost 3 % in
+    // a x X + poly X.
     __device__ void begin() {
         if constexpr (kEpi == kTrainGateGrad) {
             const void* src = first == 0 ? p.gate : p.up;
@@ -364,20 +416,99 @@ struct TrainEpilogue {
         fetch(first, x, y);
     }
 
-    // t: TMEM address of the accumulator, this warp's lane quarter.
-    __device__ void run(BoxWriter& box, uint32_t t) {
+    // t: TMEM address of the accumulator, this warp's lane quarter. The output
+    // type is a template parameter: choosing it per pair of elements doubled the
+    // instructions, and with two epilogue warps a scheduler these set the time
+    // of tiles with short sums.
+    __device__ __forceinline__ void run(BoxWriter& box, uint32_t t) {
         if (row0 >= q.m) return;
+        if constexpr (kEpi == kTrainLse) {
+            statistics(t);
+        } else if (kEpi == kTrainStore && q.out_kind != kTrainOut16) {
+#pragma unroll 1
+            for (int c = first; c < width && tn * width + c < q.n; c += 64) {
+                float v[32];
+                tmem_ld32(t + c, v);
+                box.put32(&q.out[0], v, q.out_kind == kTrainOutF32Add, c, out_row);
+            }
+        } else if (p.out_bf16) {
+            store<true>(box, t);
+        } else {
+            store<false>(box, t);
+        }
+    }
+
+    // Running maximum and sum over this thread's columns of the tile, four
+    // interleaved chains of each.
+    __device__ __forceinline__ void statistics(uint32_t t) {
         const float kNone = __int_as_float(0xff800000);
-        float alpha = 0.f, top = kNone, sum = 0.f, scale = 0.f, lse = 0.f;
+        const long long want = in_rows ? p.target[row] - p.col_base : -1;
+        float top = kNone, sum = 0.f;
+#pragma unroll 1
+        for (int c = first; c < width; c += 64) {
+            const int col = tn * width + c;
+            if (col >= q.n) break;
+            float v[32];
+            tmem_ld32(t + c, v);
+            if (want >= col && want < col + 32 && want < q.n) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (col + i == want) p.target_logit[row] = v[i];
+            }
+            if (col + 32 > q.n) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (col + i >= q.n) v[i] = kNone;
+            }
+            float best[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+            for (int i = 4; i < 32; ++i) best[i & 3] = fmaxf(best[i & 3], v[i]);
+            const float most = fmaxf(fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])), top);
+            // No column above -inf yet: subtract 0, so that exp gives 0, not NaN.
+            const float ref = most == kNone ? 0.f : most;
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 32; ++i) part[i & 3] += exp2_fast((v[i] - ref) * kLog2e);
+            sum = fmaf(sum, exp2_fast((top - ref) * kLog2e), (part[0] + part[1]) + (part[2] + part[3]));
+            top = most;
+        }
+        if (in_rows) p.partial[static_cast<long long>(2 * tn + first / 32) * q.m + row] = make_float2(top, sum);
+    }
+
+    template <bool kBf16>
+    __device__ __forceinline__ void store(BoxWriter& box, uint32_t t) {
+        float alpha = 0.f, scale = 0.f, lse = 0.f;
         long long want = -1;
         if constexpr (kEpi == kTrainStore) alpha = q.alpha_ptr != nullptr ? q.alpha * __ldg(q.alpha_ptr) : q.alpha;
-        if constexpr (kEpi == kTrainLse || kEpi == kTrainLogitGrad)
-            if (in_rows) want = p.target[row] - p.col_base;
         if constexpr (kEpi == kTrainLogitGrad)
             if (in_rows) {
+                want = p.target[row] - p.col_base;
                 scale = p.row_scale[row];
                 lse = p.lse[row];
             }
+        if (kEpi == kTrainLogitGrad || (kEpi == kTrainStore && q.beta == 0.f && !mirror)) {
+            // Two groups a turn.
+#pragma unroll 1
+            for (int c = first; c < width; c += 128) {
+                const int col = tn * width + c;
+                if (col >= q.n) break;
+                const bool two = c + 64 < width && col + 64 < q.n;
+                float v[32], w[32];
+                tmem_ld32_two(t + c, t + c + 64, two, v, w);
+                if constexpr (kEpi == kTrainStore) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        v[i] *= alpha;
+                        w[i] *= alpha;
+                    }
+                } else {
+                    logit_gradient(v, col, want, scale, lse);
+                    logit_gradient(w, col + 64, want, scale, lse);
+                }
+                box.put16_two<kBf16>(&q.out[0], v, w, two, col, col + 64, row0);
+            }
+            return;
+        }
 #pragma unroll 1
         for (int c = first; c < width; c += 64) {
             const int col = tn * width + c;
@@ -387,38 +518,29 @@ struct TrainEpilogue {
             float v[32];
             tmem_ld32(t + c, v);
             if constexpr (kEpi == kTrainStore) {
-                if (q.out_kind != kTrainOut16) {
-                    box.put32(&q.out[0], v, q.out_kind == kTrainOutF32Add, c, out_row);
-                    continue;
-                }
-                if (q.beta != 0.f) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float2 w = x.pair(i, p.in_bf16);
-                        v[2 * i] = fmaf(alpha, v[2 * i], q.beta * w.x);
-                        v[2 * i + 1] = fmaf(alpha, v[2 * i + 1], q.beta * w.y);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] *= alpha;
+                for (int i = 0; i < 16; ++i) {
+                    const float2 w = x.template pair<false>(i);   // C is FP16
+                    v[2 * i] = fmaf(alpha, v[2 * i], q.beta * w.x);
+                    v[2 * i + 1] = fmaf(alpha, v[2 * i + 1], q.beta * w.y);
                 }
-                box.put16(&q.out[0], v, p.out_bf16, col, row0);
-                if (mirror) box.put16_turned(&q.out[0], v, p.out_bf16, row0, col);
+                box.put16<kBf16>(&q.out[0], v, col, row0);
+                if (mirror) box.put16_turned<kBf16>(&q.out[0], v, row0, col);
             } else if constexpr (kEpi == kTrainGate) {
                 float u[32];
                 tmem_ld32(t + width + c, u);
                 if (p.keep) {
-                    box.put16(&q.out[1], v, p.out_bf16, col, row0);
-                    box.put16(&q.out[2], u, p.out_bf16, col, row0);
+                    box.put16<kBf16>(&q.out[1], v, col, row0);
+                    box.put16<kBf16>(&q.out[2], u, col, row0);
                 }
 #pragma unroll
                 for (int i = 0; i < 32; ++i) u[i] *= v[i] * sigmoid_f(v[i]);
-                box.put16(&q.out[0], u, p.out_bf16, col, row0);
+                box.put16<kBf16>(&q.out[0], u, col, row0);
             } else if constexpr (kEpi == kTrainGateGrad) {
                 float du[32];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float2 g = x.pair(i, p.in_bf16), u = y.pair(i, p.in_bf16);
+                    const float2 g = x.template pair<kBf16>(i), u = y.template pair<kBf16>(i);
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const float gj = j ? g.y : g.x, uj = j ? u.y : u.x, dh = v[2 * i + j];
@@ -428,47 +550,24 @@ struct TrainEpilogue {
                         du[2 * i + j] = dh * silu;
                     }
                 }
-                box.put16(&q.out[0], v, p.out_bf16, col, row0);
-                box.put16(&q.out[1], du, p.out_bf16, col, row0);
-            } else if constexpr (kEpi == kTrainLse) {
-                // Running maximum and sum over this thread's columns of the tile.
-                if (want >= col && want < col + 32 && want < q.n) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (col + i == want) p.target_logit[row] = v[i];
-                }
-                if (col + 32 > q.n) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (col + i >= q.n) v[i] = kNone;
-                }
-                float best = v[0];
-#pragma unroll
-                for (int i = 1; i < 32; ++i) best = fmaxf(best, v[i]);
-                best = fmaxf(best, top);
-                // No column above -inf yet: subtract 0, so that exp gives 0, not NaN.
-                const float ref = best == kNone ? 0.f : best;
-                float part = 0.f;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) part += exp2_fast((v[i] - ref) * kLog2e);
-                sum = fmaf(sum, exp2_fast((top - ref) * kLog2e), part);
-                top = best;
-            } else {
-                // A row without a target has factor 0 and gradient 0, whatever its logits.
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = scale == 0.f ? 0.f : exp2_fast((v[i] - lse) * kLog2e) * scale;
-                if (want >= col && want < col + 32) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (col + i == want) v[i] -= scale;
-                }
-                box.put16(&q.out[0], v, p.out_bf16, col, row0);
+                box.put16<kBf16>(&q.out[0], v, col, row0);
+                box.put16<kBf16>(&q.out[1], du, col, row0);
             }
             x = nx;
             y = ny;
         }
-        if constexpr (kEpi == kTrainLse)
-            if (in_rows) p.partial[static_cast<long long>(2 * tn + first / 32) * q.m + row] = make_float2(top, sum);
+    }
+
+    // (exp(z - lse) - [column == target]) scale. A row without a target has factor
+    // 0 and gradient 0, whatever its logits.
+    __device__ __forceinline__ void logit_gradient(float (&v)[32], int col, long long want, float scale, float lse) const {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = scale == 0.f ? 0.f : exp2_fast((v[i] - lse) * kLog2e) * scale;
+        if (want >= col && want < col + 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (col + i == want) v[i] -= scale;
+        }
     }
 };
 
@@ -504,6 +603,14 @@ __device__ __forceinline__ void tc_commit_if(uint32_t issuer, uint32_t bar) {
         asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
                      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
                      ::"r"(bar), "r"(issuer) : "memory");
+}
+
+// Frees an accumulator: arrives at the leader CTA's barrier (shared::cluster
+// address). Ordered after this warp's TMEM reads by tcgen05.wait::ld and the
+// fence before; no other memory is handed over, so no cluster-wide release,
+// which waits for the tile's stores on their way (900 to 3000 cycles a tile).
+__device__ __forceinline__ void acc_release_pair(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // A compile-time argument of the producer's inner loop, and the ways B comes.
@@ -746,7 +853,7 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) {
-                if constexpr (kPair) mbar_arrive_cluster(acc ? tempty1 : tempty0);
+                if constexpr (kPair) acc_release_pair(acc ? tempty1 : tempty0);
                 else mbar_arrive(&tempty[acc]);
             }
         }
@@ -774,46 +881,58 @@ constexpr float kLogitGradScale = 16384.f;
 // Joins a row's per-tile (max, sum) pairs: lse = max + log(sum), and its loss
 // lse - logit[target], formed as (max - logit) + log(sum). A row whose target
 // is `ignore` has loss 0; one outside the vocabulary gets NaN.
-// Block (32 rows, 32 slices of the tile list), joined in shared memory.
+// Block (kRows rows, 1024 / kRows slices of the pairs), joined in shared memory;
+// a thread has four pairs in flight. 8 rows to a block: with 32 there are few
+// blocks and a thread walks many pairs in turn (182 rows x 126940: 14 us).
+__device__ __forceinline__ float2 join_pairs(float2 a, float2 b) {
+    const float best = fmaxf(a.x, b.x);
+    const float ref = best == __int_as_float(0xff800000) ? 0.f : best;
+    // A NaN sum stays NaN.
+    return make_float2(best, a.y * exp2_fast((a.x - ref) * kLog2e) + b.y * exp2_fast((b.x - ref) * kLog2e));
+}
+
+template <int kRows>
 __global__ void __launch_bounds__(1024) lse_join_kernel(const float2* __restrict__ partial, int tiles, int m,
                                                         const float* __restrict__ target_logit,
                                                         const long long* __restrict__ target, long long vocab,
                                                         long long ignore, float* __restrict__ lse,
                                                         float* __restrict__ loss) {
-    __shared__ float2 part[32][33];
+    constexpr int kSlices = 1024 / kRows;
+    __shared__ float2 part[kSlices][kRows + 1];
     grid_dependents_launch();
     grid_dependency_wait();
-    const int row = blockIdx.x * 32 + threadIdx.x;
-    const float kNone = __int_as_float(0xff800000);
-    float top = kNone, sum = 0.f;   // a NaN sum stays NaN through every join
-    if (row < m) {
-        for (int t = threadIdx.y; t < tiles; t += 32) {
-            const float2 v = partial[static_cast<long long>(t) * m + row];
-            const float best = fmaxf(top, v.x);
-            const float ref = best == kNone ? 0.f : best;
-            sum = sum * exp2_fast((top - ref) * kLog2e) + v.y * exp2_fast((v.x - ref) * kLog2e);
-            top = best;
+    const int row = blockIdx.x * kRows + threadIdx.x;
+    const float2 none = make_float2(__int_as_float(0xff800000), 0.f);
+    float2 all = none;
+    if (row < m)
+        for (int t = threadIdx.y; t < tiles; t += 4 * kSlices) {
+            float2 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = t + kSlices * i;
+                v[i] = at < tiles ? partial[static_cast<long long>(at) * m + row] : none;
+            }
+            all = join_pairs(all, join_pairs(join_pairs(v[0], v[1]), join_pairs(v[2], v[3])));
         }
-    }
-    part[threadIdx.y][threadIdx.x] = make_float2(top, sum);
+    part[threadIdx.y][threadIdx.x] = all;
     __syncthreads();
-    if (threadIdx.y != 0 || row >= m) return;
-    for (int t = 1; t < 32; ++t) {
-        const float2 v = part[t][threadIdx.x];
-        const float best = fmaxf(top, v.x);
-        const float ref = best == kNone ? 0.f : best;
-        sum = sum * exp2_fast((top - ref) * kLog2e) + v.y * exp2_fast((v.x - ref) * kLog2e);
-        top = best;
+    for (int half = kSlices / 2; half > 0; half /= 2) {
+        if (static_cast<int>(threadIdx.y) < half)
+            part[threadIdx.y][threadIdx.x] =
+                join_pairs(part[threadIdx.y][threadIdx.x], part[threadIdx.y + half][threadIdx.x]);
+        __syncthreads();
     }
-    const float ls = logf(sum);
-    lse[row] = top + ls;
+    if (threadIdx.y != 0 || row >= m) return;
+    all = part[0][threadIdx.x];
+    const float ls = logf(all.y);
+    lse[row] = all.x + ls;
     const long long want = target[row];
     if (want == ignore) loss[row] = 0.f;
-    else loss[row] = (want >= 0 && want < vocab) ? (top - target_logit[row]) + ls : __int_as_float(0x7fffffff);
+    else loss[row] = (want >= 0 && want < vocab) ? (all.x - target_logit[row]) + ls : __int_as_float(0x7fffffff);
 }
 
 // Sum of the rows' losses (and their count for the mean), one block, in a
-// fixed order and 64 bits.
+// fixed order and 64 bits. Latency: 3-4 us up to 4096 rows.
 __global__ void __launch_bounds__(1024) loss_reduce_kernel(const float* __restrict__ loss,
                                                            const long long* __restrict__ target, int m,
                                                            long long ignore, int mean, float* __restrict__ out) {
@@ -847,7 +966,7 @@ __global__ void __launch_bounds__(1024) loss_reduce_kernel(const float* __restri
 // Row factors of the logits' gradient and the scalar that the products take:
 // dz[row] = row_scale[row] (p - onehot), gradient = alpha dz^T x and so on.
 // One loss per row: row_scale = dloss[row] / max |dloss|, so that any range of
-// incoming gradients fits 16 bits. One block.
+// incoming gradients fits 16 bits. One block; latency, 5 us up to 4096 rows.
 __global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* __restrict__ dloss, int per_row, int mean,
                                                                 const long long* __restrict__ target, int m,
                                                                 long long vocab, long long ignore,
@@ -904,7 +1023,9 @@ __global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* __r
 
 // The tiles of a product whose sums came in parts: out = alpha (part 0 + part 1
 // + ...) + beta C, added in that order and rounded once. Block (x, y): some rows
-// of tile tile0 + y; eight columns per thread.
+// of tile tile0 + y; eight columns per thread. Reads what the parts wrote, mostly
+// from L2: 3 us of a launch more, which the parts have to save (y of one token,
+// 2560 x 9728: 42 us whole, 15 + 3 in parts).
 struct JoinParams {
     const float* parts;
     int splits, tiles, tile0, tiles_m, tiles_n, group_m, tile_m, tile_n, m, n;
@@ -986,7 +1107,9 @@ __device__ __forceinline__ void orth_load8(const void* g, long long row, int c, 
 
 // Sums of squares of matrix blockIdx.y: sums[matrix][block]. Eight squares are
 // added in FP32 after dividing by their largest power of two, everything above
-// in 64 bits, so that no size of element overflows or is lost. One pass over g.
+// in 64 bits, so that no size of element overflows or is lost. One pass over g
+// (16-byte loads, one conversion to 64 bits per eight elements: 9728 x 2560
+// takes 19 us cold, element by element in 64 bits it took 114).
 template <bool kVec>
 __global__ void __launch_bounds__(256) orth_square_kernel(const void* __restrict__ g, long long batch_stride, int rows,
                                                           int cols, long long ld, int bf16,
@@ -1024,7 +1147,8 @@ __global__ void __launch_bounds__(256) orth_square_kernel(const void* __restrict
     }
 }
 
-// x = FP16(g kOrthScale / (norm + eps)), rows padded to ld_x (a multiple of 8) columns.
+// x = FP16(g kOrthScale / (norm + eps)), rows padded to ld_x (a multiple of 8)
+// columns. Memory: 19 us for 9728 x 2560.
 template <bool kVec>
 __global__ void __launch_bounds__(256) orth_scale_kernel(const void* __restrict__ g, long long batch_stride, int rows,
                                                          int cols, long long ld, int bf16,

@@ -826,7 +826,7 @@ extern "C" int hgemm_sm100_loss_forward(const HgemmSm100LossForward* a, void* st
     p.partial = partial;
     p.target_logit = target_logit;
     if ((rc = run_products(p, kTrainLse, &q.z, q.tile, 1, c)) != HGEMM_SM100_OK) return rc;
-    rc = launch(&lse_join_kernel, dim3(static_cast<unsigned>(cdiv(m, 32))), dim3(32, 32), 0, 1, c.stream, partial,
+    rc = launch(&lse_join_kernel<8>, dim3(static_cast<unsigned>(cdiv(m, 8))), dim3(8, 128), 0, 1, c.stream, partial,
                 static_cast<int>(q.parts), m, target_logit, target, static_cast<long long>(a->vocab),
                 static_cast<long long>(a->ignore_index), a->lse, loss);
     if (rc != HGEMM_SM100_OK || a->reduction == HGEMM_SM100_LOSS_NONE) return rc;
