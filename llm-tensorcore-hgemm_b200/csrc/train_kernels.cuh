@@ -65,13 +65,14 @@ static_assert(2 * kTrainMaxStages + 5 <= 30, "barrier area");
 static_assert(kTrainSmemBytes <= 232448, "shared memory");
 
 enum : int {
-    kTrainStore = 0,      // out = alpha acc + beta C (16 bits), or FP32 acc stored / added
+    kTrainStore = 0,      // out = alpha acc (16 bits), or FP32 acc stored / added
     kTrainGate = 1,       // acc = (gate | up): out = silu(gate) up, gate and up kept
     kTrainGateGrad = 2,   // acc = dh: out = dh up silu'(gate), out2 = dh silu(gate)
     kTrainLse = 3,        // per row: max and sum of exp over the tile's columns
     kTrainLogitGrad = 4,  // out = (exp(acc - lse) - [column == target]) row factor
+    kTrainStoreC = 5,     // kTrainStore with out = alpha acc + beta C
 };
-// How kTrainStore writes: 16-bit boxes, FP32 boxes, FP32 boxes added to memory.
+// How kTrainStore and kTrainStoreC write: 16-bit boxes, FP32 boxes, FP32 boxes added to memory.
 enum : int { kTrainOut16 = 0, kTrainOutF32 = 1, kTrainOutF32Add = 2 };
 
 struct alignas(64) TrainProblem {
@@ -167,7 +168,7 @@ struct Row32 {
     __device__ __forceinline__ void load(const void* base, long long off, int avail) {
         const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + off);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) w[q] = 8 * q < avail ? __ldg(src + q) : make_uint4(0u, 0u, 0u, 0u);
+        for (int q = 0; q < 4; ++q) w[q] = 8 * q < avail ? src[q] : make_uint4(0u, 0u, 0u, 0u);
     }
     template <bool kBf16>
     __device__ __forceinline__ float2 pair(int i) const {   // elements 2i, 2i + 1
@@ -193,10 +194,15 @@ struct BoxWriter {
     uint8_t* bufs;
     uint32_t next;
     uint32_t lane;
+    bool whole;    // the last group of stores reads both buffers
 
     // The next buffer, once the store that used it last has read it.
     __device__ __forceinline__ uint8_t* take() {
-        if (lane == 0) bulk_wait_group_read<1>();
+        if (lane == 0) {
+            if (whole) bulk_wait_group_read<0>();
+            else bulk_wait_group_read<1>();
+        }
+        whole = false;
         __syncwarp();
         return bufs + (next++ & 1u) * kTrainBoxBytes;
     }
@@ -232,6 +238,7 @@ struct BoxWriter {
     template <bool kBf16>
     __device__ __forceinline__ void put16_two(const CUtensorMap* map, const float (&v)[32], const float (&w)[32],
                                               bool two, int col, int col_two, int row) {
+        whole = true;
         if (lane == 0) bulk_wait_group_read<0>();
         __syncwarp();
         fill<kBf16>(bufs, v);
@@ -260,6 +267,7 @@ struct BoxWriter {
     }
 
     __device__ void put32(const CUtensorMap* map, const float (&v)[32], bool add, int col, int row) {
+        whole = true;
         if (lane == 0) bulk_wait_group_read<0>();
         __syncwarp();
         uint8_t* box = bufs;
@@ -381,7 +389,14 @@ struct TrainEpilogue {
     int row0, row, tn, width, first;   // width: the tile's output columns
     int out_row, mirror;               // row0 in the output; the tile is stored transposed too
     bool in_rows;
-    Row32 x, y;
+    int out_kind, out_bf16;
+    float alpha, beta;
+    const float* alpha_ptr;
+    const void* c0;
+    long long ldc;
+    // kTrainStoreC: C of all groups of the tile; kTrainGateGrad: the saved
+    // pre-activations of one group.
+    Row32 x[kEpi == kTrainStoreC ? 4 : 1], y;
 
     // in_tile: this warp's first row in the tile.
     __device__ TrainEpilogue(const TrainParams& p_, const TrainProblem& q_, const TileIter& it, int tile_m, int in_tile,
@@ -389,17 +404,14 @@ struct TrainEpilogue {
         : p(p_), q(q_), row0(it.tm * tile_m + in_tile), row(row0 + lane), tn(it.tn),
           width(kEpi == kTrainGate ? q_.tile_n / 2 : q_.tile_n), first(32 * group),
           out_row(q_.parted ? (it.split * q_.tiles + it.local) * tile_m + in_tile : row0),
-          mirror(q_.symmetric && it.tn > it.tm), in_rows(row < q_.m) {}
+          mirror(q_.symmetric && it.tn > it.tm), in_rows(row < q_.m), out_kind(q_.out_kind), out_bf16(p_.out_bf16),
+          alpha(q_.alpha), beta(q_.beta), alpha_ptr(q_.alpha_ptr), c0(q_.c), ldc(q_.ldc) {}
 
     __device__ __forceinline__ void fetch(int c, Row32& a, Row32& b) const {
         const int col = tn * width + c;
         const int avail = in_rows && c < width ? q.n - col : 0;
-        if constexpr (kEpi == kTrainStore) {
-            a.load(q.c, row * q.ldc + col, q.beta != 0.f ? avail : 0);
-        } else if constexpr (kEpi == kTrainGateGrad) {
-            a.load(p.gate, row * p.ld_saved + col, avail);
-            b.load(p.up, row * p.ld_saved + col, avail);
-        }
+        a.load(p.gate, row * p.ld_saved + col, avail);
+        b.load(p.up, row * p.ld_saved + col, avail);
     }
     // The rows of the saved pre-activations come from DRAM: one 128-byte line
     // per row and 64 columns into L2 while the tile is still multiplied, or each
@@ -413,7 +425,14 @@ struct TrainEpilogue {
             for (int c = 0; c < width && in_rows && tn * width + c < q.n; c += 64)
                 asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint16_t*>(src) + row * p.ld_saved + tn * width + c));
         }
-        fetch(first, x, y);
+        if constexpr (kEpi == kTrainGateGrad) fetch(first, x[0], y);
+        if constexpr (kEpi == kTrainStoreC) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int c = first + 64 * k, col = tn * width + c;
+                x[k].load(c0, row * ldc + col, in_rows && c < width ? q.n - col : 0);
+            }
+        }
     }
 
     // t: TMEM address of the accumulator, this warp's lane quarter. The output
@@ -424,14 +443,14 @@ struct TrainEpilogue {
         if (row0 >= q.m) return;
         if constexpr (kEpi == kTrainLse) {
             statistics(t);
-        } else if (kEpi == kTrainStore && q.out_kind != kTrainOut16) {
+        } else if ((kEpi == kTrainStore || kEpi == kTrainStoreC) && out_kind != kTrainOut16) {
 #pragma unroll 1
             for (int c = first; c < width && tn * width + c < q.n; c += 64) {
                 float v[32];
                 tmem_ld32(t + c, v);
-                box.put32(&q.out[0], v, q.out_kind == kTrainOutF32Add, c, out_row);
+                box.put32(&q.out[0], v, out_kind == kTrainOutF32Add, c, out_row);
             }
-        } else if (p.out_bf16) {
+        } else if (out_bf16) {
             store<true>(box, t);
         } else {
             store<false>(box, t);
@@ -477,16 +496,17 @@ struct TrainEpilogue {
 
     template <bool kBf16>
     __device__ __forceinline__ void store(BoxWriter& box, uint32_t t) {
-        float alpha = 0.f, scale = 0.f, lse = 0.f;
+        float scale = 0.f, lse = 0.f;
         long long want = -1;
-        if constexpr (kEpi == kTrainStore) alpha = q.alpha_ptr != nullptr ? q.alpha * __ldg(q.alpha_ptr) : q.alpha;
+        if constexpr (kEpi == kTrainStore || kEpi == kTrainStoreC)
+            if (alpha_ptr != nullptr) alpha *= *alpha_ptr;
         if constexpr (kEpi == kTrainLogitGrad)
             if (in_rows) {
                 want = p.target[row] - p.col_base;
                 scale = p.row_scale[row];
                 lse = p.lse[row];
             }
-        if (kEpi == kTrainLogitGrad || (kEpi == kTrainStore && q.beta == 0.f && !mirror)) {
+        if (kEpi == kTrainLogitGrad || (kEpi == kTrainStore && !mirror)) {
             // Two groups a turn.
 #pragma unroll 1
             for (int c = first; c < width; c += 128) {
@@ -509,25 +529,38 @@ struct TrainEpilogue {
             }
             return;
         }
+        if constexpr (kEpi == kTrainStoreC) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int c = first + 64 * k, col = tn * width + c;
+                if (c >= width || col >= q.n) break;
+                float v[32];
+                tmem_ld32(t + c, v);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float2 w = x[k].template pair<false>(i);   // C is FP16
+                    v[2 * i] = fmaf(alpha, v[2 * i], beta * w.x);
+                    v[2 * i + 1] = fmaf(alpha, v[2 * i + 1], beta * w.y);
+                }
+                box.put16<kBf16>(&q.out[0], v, col, row0);
+                if (mirror) box.put16_turned<kBf16>(&q.out[0], v, row0, col);
+            }
+            return;
+        }
 #pragma unroll 1
         for (int c = first; c < width; c += 64) {
             const int col = tn * width + c;
             if (col >= q.n) break;
-            Row32 nx, ny;
-            fetch(c + 64, nx, ny);
             float v[32];
-            tmem_ld32(t + c, v);
             if constexpr (kEpi == kTrainStore) {
+                tmem_ld32(t + c, v);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float2 w = x.template pair<false>(i);   // C is FP16
-                    v[2 * i] = fmaf(alpha, v[2 * i], q.beta * w.x);
-                    v[2 * i + 1] = fmaf(alpha, v[2 * i + 1], q.beta * w.y);
-                }
+                for (int i = 0; i < 32; ++i) v[i] *= alpha;
                 box.put16<kBf16>(&q.out[0], v, col, row0);
-                if (mirror) box.put16_turned<kBf16>(&q.out[0], v, row0, col);
+                box.put16_turned<kBf16>(&q.out[0], v, row0, col);
             } else if constexpr (kEpi == kTrainGate) {
                 float u[32];
+                tmem_ld32(t + c, v);
                 tmem_ld32(t + width + c, u);
                 if (p.keep) {
                     box.put16<kBf16>(&q.out[1], v, col, row0);
@@ -537,10 +570,13 @@ struct TrainEpilogue {
                 for (int i = 0; i < 32; ++i) u[i] *= v[i] * sigmoid_f(v[i]);
                 box.put16<kBf16>(&q.out[0], u, col, row0);
             } else if constexpr (kEpi == kTrainGateGrad) {
+                Row32 nx, ny;
+                fetch(c + 64, nx, ny);
+                tmem_ld32(t + c, v);
                 float du[32];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float2 g = x.template pair<kBf16>(i), u = y.template pair<kBf16>(i);
+                    const float2 g = x[0].template pair<kBf16>(i), u = y.template pair<kBf16>(i);
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const float gj = j ? g.y : g.x, uj = j ? u.y : u.x, dh = v[2 * i + j];
@@ -552,9 +588,9 @@ struct TrainEpilogue {
                 }
                 box.put16<kBf16>(&q.out[0], v, col, row0);
                 box.put16<kBf16>(&q.out[1], du, col, row0);
+                x[0] = nx;
+                y = ny;
             }
-            x = nx;
-            y = ny;
         }
     }
 
@@ -670,7 +706,9 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
     grid_dependents_launch();
-    grid_dependency_wait();                      // global memory only after the previous kernel
+    // Every role looks its first tile up before it waits for the previous
+    // kernel: the parameters come cold from constant memory, about 1.1 us of
+    // misses one after the other, which that kernel's end then hides.
     const WaitCtl wc{abort_flag, p.status, p.timeout_ns};
     const int unit = kPair ? blockIdx.x >> 1 : blockIdx.x;
     const int units = kPair ? gridDim.x >> 1 : gridDim.x;
@@ -700,6 +738,7 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
             };
             auto map_of = [](const CUtensorMap& m) { return reinterpret_cast<uint64_t>(&m); };
             uint32_t extra = p.inject ? 16u : 0u;
+            bool waiting = true;   // for the previous kernel
             // The K blocks of one segment, forwards or backwards, two to a stage.
             auto segment = [&](uint64_t ma, uint64_t mb, uint64_t mb2, auto a_mn_c, auto b_kind_c, int row0, int col0,
                                int chunks, uint32_t half_bytes, uint32_t block_bytes, int from, int to, bool back) {
@@ -707,6 +746,8 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
                 constexpr int b_kind = decltype(b_kind_c)::value;
                 int k = (back ? to - 1 : from) * kBlockK;
                 const int step = back ? -kBlockK : kBlockK;
+                if (waiting) grid_dependency_wait();
+                waiting = false;
                 for (int left = to - from; left > 0; left -= sub) {
                     if (!(kPair ? mbar_wait_cluster(&empty[stage], phase ^ 1u, wc)
                                 : mbar_wait(&empty[stage], phase ^ 1u, wc))) return false;
@@ -800,7 +841,7 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
                 const uint64_t desc_a = make_smem_desc(ring, q.a_mn ? kChunkBytes : 16u, 1024u);
                 const uint64_t desc_b = make_smem_desc(ring + b_offset, q.b_mn ? kChunkBytes : 16u, 1024u);
                 const uint32_t acc = iter & 1u, acc_phase = (iter >> 1) & 1u;
-                ++iter;
+                if (iter++ == 0) grid_dependency_wait();   // the time limits of waits start then
                 if (!__all_sync(0xffffffffu, kPair ? mbar_wait_cluster(&tempty[acc], acc_phase ^ 1u, wc)
                                                    : mbar_wait(&tempty[acc], acc_phase ^ 1u, wc))) { ok = false; break; }
                 tc_fence_after_sync();
@@ -837,7 +878,7 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
     } else {
         const uint32_t tempty0 = kPair ? map_to_rank(smem_addr(&tempty[0]), 0) : 0u;
         const uint32_t tempty1 = kPair ? map_to_rank(smem_addr(&tempty[1]), 0) : 0u;
-        BoxWriter box{smem + kTrainRingBytes + warp * 2u * kTrainBoxBytes, 0u, lane};
+        BoxWriter box{smem + kTrainRingBytes + warp * 2u * kTrainBoxBytes, 0u, lane, false};
         const int quarter = static_cast<int>(warp & 3u), group = static_cast<int>(warp >> 2);
         uint32_t iter = 0;
         while (it.next(p)) {
@@ -845,6 +886,7 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
             ++iter;
             TrainEpilogue<kEpi> epi(p, p.prob[it.prob], it, kTileM, static_cast<int>(rank) * 128 + quarter * 32,
                                     static_cast<int>(lane), group);
+            if (iter == 1) grid_dependency_wait();
             epi.begin();
             const bool got = kPair ? mbar_wait_cluster(&tfull[acc], acc_phase, wc) : mbar_wait(&tfull[acc], acc_phase, wc);
             if (!__all_sync(0xffffffffu, got)) break;
@@ -892,11 +934,11 @@ __device__ __forceinline__ float2 join_pairs(float2 a, float2 b) {
 }
 
 template <int kRows>
-__global__ void __launch_bounds__(1024) lse_join_kernel(const float2* __restrict__ partial, int tiles, int m,
-                                                        const float* __restrict__ target_logit,
-                                                        const long long* __restrict__ target, long long vocab,
-                                                        long long ignore, float* __restrict__ lse,
-                                                        float* __restrict__ loss) {
+__global__ void __launch_bounds__(1024) lse_join_kernel(const float2* partial, int tiles, int m,
+                                                        const float* target_logit,
+                                                        const long long* target, long long vocab,
+                                                        long long ignore, float* lse,
+                                                        float* loss) {
     constexpr int kSlices = 1024 / kRows;
     __shared__ float2 part[kSlices][kRows + 1];
     grid_dependents_launch();
@@ -933,9 +975,9 @@ __global__ void __launch_bounds__(1024) lse_join_kernel(const float2* __restrict
 
 // Sum of the rows' losses (and their count for the mean), one block, in a
 // fixed order and 64 bits. Latency: 3-4 us up to 4096 rows.
-__global__ void __launch_bounds__(1024) loss_reduce_kernel(const float* __restrict__ loss,
-                                                           const long long* __restrict__ target, int m,
-                                                           long long ignore, int mean, float* __restrict__ out) {
+__global__ void __launch_bounds__(1024) loss_reduce_kernel(const float* loss,
+                                                           const long long* target, int m,
+                                                           long long ignore, int mean, float* out) {
     __shared__ double sums[32];
     __shared__ int counts[32];
     grid_dependents_launch();
@@ -967,11 +1009,11 @@ __global__ void __launch_bounds__(1024) loss_reduce_kernel(const float* __restri
 // dz[row] = row_scale[row] (p - onehot), gradient = alpha dz^T x and so on.
 // One loss per row: row_scale = dloss[row] / max |dloss|, so that any range of
 // incoming gradients fits 16 bits. One block; latency, 5 us up to 4096 rows.
-__global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* __restrict__ dloss, int per_row, int mean,
-                                                                const long long* __restrict__ target, int m,
+__global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* dloss, int per_row, int mean,
+                                                                const long long* target, int m,
                                                                 long long vocab, long long ignore,
-                                                                float* __restrict__ row_scale,
-                                                                float* __restrict__ alpha) {
+                                                                float* row_scale,
+                                                                float* alpha) {
     __shared__ float tops[32];
     __shared__ int counts[32];
     grid_dependents_launch();
@@ -1061,7 +1103,7 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const JoinParams p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] *= alpha;
     if (p.beta != 0.f) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.c) + row * p.ldc + col));
+        const uint4 w = *(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.c) + row * p.ldc + col));
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -1091,7 +1133,7 @@ constexpr float kOrthScale = 256.f;
 template <bool kVec>
 __device__ __forceinline__ void orth_load8(const void* g, long long row, int c, int cols, int bf16, float (&v)[8]) {
     if constexpr (kVec) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(g) + row + c));
+        const uint4 w = *(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(g) + row + c));
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -1111,9 +1153,9 @@ __device__ __forceinline__ void orth_load8(const void* g, long long row, int c, 
 // (16-byte loads, one conversion to 64 bits per eight elements: 9728 x 2560
 // takes 19 us cold, element by element in 64 bits it took 114).
 template <bool kVec>
-__global__ void __launch_bounds__(256) orth_square_kernel(const void* __restrict__ g, long long batch_stride, int rows,
+__global__ void __launch_bounds__(256) orth_square_kernel(const void* g, long long batch_stride, int rows,
                                                           int cols, long long ld, int bf16,
-                                                          double* __restrict__ sums) {
+                                                          double* sums) {
     __shared__ double part[8];
     grid_dependents_launch();
     grid_dependency_wait();
@@ -1150,10 +1192,10 @@ __global__ void __launch_bounds__(256) orth_square_kernel(const void* __restrict
 // x = FP16(g kOrthScale / (norm + eps)), rows padded to ld_x (a multiple of 8)
 // columns. Memory: 19 us for 9728 x 2560.
 template <bool kVec>
-__global__ void __launch_bounds__(256) orth_scale_kernel(const void* __restrict__ g, long long batch_stride, int rows,
+__global__ void __launch_bounds__(256) orth_scale_kernel(const void* g, long long batch_stride, int rows,
                                                          int cols, long long ld, int bf16,
-                                                         const double* __restrict__ sums, int num_sums, double eps,
-                                                         __half* __restrict__ x, long long ld_x, long long x_stride) {
+                                                         const double* sums, int num_sums, double eps,
+                                                         __half* x, long long ld_x, long long x_stride) {
     __shared__ float factor;
     grid_dependents_launch();
     grid_dependency_wait();
@@ -1186,9 +1228,9 @@ __global__ void __launch_bounds__(256) orth_scale_kernel(const void* __restrict_
 
 // out[r, c] = scale src[r, c], for outputs whose rows TMA cannot store to (scale
 // 1, src in the output's type) and for no step at all (X itself).
-__global__ void __launch_bounds__(256) orth_copy_kernel(const void* __restrict__ src, long long ld_src,
+__global__ void __launch_bounds__(256) orth_copy_kernel(const void* src, long long ld_src,
                                                         long long src_stride, int src_bf16, float scale,
-                                                        void* __restrict__ out, int rows, int cols, int out_bf16) {
+                                                        void* out, int rows, int cols, int out_bf16) {
     grid_dependents_launch();
     grid_dependency_wait();
     const long long from = blockIdx.y * src_stride, to = static_cast<long long>(blockIdx.y) * rows * cols;
@@ -1334,7 +1376,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const Ort
     double sum = 0.;
     if (p.vec_in) {
         walk(true, [&](int s, int l) {
-            const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.g) + base + far(p.ld, s, l)));
+            const uint4 w = *(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.g) + base + far(p.ld, s, l)));
             const uint32_t u[4] = {w.x, w.y, w.z, w.w};
             float v[8], top = 0.f, part = 0.f;
 #pragma unroll
@@ -1355,7 +1397,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const Ort
         });
     } else {
         walk(false, [&](int s, int l) {
-            const uint16_t w = __ldg(static_cast<const uint16_t*>(p.g) + base + far(p.ld, s, l));
+            const uint16_t w = *(static_cast<const uint16_t*>(p.g) + base + far(p.ld, s, l));
             *reinterpret_cast<uint16_t*>(x_at(s, l)) = w;
             const double v = static_cast<double>(to_f32(&w, 0, p.bf16));
             sum += v * v;

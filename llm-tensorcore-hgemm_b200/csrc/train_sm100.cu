@@ -106,11 +106,11 @@ struct KernelEntry {
     std::atomic<uint64_t> ready{0};   // bit d: attributes set on device d
 };
 #define HG_TRAIN(PAIR, EPI) KernelEntry { &train_gemm_kernel<PAIR, EPI> }
-KernelEntry g_kernels[2][5] = {
+KernelEntry g_kernels[2][6] = {
     {HG_TRAIN(false, kTrainStore), HG_TRAIN(false, kTrainGate), HG_TRAIN(false, kTrainGateGrad),
-     HG_TRAIN(false, kTrainLse), HG_TRAIN(false, kTrainLogitGrad)},
+     HG_TRAIN(false, kTrainLse), HG_TRAIN(false, kTrainLogitGrad), HG_TRAIN(false, kTrainStoreC)},
     {HG_TRAIN(true, kTrainStore), HG_TRAIN(true, kTrainGate), HG_TRAIN(true, kTrainGateGrad),
-     HG_TRAIN(true, kTrainLse), HG_TRAIN(true, kTrainLogitGrad)},
+     HG_TRAIN(true, kTrainLse), HG_TRAIN(true, kTrainLogitGrad), HG_TRAIN(true, kTrainStoreC)},
 };
 
 // Launch with programmatic stream serialisation (the kernels wait for the
@@ -1097,7 +1097,7 @@ extern "C" int hgemm_sm100_orthogonalize(const HgemmSm100Orthogonalize* a, void*
             init_params(p, c);
             p.in_bf16 = 0;
             p.out_bf16 = out_bf16;
-            int r = run_products(p, kTrainStore, s, t, n, c);
+            int r = run_products(p, s[0].c != nullptr ? kTrainStoreC : kTrainStore, s, t, n, c);
             if (r == HGEMM_SM100_OK && n == 1) r = join_parts(s[0], t, c, 0, out_bf16);
             if (r != HGEMM_SM100_OK) return r;
         }
