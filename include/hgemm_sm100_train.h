@@ -49,7 +49,8 @@ typedef struct HgemmSm100TrainCommon {
 } HgemmSm100TrainCommon;
 
 /* Gated feed-forward block, forward: h = silu(x Wg^T) * (x Wu^T), y = h Wd^T.
- * gate_pre / up_pre (both or neither): x Wg^T and x Wu^T, for the gradient. */
+ * silu / slope (both or neither), for the gradient: silu(g) and u silu'(g) with
+ * g = x Wg^T, u = x Wu^T, the factors that turn dh into du and dg. */
 typedef struct HgemmSm100FfnForward {
     HgemmSm100TrainCommon common;
     const void* x;         /* [tokens x ldx]                                  */
@@ -58,8 +59,8 @@ typedef struct HgemmSm100FfnForward {
     const void* down;      /* Wd [out x inter]                                */
     void* y;               /* [tokens x out]                                  */
     void* h;               /* [tokens x inter]                                */
-    void* gate_pre;        /* [tokens x inter] or NULL                        */
-    void* up_pre;          /* [tokens x inter] or NULL                        */
+    void* silu;            /* [tokens x inter] or NULL                        */
+    void* slope;          /* [tokens x inter] or NULL                        */
     void* workspace;       /* hgemm_sm100_ffn_forward_workspace bytes (may be 0) */
     uint64_t workspace_bytes;
     int64_t tokens, hidden, inter, out, ldx;
@@ -67,7 +68,7 @@ typedef struct HgemmSm100FfnForward {
 size_t hgemm_sm100_ffn_forward_workspace(const HgemmSm100FfnForward* args);
 int hgemm_sm100_ffn_forward(const HgemmSm100FfnForward* args, void* stream);
 
-/* Its gradient. dh = dy Wd, du = dh silu(g), dg = dh u silu'(g) (rounded to the
+/* Its gradient. dh = dy Wd, du = dh silu, dg = dh slope (rounded to the
  * call's type, as operands of the products); dx = dg Wg + du Wu, dgate = dg^T x,
  * dup = du^T x, ddown = dy^T h. Outputs that are NULL are not computed. */
 typedef struct HgemmSm100FfnBackward {
@@ -77,8 +78,8 @@ typedef struct HgemmSm100FfnBackward {
     const void* gate;
     const void* up;
     const void* down;
-    const void* gate_pre;  /* [tokens x inter], from the forward call         */
-    const void* up_pre;
+    const void* silu;      /* [tokens x inter], from the forward call         */
+    const void* slope;
     const void* h;
     void* dgate_pre;       /* scratch [tokens x inter]: dg                    */
     void* dup_pre;         /* scratch [tokens x inter]: du                    */

@@ -97,7 +97,7 @@ FfnSizes ffn_sizes(const Tensor& x, const Tensor& gate, const Tensor& down) {
 
 struct FfnForward {
     Tensor y;
-    Tensor kept;   // [tokens, inter] (h), or [3, tokens, inter]: h, gate and up pre-activations; padded sizes
+    Tensor kept;   // [tokens, inter] (h), or [3, tokens, inter]: h, silu(g), u silu'(g); padded sizes
 };
 
 FfnForward ffn_forward(const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down, const FfnSizes& s,
@@ -120,8 +120,8 @@ FfnForward ffn_forward(const Tensor& x, const Tensor& gate, const Tensor& up, co
     a.down = dp.data_ptr();
     a.y = r.y.data_ptr();
     a.h = kept;
-    a.gate_pre = keep ? kept + plane : nullptr;
-    a.up_pre = keep ? kept + 2 * plane : nullptr;
+    a.silu = keep ? kept + plane : nullptr;
+    a.slope = keep ? kept + 2 * plane : nullptr;
     a.tokens = s.tokens;
     a.hidden = s.hidden8;
     a.inter = s.inter8;
@@ -183,8 +183,8 @@ class GatedFfn : public torch::autograd::Function<GatedFfn> {
         a.up = up_.data_ptr();
         a.down = dp.data_ptr();
         a.h = kept;
-        a.gate_pre = kept + plane;
-        a.up_pre = kept + 2 * plane;
+        a.silu = kept + plane;
+        a.slope = kept + 2 * plane;
         a.dgate_pre = pre.data_ptr();
         a.dup_pre = static_cast<uint8_t*>(pre.data_ptr()) + plane;
         a.dx = need_x ? dx.data_ptr() : nullptr;

@@ -25,8 +25,8 @@
 //    statistics, the logits' gradient, a x X + acc) on the FP32 accumulators.
 //
 // kPair: tiles of 256 x tile_n per CTA pair (cta_group::2); otherwise 128 x
-// tile_n per CTA. tile_n is a run-time multiple of 32 (pairs: 64) up to 256,
-// so the host cuts the columns into a whole number of waves.
+// tile_n per CTA. tile_n is a run-time multiple of 64 up to 256, which the host
+// picks by what the waves of tiles are estimated to take.
 // Roles per CTA: warps 0-7 epilogue (one TMEM lane = one output row per
 // thread; warps w and w + 4 share a row quarter and take every second group of
 // 32 columns), warp 8 TMA producer, warp 9 MMA issuer; two accumulators, so a
@@ -66,8 +66,8 @@ static_assert(kTrainSmemBytes <= 232448, "shared memory");
 
 enum : int {
     kTrainStore = 0,      // out = alpha acc (16 bits), or FP32 acc stored / added
-    kTrainGate = 1,       // acc = (gate | up): out = silu(gate) up, gate and up kept
-    kTrainGateGrad = 2,   // acc = dh: out = dh up silu'(gate), out2 = dh silu(gate)
+    kTrainGate = 1,       // acc = (gate | up): out = silu(gate) up; silu(gate) and up silu'(gate) kept
+    kTrainGateGrad = 2,   // acc = dh: out = dh (up silu'(gate)), out[1] = dh silu(gate), from what was kept
     kTrainLse = 3,        // per row: max and sum of exp over the tile's columns
     kTrainLogitGrad = 4,  // out = (exp(acc - lse) - [column == target]) row factor
     kTrainStoreC = 5,     // kTrainStore with out = alpha acc + beta C
@@ -82,7 +82,7 @@ struct alignas(64) TrainProblem {
     int m, n;              // output rows and columns (dual: columns of one half)
     int tile_n;            // accumulator columns of a tile (dual: both halves)
     int nkb0, nkb;         // K blocks of the first segment, of both
-    int a_mn, b_mn, dual;
+    int a_mn, b_mn;
     int tiles_m, tiles_n, group_m;
     int symmetric;         // tiles are those of the upper triangle, row by row
     int tile0, tiles;      // this problem's tiles of all: tile0 .. tile0 + tiles - 1
@@ -98,7 +98,6 @@ struct alignas(64) TrainProblem {
 
 struct alignas(64) TrainParams {
     TrainProblem prob[kTrainMaxProblems];
-    int num_problems;
     int heavy_tiles, light_tiles;  // tiles of problem 0 / of the others
     int light_skip;                // waves the units with one heavy tile more sit out
     int stages, sub;               // ring stages, K blocks of 64 in each
@@ -108,11 +107,11 @@ struct alignas(64) TrainParams {
     int* status;
     unsigned long long timeout_ns;
     int inject;                    // test only: arm the first stage with 16 bytes more
-    // kTrainGateGrad: the saved pre-activations, 16-bit [m x ld_saved].
-    const void* gate;
-    const void* up;
-    long long ld_saved;
-    int keep;                      // kTrainGate: store gate and up too (out[1], out[2])
+    // kTrainGateGrad: what the forward pass kept, 16-bit [m x ld_kept].
+    const void* silu;              // silu(gate)
+    const void* slope;             // up silu'(gate)
+    long long ld_kept;
+    int keep;                      // kTrainGate: store these too (out[1], out[2])
     // kTrainLse / kTrainLogitGrad, per row.
     const long long* target;
     long long col_base;            // vocabulary index of column 0
@@ -174,6 +173,30 @@ struct Row32 {
     __device__ __forceinline__ float2 pair(int i) const {   // elements 2i, 2i + 1
         const uint4& v = w[i >> 2];
         return unpack2((i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w, kBf16);
+    }
+};
+
+// A 32 x 32 patch of a 16-bit matrix in a warp's registers, loaded ahead of its
+// use: lane l holds 16 bytes (columns 8 (l % 4) ..) of rows l / 4, l / 4 + 8, ...
+// Four lanes share a row's 64 bytes, so a load touches 8 lines, not 32.
+struct Patch32 {
+    uint4 w[4];
+    // Element (row0, col0) is the patch's first; rows and columns from `rows`,
+    // `cols` on (counted from there) are zero. cols is a multiple of 8.
+    __device__ __forceinline__ void load(const void* base, long long ld, int row0, int col0, int rows, int cols, uint32_t lane) {
+        const int r = static_cast<int>(lane >> 2), c = static_cast<int>(lane & 3u) * 8;
+        const uint16_t* src = static_cast<const uint16_t*>(base) + (row0 + r) * ld + col0 + c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i, src += 8 * ld)
+            w[i] = r + 8 * i < rows && c < cols ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    // Into a box (64-byte rows, swizzled as BoxWriter's).
+    __device__ __forceinline__ void put(uint8_t* box, uint32_t lane) const {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t r = (lane >> 2) + 8u * i;
+            *reinterpret_cast<uint4*>(box + r * 64u + (((lane & 3u) ^ ((r >> 1) & 3u)) << 4)) = w[i];
+        }
     }
 };
 
@@ -252,6 +275,15 @@ struct BoxWriter {
         }
     }
 
+    // This lane's row of a box.
+    __device__ __forceinline__ Row32 row_of(const uint8_t* box) const {
+        Row32 r;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j)
+            r.w[j] = *reinterpret_cast<const uint4*>(box + lane * 64u + ((j ^ ((lane >> 1) & 3u)) << 4));
+        return r;
+    }
+
     // The transposed box: lane = column `col` + lane, v = rows row .. row + 31.
     template <bool kBf16>
     __device__ __forceinline__ void put16_turned(const CUtensorMap* map, const float (&v)[32], int col, int row) {
@@ -287,11 +319,11 @@ struct BoxWriter {
     }
 };
 
-// Two accumulator groups (the second one with `two`), loaded together.
-__device__ __forceinline__ void tmem_ld32_two(uint32_t t, uint32_t t_two, bool two, float (&v)[32], float (&w)[32]) {
+// Two accumulator groups, loaded together.
+__device__ __forceinline__ void tmem_ld32_two(uint32_t t, uint32_t t_two, float (&v)[32], float (&w)[32]) {
     uint32_t a[32], b[32];
     tmem_ld_32x32b_x32(t, a);
-    if (two) tmem_ld_32x32b_x32(t_two, b);
+    tmem_ld_32x32b_x32(t_two, b);
     tmem_wait_ld();
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
@@ -379,9 +411,10 @@ struct TileIter {
 // ---------------------------------------------------------------- epilogues ---
 
 // One epilogue warp's part of a tile: rows row0 + lane, the groups of 32 columns
-// with index group, group + 2, ... of tile column tn. begin() starts the loads
-// of the first group (before the accumulator is ready); run() goes through the
-// groups with the next one's loads in flight. Called by the whole warp.
+// with index group, group + 2, ... of tile column tn. begin() starts loads before
+// the accumulator is ready (C of all groups: a x X + poly X of 1024 x 2560 took
+// 2.8 us of epilogue with a group ahead); run() goes through the groups. Called
+// by the whole warp.
 template <int kEpi>
 struct TrainEpilogue {
     const TrainParams& p;
@@ -394,9 +427,9 @@ struct TrainEpilogue {
     const float* alpha_ptr;
     const void* c0;
     long long ldc;
-    // kTrainStoreC: C of all groups of the tile; kTrainGateGrad: the saved
-    // pre-activations of one group.
-    Row32 x[kEpi == kTrainStoreC ? 4 : 1], y;
+    Row32 x[kEpi == kTrainStoreC ? 4 : 1];         // C of all groups of the tile
+    Patch32 silu, slope;                           // kTrainGateGrad: what was kept, of one group
+    uint32_t lane_;
 
     // in_tile: this warp's first row in the tile.
     __device__ TrainEpilogue(const TrainParams& p_, const TrainProblem& q_, const TileIter& it, int tile_m, int in_tile,
@@ -405,27 +438,24 @@ struct TrainEpilogue {
           width(kEpi == kTrainGate ? q_.tile_n / 2 : q_.tile_n), first(32 * group),
           out_row(q_.parted ? (it.split * q_.tiles + it.local) * tile_m + in_tile : row0),
           mirror(q_.symmetric && it.tn > it.tm), in_rows(row < q_.m), out_kind(q_.out_kind), out_bf16(p_.out_bf16),
-          alpha(q_.alpha), beta(q_.beta), alpha_ptr(q_.alpha_ptr), c0(q_.c), ldc(q_.ldc) {}
+          alpha(q_.alpha), beta(q_.beta), alpha_ptr(q_.alpha_ptr), c0(q_.c), ldc(q_.ldc),
+          lane_(static_cast<uint32_t>(lane)) {}
 
-    __device__ __forceinline__ void fetch(int c, Row32& a, Row32& b) const {
-        const int col = tn * width + c;
-        const int avail = in_rows && c < width ? q.n - col : 0;
-        a.load(p.gate, row * p.ld_saved + col, avail);
-        b.load(p.up, row * p.ld_saved + col, avail);
+    __device__ __forceinline__ void fetch(int c) {
+        const int col = tn * width + c, cols = c < width ? q.n - col : 0;
+        silu.load(p.silu, p.ld_kept, row0, col, q.m - row0, cols, lane_);
+        slope.load(p.slope, p.ld_kept, row0, col, q.m - row0, cols, lane_);
     }
-    // The rows of the saved pre-activations come from DRAM: one 128-byte line
-    // per row and 64 columns into L2 while the tile is still multiplied, or each
-    // group's loads would wait for memory in turn (192 -> 175 us for dh at
-    // 4096 x 9728 x 2560, with the approximate reciprocal). Boxes through TMA
-    // instead took a stage from the ring and gained 2 % there, and lost 3 % in
-    // a x X + poly X.
+    // What was kept comes from DRAM: one 128-byte line per row and 64 columns into
+    // L2 while the tile is still multiplied, or each group's loads would wait for
+    // memory in turn.
     __device__ void begin() {
         if constexpr (kEpi == kTrainGateGrad) {
-            const void* src = first == 0 ? p.gate : p.up;
+            const void* src = first == 0 ? p.silu : p.slope;
             for (int c = 0; c < width && in_rows && tn * width + c < q.n; c += 64)
-                asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint16_t*>(src) + row * p.ld_saved + tn * width + c));
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint16_t*>(src) + row * p.ld_kept + tn * width + c));
+            fetch(first);
         }
-        if constexpr (kEpi == kTrainGateGrad) fetch(first, x[0], y);
         if constexpr (kEpi == kTrainStoreC) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -514,7 +544,7 @@ struct TrainEpilogue {
                 if (col >= q.n) break;
                 const bool two = c + 64 < width && col + 64 < q.n;
                 float v[32], w[32];
-                tmem_ld32_two(t + c, t + c + 64, two, v, w);
+                tmem_ld32_two(t + c, two ? t + c + 64 : t + c, v, w);
                 if constexpr (kEpi == kTrainStore) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
@@ -563,33 +593,53 @@ struct TrainEpilogue {
                 tmem_ld32(t + c, v);
                 tmem_ld32(t + width + c, u);
                 if (p.keep) {
-                    box.put16<kBf16>(&q.out[1], v, col, row0);
-                    box.put16<kBf16>(&q.out[2], u, col, row0);
-                }
+                    float d[32];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) u[i] *= v[i] * sigmoid_f(v[i]);
-                box.put16<kBf16>(&q.out[0], u, col, row0);
+                    for (int i = 0; i < 32; ++i) {
+                        const float s = sigmoid_f(v[i]);
+                        v[i] *= s;
+                        // silu' = s (1 + g (1 - s)) = s + silu (1 - s)
+                        d[i] = u[i] * fmaf(v[i], 1.f - s, s);
+                        u[i] *= v[i];
+                    }
+                    box.put16<kBf16>(&q.out[0], u, col, row0);
+                    box.put16<kBf16>(&q.out[1], v, col, row0);
+                    box.put16<kBf16>(&q.out[2], d, col, row0);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) u[i] *= v[i] * sigmoid_f(v[i]);
+                    box.put16<kBf16>(&q.out[0], u, col, row0);
+                }
             } else if constexpr (kEpi == kTrainGateGrad) {
-                Row32 nx, ny;
-                fetch(c + 64, nx, ny);
+                // The patches of this group through the two boxes to their rows'
+                // lanes, and the results into the same places.
+                uint8_t* other = box.bufs + kTrainBoxBytes;
+                if (box.lane == 0) bulk_wait_group_read<0>();
+                __syncwarp();
+                silu.put(box.bufs, box.lane);
+                slope.put(other, box.lane);
+                fetch(c + 64);
+                __syncwarp();
+                const Row32 s = box.row_of(box.bufs), d = box.row_of(other);
                 tmem_ld32(t + c, v);
                 float du[32];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float2 g = x[0].template pair<kBf16>(i), u = y.template pair<kBf16>(i);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const float gj = j ? g.y : g.x, uj = j ? u.y : u.x, dh = v[2 * i + j];
-                        const float s = sigmoid_f(gj), silu = gj * s;
-                        // silu' = s (1 + g (1 - s)) = s + silu (1 - s)
-                        v[2 * i + j] = dh * uj * fmaf(silu, 1.f - s, s);
-                        du[2 * i + j] = dh * silu;
-                    }
+                    const float2 si = s.template pair<kBf16>(i), di = d.template pair<kBf16>(i);
+                    du[2 * i] = v[2 * i] * si.x;
+                    du[2 * i + 1] = v[2 * i + 1] * si.y;
+                    v[2 * i] *= di.x;
+                    v[2 * i + 1] *= di.y;
                 }
-                box.put16<kBf16>(&q.out[0], v, col, row0);
-                box.put16<kBf16>(&q.out[1], du, col, row0);
-                x[0] = nx;
-                y = ny;
+                box.fill<kBf16>(box.bufs, v);
+                box.fill<kBf16>(other, du);
+                fence_async_shared();
+                __syncwarp();
+                if (box.lane == 0) {
+                    tma_store_2d(&q.out[0], box.bufs, col, row0);
+                    tma_store_2d(&q.out[1], other, col, row0);
+                    bulk_commit_group();
+                }
             }
         }
     }
@@ -669,7 +719,7 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     constexpr int kTileM = kPair ? 256 : 128;
-        const uint32_t warp = warp_index();
+    const uint32_t warp = warp_index();
     const uint32_t lane = threadIdx.x & 31u;
     const uint32_t rank = kPair ? cluster_ctarank() : 0u;
     const bool leader = rank == 0;
@@ -869,7 +919,7 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
                 }
                 if (ok) tc_commit_if<kPair>(issuer, smem_addr(&tfull[acc]));
             }
-            if (!ok && lane == 0) {
+            if (!ok && issuer) {
                 if constexpr (kPair) tc_commit_pair(smem_addr(drain));
                 else tc_commit(drain);
                 mbar_wait_drain(drain, 0, kDrainLimitNs);

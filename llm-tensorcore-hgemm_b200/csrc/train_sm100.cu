@@ -388,7 +388,6 @@ int run_products(TrainParams& p, int epi, const Product* products, const Tile& t
         q.nkb = static_cast<int>(s.kblocks());
         q.a_mn = s.a0.mn;
         q.b_mn = s.b0.mn;
-        q.dual = s.dual;
         q.tiles_m = static_cast<int>(cdiv(s.m, tile_rows(pair)));
         q.tiles_n = static_cast<int>(cdiv(s.n, cols));
         q.group_m = group_height(s.m, s.k0 + s.k1, pair, units);
@@ -431,7 +430,6 @@ int run_products(TrainParams& p, int epi, const Product* products, const Tile& t
         if (problems > 1) light += tiles * q.splits;
     }
     if (total >= (int64_t{1} << 31)) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
-    p.num_problems = problems;
     p.heavy_tiles = static_cast<int>(total - light);
     p.light_tiles = static_cast<int>(light);
     const int grid_units = static_cast<int>(std::min<int64_t>(total, units));
@@ -604,7 +602,7 @@ extern "C" int hgemm_sm100_ffn_forward(const HgemmSm100FfnForward* a, void* stre
     if (!matrix_ok(a->x, a->ldx, a->hidden) || !matrix_ok(a->gate, 8, 8) || !matrix_ok(a->up, 8, 8) ||
         !matrix_ok(a->down, 8, 8) || !matrix_ok(a->y, 8, 8) || !matrix_ok(a->h, 8, 8))
         return HGEMM_SM100_ERR_INVALID_ARGUMENT;
-    if ((a->gate_pre == nullptr) != (a->up_pre == nullptr) || !aligned16(a->gate_pre) || !aligned16(a->up_pre))
+    if ((a->silu == nullptr) != (a->slope == nullptr) || !aligned16(a->silu) || !aligned16(a->slope))
         return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     Context c;
     int rc = begin(&c, a->common, stream);
@@ -625,11 +623,11 @@ extern "C" int hgemm_sm100_ffn_forward(const HgemmSm100FfnForward* a, void* stre
     g.b1 = {a->up, a->hidden, false};
     g.dual = true;
     g.out = a->h;
-    g.out1 = a->gate_pre;
-    g.out2 = a->up_pre;
+    g.out1 = a->silu;
+    g.out2 = a->slope;
     g.ld_out = a->inter;
     init_params(p, c);
-    p.keep = a->gate_pre != nullptr;
+    p.keep = a->silu != nullptr;
     if ((rc = run_product(p, kTrainGate, g, c)) != HGEMM_SM100_OK) return rc;
 
     return run_and_join(d, down_tile, a->workspace, c);
@@ -645,8 +643,8 @@ extern "C" size_t hgemm_sm100_ffn_backward_workspace(const HgemmSm100FfnBackward
 extern "C" int hgemm_sm100_ffn_backward(const HgemmSm100FfnBackward* a, void* stream) {
     if (a == nullptr || !ffn_sizes_ok(a->tokens, a->hidden, a->inter, a->out)) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     if (!matrix_ok(a->dy, a->lddy, a->out) || !matrix_ok(a->x, a->ldx, a->hidden) || !matrix_ok(a->gate, 8, 8) ||
-        !matrix_ok(a->up, 8, 8) || !matrix_ok(a->down, 8, 8) || !matrix_ok(a->gate_pre, 8, 8) ||
-        !matrix_ok(a->up_pre, 8, 8) || !matrix_ok(a->h, 8, 8) || !matrix_ok(a->dgate_pre, 8, 8) ||
+        !matrix_ok(a->up, 8, 8) || !matrix_ok(a->down, 8, 8) || !matrix_ok(a->silu, 8, 8) ||
+        !matrix_ok(a->slope, 8, 8) || !matrix_ok(a->h, 8, 8) || !matrix_ok(a->dgate_pre, 8, 8) ||
         !matrix_ok(a->dup_pre, 8, 8) || !aligned16(a->dx) || !aligned16(a->dgate) || !aligned16(a->dup) ||
         !aligned16(a->ddown))
         return HGEMM_SM100_ERR_INVALID_ARGUMENT;
@@ -672,9 +670,9 @@ extern "C" int hgemm_sm100_ffn_backward(const HgemmSm100FfnBackward* a, void* st
         h.out1 = a->dup_pre;
         h.ld_out = a->inter;
         init_params(p, c);
-        p.gate = a->gate_pre;
-        p.up = a->up_pre;
-        p.ld_saved = a->inter;
+        p.silu = a->silu;
+        p.slope = a->slope;
+        p.ld_kept = a->inter;
         if ((rc = run_product(p, kTrainGateGrad, h, c)) != HGEMM_SM100_OK) return rc;
     }
     if (g.dx >= 0) g.s[g.dx].parts = static_cast<float*>(a->workspace);

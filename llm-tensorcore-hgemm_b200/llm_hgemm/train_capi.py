@@ -28,9 +28,9 @@ def _struct(name: str, pointers: str, sizes: str, rest=()):
     return type(name, (ctypes.Structure,), {"_fields_": fields + list(rest)})
 
 
-FfnForward = _struct("FfnForward", "x gate up down y h gate_pre up_pre workspace",
+FfnForward = _struct("FfnForward", "x gate up down y h silu slope workspace",
                      "workspace_bytes tokens hidden inter out ldx")
-FfnBackward = _struct("FfnBackward", "dy x gate up down gate_pre up_pre h dgate_pre dup_pre dx dgate dup ddown workspace",
+FfnBackward = _struct("FfnBackward", "dy x gate up down silu slope h dgate_pre dup_pre dx dgate dup ddown workspace",
                       "workspace_bytes tokens hidden inter out ldx lddy")
 _REDUCTION = [("reduction", c_int32), ("reserved", c_int32)]
 LossForward = _struct("LossForward", "x weight target loss lse workspace",

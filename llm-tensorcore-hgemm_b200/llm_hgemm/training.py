@@ -29,8 +29,8 @@ def gated_ffn(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch
     ``x`` is ``[..., H]`` (any strides), ``gate`` and ``up`` ``[I, H]``, ``down``
     ``[O, I]``; the result is ``[..., O]``. Two launches: gate and up are one
     product whose epilogue writes the gated activation, then the down
-    projection. Where a gradient is wanted the pre-activations and the gated
-    activation are kept (``3 * tokens * I`` elements); the backward pass is two
+    projection. Where a gradient is wanted the gated activation and its two
+    derivatives are kept (``3 * tokens * I`` elements); the backward pass is two
     launches more, one whose epilogue turns the activation's gradient into
     those of the pre-activations, and one for all wanted gradients together.
     H, I and O that are no multiples of 8 work through padded copies.

@@ -699,7 +699,7 @@ def test_a_training_step_of_a_small_model():
 def test_model_training_step():
     """A small decoder with ``trainable_mlps`` and ``linear_cross_entropy``: each
     FP16 model's gradients against the FP32 model's. Ours round the MLP three
-    times (gate and up pre-activations, product) where the stock model rounds
+    times (the product and its two derivatives) where the stock model rounds
     four times, and the logits never: no parameter may be further off than 1.5
     times the stock model's worst."""
     import importlib.util

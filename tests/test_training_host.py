@@ -45,7 +45,7 @@ def ffn_args(**change):
 
 @pytest.mark.parametrize("change", [
     {"tokens": 0}, {"tokens": -1}, {"tokens": 2 ** 31}, {"hidden": 60}, {"inter": 4}, {"out": 0}, {"x": None},
-    {"gate": None}, {"y": None}, {"h": (1 << 20) + 8}, {"ldx": 56}, {"ldx": 68}, {"gate_pre": 1 << 20},
+    {"gate": None}, {"y": None}, {"h": (1 << 20) + 8}, {"ldx": 56}, {"ldx": 68}, {"silu": 1 << 20},
     {"common": train_capi.Common(dtype=2)}, {"common": train_capi.Common(splits=17)}, {"common": train_capi.Common(splits=-1)},
     {"common": train_capi.Common(flags=capi.FLAG_OUT_F32)},
 ], ids=str)

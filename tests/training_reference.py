@@ -64,12 +64,13 @@ def ffn(x, gate, up, down, dy=None):
     if dy is None:
         return out
     dy = dy.double()
-    # The backward pass reads g and u rounded.
-    eg, eu = rounded(g, eg, dtype), rounded(u, eu, dtype)
+    # The backward pass multiplies by silu(g) and u silu'(g) as kept, rounded.
+    es = rounded(silu, slope.abs() * eg + fast * silu.abs(), dtype)
+    ed = rounded(u * slope, eu * slope.abs() + u.abs() * (bend.abs() * eg + fast), dtype)
     dh, edh = product(dy, None, down, None)
     du, dg = dh * silu, dh * u * slope
-    edu = rounded(du, edh * silu.abs() + dh.abs() * (slope.abs() * eg + fast * silu.abs()), dtype)
-    edg = rounded(dg, edh * (u * slope).abs() + dh.abs() * (eu * slope.abs() + u.abs() * (bend.abs() * eg + fast)), dtype)
+    edu = rounded(du, edh * silu.abs() + dh.abs() * es, dtype)
+    edg = rounded(dg, edh * (u * slope).abs() + dh.abs() * ed, dtype)
     a, ea = product(dg, edg, gate, None)
     b, eb = product(du, edu, up, None)
     dx, edx = a + b, ea + eb + gamma(1) * (a.abs() + b.abs())
