@@ -1178,6 +1178,17 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const JoinParams p) {
 // leaves room on both sides.
 constexpr float kOrthScale = 256.f;
 
+// kOrthScale / norm as two FP32 factors for one after the other, the first a
+// power of two (so that the product is rounded once): a single one is infinite
+// for norms below 2^-120, which BF16 elements can have.
+__device__ __forceinline__ float2 orth_factors(double norm) {
+    const double f = static_cast<double>(kOrthScale) / norm;
+    // A norm of zero, infinity or NaN gives what the formula gives.
+    if (!(f > 0.) || isinf(f)) return make_float2(static_cast<float>(f), 1.f);
+    const int half = ilogb(f) / 2;
+    return make_float2(static_cast<float>(ldexp(1., half)), static_cast<float>(ldexp(f, -half)));
+}
+
 // Eight elements of a row from column c on, zero from `cols` on. kVec: rows are
 // 16-byte aligned and whole vectors.
 template <bool kVec>
@@ -1195,6 +1206,15 @@ __device__ __forceinline__ void orth_load8(const void* g, long long row, int c, 
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? to_f32(g, row + c + j, bf16) : 0.f;
     }
+}
+
+// Elements times `down` have squares within FP32; the result is 1 / down. The
+// power of two of the largest of them, or 2^100 from 2^-125 down (whose inverse
+// or squares FP32 does not have) and 2^-100 from 2^126 up.
+__device__ __forceinline__ double square_scale(float top, float& down) {
+    const uint32_t e = __float_as_uint(top) & 0x7f800000u;
+    down = e < 0x01000000u ? 0x1p100f : e >= 0x7e800000u ? 0x1p-100f : __uint_as_float(0x7f000000u - e);
+    return e < 0x01000000u ? 0x1p-100 : e >= 0x7e800000u ? 0x1p100 : static_cast<double>(__uint_as_float(e));
 }
 
 // Sums of squares of matrix blockIdx.y: sums[matrix][block]. Eight squares are
@@ -1221,11 +1241,8 @@ __global__ void __launch_bounds__(256) orth_square_kernel(const void* g, long lo
         float top = 0.f, sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
-        // 2^-e of the largest element (its mantissa cleared); 1 for zeros, infinities and NaN.
-        const uint32_t e = __float_as_uint(top) & 0x7f800000u;
-        const bool plain = e >= 0x01000000u && e < 0x7e800000u;
-        const float down = plain ? __uint_as_float(0x7f000000u - e) : 1.f;
-        const double up = plain ? static_cast<double>(__uint_as_float(e)) : 1.;
+        float down;
+        const double up = square_scale(top, down);
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum = fmaf(v[j] * down, v[j] * down, sum);
         s += static_cast<double>(sum) * up * up;
@@ -1246,17 +1263,17 @@ __global__ void __launch_bounds__(256) orth_scale_kernel(const void* g, long lon
                                                          int cols, long long ld, int bf16,
                                                          const double* sums, int num_sums, double eps,
                                                          __half* x, long long ld_x, long long x_stride) {
-    __shared__ float factor;
+    __shared__ float2 factors;
     grid_dependents_launch();
     grid_dependency_wait();
     if (threadIdx.x < 32) {
         double s = 0.;
         for (int i = threadIdx.x; i < num_sums; i += 32) s += sums[static_cast<long long>(blockIdx.y) * num_sums + i];
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (threadIdx.x == 0) factor = static_cast<float>(static_cast<double>(kOrthScale) / (sqrt(s) + eps));
+        if (threadIdx.x == 0) factors = orth_factors(sqrt(s) + eps);
     }
     __syncthreads();
-    const float f = factor;
+    const float f = factors.x, f2 = factors.y;
     const long long base = blockIdx.y * batch_stride;
     __half* dst = x + blockIdx.y * x_stride;
     const int groups = (cols + 7) / 8;
@@ -1268,10 +1285,10 @@ __global__ void __launch_bounds__(256) orth_scale_kernel(const void* g, long lon
         float v[8];
         orth_load8<kVec>(g, base + r * ld, c, cols, bf16, v);
         uint4 w;
-        w.x = pack2(v[0] * f, v[1] * f, 0);
-        w.y = pack2(v[2] * f, v[3] * f, 0);
-        w.z = pack2(v[4] * f, v[5] * f, 0);
-        w.w = pack2(v[6] * f, v[7] * f, 0);
+        w.x = pack2(v[0] * f * f2, v[1] * f * f2, 0);
+        w.y = pack2(v[2] * f * f2, v[3] * f * f2, 0);
+        w.z = pack2(v[4] * f * f2, v[5] * f * f2, 0);
+        w.w = pack2(v[6] * f * f2, v[7] * f * f2, 0);
         *reinterpret_cast<uint4*>(dst + r * ld_x + c) = w;
     }
 }
@@ -1353,7 +1370,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const Ort
     uint64_t* bars = reinterpret_cast<uint64_t*>(qs + kOrthSquareBytes);   // [2]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    float* factor = reinterpret_cast<float*>(tmem_slot + 2);
+    float2* factors = reinterpret_cast<float2*>(tmem_slot + 2);
     double* warp_sums = reinterpret_cast<double*>(bars + 4);       // [8]
     double* cta_sums = warp_sums + 8;                              // [16]
 
@@ -1437,10 +1454,8 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const Ort
                 if (p.tall) *reinterpret_cast<uint16_t*>(x_at(s + j, l)) = static_cast<uint16_t>(u[j >> 1] >> ((j & 1) * 16));
             }
             if (!p.tall) *reinterpret_cast<uint4*>(x_at(s, l)) = w;
-            const uint32_t e = __float_as_uint(top) & 0x7f800000u;
-            const bool plain = e >= 0x01000000u && e < 0x7e800000u;
-            const float down = plain ? __uint_as_float(0x7f000000u - e) : 1.f;
-            const double up = plain ? static_cast<double>(__uint_as_float(e)) : 1.;
+            float down;
+            const double up = square_scale(top, down);
 #pragma unroll
             for (int j = 0; j < 8; ++j) part = fmaf(v[j] * down, v[j] * down, part);
             sum += static_cast<double>(part) * up * up;
@@ -1467,10 +1482,10 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const Ort
     if (threadIdx.x == 0) {
         sum = 0.;
         for (uint32_t i = 0; i < ctas; ++i) sum += cta_sums[i];
-        *factor = static_cast<float>(static_cast<double>(kOrthScale) / (sqrt(sum) + p.eps));
+        *factors = orth_factors(sqrt(sum) + p.eps);
     }
     __syncthreads();
-    const float f = *factor;
+    const float f = factors->x, f2 = factors->y;
     // Scaled in place (columns outside X are zero).
     for (uint32_t i = threadIdx.x; i < blocks * (kOrthBlockBytes / 16u); i += kOrthThreads) {
         uint4 w = reinterpret_cast<uint4*>(xs)[i];
@@ -1478,7 +1493,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const Ort
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float2 h = unpack2(u[j], p.bf16);
-            u[j] = pack2(h.x * f, h.y * f, 0);
+            u[j] = pack2(h.x * f * f2, h.y * f * f2, 0);
         }
         reinterpret_cast<uint4*>(xs)[i] = w;
     }

@@ -541,6 +541,24 @@ def test_orthogonalize_steps_coefficients_and_zeros():
     assert llm_hgemm.orthogonalize(zero[:0]).shape == (0, 50)
 
 
+@pytest.mark.parametrize("size", [(8, 24), (9, 23), (136, 200)], ids=str)
+def test_orthogonalize_of_the_smallest_and_largest_elements(size):
+    """Without eps the result does not depend on a power of two in g, over all of
+    BF16's normal numbers: at the first scale 256 / norm is beyond FP32 (elements
+    of 2^-126 to 2^-123, a few of them in the large matrix)."""
+    g = normal(11, *size, dtype=torch.bfloat16)
+    g = torch.where(g < 0, -1.0, 1.0).bfloat16() * g.abs().clamp(0.5, 4)
+    if g.numel() > 1000:
+        keep = torch.rand(size, generator=torch.Generator(device="cuda").manual_seed(12), device="cuda") < 0.005
+        g = torch.where(keep, g, torch.zeros_like(g))
+    assert float(g.double().norm()) * 2.0 ** -125 < 2.0 ** -120
+    want = llm_hgemm.orthogonalize(g, eps=0.0)
+    assert bool(want.isfinite().all())
+    for exponent in (-125, -100, 100, 125):
+        h = (g.double() * 2.0 ** exponent).bfloat16()
+        assert torch.equal(llm_hgemm.orthogonalize(h, eps=0.0), want)
+
+
 @pytest.mark.parametrize("pair", [0, train_capi.TILE_PAIR], ids=["single", "pair"])
 @pytest.mark.parametrize("width", TILES)
 @pytest.mark.parametrize("size", [(300, 700), (700, 300)], ids=str)
