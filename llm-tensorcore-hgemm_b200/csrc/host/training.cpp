@@ -2,6 +2,7 @@
 #include "training.h"
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -64,6 +65,29 @@ void check_status(int rc, const char* what) {
 void no_double_backward(const char* what) {
     // Gradient mode is on inside a backward pass only under create_graph=True.
     TORCH_CHECK(!torch::GradMode::is_enabled(), what, " has no second derivative (create_graph=True)");
+}
+
+// A gradient goes on to the node of its leaf, which lives on as long as any graph
+// of that leaf does, on the stream where the first of them was recorded. In a
+// capture the engine would make that stream wait for the captured one; where it
+// is no part of the capture this ends the process, so it is refused here.
+void check_capture(const char* what) {
+    using c10::cuda::CaptureStatus;
+    const c10::cuda::CUDAStream here = c10::cuda::getCurrentCUDAStream();
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == CaptureStatus::None) return;
+    const auto node = torch::autograd::get_current_node();
+    if (node == nullptr) return;
+    for (const torch::autograd::Edge& edge : node->next_edges()) {
+        if (!edge.is_valid()) continue;
+        const std::optional<c10::Stream> next = edge.function->stream();
+        if (!next.has_value() || *next == here.unwrap()) continue;
+        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+        const cudaError_t rc = cudaStreamIsCapturing(c10::cuda::CUDAStream(*next).stream(), &status);
+        if (rc != cudaSuccess) (void)cudaGetLastError();   // the legacy stream, never part of a capture
+        TORCH_CHECK(rc == cudaSuccess && status == cudaStreamCaptureStatusActive, what,
+                    " backward cannot be captured into a CUDA graph while a graph of the same tensors from outside the "
+                    "capture is alive: delete its outputs first");
+    }
 }
 
 // An uninitialised tensor on the device of `like`, without the dispatcher's way.
@@ -160,6 +184,7 @@ class GatedFfn : public torch::autograd::Function<GatedFfn> {
         const FfnSizes s = ffn_sizes(x, gate, down);
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
         const c10::cuda::CUDAGuard device_guard(x.device());
+        check_capture("gated_ffn");
         const Tensor dy = operand(rows_of(grads[0], s.tokens, s.out), s.tokens, s.out8, false);
         const Tensor xp = operand(rows_of(x, s.tokens, s.hidden), s.tokens, s.hidden8, false);
         const Tensor gp = operand(gate, s.inter8, s.hidden8, true), up_ = operand(up, s.inter8, s.hidden8, true);
@@ -267,6 +292,7 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
         const variable_list v = ctx->get_saved_variables();
         const Tensor &x = v[0], &weight = v[1], &target = v[2], &lse = v[3];
         const c10::cuda::CUDAGuard device_guard(x.device());
+        check_capture("linear_cross_entropy");
         const int64_t tokens = target.numel(), hidden = weight.size(1), hidden8 = round8(hidden);
         const Tensor xp = operand(rows_of(x, tokens, hidden), tokens, hidden8, false);
         const Tensor wp = operand(weight, weight.size(0), hidden8, true);

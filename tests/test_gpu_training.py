@@ -2,6 +2,10 @@
 bounds of tests/training_reference.py: tile shapes, types, odd and ragged sizes,
 ignored and invalid targets, strides, streams, captured graphs, differences."""
 
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 from torch import nn
@@ -656,6 +660,134 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         for a, b in zip(out, w):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("what", ["ffn", "loss"])
+def test_captured_backward_beside_an_eager_graph_is_refused(what):
+    x, gate, up, down, w, t, dy = all_inputs()
+
+    def call():
+        if what == "loss":
+            return llm_hgemm.linear_cross_entropy(x, w, t), [x, w]
+        return llm_hgemm.gated_ffn(x, gate, up, down).float().sum(), [x, gate, up, down]
+
+    def capture():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y, leaves = call()
+            out = torch.autograd.grad(y, leaves)
+        return graph, out
+
+    want = torch.autograd.grad(*call())
+    eager, _ = call()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        capture()
+    torch.cuda.synchronize()
+    for got, v in zip(torch.autograd.grad(eager, call()[1]), want):   # the eager graph still works
+        assert torch.equal(got, v)
+    del eager
+    graph, out = capture()
+    graph.replay()
+    torch.cuda.synchronize()
+    for got, v in zip(out, want):
+        assert torch.equal(got, v)
+
+
+FIRST_CALL = """
+import torch, llm_hgemm
+gen = torch.Generator(device="cuda").manual_seed(1)
+r = lambda *s: torch.randn(s, generator=gen, device="cuda").half() / 8
+x, gate, up, down, w, g = r(40, 64), r(96, 64), r(96, 64), r(64, 96), r(500, 64), r(200, 300)
+t = torch.arange(40, device="cuda")
+run = lambda: (llm_hgemm.gated_ffn(x, gate, up, down), llm_hgemm.linear_cross_entropy(x, w, t),
+               llm_hgemm.orthogonalize(g), llm_hgemm.orthogonalize(g[:50]))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = run()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, run()))
+print("same")
+"""
+
+
+def test_first_call_of_a_process_captured():
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL], capture_output=True, text=True, timeout=300,
+                          env={**os.environ, "PYTHONPATH": os.pathsep.join(p for p in sys.path if p)})
+    assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]
+
+
+def test_ffn_past_32_bits():
+    """tokens x inter beyond 2^31: the last rows, and the last columns' weight
+    gradients (of the last rows alone, so that the bound of 131080 FP32 additions
+    stays below the values)."""
+    tokens, hidden, inter = 131080, 64, 17408
+    x, gate, up, down, dy = ffn_inputs(tokens, hidden, inter, 64, torch.float16)
+    dy[:-64] = 0
+    leaves = [v.requires_grad_() for v in (x, gate, up, down)]
+    y = llm_hgemm.gated_ffn(*leaves)
+    dx, dgate, dup, ddown = torch.autograd.grad(y, leaves, dy)
+    want = ref.ffn(x[-40:], gate, up, down, dy[-40:])
+    within(y.detach()[-40:], want[0])
+    within(dx[-40:], want[1])
+    assert not dx[:-64].any()
+    last = ref.ffn(x, gate[-8:], up[-8:], down[:, -8:], dy)
+    within(dgate[-8:], last[2])
+    within(dup[-8:], last[3])
+    within(ddown[:, -8:], last[4])
+
+
+def test_loss_past_32_bits():
+    """vocabulary x hidden beyond 2^31. All of W but its first and last 1000 rows is
+    zero: there the logits are 0, and one entry with probability stands for them."""
+    tokens, hidden, vocab, ends = 16, 1024, 2100000, 1000
+    x = normal(1, tokens, hidden, dtype=torch.bfloat16, scale=0.1)
+    some = normal(2, 2 * ends, hidden, dtype=torch.bfloat16)
+    w = torch.zeros(vocab, hidden, dtype=torch.bfloat16, device="cuda")
+    w[:ends], w[-ends:] = some[:ends], some[ends:]
+    t = torch.where(torch.arange(tokens, device="cuda") % 2 == 0, 7, vocab - 7)
+    x.requires_grad_(), w.requires_grad_()
+    value = llm_hgemm.linear_cross_entropy(x, w, t, reduction="sum")
+    dx, dw = torch.autograd.grad(value, [x, w])
+    z = x.detach().double() @ some.double().T
+    lse = torch.log(z.exp().sum(1) + (vocab - 2 * ends))
+    at = torch.where(t < ends, t, t - vocab + 2 * ends)
+    d = torch.exp(z - lse[:, None])
+    d[torch.arange(tokens, device="cuda"), at] -= 1
+    # Relative error of a probability: FP32 sums of 1024 products, at most
+    # (1024 + 8) 2^-23 sum |x w|, for the logit and the statistics; 2^-24 for each of
+    # at most 40 + V / 32 additions; some 2^-20 for exp. Then dz is rounded once.
+    logit = 1032 * 2.0 ** -23 * float((x.detach().double().abs() @ some.double().abs().T).max())
+    off = 2 * logit + (40 + vocab / 32) * 2.0 ** -24 + 2.0 ** -20
+    assert off < 0.06
+    total = (lse - z.gather(1, at[:, None])[:, 0]).sum()
+    assert abs(float(value.detach().double() - total)) <= tokens * (off + 2.0 ** -20 * float(lse.max()))
+    for got, p, q in ((dx, d, some.double()), (torch.cat([dw[:ends], dw[-ends:]]), d.T, x.detach().double())):
+        v, most = p @ q, p.abs() @ q.abs()
+        err = (off + 2.0 ** -8 + 1032 * 2.0 ** -23) * most + 2.0 ** -8 * v.abs() * 1.1 + 1e-30
+        assert bool(((got.double() - v).abs() <= err).all())
+    # A row of the zeros: -p of that column times x, in every one of them.
+    p0 = torch.exp(-lse)
+    v, most = p0 @ x.detach().double(), p0 @ x.detach().double().abs()
+    err = (off + 2.0 ** -7) * most + 2.0 ** -8 * v.abs()
+    for row in (ends, vocab // 2, vocab - ends - 1):
+        assert bool(((dw[row].double() - v).abs() <= err).all())
+
+
+def test_orthogonalize_past_32_bits():
+    """rows x cols beyond 2^31, zero but for the first and last 1000 rows: their
+    update is that of the 2000 rows alone."""
+    rows, cols, ends = 16000000, 136, 1000
+    some = normal(3, 2 * ends, cols, dtype=torch.bfloat16)
+    g = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    g[:ends], g[-ends:] = some[:ends], some[ends:]
+    value, err = ref.orthogonalize(some, 5, NEWTON_SCHULZ, 1e-7)
+    got = llm_hgemm.orthogonalize(g)
+    assert not got[ends:-ends].any()
+    got = torch.cat([got[:ends], got[-ends:]])
+    assert float(torch.linalg.vector_norm(got.double() - value)) <= err
 
 
 def test_injected_stall_times_out_and_context_survives():
