@@ -36,12 +36,12 @@
 // as in the inference kernels (status word, drained copies, freed TMEM).
 //
 // What bounds it (2048 tokens, hidden 2560, under ncu): the tensor pipe where
-// the epilogue stores nothing (softmax statistics: 91 % active, 1.7 PFLOP/s in
-// a burst); 80-85 % where it stores 16 bits (logit gradients, the weights'
-// gradients); 73 % with three outputs (gate, kept pre-activations); 46 % where
-// it reads two matrices and writes two (gradient of the gate), DRAM at 24 % and
-// L2 at 50 % throughout. Long back-to-back runs are held by the power limit
-// instead (1.2-1.35 PFLOP/s). A K block of a 256 x 256 pair tile takes about
+// the epilogue stores nothing (softmax statistics: 92 % active, 1.65 PFLOP/s);
+// 82-86 % where it stores 16 bits (logit gradients, the weights' gradients);
+// 74 % with three outputs (gate); 49 % where it reads two matrices and writes
+// two (gradient of the gate). DRAM is at 11-24 % and L2 at 42-52 % throughout.
+// Long back-to-back runs are held by the power limit instead (sampled: 1.24 to
+// 1.55 GHz of 1.965, the power cap active all the time; 1.2-1.35 PFLOP/s). A K block of a 256 x 256 pair tile takes about
 // 590 cycles of which the MMAs are 512.
 #pragma once
 
@@ -1024,7 +1024,7 @@ __global__ void __launch_bounds__(1024) lse_join_kernel(const float2* partial, i
 }
 
 // Sum of the rows' losses (and their count for the mean), one block, in a
-// fixed order and 64 bits. Latency: 3-4 us up to 4096 rows.
+// fixed order and 64 bits. Latency: 3.6-4.5 us for 24 to 4096 rows.
 __global__ void __launch_bounds__(1024) loss_reduce_kernel(const float* loss,
                                                            const long long* target, int m,
                                                            long long ignore, int mean, float* out) {
@@ -1058,7 +1058,7 @@ __global__ void __launch_bounds__(1024) loss_reduce_kernel(const float* loss,
 // Row factors of the logits' gradient and the scalar that the products take:
 // dz[row] = row_scale[row] (p - onehot), gradient = alpha dz^T x and so on.
 // One loss per row: row_scale = dloss[row] / max |dloss|, so that any range of
-// incoming gradients fits 16 bits. One block; latency, 5 us up to 4096 rows.
+// incoming gradients fits 16 bits. One block; latency, 4.6-5.7 us for 24 to 4096 rows.
 __global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* dloss, int per_row, int mean,
                                                                 const long long* target, int m,
                                                                 long long vocab, long long ignore,
