@@ -178,6 +178,9 @@ struct Product {
     float* parts = nullptr;
     bool add_parts = false;
     bool triangle = false;
+    // The sum's length that the raster goes by, where launches of different
+    // lengths add to the same parts (a part's place is its tile's raster number).
+    int64_t raster_k = 0;
     int64_t kblocks() const { return cdiv(k0, kBlockK) + cdiv(k1, kBlockK); }
 };
 
@@ -316,7 +319,9 @@ size_t parts_bytes(const Product& p, const Tile& t) {
 
 // Raster group height: the tallest of 8, 16, 32 tile rows whose one-wave
 // footprint of A and B panels stays within 48 MB (the pair kernels' rule).
-int group_height(int64_t m, int64_t k, bool pair, int units) {
+int group_height(const Product& p, bool pair, int sms) {
+    const int64_t m = p.m, k = p.raster_k > 0 ? p.raster_k : p.k0 + p.k1;
+    const int units = pair ? sms / 2 : sms;
     const int rows = pair ? 256 : 128;
     const double panel = 2.0 * rows * static_cast<double>(k);
     int g = 8;
@@ -390,7 +395,7 @@ int run_products(TrainParams& p, int epi, const Product* products, const Tile& t
         q.b_mn = s.b0.mn;
         q.tiles_m = static_cast<int>(cdiv(s.m, tile_rows(pair)));
         q.tiles_n = static_cast<int>(cdiv(s.n, cols));
-        q.group_m = group_height(s.m, s.k0 + s.k1, pair, units);
+        q.group_m = group_height(s, pair, c.dev->sms);
         q.symmetric = s.triangle;
         q.tile0 = static_cast<int>(parted ? all - s.parted : 0);
         q.tiles = static_cast<int>(tiles);
@@ -471,7 +476,7 @@ int join_parts(const Product& s, const Tile& t, const Context& c, int in_bf16, i
     p.tile_n = t.n;
     p.tiles_m = static_cast<int>(cdiv(s.m, p.tile_m));
     p.tiles_n = static_cast<int>(cdiv(s.n, t.n));
-    p.group_m = group_height(s.m, s.k0 + s.k1, t.pair, t.pair ? c.dev->sms / 2 : c.dev->sms);
+    p.group_m = group_height(s, t.pair, c.dev->sms);
     p.m = static_cast<int>(s.m);
     p.n = static_cast<int>(s.n);
     p.alpha = s.alpha;
@@ -732,6 +737,7 @@ LossPiece plan_piece(const HgemmSm100LossBackward& a, int64_t nv, int64_t piece,
         d.m = a.tokens;
         d.n = d.ld_out = a.hidden;
         d.k0 = nv;
+        d.raster_k = piece;   // a short last piece adds to the tiles of the others
         d.a0 = {nullptr, piece, false};
         d.b0 = {nullptr, a.hidden, true};
         d.splittable = true;
