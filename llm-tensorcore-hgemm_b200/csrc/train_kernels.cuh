@@ -69,7 +69,7 @@ enum : int {
     kTrainGate = 1,       // acc = (gate | up): out = silu(gate) up; silu(gate) and up silu'(gate) kept
     kTrainGateGrad = 2,   // acc = dh: out = dh (up silu'(gate)), out[1] = dh silu(gate), from what was kept
     kTrainLse = 3,        // per row: max and sum of exp over the tile's columns
-    kTrainLogitGrad = 4,  // out = (exp(acc - lse) - [column == target]) row factor
+    kTrainLogitGrad = 4,  // out = (exp(acc - lse) - [column == target]) row factor; out[1] with another factor
     kTrainStoreC = 5,     // kTrainStore with out = alpha acc + beta C
 };
 // How kTrainStore and kTrainStoreC write: 16-bit boxes, FP32 boxes, FP32 boxes added to memory.
@@ -92,6 +92,7 @@ struct alignas(64) TrainProblem {
     int out_kind;
     float alpha, beta;
     const float* alpha_ptr;    // multiplies alpha (device memory; may be null)
+    const float* alpha_rows;   // kTrainStore: multiplies alpha, per row (may be null)
     const void* c;             // FP16 [m x ldc] for beta != 0
     long long ldc;
 };
@@ -119,6 +120,7 @@ struct alignas(64) TrainParams {
     float* target_logit;           // kTrainLse: written by the tile holding the target
     const float* lse;
     const float* row_scale;
+    const float* row_ratio;        // kTrainLogitGrad: out[1] = row_ratio out[0] too (may be null)
 };
 
 // ------------------------------------------------------------- small parts ---
@@ -526,15 +528,18 @@ struct TrainEpilogue {
 
     template <bool kBf16>
     __device__ __forceinline__ void store(BoxWriter& box, uint32_t t) {
-        float scale = 0.f, lse = 0.f;
+        float scale = 0.f, lse = 0.f, ratio = 0.f;
         long long want = -1;
         if constexpr (kEpi == kTrainStore || kEpi == kTrainStoreC)
             if (alpha_ptr != nullptr) alpha *= *alpha_ptr;
+        if constexpr (kEpi == kTrainStore)
+            if (q.alpha_rows != nullptr && in_rows) alpha *= q.alpha_rows[row];
         if constexpr (kEpi == kTrainLogitGrad)
             if (in_rows) {
                 want = p.target[row] - p.col_base;
                 scale = p.row_scale[row];
                 lse = p.lse[row];
+                if (p.row_ratio != nullptr) ratio = p.row_ratio[row];
             }
         if (kEpi == kTrainLogitGrad || (kEpi == kTrainStore && !mirror)) {
             // Two groups a turn.
@@ -556,6 +561,16 @@ struct TrainEpilogue {
                     logit_gradient(w, col + 64, want, scale, lse);
                 }
                 box.put16_two<kBf16>(&q.out[0], v, w, two, col, col + 64, row0);
+                if constexpr (kEpi == kTrainLogitGrad) {
+                    if (p.row_ratio != nullptr) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            v[i] *= ratio;
+                            w[i] *= ratio;
+                        }
+                        box.put16_two<kBf16>(&q.out[1], v, w, two, col, col + 64, row0);
+                    }
+                }
             }
             return;
         }
@@ -966,8 +981,9 @@ __global__ void __launch_bounds__(kTrainThreads, 1) train_gemm_kernel(const __gr
 
 // -------------------------------------------------- cross entropy, row parts ---
 
-// Factor on the stored logit gradients, so that a probability of 1 / vocabulary
-// stays a normal FP16 number; the products' epilogues take it out again.
+// Factor on the stored logit gradients of one incoming gradient, so that a
+// probability of 1 / vocabulary stays a normal FP16 number (151936 entries:
+// 0.1); the products' epilogues take it out again.
 constexpr float kLogitGradScale = 16384.f;
 
 // Joins a row's per-tile (max, sum) pairs: lse = max + log(sum), and its loss
@@ -1055,15 +1071,24 @@ __global__ void __launch_bounds__(1024) loss_reduce_kernel(const float* loss,
     *out = static_cast<float>(mean ? s / c : s);   // no target at all: 0 / 0 = NaN for the mean
 }
 
-// Row factors of the logits' gradient and the scalar that the products take:
-// dz[row] = row_scale[row] (p - onehot), gradient = alpha dz^T x and so on.
-// One loss per row: row_scale = dloss[row] / max |dloss|, so that any range of
-// incoming gradients fits 16 bits. One block; latency, 4.6-5.7 us for 24 to 4096 rows.
-__global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* dloss, int per_row, int mean,
+// Row factors of the logits' gradient, and what takes them out of the products:
+//   dz[row] = row_scale[row] (p - onehot), dW = alpha dz^T x, dx = alpha dz W.
+// One incoming gradient for all rows: row_scale is 2^14 and alpha has the rest.
+// One per row, kScaleBf16: BF16 has FP32's range, so row_scale = dloss[row] and
+// alpha = 1. FP16 with one scale for all rows loses probabilities of small
+// gradients: 1/151936 is subnormal in a row with 1/1800 of the largest, and zero
+// with 1/3.6e6. A sum over rows (dW) needs one scale, a row of dx does not, so dz
+// is written in both where both are wanted. kScaleRows: row_scale = dloss[row]
+// 2^(15 - e), e the row's own exponent, and dx = row_alpha[row] dz W; row_ratio =
+// 2^(e - E), E the largest exponent, turns such a dz into the common scale's.
+// kScaleCommon: that scale alone, dloss[row] 2^(15 - E); alpha = 2^(E - 15).
+// One block; latency, 4.6-5.7 us for 24 to 4096 rows.
+enum : int { kScaleOne = 0, kScaleBf16 = 1, kScaleCommon = 2, kScaleRows = 3 };
+__global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* dloss, int kind, int mean,
                                                                 const long long* target, int m,
                                                                 long long vocab, long long ignore,
-                                                                float* row_scale,
-                                                                float* alpha) {
+                                                                float* row_scale, float* row_alpha,
+                                                                float* row_ratio, float* alpha) {
     __shared__ float tops[32];
     __shared__ int counts[32];
     grid_dependents_launch();
@@ -1074,7 +1099,7 @@ __global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* dlo
     for (int i = threadIdx.x; i < m; i += 1024) {
         if (target[i] == ignore) continue;
         ++c;
-        if (per_row) {
+        if (kind != kScaleOne) {
             const float a = fabsf(dloss[i]);
             odd |= !(a <= 3.4028235e38f);
             top = fmaxf(top, a);
@@ -1096,20 +1121,40 @@ __global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* dlo
         top = fmaxf(top, tops[i]);
         c += counts[i];
     }
+    int most = 0;
+    if (top > 0.f && top <= 3.4028235e38f) frexpf(top, &most);
     const float nan = __int_as_float(0x7fffffff);
     for (int i = threadIdx.x; i < m; i += 1024) {
         const long long want = target[i];
-        float r = 0.f;
+        float r = 0.f, own_alpha = 1.f, ratio = 1.f;
         if (want != ignore) {
-            r = (want >= 0 && want < vocab) ? kLogitGradScale : nan;
-            if (per_row) r *= top > 0.f ? dloss[i] / top : 0.f;   // inf / inf: NaN, as it should be
+            const float d = kind == kScaleOne ? kLogitGradScale : dloss[i];
+            r = d;
+            if (kind >= kScaleCommon && d != 0.f && fabsf(d) <= 3.4028235e38f) {
+                int e;
+                r = ldexpf(frexpf(d, &e), 15);
+                own_alpha = ldexpf(1.f, e - 15);
+                ratio = ldexpf(1.f, e - most);
+                if (kind == kScaleCommon) r *= ratio;
+            }
+            if (want < 0 || want >= vocab) r = nan;
         }
         row_scale[i] = r;
+        if (kind == kScaleRows) {
+            row_alpha[i] = own_alpha;
+            row_ratio[i] = ratio;
+        }
     }
     if (threadIdx.x == 0) {
-        float a = per_row ? top : dloss[0];
-        if (mean) a = c > 0 ? a / static_cast<float>(c) : 0.f;
-        *alpha = a / kLogitGradScale;
+        float a = 1.f;
+        if (kind == kScaleOne) {
+            a = dloss[0];
+            if (mean) a = c > 0 ? a / static_cast<float>(c) : 0.f;
+            a /= kLogitGradScale;
+        } else if (kind >= kScaleCommon) {
+            a = ldexpf(1.f, most - 15);
+        }
+        *alpha = a;
     }
 }
 
@@ -1123,6 +1168,7 @@ struct JoinParams {
     int splits, tiles, tile0, tiles_m, tiles_n, group_m, tile_m, tile_n, m, n;
     float alpha, beta;
     const float* alpha_ptr;    // multiplies alpha; may be null
+    const float* alpha_rows;   // multiplies alpha, per row; may be null
     const void* c;
     long long ldc;
     void* out;                 // 16-byte aligned rows
@@ -1149,7 +1195,8 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const JoinParams p) {
         v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
         v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
     }
-    const float alpha = p.alpha_ptr != nullptr ? p.alpha * *p.alpha_ptr : p.alpha;
+    float alpha = p.alpha_ptr != nullptr ? p.alpha * *p.alpha_ptr : p.alpha;
+    if (p.alpha_rows != nullptr) alpha *= p.alpha_rows[row];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] *= alpha;
     if (p.beta != 0.f) {

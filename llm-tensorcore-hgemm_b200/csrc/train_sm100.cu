@@ -167,6 +167,7 @@ struct Product {
     void* out2 = nullptr;
     float alpha = 1.f, beta = 0.f;
     const float* alpha_ptr = nullptr;
+    const float* alpha_rows = nullptr;
     const void* c = nullptr;
     int64_t ldc = 0;
     bool splittable = false;   // sums may be cut into parts
@@ -406,6 +407,7 @@ int run_products(TrainParams& p, int epi, const Product* products, const Tile& t
         q.alpha = s.alpha;
         q.beta = parted ? 0.f : s.beta;   // the join adds it
         q.alpha_ptr = s.alpha_ptr;
+        q.alpha_rows = s.alpha_rows;
         q.c = s.c;
         q.ldc = s.ldc;
         // Few rows (K-major): only those are loaded. What the MMA reads in place
@@ -482,6 +484,7 @@ int join_parts(const Product& s, const Tile& t, const Context& c, int in_bf16, i
     p.alpha = s.alpha;
     p.beta = s.beta;
     p.alpha_ptr = s.alpha_ptr;
+    p.alpha_rows = s.alpha_rows;
     p.c = s.c;
     p.ldc = s.ldc;
     p.out = s.out;
@@ -712,12 +715,25 @@ LossForwardPlan plan_loss_forward(const HgemmSm100LossForward& a, int sms) {
     return q;
 }
 
+// How the logits' gradient is scaled (logit_grad_setup_kernel).
+int loss_scale(const HgemmSm100LossBackward& a) {
+    if (a.reduction != HGEMM_SM100_LOSS_NONE) return kScaleOne;
+    if (a.common.dtype == HGEMM_SM100_TRAIN_BF16) return kScaleBf16;
+    return a.dx != nullptr ? kScaleRows : kScaleCommon;
+}
+
+// Rows of their own scale serve dx; dW needs dz in the common one as well.
+int64_t loss_planes(const HgemmSm100LossBackward& a) {
+    return loss_scale(a) == kScaleRows && a.dweight != nullptr ? 2 : 1;
+}
+
 // Vocabulary entries of a piece: as many as keep its dz (tokens x piece, 16
-// bits) within 96 MB, so that it stays in L2 between the product that writes
-// it and the two that read it, in whole 256-column tiles, at least 2048.
+// bits, once or twice) within 96 MB, so that it stays in L2 between the product
+// that writes it and the two that read it, in whole 256-column tiles, at least
+// 2048.
 int64_t loss_piece(const HgemmSm100LossBackward& a) {
     if (a.piece > 0) return std::min<int64_t>(round_up(a.piece, 8), round_up(a.vocab, 8));
-    int64_t n = (int64_t{96} << 20) / (2 * a.tokens) / 256 * 256;
+    int64_t n = (int64_t{96} << 20) / (2 * loss_planes(a) * a.tokens) / 256 * 256;
     n = std::max<int64_t>(n, 2048);
     if (n >= a.vocab) return round_up(a.vocab, 8);
     return round_up(cdiv(a.vocab, cdiv(a.vocab, n)), 256);   // equal pieces
@@ -759,14 +775,16 @@ struct LossBackwardPlan {
     bool sums = false;     // dx goes through FP32 sums: several pieces, or parts of one
     int splits = 1;        // of dx, in every piece alike
     Tile tile;
-    size_t dz_bytes = 0, sum_bytes = 0, row_bytes = 0;
-    size_t bytes() const { return dz_bytes + sum_bytes + row_bytes + 256; }
+    int64_t planes = 1;    // of dz
+    size_t dz_bytes = 0, sum_bytes = 0, row_bytes = 0;   // of one plane, of dx, of one number per row
+    size_t bytes() const { return planes * dz_bytes + sum_bytes + 3 * row_bytes + 256; }
 };
 
 LossBackwardPlan plan_loss_backward(const HgemmSm100LossBackward& a, int sms) {
     LossBackwardPlan q;
     q.piece = loss_piece(a);
     q.pieces = cdiv(a.vocab, q.piece);
+    q.planes = loss_planes(a);
     q.dz_bytes = static_cast<size_t>(round_up(a.tokens * q.piece * 2, 256));
     q.row_bytes = static_cast<size_t>(round_up(a.tokens * 4, 256));
     if (a.dx == nullptr && a.dweight == nullptr) return q;
@@ -856,16 +874,26 @@ extern "C" int hgemm_sm100_loss_backward(const HgemmSm100LossBackward* a, void* 
     if (a->workspace_bytes < q.bytes()) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     if (a->dx == nullptr && a->dweight == nullptr) return HGEMM_SM100_OK;
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-    void* dz = ws;
-    float* sums = reinterpret_cast<float*>(ws + q.dz_bytes);
-    float* row_scale = reinterpret_cast<float*>(ws + q.dz_bytes + q.sum_bytes);
-    float* alpha = reinterpret_cast<float*>(ws + q.dz_bytes + q.sum_bytes + q.row_bytes);
+    uint8_t* dz = ws;                                          // as dx takes it
+    uint8_t* dz_common = ws + (q.planes - 1) * q.dz_bytes;     // as dW does
+    float* sums = reinterpret_cast<float*>(ws + q.planes * q.dz_bytes);
+    uint8_t* rows = ws + q.planes * q.dz_bytes + q.sum_bytes;
+    float* row_scale = reinterpret_cast<float*>(rows);
+    float* row_alpha = reinterpret_cast<float*>(rows + q.row_bytes);
+    float* row_ratio = reinterpret_cast<float*>(rows + 2 * q.row_bytes);
+    float* alpha = reinterpret_cast<float*>(rows + 3 * q.row_bytes);
+    const int scale = loss_scale(*a);
+    // What takes the factors out of dx.
+    auto scale_dx = [&](Product& d) {
+        if (scale == kScaleRows) d.alpha_rows = row_alpha;
+        else d.alpha_ptr = alpha;
+    };
     const long long* target = reinterpret_cast<const long long*>(a->target);
 
     rc = launch(&logit_grad_setup_kernel, dim3(1), dim3(1024), 0, 1, c.stream, a->dloss,
-                a->reduction == HGEMM_SM100_LOSS_NONE ? 1 : 0, a->reduction == HGEMM_SM100_LOSS_MEAN ? 1 : 0, target,
-                static_cast<int>(a->tokens), static_cast<long long>(a->vocab),
-                static_cast<long long>(a->ignore_index), row_scale, alpha);
+                scale, a->reduction == HGEMM_SM100_LOSS_MEAN ? 1 : 0, target, static_cast<int>(a->tokens),
+                static_cast<long long>(a->vocab), static_cast<long long>(a->ignore_index), row_scale, row_alpha,
+                row_ratio, alpha);
     if (rc != HGEMM_SM100_OK) return rc;
 
     TrainParams p;
@@ -879,12 +907,14 @@ extern "C" int hgemm_sm100_loss_backward(const HgemmSm100LossBackward* a, void* 
         z.a0 = {a->x, a->ldx, false};
         z.b0 = {w, a->hidden, false};
         z.out = dz;
+        z.out1 = q.planes == 2 ? dz_common : nullptr;
         z.ld_out = q.piece;
         init_params(p, c);
         p.target = target;
         p.col_base = v0;
         p.lse = a->lse;
         p.row_scale = row_scale;
+        p.row_ratio = q.planes == 2 ? row_ratio : nullptr;
         if ((rc = run_product(p, kTrainLogitGrad, z, c)) != HGEMM_SM100_OK) return rc;
 
         LossPiece g = plan_piece(*a, nv, q.piece, c.dev->sms);
@@ -898,11 +928,11 @@ extern "C" int hgemm_sm100_loss_backward(const HgemmSm100LossBackward* a, void* 
             d.parts = sums;
             d.add_parts = i > 0;
             d.out = a->dx;
-            d.alpha_ptr = alpha;
+            scale_dx(d);
         }
         if (a->dweight != nullptr) {
             Product& d = g.s[n++];
-            d.a0.ptr = dz;
+            d.a0.ptr = dz_common;
             d.out = static_cast<uint8_t*>(a->dweight) + v0 * a->hidden * 2;
             d.alpha_ptr = alpha;
         }
@@ -916,7 +946,7 @@ extern "C" int hgemm_sm100_loss_backward(const HgemmSm100LossBackward* a, void* 
     d.parted = tile_count(d, q.tile);
     d.parts = sums;
     d.out = a->dx;
-    d.alpha_ptr = alpha;
+    scale_dx(d);
     return join_parts(d, q.tile, c, p.in_bf16, p.out_bf16);
 }
 

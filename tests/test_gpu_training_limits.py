@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+import llm_hgemm
 from llm_hgemm import train_capi
 from tests import training_reference as ref
 from tests.gpu_helpers import require_cuda
@@ -29,3 +30,31 @@ def test_loss_short_last_piece_of_many_tile_rows(tokens, vocab, piece, tile):
     got = loss_through_c(x, w, t, dl, tile, piece, train_capi.LOSS_SUM)
     for g, v in zip((got[0][0], got[1], got[2]), want):
         within(g, v)
+
+
+@pytest.mark.parametrize("wanted, piece", [("both", 0), ("both", 4096), ("x", 0), ("weight", 0)])
+@pytest.mark.parametrize("dtype, sizes", [
+    (torch.float16, [2e4, 1e-3, 1.0, -3e-3, 0.0, 5e-5]),
+    (torch.bfloat16, [1e20, 1e-20, 1.0, -3e-22, 0.0, 5e4]),
+], ids=["fp16", "bf16"])
+def test_loss_gradients_of_small_and_large_rows(dtype, sizes, wanted, piece):
+    """Every row of dx is as good as if it were the only one, whatever the other
+    rows' incoming gradients. The weights have a mean, so that the probabilities'
+    part of a row (each of them 1/20011) is as large as its target's."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    w = (0.5 + 0.05 * torch.randn(20011, 64, generator=gen, device="cuda")).to(dtype)
+    x = (0.05 * torch.randn(6, 64, generator=gen, device="cuda")).to(dtype)
+    t = torch.arange(6, device="cuda") * 3000
+    dl = torch.tensor(sizes, device="cuda")
+    if piece:
+        _, dx, dw = loss_through_c(x, w, t, dl, piece=piece, reduction=train_capi.LOSS_NONE)
+    else:
+        leaves = [v.requires_grad_() for v, name in ((x, "x"), (w, "weight")) if wanted in ("both", name)]
+        grads = list(torch.autograd.grad(llm_hgemm.linear_cross_entropy(x, w, t, reduction="none"), leaves, dl))
+        dx = grads.pop(0) if wanted != "weight" else None
+        dw = grads.pop(0) if wanted != "x" else None
+    if dx is not None:
+        for i in range(6):
+            within(dx[i:i + 1], ref.loss(x[i:i + 1], w, t[i:i + 1], "none", -100, dl[i:i + 1])[1])
+    if dw is not None:
+        within(dw, ref.loss(x, w, t, "none", -100, dl)[2])
