@@ -1074,6 +1074,8 @@ __global__ void __launch_bounds__(1024) loss_reduce_kernel(const float* loss,
 // Row factors of the logits' gradient, and what takes them out of the products:
 //   dz[row] = row_scale[row] (p - onehot), dW = alpha dz^T x, dx = alpha dz W.
 // One incoming gradient for all rows: row_scale is 2^14 and alpha has the rest.
+// Infinity and NaN go to the rows they belong to, where alpha would bring them
+// to the others (0 x inf); an ignored row's gradient is 0 in any case.
 // One per row, kScaleBf16: BF16 has FP32's range, so row_scale = dloss[row] and
 // alpha = 1. FP16 with one scale for all rows loses probabilities of small
 // gradients: 1/151936 is subnormal in a row with 1/1800 of the largest, and zero
@@ -1093,19 +1095,18 @@ __global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* dlo
     __shared__ int counts[32];
     grid_dependents_launch();
     grid_dependency_wait();
-    float top = 0.f;
+    const float kMost = 3.4028235e38f;   // the largest finite number
+    const bool one_finite = kind == kScaleOne && fabsf(dloss[0]) <= kMost;
+    float top = 0.f;                      // of the finite ones
     int c = 0;
-    bool odd = false;
     for (int i = threadIdx.x; i < m; i += 1024) {
         if (target[i] == ignore) continue;
         ++c;
-        if (kind != kScaleOne) {
+        if (kind >= kScaleCommon) {
             const float a = fabsf(dloss[i]);
-            odd |= !(a <= 3.4028235e38f);
-            top = fmaxf(top, a);
+            if (a <= kMost) top = fmaxf(top, a);
         }
     }
-    if (odd) top = __int_as_float(0x7f800000);
     for (int o = 16; o > 0; o >>= 1) {
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         c += __shfl_xor_sync(0xffffffffu, c, o);
@@ -1122,15 +1123,15 @@ __global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* dlo
         c += counts[i];
     }
     int most = 0;
-    if (top > 0.f && top <= 3.4028235e38f) frexpf(top, &most);
+    if (top > 0.f) frexpf(top, &most);
     const float nan = __int_as_float(0x7fffffff);
     for (int i = threadIdx.x; i < m; i += 1024) {
         const long long want = target[i];
         float r = 0.f, own_alpha = 1.f, ratio = 1.f;
         if (want != ignore) {
-            const float d = kind == kScaleOne ? kLogitGradScale : dloss[i];
-            r = d;
-            if (kind >= kScaleCommon && d != 0.f && fabsf(d) <= 3.4028235e38f) {
+            const float d = kind == kScaleOne ? dloss[0] : dloss[i];
+            r = one_finite ? kLogitGradScale : d;
+            if (kind >= kScaleCommon && d != 0.f && fabsf(d) <= kMost) {
                 int e;
                 r = ldexpf(frexpf(d, &e), 15);
                 own_alpha = ldexpf(1.f, e - 15);
@@ -1147,7 +1148,7 @@ __global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* dlo
     }
     if (threadIdx.x == 0) {
         float a = 1.f;
-        if (kind == kScaleOne) {
+        if (one_finite) {
             a = dloss[0];
             if (mean) a = c > 0 ? a / static_cast<float>(c) : 0.f;
             a /= kLogitGradScale;

@@ -7,7 +7,7 @@ import llm_hgemm
 from llm_hgemm import train_capi
 from tests import training_reference as ref
 from tests.gpu_helpers import require_cuda
-from tests.test_gpu_training import loss_inputs, loss_through_c, within
+from tests.test_gpu_training import DTYPES, IDS, loss_inputs, loss_through_c, within
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +58,25 @@ def test_loss_gradients_of_small_and_large_rows(dtype, sizes, wanted, piece):
             within(dx[i:i + 1], ref.loss(x[i:i + 1], w, t[i:i + 1], "none", -100, dl[i:i + 1])[1])
     if dw is not None:
         within(dw, ref.loss(x, w, t, "none", -100, dl)[2])
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_loss_infinite_gradients_stay_in_their_rows(dtype, bad):
+    """An incoming gradient that is infinite or NaN reaches its own row of dx, or
+    all rows with a target where there is one for all, and no ignored row."""
+    x, w, t = loss_inputs(40, 64, 500, dtype)
+    t[3], t[7] = -100, 5
+    keep = t != -100
+    x.requires_grad_()
+    dl = torch.linspace(-2.0, 3.0, 40, device="cuda")
+    want = ref.loss(x, w, t, "none", -100, dl)[1]
+    dl[7] = bad
+    (dx,) = torch.autograd.grad(llm_hgemm.linear_cross_entropy(x, w, t, reduction="none"), x, dl)
+    others = torch.arange(40, device="cuda") != 7
+    assert not dx[7].isfinite().any()
+    within(dx[others], (want[0][others], want[1][others]))
+    for reduction in ("sum", "mean"):
+        value = llm_hgemm.linear_cross_entropy(x, w, t, reduction=reduction)
+        (dx,) = torch.autograd.grad(value, x, torch.tensor(bad, device="cuda"))
+        assert not dx[keep].isfinite().any() and not dx[~keep].any()
