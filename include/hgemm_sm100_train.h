@@ -117,7 +117,9 @@ int hgemm_sm100_loss_forward(const HgemmSm100LossForward* args, void* stream);
 
 /* Its gradient for an incoming gradient dloss ([tokens] for NONE, else [1]):
  * dz = (softmax(z) - onehot(target)) * row factor, dx = dz W, dweight = dz^T x.
- * The vocabulary is taken in pieces; of dz only one piece exists at a time. */
+ * The vocabulary is taken in pieces; of dz only one piece exists at a time.
+ * Rows whose target is `ignore_index` get zeros in dx and add nothing to
+ * dweight, even where x or dloss hold infinity or NaN there. */
 typedef struct HgemmSm100LossBackward {
     HgemmSm100TrainCommon common;
     const void* x;

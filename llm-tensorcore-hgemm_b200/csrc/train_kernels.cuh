@@ -1084,17 +1084,33 @@ __global__ void __launch_bounds__(1024) loss_reduce_kernel(const float* loss,
 // 2^(15 - e), e the row's own exponent, and dx = row_alpha[row] dz W; row_ratio =
 // 2^(e - E), E the largest exponent, turns such a dz into the common scale's.
 // kScaleCommon: that scale alone, dloss[row] 2^(15 - E); alpha = 2^(E - 15).
-// One block; latency, 4.6-5.7 us for 24 to 4096 rows.
+// Block 0; latency, 4.6-5.7 us for 24 to 4096 rows. Further blocks, where dW is
+// wanted, copy x with zeros for the ignored rows: their dz is 0, but dz^T x would
+// still take infinity and NaN from them (padding may hold anything).
 enum : int { kScaleOne = 0, kScaleBf16 = 1, kScaleCommon = 2, kScaleRows = 3 };
 __global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* dloss, int kind, int mean,
                                                                 const long long* target, int m,
                                                                 long long vocab, long long ignore,
                                                                 float* row_scale, float* row_alpha,
-                                                                float* row_ratio, float* alpha) {
+                                                                float* row_ratio, float* alpha, const void* x,
+                                                                long long ldx, int hidden, void* x_kept) {
     __shared__ float tops[32];
     __shared__ int counts[32];
     grid_dependents_launch();
     grid_dependency_wait();
+    if (blockIdx.x > 0) {
+        const int per_row = hidden / 8;
+        const long long total = static_cast<long long>(m) * per_row, stride = (gridDim.x - 1) * 1024ll;
+#pragma unroll 4
+        for (long long i = (blockIdx.x - 1) * 1024ll + threadIdx.x; i < total; i += stride) {
+            const long long r = i / per_row;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (target[r] != ignore)
+                v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + r * ldx + (i - r * per_row) * 8);
+            static_cast<uint4*>(x_kept)[i] = v;
+        }
+        return;
+    }
     const float kMost = 3.4028235e38f;   // the largest finite number
     const bool one_finite = kind == kScaleOne && fabsf(dloss[0]) <= kMost;
     float top = 0.f;                      // of the finite ones

@@ -777,7 +777,8 @@ struct LossBackwardPlan {
     Tile tile;
     int64_t planes = 1;    // of dz
     size_t dz_bytes = 0, sum_bytes = 0, row_bytes = 0;   // of one plane, of dx, of one number per row
-    size_t bytes() const { return planes * dz_bytes + sum_bytes + 3 * row_bytes + 256; }
+    size_t x_bytes = 0;    // x without the ignored rows
+    size_t bytes() const { return planes * dz_bytes + sum_bytes + 3 * row_bytes + 256 + x_bytes; }
 };
 
 LossBackwardPlan plan_loss_backward(const HgemmSm100LossBackward& a, int sms) {
@@ -787,6 +788,7 @@ LossBackwardPlan plan_loss_backward(const HgemmSm100LossBackward& a, int sms) {
     q.planes = loss_planes(a);
     q.dz_bytes = static_cast<size_t>(round_up(a.tokens * q.piece * 2, 256));
     q.row_bytes = static_cast<size_t>(round_up(a.tokens * 4, 256));
+    if (a.dweight != nullptr) q.x_bytes = static_cast<size_t>(a.tokens * a.hidden * 2);
     if (a.dx == nullptr && a.dweight == nullptr) return q;
     const int64_t last = a.vocab - (q.pieces - 1) * q.piece;
     const LossPiece g = plan_piece(a, std::min(q.piece, a.vocab), q.piece, sms);
@@ -882,6 +884,7 @@ extern "C" int hgemm_sm100_loss_backward(const HgemmSm100LossBackward* a, void* 
     float* row_alpha = reinterpret_cast<float*>(rows + q.row_bytes);
     float* row_ratio = reinterpret_cast<float*>(rows + 2 * q.row_bytes);
     float* alpha = reinterpret_cast<float*>(rows + 3 * q.row_bytes);
+    void* x_kept = rows + 3 * q.row_bytes + 256;
     const int scale = loss_scale(*a);
     // What takes the factors out of dx.
     auto scale_dx = [&](Product& d) {
@@ -890,10 +893,14 @@ extern "C" int hgemm_sm100_loss_backward(const HgemmSm100LossBackward* a, void* 
     };
     const long long* target = reinterpret_cast<const long long*>(a->target);
 
-    rc = launch(&logit_grad_setup_kernel, dim3(1), dim3(1024), 0, 1, c.stream, a->dloss,
+    // Copying blocks: four 16-byte pieces a thread, two waves of blocks at most.
+    const int64_t copying = a->dweight == nullptr
+                                ? 0
+                                : std::min<int64_t>(cdiv(a->tokens * (a->hidden / 8), 4096), 4 * c.dev->sms);
+    rc = launch(&logit_grad_setup_kernel, dim3(static_cast<unsigned>(1 + copying)), dim3(1024), 0, 1, c.stream, a->dloss,
                 scale, a->reduction == HGEMM_SM100_LOSS_MEAN ? 1 : 0, target, static_cast<int>(a->tokens),
                 static_cast<long long>(a->vocab), static_cast<long long>(a->ignore_index), row_scale, row_alpha,
-                row_ratio, alpha);
+                row_ratio, alpha, a->x, static_cast<long long>(a->ldx), static_cast<int>(a->hidden), x_kept);
     if (rc != HGEMM_SM100_OK) return rc;
 
     TrainParams p;
@@ -933,6 +940,7 @@ extern "C" int hgemm_sm100_loss_backward(const HgemmSm100LossBackward* a, void* 
         if (a->dweight != nullptr) {
             Product& d = g.s[n++];
             d.a0.ptr = dz_common;
+            d.b0 = {x_kept, a->hidden, true};
             d.out = static_cast<uint8_t*>(a->dweight) + v0 * a->hidden * 2;
             d.alpha_ptr = alpha;
         }

@@ -49,7 +49,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     ``x`` is ``[..., H]``, ``weight`` ``[V, H]``, ``target`` ``[...]`` (int64 or
     int32). ``reduction``: ``"none"`` (shape of ``target``), ``"mean"`` over the
     targets that are not ``ignore_index`` (NaN when there is none) or
-    ``"sum"``. Ignored targets have loss 0 and gradient 0. A target outside
+    ``"sum"``. Ignored targets have loss 0 and gradient 0, and add
+    nothing to the weight's, whatever ``x`` holds there. A target outside
     ``[0, V)`` that is not ``ignore_index`` gives that token a NaN loss (and NaN
     gradients) instead of a device assertion. The forward pass keeps one number
     per token; the backward pass forms the logits again, a piece of the

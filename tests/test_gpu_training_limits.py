@@ -80,3 +80,30 @@ def test_loss_infinite_gradients_stay_in_their_rows(dtype, bad):
         value = llm_hgemm.linear_cross_entropy(x, w, t, reduction=reduction)
         (dx,) = torch.autograd.grad(value, x, torch.tensor(bad, device="cuda"))
         assert not dx[keep].isfinite().any() and not dx[~keep].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+@pytest.mark.parametrize("size", [(40, 64, 500), (333, 37, 1001), (1500, 264, 700)], ids=str)
+def test_loss_ignored_rows_may_hold_anything(size, reduction, dtype):
+    """Infinity and NaN in ignored rows reach neither the loss, dx nor dW."""
+    x, w, t = loss_inputs(*size, dtype)
+    t[3] = t[9] = t[-1] = -100
+    keep = t != -100
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    dl = (torch.rand(size[0], generator=gen, device="cuda") if reduction == "none" else torch.ones((), device="cuda"))
+    want = ref.loss(x[keep], w, t[keep], reduction, -100, dl[keep] if reduction == "none" else dl)
+    poisoned = x.clone()
+    poisoned[~keep] = float("inf")
+    poisoned[3] = float("nan")
+    poisoned[9, 1:] = x[9, 1:]
+    poisoned.requires_grad_(), w.requires_grad_()
+    value = llm_hgemm.linear_cross_entropy(poisoned, w, t, reduction=reduction)
+    dx, dw = torch.autograd.grad(value, [poisoned, w], dl)
+    value = value.detach()
+    within(value[keep] if reduction == "none" else value, want[0])
+    assert not dx[~keep].any()
+    within(dx[keep], want[1])
+    within(dw, want[2])
+    (alone,) = torch.autograd.grad(llm_hgemm.linear_cross_entropy(poisoned.detach(), w, t, reduction=reduction), w, dl)
+    within(alone, want[2])
