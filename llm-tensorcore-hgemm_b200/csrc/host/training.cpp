@@ -67,6 +67,13 @@ void no_double_backward(const char* what) {
     TORCH_CHECK(!torch::GradMode::is_enabled(), what, " has no second derivative (create_graph=True)");
 }
 
+// A dual tensor needs no requires_grad: without this its tangent would be dropped,
+// which reads as zero.
+void no_forward_mode(const char* what, std::initializer_list<const Tensor*> tensors) {
+    for (const Tensor* t : tensors)
+        TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative");
+}
+
 // A gradient goes on to the node of its leaf, which lives on as long as any graph
 // of that leaf does, on the stream where the first of them was recorded. In a
 // capture the engine would make that stream wait for the captured one; where it
@@ -331,6 +338,7 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
 }  // namespace
 
 Tensor gated_ffn(const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down) {
+    no_forward_mode("gated_ffn", {&x, &gate, &up, &down});
     check_input(x);
     check_matrix(gate, "gate", x);
     check_matrix(up, "up", x);
@@ -355,6 +363,7 @@ Tensor gated_ffn(const Tensor& x, const Tensor& gate, const Tensor& up, const Te
 
 Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor& target, const std::string& reduction,
                             int64_t ignore_index) {
+    no_forward_mode("linear_cross_entropy", {&x, &weight});
     check_input(x);
     check_matrix(weight, "weight", x);
     TORCH_CHECK(weight.numel() > 0, "weight must not be empty");

@@ -36,7 +36,7 @@ def gated_ffn(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch
     launches more, one whose epilogue turns the activation's gradient into
     those of the pre-activations, and one for all wanted gradients together.
     H, I and O that are no multiples of 8 work through padded copies.
-    Gradients of gradients are refused.
+    Gradients of gradients and forward mode are refused.
     """
     return _C.gated_ffn(x, gate, up, down)
 
@@ -54,7 +54,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     ``[0, V)`` that is not ``ignore_index`` gives that token a NaN loss (and NaN
     gradients) instead of a device assertion. The forward pass keeps one number
     per token; the backward pass forms the logits again, a piece of the
-    vocabulary at a time. Gradients of gradients are refused.
+    vocabulary at a time. Gradients of gradients and forward mode are refused.
     """
     return _C.linear_cross_entropy(x, weight, target, reduction, ignore_index)
 
