@@ -25,7 +25,7 @@ from torch import nn
 
 from .dispatch import last_selected
 from .ops import hgemm, interleave_gate_up
-from .training import TrainableSwiGLU
+from .training import TrainableSwiGLU, is_plain_linear, runs_as_is
 
 
 class FrozenHgemmLinear(nn.Module):
@@ -248,19 +248,31 @@ def fuse_projections(module: nn.Module, implementation: str = "shape_auto") -> d
     return counts
 
 
+def _is_plain_mlp(module: nn.Module) -> bool:
+    """Whether ``TrainableSwiGLU`` computes what ``module`` does: three plain
+    projections, SiLU, and nothing that would be lost."""
+    linears = [getattr(module, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
+    act = getattr(module, "act_fn", None)
+    extra = set(dict(module.named_children())) - {"gate_proj", "up_proj", "down_proj", "act_fn"}
+    return (all(is_plain_linear(lin) and lin.weight.dtype in (torch.float16, torch.bfloat16) for lin in linears)
+            and not extra and not module._parameters and not module._buffers and runs_as_is(module)
+            and not (isinstance(act, nn.Module) and not runs_as_is(act)) and _is_silu(act))
+
+
 def trainable_mlps(module: nn.Module) -> int:
     """Replaces every SwiGLU MLP below ``module`` (children ``gate_proj``,
     ``up_proj``, ``down_proj``, bias-free FP16 or BF16, with a SiLU ``act_fn``)
     by a ``TrainableSwiGLU`` holding the same linears: forward and backward run
-    on this library's kernels, parameters and their names stay. Returns how
-    many were replaced."""
+    on this library's kernels, parameters and their names stay. An MLP that does
+    more stays as it is: other children, parameters or buffers (dropout, a
+    scale), projections with a ``forward`` of their own (quantisation,
+    adapters), hooks on any of them. Returns how many were replaced."""
     count = 0
     for name, child in list(module.named_children()):
-        mlp = [getattr(child, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
-        if (all(isinstance(lin, nn.Linear) and lin.bias is None
-                and lin.weight.dtype in (torch.float16, torch.bfloat16) for lin in mlp)
-                and _is_silu(getattr(child, "act_fn", None))):
-            setattr(module, name, TrainableSwiGLU(*mlp))
+        if _is_plain_mlp(child):
+            block = TrainableSwiGLU(child.gate_proj, child.up_proj, child.down_proj)
+            block.training = child.training
+            setattr(module, name, block)
             count += 1
         else:
             count += trainable_mlps(child)

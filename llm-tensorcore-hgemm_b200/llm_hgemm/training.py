@@ -75,20 +75,40 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5,
     return _C.orthogonalize(g, steps, a, b, c, eps)
 
 
+def runs_as_is(module: nn.Module) -> bool:
+    """Whether calling ``module`` is its class's ``forward`` and nothing else: no
+    hooks, no ``forward`` or ``__call__`` of its own."""
+    return not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
+                or module._backward_pre_hooks or "forward" in vars(module)
+                or type(module).__call__ is not nn.Module.__call__)
+
+
+def is_plain_linear(module) -> bool:
+    """Whether calling ``module`` multiplies by its weight and nothing else, so that
+    an operator may read the weight instead: no bias, no subclass with another
+    ``forward`` (quantisation, adapters), no hooks."""
+    return (isinstance(module, nn.Linear) and module.bias is None and type(module).forward is nn.Linear.forward
+            and runs_as_is(module))
+
+
 class TrainableSwiGLU(nn.Module):
     """SwiGLU MLP that trains through :func:`gated_ffn`; the counterpart of the
     inference-only ``HgemmSwiGLU``. It holds the projections it is built from
     as ``gate_proj``, ``up_proj`` and ``down_proj``, so parameters, state dict
-    and optimizers stay as they are."""
+    and optimizers stay as they are. The projections' weights are used, they are
+    not called: ones with another ``forward`` or with hooks are refused, also
+    where these came after the block was built."""
 
     def __init__(self, gate: nn.Linear, up: nn.Linear, down: nn.Linear):
         super().__init__()
-        for lin in (gate, up, down):
-            if not isinstance(lin, nn.Linear) or lin.bias is not None:
-                raise ValueError("requires bias-free nn.Linear projections")
+        if not all(is_plain_linear(lin) for lin in (gate, up, down)):
+            raise ValueError("requires bias-free nn.Linear projections without hooks or a forward of their own")
         if gate.weight.shape != up.weight.shape or down.in_features != gate.out_features:
             raise ValueError("gate/up/down shapes do not form an MLP")
         self.gate_proj, self.up_proj, self.down_proj = gate, up, down
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        for lin in (self.gate_proj, self.up_proj, self.down_proj):
+            if not is_plain_linear(lin):
+                raise RuntimeError("a projection got hooks, a bias or another forward, which this block does not run")
         return gated_ffn(x, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight)
