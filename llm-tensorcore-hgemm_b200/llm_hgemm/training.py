@@ -97,7 +97,8 @@ class TrainableSwiGLU(nn.Module):
     as ``gate_proj``, ``up_proj`` and ``down_proj``, so parameters, state dict
     and optimizers stay as they are. The projections' weights are used, they are
     not called: ones with another ``forward`` or with hooks are refused, also
-    where these came after the block was built."""
+    where these came after the block was built. Under ``torch.autocast`` the
+    input and the weights are cast to its type, as ``nn.Linear`` does."""
 
     def __init__(self, gate: nn.Linear, up: nn.Linear, down: nn.Linear):
         super().__init__()
@@ -111,4 +112,8 @@ class TrainableSwiGLU(nn.Module):
         for lin in (self.gate_proj, self.up_proj, self.down_proj):
             if not is_plain_linear(lin):
                 raise RuntimeError("a projection got hooks, a bias or another forward, which this block does not run")
-        return gated_ffn(x, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight)
+        weights = (self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight)
+        if torch.is_autocast_enabled("cuda"):     # what the projections' F.linear does there
+            dtype = torch.get_autocast_dtype("cuda")
+            x, *weights = (t.to(dtype) for t in (x, *weights))
+        return gated_ffn(x, *weights)
