@@ -27,4 +27,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("reduction") = "mean", py::arg("ignore_index") = -100);
     m.def("orthogonalize", &orthogonalize, py::arg("g"), py::arg("steps"), py::arg("a"), py::arg("b"), py::arg("c"),
           py::arg("eps"));
+    m.def("training_status", &training_status, py::arg("clear"));
+    m.def("training_status_address", &training_status_address);
 }

@@ -7,6 +7,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <cmath>
+#include <cstring>
 #include <limits>
 
 #include "hgemm_sm100_train.h"
@@ -52,8 +53,30 @@ Tensor cut(const Tensor& t, int64_t rows, int64_t cols) {
     return t.narrow(0, 0, rows).narrow(1, 0, cols).contiguous();
 }
 
+// Where kernels of this process record a wait that ran out: a word in host memory
+// that every device can write, so that the next call finds it without waiting for
+// the device. Never freed: captured graphs hold its address.
+volatile int32_t* status_word() {
+    static int32_t* const word = [] {
+        // Allowed while another stream is captured; the allocation is no part of it.
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+        void* p = nullptr;
+        const cudaError_t rc = cudaHostAlloc(&p, 64, cudaHostAllocPortable | cudaHostAllocMapped);
+        C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+        C10_CUDA_CHECK(rc);
+        std::memset(p, 0, 64);
+        return static_cast<int32_t*>(p);
+    }();
+    return word;
+}
+
 HgemmSm100TrainCommon common_of(const Tensor& x) {
+    const int32_t failed = training_status(true);
+    TORCH_CHECK(failed == HGEMM_SM100_OK, "a kernel of an earlier call of the training operators failed (",
+                hgemm_sm100_status_string(failed), "); what it returned, and what came of it, is not valid");
     HgemmSm100TrainCommon c{};
+    c.status = const_cast<int32_t*>(status_word());
     c.dtype = x.scalar_type() == torch::kBFloat16 ? HGEMM_SM100_TRAIN_BF16 : HGEMM_SM100_TRAIN_F16;
     return c;
 }
@@ -336,6 +359,15 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
 };
 
 }  // namespace
+
+int64_t training_status_address() { return static_cast<int64_t>(reinterpret_cast<uintptr_t>(status_word())); }
+
+int32_t training_status(bool clear) {
+    volatile int32_t* const word = status_word();
+    const int32_t value = *word;
+    if (clear && value != 0) *word = 0;
+    return value;
+}
 
 Tensor gated_ffn(const Tensor& x, const Tensor& gate, const Tensor& up, const Tensor& down) {
     no_forward_mode("gated_ffn", {&x, &gate, &up, &down});

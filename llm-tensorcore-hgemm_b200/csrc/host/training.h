@@ -20,3 +20,10 @@ torch::Tensor linear_cross_entropy(const torch::Tensor& x, const torch::Tensor& 
 
 // The last two dimensions of g orthogonalised by Newton-Schulz steps.
 torch::Tensor orthogonalize(const torch::Tensor& g, int64_t steps, double a, double b, double c, double eps);
+
+// Status of the kernels launched by the functions above so far, as far as they
+// have run (0, or HGEMM_SM100_ERR_PIPELINE_TIMEOUT); with `clear` it is reset.
+// Does not wait for the device. The next of those calls raises it too.
+int32_t training_status(bool clear);
+// Address of that word, writable by the host and all devices.
+int64_t training_status_address();

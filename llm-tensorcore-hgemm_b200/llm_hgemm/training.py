@@ -19,6 +19,7 @@ import torch
 from torch import nn
 
 from . import _C
+from .capi import status_string
 
 #: Coefficients of the quintic Newton-Schulz step of the Muon optimizer.
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
@@ -73,6 +74,18 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5,
     """
     a, b, c = coefficients
     return _C.orthogonalize(g, steps, a, b, c, eps)
+
+
+def check_status() -> None:
+    """Waits for the current device and raises ``RuntimeError`` if a kernel of an
+    operator above gave up: every wait inside the kernels has a time limit, after
+    which they return with their results incomplete. Each call of an operator
+    raises it as well, for those of earlier calls that have run by then, so this is
+    for the end of a run and for replayed graphs. Raising clears it."""
+    torch.cuda.synchronize()
+    status = _C.training_status(True)
+    if status != 0:
+        raise RuntimeError(f"a kernel of the training operators failed ({status_string(status)}); its results are not valid")
 
 
 def runs_as_is(module: nn.Module) -> bool:

@@ -1,13 +1,15 @@
 """Training operators where a call meets a limit of its kernels (GPU)."""
 
+import ctypes
+
 import pytest
 import torch
 
 import llm_hgemm
-from llm_hgemm import train_capi
+from llm_hgemm import _C, capi, train_capi, training
 from tests import training_reference as ref
 from tests.gpu_helpers import require_cuda
-from tests.test_gpu_training import DTYPES, IDS, loss_inputs, loss_through_c, within
+from tests.test_gpu_training import DTYPES, IDS, ffn_inputs, ffn_through_c, loss_inputs, loss_through_c, within
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +109,45 @@ def test_loss_ignored_rows_may_hold_anything(size, reduction, dtype):
     within(dw, want[2])
     (alone,) = torch.autograd.grad(llm_hgemm.linear_cross_entropy(poisoned.detach(), w, t, reduction=reduction), w, dl)
     within(alone, want[2])
+
+
+class StatusWord:
+    """The word that the torch functions give to their kernels, as an argument of the C calls."""
+
+    def data_ptr(self):
+        return _C.training_status_address()
+
+
+def test_a_wait_that_ran_out_raises():
+    inputs = ffn_inputs(390, 520, 712, 520, torch.bfloat16)
+    training.check_status()
+    want = llm_hgemm.gated_ffn(*inputs[:4])
+
+    def stall():
+        ffn_through_c(*inputs, 128, flags=capi.FLAG_TEST_INJECT_TX, status=StatusWord(), timeout_ns=50_000_000)
+        torch.cuda.synchronize()
+
+    stall()
+    with pytest.raises(RuntimeError, match="earlier call of the training operators failed"):
+        llm_hgemm.gated_ffn(*inputs[:4])
+    assert torch.equal(llm_hgemm.gated_ffn(*inputs[:4]), want)     # raised once
+    stall()
+    with pytest.raises(RuntimeError, match="kernel of the training operators failed"):
+        training.check_status()
+    training.check_status()
+
+
+def test_every_operator_raises_for_an_earlier_failure():
+    x, gate, up, down, dy = ffn_inputs(40, 64, 136, 64, torch.float16)
+    w, t = gate, torch.arange(40, device="cuda")
+    x.requires_grad_()
+    y, loss = llm_hgemm.gated_ffn(x, gate, up, down), llm_hgemm.linear_cross_entropy(x, w, t)
+    word = ctypes.c_int32.from_address(_C.training_status_address())
+    for call in (lambda: llm_hgemm.gated_ffn(x, gate, up, down), lambda: llm_hgemm.linear_cross_entropy(x, w, t),
+                 lambda: llm_hgemm.orthogonalize(gate), lambda: torch.autograd.grad(y, x, dy, retain_graph=True),
+                 lambda: torch.autograd.grad(loss, x, retain_graph=True)):
+        word.value = capi.ERR_PIPELINE_TIMEOUT
+        with pytest.raises(RuntimeError, match="earlier call"):
+            call()
+        assert word.value == 0
+        call()
