@@ -99,24 +99,23 @@ void no_forward_mode(const char* what, std::initializer_list<const Tensor*> tens
 
 // A gradient goes on to the node of its leaf, which lives on as long as any graph
 // of that leaf does, on the stream where the first of them was recorded. In a
-// capture the engine would make that stream wait for the captured one; where it
-// is no part of the capture this ends the process, so it is refused here.
+// capture the engine makes that stream wait for the captured one and joins it
+// again at the end, which any other stream can do (torch.cuda.make_graphed_callables
+// leaves its warm-up's there). The legacy default stream can be no part of a
+// capture: there the engine's wait ends the process, so it is refused here.
 void check_capture(const char* what) {
     using c10::cuda::CaptureStatus;
-    const c10::cuda::CUDAStream here = c10::cuda::getCurrentCUDAStream();
     if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == CaptureStatus::None) return;
     const auto node = torch::autograd::get_current_node();
     if (node == nullptr) return;
-    for (const torch::autograd::Edge& edge : node->next_edges()) {
-        if (!edge.is_valid()) continue;
-        const std::optional<c10::Stream> next = edge.function->stream();
-        if (!next.has_value() || *next == here.unwrap()) continue;
-        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-        const cudaError_t rc = cudaStreamIsCapturing(c10::cuda::CUDAStream(*next).stream(), &status);
-        if (rc != cudaSuccess) (void)cudaGetLastError();   // the legacy stream, never part of a capture
-        TORCH_CHECK(rc == cudaSuccess && status == cudaStreamCaptureStatusActive, what,
-                    " backward cannot be captured into a CUDA graph while a graph of the same tensors from outside the "
-                    "capture is alive: delete its outputs first");
+    for (uint32_t i = 0; i < node->num_outputs(); ++i) {
+        if (!node->task_should_compute_output(i)) continue;
+        const std::optional<c10::Stream> next = node->next_edge(i).function->stream();
+        if (!next.has_value()) continue;
+        const cudaStream_t stream = c10::cuda::CUDAStream(*next).stream();
+        TORCH_CHECK(stream != nullptr && stream != cudaStreamLegacy, what,
+                    " backward cannot be captured into a CUDA graph while a graph of the same tensors from the default "
+                    "stream is alive: delete its outputs first");
     }
 }
 

@@ -8,9 +8,10 @@ They take FP16 or BF16 CUDA tensors and weights in ``nn.Linear``'s layout
 packed, so an optimizer may change them between calls. Sums are FP32. Launches
 go to the current stream of the tensors' device; scratch comes from torch's
 caching allocator, so calls on different streams and captured graphs do not
-share any. A backward pass can be captured into a CUDA graph together with its
-forward pass; it is refused while an eager graph of the same leaf tensors lives
-(delete the eager call's outputs first). Like the rest of the package there is no CPU or library fallback.
+share any. A backward pass can be captured into a CUDA graph, together with its forward
+pass or after it (``torch.cuda.make_graphed_callables``); it is refused while an
+eager graph of the same tensors from the default stream lives (delete the eager
+call's outputs first). Like the rest of the package there is no CPU or library fallback.
 """
 
 from __future__ import annotations
