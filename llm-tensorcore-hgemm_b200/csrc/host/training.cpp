@@ -34,13 +34,17 @@ void check_input(const Tensor& x) {
     TORCH_CHECK(x.dim() >= 1, "x must have at least one dimension");
 }
 
+// The values in memory: torch may hold a tensor negated by a bit alone (the
+// imaginary part of a conjugate).
+Tensor as_stored(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // A [rows, cols] operand as the kernels take it: unit column stride, 16-byte
 // aligned rows, both sides padded with zeros to what is asked for. The tensor
 // itself where it already is that, else a copy. `dense`: no gap between rows.
 Tensor operand(const Tensor& t, int64_t rows, int64_t cols, bool dense) {
-    Tensor r = t;
+    Tensor r = as_stored(t);
     if (t.size(0) != rows || t.size(1) != cols)
-        r = torch::constant_pad_nd(t, {0, cols - t.size(1), 0, rows - t.size(0)});
+        r = torch::constant_pad_nd(r, {0, cols - t.size(1), 0, rows - t.size(0)});
     const int64_t ld = r.stride(0);
     const bool as_is = r.stride(1) == 1 && (ld == cols || (!dense && ld > cols && ld % 8 == 0)) &&
                        reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0;
@@ -325,7 +329,7 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
         const int64_t tokens = target.numel(), hidden = weight.size(1), hidden8 = round8(hidden);
         const Tensor xp = operand(rows_of(x, tokens, hidden), tokens, hidden8, false);
         const Tensor wp = operand(weight, weight.size(0), hidden8, true);
-        const Tensor dloss = grads[0].contiguous();
+        const Tensor dloss = as_stored(grads[0]).contiguous();
         const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
         Tensor dx, dw;
         if (need_x) dx = fresh({tokens, hidden8}, x.scalar_type(), x);
@@ -419,7 +423,7 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
     const c10::cuda::CUDAGuard device_guard(x.device());
     Tensor flat = target.dim() == 1 ? target : target.reshape({tokens});
     if (flat.scalar_type() != torch::kInt64) flat = flat.to(torch::kInt64);
-    flat = flat.contiguous();
+    flat = as_stored(flat).contiguous();
     const bool keep = torch::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad());
     const Tensor loss = keep ? LinearCrossEntropy::apply(x, weight, flat, tokens, static_cast<int64_t>(kind),
                                                          ignore_index)
@@ -441,7 +445,7 @@ Tensor orthogonalize(const Tensor& g, int64_t steps, double a, double b, double 
     if (g.numel() == 0) return out;
     const int64_t rows = g.size(-2), cols = g.size(-1), batch = g.numel() / (rows * cols);
     TORCH_CHECK(batch <= 65535, "at most 65535 matrices in one call, got ", batch);
-    Tensor m = g.detach().reshape({batch, rows, cols});
+    Tensor m = as_stored(g.detach()).reshape({batch, rows, cols});
     if (m.stride(2) != 1 || m.stride(1) < cols || m.stride(0) < 0) m = m.contiguous();
     HgemmSm100Orthogonalize args{};
     args.common = common_of(g);

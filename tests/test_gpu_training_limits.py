@@ -151,3 +151,29 @@ def test_every_operator_raises_for_an_earlier_failure():
             call()
         assert word.value == 0
         call()
+
+
+def test_values_negated_by_a_bit():
+    """torch holds the imaginary part of a conjugate as its negative, by a bit of
+    the tensor: as an input, and as the gradient that comes in behind one."""
+    x, gate, up, down, dy = ffn_inputs(20, 64, 136, 72, torch.float16)
+    neg = torch._neg_view
+    assert neg(x).is_neg() and torch.equal(neg(x), -x)
+    for k in range(4):
+        args = [x, gate, up, down]
+        args[k] = -args[k]
+        want = llm_hgemm.gated_ffn(*args)
+        args[k] = neg([x, gate, up, down][k])
+        assert torch.equal(llm_hgemm.gated_ffn(*args), want)
+    x.requires_grad_()
+    y = llm_hgemm.gated_ffn(x, gate, up, down)
+    (want,) = torch.autograd.grad(y, x, -dy, retain_graph=True)
+    assert torch.equal(torch.autograd.grad(y, x, neg(dy))[0], want)
+    assert torch.equal(llm_hgemm.orthogonalize(neg(gate)), llm_hgemm.orthogonalize(-gate))
+    assert torch.equal(llm_hgemm.orthogonalize(neg(gate[:, :8])), llm_hgemm.orthogonalize(-gate[:, :8]))
+    t = torch.arange(20, device="cuda")
+    assert torch.equal(llm_hgemm.linear_cross_entropy(x, gate, neg(-t)), llm_hgemm.linear_cross_entropy(x, gate, t))
+    loss = llm_hgemm.linear_cross_entropy(x, gate, t)
+    (want,) = torch.autograd.grad(loss, x, torch.tensor(-3.0, device="cuda"), retain_graph=True)
+    z = torch.complex(torch.zeros((), device="cuda"), loss).conj()
+    assert torch.equal(torch.autograd.grad(3 * z.imag, x)[0], want)
