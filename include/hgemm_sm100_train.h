@@ -12,7 +12,8 @@
  * contents do, two calls that may overlap need one each.
  *
  * Matrices are row-major with FP16 or BF16 elements (one type per call) and
- * FP32 accumulation. Bases must be 16-byte aligned; leading dimensions, hidden
+ * FP32 accumulation. Bases of matrices must be 16-byte aligned (except where it
+ * says otherwise), those of other arrays to their elements; leading dimensions, hidden
  * and inner sizes multiples of 8 elements (the Python layer pads other sizes).
  * Token counts, vocabularies and the sides of an orthogonalised matrix take
  * any value from 1 on.

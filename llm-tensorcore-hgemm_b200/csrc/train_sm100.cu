@@ -343,7 +343,11 @@ struct Context {
     HgemmSm100TrainCommon common{};
 };
 
+bool aligned(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+bool aligned16(const void* p) { return aligned(p, 16); }
+
 int begin(Context* c, const HgemmSm100TrainCommon& common, void* stream) {
+    if (!aligned(common.status, 4)) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     if (common.dtype != HGEMM_SM100_TRAIN_F16 && common.dtype != HGEMM_SM100_TRAIN_BF16)
         return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     if (common.flags & ~HGEMM_SM100_FLAG_TEST_INJECT_TX) return HGEMM_SM100_ERR_INVALID_ARGUMENT;
@@ -514,7 +518,6 @@ int run_and_join(Product& s, const Tile& t, void* parts, const Context& c) {
     return rc != HGEMM_SM100_OK ? rc : join_parts(s, t, c, p.in_bf16, p.out_bf16);
 }
 
-bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 bool size_ok(int64_t v) { return v > 0 && v <= kMaxSize; }
 bool size8_ok(int64_t v) { return size_ok(v) && v % 8 == 0; }
 // A matrix operand: present, aligned, its pitch a multiple of 8 and at least `cols`.
@@ -815,7 +818,8 @@ LossBackwardPlan plan_loss_backward(const HgemmSm100LossBackward& a, int sms) {
 template <typename Args>
 bool loss_args_ok(const Args& a) {
     return size_ok(a.tokens) && size8_ok(a.hidden) && size_ok(a.vocab) && matrix_ok(a.x, a.ldx, a.hidden) &&
-           matrix_ok(a.weight, 8, 8) && a.target != nullptr && a.lse != nullptr &&
+           matrix_ok(a.weight, 8, 8) && a.target != nullptr && aligned(a.target, 8) && a.lse != nullptr &&
+           aligned(a.lse, 4) &&
            a.reduction >= HGEMM_SM100_LOSS_NONE && a.reduction <= HGEMM_SM100_LOSS_SUM;
 }
 
@@ -829,7 +833,8 @@ extern "C" size_t hgemm_sm100_loss_forward_workspace(const HgemmSm100LossForward
 }
 
 extern "C" int hgemm_sm100_loss_forward(const HgemmSm100LossForward* a, void* stream) {
-    if (a == nullptr || !loss_args_ok(*a) || a->loss == nullptr || a->workspace == nullptr || !aligned16(a->workspace))
+    if (a == nullptr || !loss_args_ok(*a) || a->loss == nullptr || !aligned(a->loss, 4) ||
+        a->workspace == nullptr || !aligned16(a->workspace))
         return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     Context c;
     int rc = begin(&c, a->common, stream);
@@ -866,7 +871,7 @@ extern "C" size_t hgemm_sm100_loss_backward_workspace(const HgemmSm100LossBackwa
 }
 
 extern "C" int hgemm_sm100_loss_backward(const HgemmSm100LossBackward* a, void* stream) {
-    if (a == nullptr || !loss_args_ok(*a) || a->dloss == nullptr || a->workspace == nullptr ||
+    if (a == nullptr || !loss_args_ok(*a) || a->dloss == nullptr || !aligned(a->dloss, 4) || a->workspace == nullptr ||
         !aligned16(a->workspace) || !aligned16(a->dx) || !aligned16(a->dweight) || a->piece < 0)
         return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     Context c;
@@ -1084,11 +1089,11 @@ extern "C" size_t hgemm_sm100_orthogonalize_workspace(const HgemmSm100Orthogonal
 }
 
 extern "C" int hgemm_sm100_orthogonalize(const HgemmSm100Orthogonalize* a, void* stream) {
-    if (a == nullptr || !orth_sizes_ok(*a) || a->g == nullptr || a->out == nullptr || a->ldg < a->cols ||
-        a->batch_stride < 0 || !(a->eps >= 0))
+    if (a == nullptr || !orth_sizes_ok(*a) || a->g == nullptr || a->out == nullptr || !aligned(a->g, 2) ||
+        !aligned(a->out, 2) || a->ldg < a->cols || a->batch_stride < 0 || !(a->eps >= 0))
         return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     const int ctas = orth_cluster_ctas(*a);
-    if (ctas == 0 && (a->workspace == nullptr || reinterpret_cast<uintptr_t>(a->workspace) % 256 != 0))
+    if (ctas == 0 && (a->workspace == nullptr || !aligned(a->workspace, 256)))
         return HGEMM_SM100_ERR_INVALID_ARGUMENT;
     Context c;
     int rc = begin(&c, a->common, stream);
