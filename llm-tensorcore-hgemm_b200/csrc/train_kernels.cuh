@@ -1076,8 +1076,9 @@ __global__ void __launch_bounds__(1024) loss_reduce_kernel(const float* loss,
 // One incoming gradient for all rows: row_scale is 2^14 and alpha has the rest.
 // Infinity and NaN go to the rows they belong to, where alpha would bring them
 // to the others (0 x inf); an ignored row's gradient is 0 in any case.
-// One per row, kScaleBf16: BF16 has FP32's range, so row_scale = dloss[row] and
-// alpha = 1. FP16 with one scale for all rows loses probabilities of small
+// One per row, kScaleBf16: row_scale = dloss[row] 2^k, alpha = 2^-k, with the
+// largest at 2^60 (k at most 100, which FP32 has the inverse of): BF16's range
+// then holds probabilities in rows with 1e-40 of it. FP16 with one scale for all rows loses probabilities of small
 // gradients: 1/151936 is subnormal in a row with 1/1800 of the largest, and zero
 // with 1/3.6e6. A sum over rows (dW) needs one scale, a row of dx does not, so dz
 // is written in both where both are wanted. kScaleRows: row_scale = dloss[row]
@@ -1118,7 +1119,7 @@ __global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* dlo
     for (int i = threadIdx.x; i < m; i += 1024) {
         if (target[i] == ignore) continue;
         ++c;
-        if (kind >= kScaleCommon) {
+        if (kind != kScaleOne) {
             const float a = fabsf(dloss[i]);
             if (a <= kMost) top = fmaxf(top, a);
         }
@@ -1140,13 +1141,14 @@ __global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* dlo
     }
     int most = 0;
     if (top > 0.f) frexpf(top, &most);
+    const int up = min(60 - most, 100);   // kScaleBf16
     const float nan = __int_as_float(0x7fffffff);
     for (int i = threadIdx.x; i < m; i += 1024) {
         const long long want = target[i];
         float r = 0.f, own_alpha = 1.f, ratio = 1.f;
         if (want != ignore) {
             const float d = kind == kScaleOne ? dloss[0] : dloss[i];
-            r = one_finite ? kLogitGradScale : d;
+            r = one_finite ? kLogitGradScale : kind == kScaleBf16 ? ldexpf(d, up) : d;
             if (kind >= kScaleCommon && d != 0.f && fabsf(d) <= kMost) {
                 int e;
                 r = ldexpf(frexpf(d, &e), 15);
@@ -1170,6 +1172,8 @@ __global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* dlo
             a /= kLogitGradScale;
         } else if (kind >= kScaleCommon) {
             a = ldexpf(1.f, most - 15);
+        } else if (kind == kScaleBf16) {
+            a = ldexpf(1.f, -up);
         }
         *alpha = a;
     }

@@ -38,7 +38,9 @@ def test_loss_short_last_piece_of_many_tile_rows(tokens, vocab, piece, tile):
 @pytest.mark.parametrize("dtype, sizes", [
     (torch.float16, [2e4, 1e-3, 1.0, -3e-3, 0.0, 5e-5]),
     (torch.bfloat16, [1e20, 1e-20, 1.0, -3e-22, 0.0, 5e4]),
-], ids=["fp16", "bf16"])
+    (torch.bfloat16, [1e-35, -3e-35, 2e-36, 1e-35, 0.0, 1e-37]),
+    (torch.bfloat16, [3.4e38, -3.4e38, 1.0, 1e30, 0.0, 1e8]),
+], ids=["fp16", "bf16", "bf16 tiny", "bf16 huge"])
 def test_loss_gradients_of_small_and_large_rows(dtype, sizes, wanted, piece):
     """Every row of dx is as good as if it were the only one, whatever the other
     rows' incoming gradients. The weights have a mean, so that the probabilities'
