@@ -32,14 +32,15 @@
 // 32 columns), warp 8 TMA producer, warp 9 MMA issuer; two accumulators, so a
 // tile's epilogue runs under the next tile's MMAs; eight warps, because the last
 // tile's epilogue is exposed and the gradient of the gate is a long one (dh at
-// 4096 x 9728 x 2560: 278 us with four, 192 with eight). Every wait is bounded
+// 4096 x 9728 x 2560: 278 us with four, 192 with eight, 168 since its side inputs
+// come in coalesced patches). Every wait is bounded
 // as in the inference kernels (status word, drained copies, freed TMEM).
 //
 // What bounds it (2048 tokens, hidden 2560, under ncu): the tensor pipe where
-// the epilogue stores nothing (softmax statistics: 92 % active, 1.65 PFLOP/s);
-// 82-86 % where it stores 16 bits (logit gradients, the weights' gradients);
-// 74 % with three outputs (gate); 49 % where it reads two matrices and writes
-// two (gradient of the gate). DRAM is at 11-24 % and L2 at 42-52 % throughout.
+// the epilogue stores nothing (softmax statistics: 91 % active, 1.66 PFLOP/s);
+// 82-85 % where it stores 16 bits (logit gradients, the weights' gradients);
+// 75 % with three outputs (gate); 50 % where it reads two matrices and writes
+// two (gradient of the gate). DRAM is at 11-24 % and L2 at 43-54 % throughout.
 // Long back-to-back runs are held by the power limit instead (sampled: 1.24 to
 // 1.55 GHz of 1.965, the power cap active all the time; 1.2-1.35 PFLOP/s). A K block of a 256 x 256 pair tile takes about
 // 590 cycles of which the MMAs are 512.
@@ -1085,9 +1086,10 @@ __global__ void __launch_bounds__(1024) loss_reduce_kernel(const float* loss,
 // 2^(15 - e), e the row's own exponent, and dx = row_alpha[row] dz W; row_ratio =
 // 2^(e - E), E the largest exponent, turns such a dz into the common scale's.
 // kScaleCommon: that scale alone, dloss[row] 2^(15 - E); alpha = 2^(E - 15).
-// Block 0; latency, 4.6-5.7 us for 24 to 4096 rows. Further blocks, where dW is
+// Block 0; latency, 4.6-5.9 us for 24 to 4096 rows. Further blocks, where dW is
 // wanted, copy x with zeros for the ignored rows: their dz is 0, but dz^T x would
-// still take infinity and NaN from them (padding may hold anything).
+// still take infinity and NaN from them (padding may hold anything). With the copy
+// 6-7 us at 777 x 1024, 11-13 us at 4096 x 2560 (42 MB, cold).
 enum : int { kScaleOne = 0, kScaleBf16 = 1, kScaleCommon = 2, kScaleRows = 3 };
 __global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* dloss, int kind, int mean,
                                                                 const long long* target, int m,
@@ -1182,8 +1184,8 @@ __global__ void __launch_bounds__(1024) logit_grad_setup_kernel(const float* dlo
 // The tiles of a product whose sums came in parts: out = alpha (part 0 + part 1
 // + ...) + beta C, added in that order and rounded once. Block (x, y): some rows
 // of tile tile0 + y; eight columns per thread. Reads what the parts wrote, mostly
-// from L2: 3 us of a launch more, which the parts have to save (y of one token,
-// 2560 x 9728: 42 us whole, 15 + 3 in parts).
+// from L2: a launch more, which the parts have to save (y of one token,
+// 2560 x 9728, cold: 42 us whole, 14 + 5 in parts).
 struct JoinParams {
     const float* parts;
     int splits, tiles, tile0, tiles_m, tiles_n, group_m, tile_m, tile_n, m, n;

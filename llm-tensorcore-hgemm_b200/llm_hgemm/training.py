@@ -4,8 +4,11 @@ weight, each with hand-written sm_100a kernels (no reference counterpart: the
 reference, llm_hgemm/integration.py:8-46, is inference-only).
 
 They take FP16 or BF16 CUDA tensors and weights in ``nn.Linear``'s layout
-(``[out_features, in_features]``), which are read where they are: nothing is
-packed, so an optimizer may change them between calls. Sums are FP32. Launches
+(``[out_features, in_features]``), which are read on every call: nothing is
+packed or kept, so an optimizer may change them between calls. A weight without
+gaps between its rows, with 16-byte aligned rows and sizes that are multiples of
+8, is read where it is; any other (a slice of columns, say) is copied in each
+forward and each backward pass. Sums are FP32. Launches
 go to the current stream of the tensors' device; scratch comes from torch's
 caching allocator, so calls on different streams and captured graphs do not
 share any. A backward pass can be captured into a CUDA graph, together with its forward
@@ -37,7 +40,8 @@ def gated_ffn(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch
     derivatives are kept (``3 * tokens * I`` elements); the backward pass is two
     launches more, one whose epilogue turns the activation's gradient into
     those of the pre-activations, and one for all wanted gradients together.
-    H, I and O that are no multiples of 8 work through padded copies.
+    Where the sums of the result or of ``x``'s gradient come in parts (few
+    tokens, a nearly empty last wave), one more launch adds them, each way. H, I and O that are no multiples of 8 work through padded copies.
     Gradients of gradients and forward mode are refused.
     """
     return _C.gated_ffn(x, gate, up, down)
@@ -71,7 +75,9 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5,
 
     Leading dimensions are a batch of matrices, each normalised by itself. A
     zero matrix gives zeros. The steps run on FP16 elements (scaled by a power
-    of two) whatever the dtype of ``g``. No gradient is recorded.
+    of two) whatever the dtype of ``g``, so no element may pass 255 on the way, or
+    65504 in ``A`` and the polynomial: coefficients that keep the singular values
+    near 1 stay far below. No gradient is recorded.
     """
     a, b, c = coefficients
     return _C.orthogonalize(g, steps, a, b, c, eps)
